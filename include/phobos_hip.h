@@ -304,6 +304,170 @@ int phx_flash_attention_bh_noalloc(phx_stream s, phx_kernel k, uint64_t q, uint6
                                    uint64_t v, uint64_t o, int64_t BH, int64_t Nq, int64_t Nk,
                                    int64_t D, float scale);
 
+/* ------------------------------------------------------------ decode operators */
+/* What answering with a model takes beside the leaf kernels above: products
+ * of a few rows with weights held in 4 bits, attention over a cache of keys
+ * and values held in 4 bits in pages, and the pages themselves.  No
+ * counterparts in the reference, whose attention reads dense K and V
+ * (examples/flash_attention_fp16.ph:1-44) and whose store gives out whole
+ * tiles (tile_store.rs:14-83).
+ *
+ * Every entry below that takes a stream launches on it and returns; it never
+ * allocates or waits, so it can be captured into a graph (the first use of a
+ * kernel loads its code object, in a capture too).  The device given to
+ * phx_init has to be the calling thread's current one and the stream's
+ * (PHX_E_INVALID otherwise).  Arguments are checked before anything is
+ * launched; what lies in device memory (lengths, tables, row starts) is
+ * checked by the kernels, which read and write nothing outside the pool, the
+ * tables and the rows they were given, whatever it holds. */
+typedef enum { PHX_F32 = 0, PHX_F16 = 1 } phx_dtype;
+
+/* --- products of few rows with 4-bit weights ---
+ * W is [K, N] as B of a GEMM: codes 0 .. 15, a scale (f16) and optionally a
+ * zero point (u8, 8 where zeros is 0) for each group of `group` (32, 64 or
+ * 128) rows of a column, both [ceil(K/group), N] row-major.  A weight stands
+ * for (code - zero) * scale.
+ * Packed codes: tiles of 16 columns by 128 rows, [ceil(N/16)][ceil(K/128)] of
+ * them, 1 KiB each; dword [q][r][j] (q, j < 4; r < 16) of a tile holds column
+ * r of the tile at its rows 32j + 8q + i, i = 0 .. 7, element i in bits
+ * 4 (i/2 + 4 (i%2)) and up.  Padding codes may be anything. */
+size_t phx_w4_packed_bytes(int64_t N, int64_t K);
+/* codes: u8 [K, N] row-major, device memory, the low four bits of each. */
+int phx_w4_pack(phx_stream s, uint64_t codes, uint64_t packed, int64_t N, int64_t K);
+/* C = alpha*A@W + beta*C over 0 <= M <= 64 rows (more is a GEMM's work), A
+ * [M, K] and C [M, N] of type t with rows lda and ldc elements apart (0: K
+ * and N).  K % 8 == 0, any N; A's rows and the packed codes start 16-byte
+ * aligned (lda % 8 == 0 for f16, % 4 for f32).  Codes less zero points and
+ * f16 operands enter the products exactly, f32 operands with all their bits;
+ * products, sums and scales are f32, and C is rounded once from
+ * fl(fl(alpha*acc) + fl(beta*c)), not read when beta == 0.  C overlaps no
+ * other operand. */
+int phx_gemv_w4(phx_stream s, phx_dtype t, uint64_t a, uint64_t w, uint64_t scales,
+                uint64_t zeros, uint64_t c, int64_t M, int64_t N, int64_t K, int64_t group,
+                float alpha, float beta, int64_t lda, int64_t ldc);
+
+/* --- a cache of keys and values in 4 bits ---
+ * A pool of pages, 256-byte aligned, each of page_tokens (32, 64, 128 or 256)
+ * token slots for every one of `heads` KV heads of head_dim (64 or 128)
+ * elements: for each head page_tokens*(head_dim+8) bytes,
+ *   K's codes  [page_tokens][head_dim/2], element 2i in the low nibble;
+ *   V's codes  [page_tokens/4][head_dim/8][4] dwords: token 4a+r, elements
+ *              8e .. 8e+7 from the low nibble up at [a][e][r];
+ *   K's (f16 scale, f16 minimum) [page_tokens], then V's.
+ * A code c stands for c*scale + minimum; scales are positive. */
+typedef struct {
+    uint64_t pool;
+    int64_t pages;
+    int32_t heads;
+    int32_t head_dim;
+    int32_t page_tokens;
+} phx_kv4_cache;
+/* Bytes of one page, 0 for sizes the cache does not take. */
+size_t phx_kv4_page_bytes(int32_t heads, int32_t head_dim, int32_t page_tokens);
+
+/* The sequences of a call.  Sequence b holds lens[b] tokens, those of this
+ * call among them (cut to 0 .. min(max_len, table_stride*page_tokens)), in the
+ * pages table[b][0 ..]; its T rows of the call are its last T tokens, at
+ * positions lens[b]-T .. lens[b]-1.  Rows are those from q_starts[b] up to
+ * q_starts[b+1] (at most max_q of them), or with q_starts 0 the max_q rows
+ * from b*max_q.  `rows` is how many rows the call's tensors have; a row at or
+ * past it, or below 0, does not exist.  Entries of the table that a sequence
+ * does not reach may be anything; one that it reaches and that is no page
+ * (below 0 or at least `pages`) is a page of no tokens.  Two sequences may
+ * share pages that the call only reads. */
+typedef struct {
+    uint64_t table;        /* i32 [batch][table_stride] */
+    int64_t table_stride;  /* entries per sequence */
+    uint64_t lens;         /* i32 [batch] */
+    uint64_t q_starts;     /* i32 [batch+1], or 0 */
+    int64_t batch;
+    int64_t max_q;
+    int64_t max_len;       /* no length is longer: sets how a launch is split */
+    int64_t rows;
+} phx_kv4_batch;
+
+/* Quantises the rows' K and V [rows][heads][head_dim] (type t, token rows ldk
+ * and ldv elements apart, 0: heads*head_dim) and writes them to their
+ * positions in the pages.  Per token and head minimum = f16(min x), scale =
+ * max(f16((max x - min x)/15), 2^-24), code = rint((x - minimum)/scale) of
+ * the exact quotient, ties to even, cut to 0 .. 15.  Values are finite and
+ * within f16's range.  Rows at positions below 0 are not written. */
+int phx_kv4_append(phx_stream s, const phx_kv4_cache *cache, const phx_kv4_batch *batch,
+                   phx_dtype t, uint64_t k, uint64_t v, int64_t ldk, int64_t ldv);
+/* The rows' K and V as the cache holds them, c*scale + minimum in f32 rounded
+ * once to type t: the inverse of append, e.g. for phx_flash_attention_bh over
+ * what a cache holds.  Rows at positions below 0 or in no page are zeros. */
+int phx_kv4_read(phx_stream s, const phx_kv4_cache *cache, const phx_kv4_batch *batch,
+                 phx_dtype t, uint64_t k, uint64_t v, int64_t ldk, int64_t ldv);
+/* O = softmax(scale * Q K^T) V of the rows' Q [rows][q_heads][head_dim] over
+ * the keys of their sequence: with causal those up to the row's own position,
+ * else all.  q_heads is a multiple of the cache's heads; query head h reads KV
+ * head h / (q_heads / heads).  A row without keys gets zeros.  Q and O are of
+ * type t, rows ldq and ldo elements apart (0: q_heads*head_dim), and start
+ * 16-byte aligned (ldq, ldo % 8 == 0 for f16, % 4 for f32).  Codes and f16
+ * queries enter the products exactly, f32 queries and the softmax's weights as
+ * two f16 terms (22 bits); scores, statistics and sums are f32.
+ * A launch too small to fill the GPU is split over the keys when s has a
+ * workspace bound that holds the parts (phx_stream_set_workspace,
+ * phx_kv4_split_plan), else it runs unsplit.  A captured launch keeps the
+ * workspace it was captured with: two graphs with the same one must not run
+ * at the same time. */
+int phx_kv4_attention(phx_stream s, const phx_kv4_cache *cache, const phx_kv4_batch *batch,
+                      phx_dtype t, uint64_t q, uint64_t o, int64_t q_heads, float scale,
+                      int causal, int64_t ldq, int64_t ldo);
+/* The split such a launch runs with where at least *workspace_bytes are bound
+ * (fewer parts with less): *splits parts of every sequence's keys, 1 and 0
+ * bytes for none. */
+int phx_kv4_split_plan(const phx_kv4_cache *cache, const phx_kv4_batch *batch, int64_t q_heads,
+                       int *splits, size_t *workspace_bytes);
+
+/* --- pages ---
+ * Which page belongs to which sequence, on the host: a pool of `pages` pages
+ * of page_tokens tokens, shared by sequences that were forked and copied when
+ * one of them is about to write where another reads.  One table serves every
+ * layer.  Calls on one pool may come from several threads. */
+typedef struct phx_pages_s *phx_pages;
+int phx_pages_create(phx_pages *p, int32_t pages, int32_t page_tokens);
+int phx_pages_destroy(phx_pages p);
+/* A new, empty sequence; ids count up from 0 and are not used again. */
+int phx_pages_new(phx_pages p, int64_t *seq);
+/* Sets a sequence's length: more tokens take new pages (the lowest free), and
+ * a partly filled last page that another sequence shares is replaced by a
+ * copy of its own; fewer return the pages past the end.  PHX_E_EXHAUSTED, with
+ * nothing changed, when the pages do not suffice. */
+int phx_pages_resize(phx_pages p, int64_t seq, int64_t tokens);
+/* A new sequence of the same tokens, in the same pages. */
+int phx_pages_fork(phx_pages p, int64_t seq, int64_t *child);
+int phx_pages_free(phx_pages p, int64_t seq);
+/* Moves the pages in use to the lowest numbers (the tables change); refused
+ * while copies are pending. */
+int phx_pages_compact(phx_pages p);
+/* A sequence's pages: *count of them (nullable), the first cap into out. */
+int phx_pages_table(phx_pages p, int64_t seq, int32_t *out, int64_t cap, int64_t *count);
+/* Pages in use (those that pending copies hold among them), one past the
+ * highest of them, and pending copies (each nullable). */
+int phx_pages_stats(phx_pages p, int64_t *used, int64_t *top, int64_t *pending);
+/* The pending copies, src[i] to dst[i]: *count (nullable) of them, the first
+ * cap into src and dst.  With clear they are no longer pending, as the caller
+ * runs them (PHX_E_INVALID, and none is cleared, when there are more than cap). */
+int phx_pages_pending(phx_pages p, int32_t *src, int32_t *dst, int64_t cap, int64_t *count,
+                      int clear);
+/* Launches the pending copies in the pool at `pool` and clears them: to be
+ * called on the stream of the cache's work after resizes and compactions and
+ * before the cache is read or written with the new tables.  Arguments as
+ * phx_pages_copy.  If it fails they stay pending. */
+int phx_pages_apply(phx_pages p, phx_stream s, uint64_t pool, size_t page_bytes, int64_t layers,
+                    uint64_t layer_stride);
+/* Copies page src[i] to page dst[i], i < n, in each of `layers` pools
+ * layer_stride bytes apart, of `pages` pages of page_bytes (a multiple of 16,
+ * as the addresses) each.  src and dst are host arrays, read before the call
+ * returns.  A page may be the source of several copies; no page may be the
+ * destination of two, nor destination and source (PHX_E_INVALID; a page
+ * copied to itself is left out). */
+int phx_pages_copy(phx_stream s, uint64_t pool, int64_t pages, size_t page_bytes,
+                   const int32_t *src, const int32_t *dst, int64_t n, int64_t layers,
+                   uint64_t layer_stride);
+
 /* ------------------------------------------------------------ inputs */
 /* Lcg::unit_f32s (phobos-base/src/rng.rs:9-25) into host memory. */
 int phx_lcg_fill_f32(uint64_t seed, size_t n, float *out);

@@ -23,6 +23,9 @@ int kernel_abi(phx_kernel k, int *bits, uint32_t block[3]);
 int launch_raw(hipFunction_t f, const uint32_t grid[3], const uint32_t block[3], uint32_t shmem,
                hipStream_t s, void **args);
 int aux_function(const char *file, const char *entry, hipFunction_t *out);
+// PHX_OK if the device given to phx_init is the calling thread's current one
+// and the stream's
+int on_device(hipStream_t s);
 // split-key flash attention (phx_runtime.cpp)
 int flash_split(phx_kernel k, int64_t BH, int64_t Nq, int64_t Nk);
 size_t flash_split_bytes(int64_t BH, int64_t Nq, int sp);

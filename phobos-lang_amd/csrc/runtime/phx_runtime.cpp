@@ -136,6 +136,31 @@ int builtin(phx_kernel k, hipFunction_t *out) {
     return PHX_OK;
 }
 
+int on_device(hipStream_t s) {
+    if (int rc = ensure_init()) return rc;
+    int dev = -1;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return hip_error(e, "hipGetDevice");
+    if (dev != g.device)
+        return set_error(PHX_E_INVALID, "device %d is current, phx_init was given %d", dev, g.device);
+    if (!s) return PHX_OK;
+    hipDevice_t of = -1;
+    e = hipStreamGetDevice(s, &of);
+    if (e != hipSuccess) return hip_error(e, "hipStreamGetDevice");
+    if (of != g.device)
+        return set_error(PHX_E_INVALID, "the stream is of device %d, phx_init was given %d", (int)of,
+                         g.device);
+    return PHX_OK;
+}
+
+// While it lives, the calling thread may load code objects although a stream
+// is being captured: a load is no part of the graph.
+struct OutsideCapture {
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    OutsideCapture() { (void)hipThreadExchangeStreamCaptureMode(&mode); }
+    ~OutsideCapture() { (void)hipThreadExchangeStreamCaptureMode(&mode); }
+};
+
 static int find_aux(const char *file, const char *entry, hipFunction_t *out);
 
 // Entry points of the built-in code objects that no .ph kernel names (the
@@ -165,6 +190,7 @@ int aux_function(const char *file, const char *entry, hipFunction_t *out) {
 
 static int find_aux(const char *file, const char *entry, hipFunction_t *out) {
     std::lock_guard<std::mutex> lock(g.mu);
+    OutsideCapture outside;
     const std::string key = std::string(file) + ":" + entry;
     auto fit = g.aux.find(key);
     if (fit != g.aux.end()) {

@@ -46,7 +46,11 @@ KERNEL_NAMES = {
 
 CODE_OBJECTS = ["saxpy_fp32.hsaco", "gemm_fp32.hsaco", "gemm_fp16tc_fp32acc.hsaco",
                 "gemm_fp16.hsaco", "flash_attention_fp32.hsaco", "flash_attention_fp16.hsaco",
-                "matmul_cluster_fp32.hsaco"]
+                "matmul_cluster_fp32.hsaco", "gemv_w4.hsaco", "kv4.hsaco", "pages.hsaco"]
+
+# phx_dtype of the decode operators
+F32 = 0
+F16 = 1
 
 PHX_E_INVALID = 1001
 PHX_E_NOT_INIT = 1002
@@ -67,6 +71,20 @@ class TileArg(ctypes.Structure):
 
 class ScalarArg(ctypes.Structure):
     _fields_ = [("pos", ctypes.c_uint32), ("bytes", ctypes.c_uint32), ("bits", ctypes.c_uint64)]
+
+
+class Kv4Cache(ctypes.Structure):
+    """phx_kv4_cache: a pool of 4-bit key and value pages (device address)."""
+    _fields_ = [("pool", ctypes.c_uint64), ("pages", ctypes.c_int64), ("heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("page_tokens", ctypes.c_int32)]
+
+
+class Kv4Batch(ctypes.Structure):
+    """phx_kv4_batch: the sequences of a call (device addresses of i32 arrays)."""
+    _fields_ = [("table", ctypes.c_uint64), ("table_stride", ctypes.c_int64),
+                ("lens", ctypes.c_uint64), ("q_starts", ctypes.c_uint64),
+                ("batch", ctypes.c_int64), ("max_q", ctypes.c_int64),
+                ("max_len", ctypes.c_int64), ("rows", ctypes.c_int64)]
 
 
 _LIB = None
@@ -151,6 +169,33 @@ def lib():
     L.phx_flash_attention_bh.argtypes = [_vp, ctypes.c_int, _u64, _u64, _u64, _u64, _i64, _i64,
                                          _i64, _i64, ctypes.c_float]
     L.phx_flash_attention_bh_noalloc.argtypes = L.phx_flash_attention_bh.argtypes
+    L.phx_w4_packed_bytes.argtypes = [_i64, _i64]
+    L.phx_w4_packed_bytes.restype = _sz
+    L.phx_w4_pack.argtypes = [_vp, _u64, _u64, _i64, _i64]
+    L.phx_gemv_w4.argtypes = [_vp, ctypes.c_int] + [_u64] * 5 + [_i64] * 4 + \
+        [ctypes.c_float] * 2 + [_i64] * 2
+    _cache, _batch = ctypes.POINTER(Kv4Cache), ctypes.POINTER(Kv4Batch)
+    L.phx_kv4_page_bytes.argtypes = [ctypes.c_int32] * 3
+    L.phx_kv4_page_bytes.restype = _sz
+    L.phx_kv4_append.argtypes = [_vp, _cache, _batch, ctypes.c_int, _u64, _u64, _i64, _i64]
+    L.phx_kv4_read.argtypes = L.phx_kv4_append.argtypes
+    L.phx_kv4_attention.argtypes = [_vp, _cache, _batch, ctypes.c_int, _u64, _u64, _i64,
+                                    ctypes.c_float, ctypes.c_int, _i64, _i64]
+    L.phx_kv4_split_plan.argtypes = [_cache, _batch, _i64, ctypes.POINTER(ctypes.c_int),
+                                     ctypes.POINTER(_sz)]
+    _pi64, _pi32 = ctypes.POINTER(_i64), ctypes.POINTER(ctypes.c_int32)
+    L.phx_pages_create.argtypes = [ctypes.POINTER(_vp), ctypes.c_int32, ctypes.c_int32]
+    L.phx_pages_destroy.argtypes = [_vp]
+    L.phx_pages_new.argtypes = [_vp, _pi64]
+    L.phx_pages_resize.argtypes = [_vp, _i64, _i64]
+    L.phx_pages_fork.argtypes = [_vp, _i64, _pi64]
+    L.phx_pages_free.argtypes = [_vp, _i64]
+    L.phx_pages_compact.argtypes = [_vp]
+    L.phx_pages_table.argtypes = [_vp, _i64, _pi32, _i64, _pi64]
+    L.phx_pages_stats.argtypes = [_vp, _pi64, _pi64, _pi64]
+    L.phx_pages_pending.argtypes = [_vp, _pi32, _pi32, _i64, _pi64, ctypes.c_int]
+    L.phx_pages_apply.argtypes = [_vp, _vp, _u64, _sz, _i64, _u64]
+    L.phx_pages_copy.argtypes = [_vp, _u64, _i64, _sz, _vp, _vp, _i64, _i64, _u64]
     L.phx_size_class.argtypes = [_sz]
     L.phx_size_class.restype = _sz
     L.phx_arena_create.argtypes = [ctypes.POINTER(_vp), _sz]
@@ -399,6 +444,175 @@ def launch_flash_bh(stream, kernel, q, k, v, o, BH, Nq, Nk, D, scale):
                                        _addr(k, e * BH * Nk * D, "K"),
                                        _addr(v, e * BH * Nk * D, "V"),
                                        _addr(o, e * BH * Nq * D, "O"), BH, Nq, Nk, D, scale))
+
+
+# ------------------------------------------------------------------- decode operators
+_ESZ = {F32: 4, F16: 2}
+
+
+def _span(rows, ld, width, esz):
+    """Bytes from the first to past the last of `rows` rows, ld elements apart."""
+    return ((rows - 1) * (ld or width) + width) * esz if rows else 0
+
+
+def w4_packed_bytes(N, K):
+    return lib().phx_w4_packed_bytes(N, K)
+
+
+def w4_pack(stream, codes, packed, N, K):
+    """Codes u8 [K, N] (0 .. 15) into the tiles launch_gemv_w4 reads."""
+    check(lib().phx_w4_pack(_sh(stream), _addr(codes, N * K, "codes"),
+                            _addr(packed, w4_packed_bytes(N, K), "packed"), N, K))
+
+
+def w4_quantize(b, group):
+    """Codes u8 [K, N], scales f16 and zero points u8 [ceil(K/group), N] of
+    weights b [K, N]: each group's range, widened to hold 0, in 15 steps, so
+    that a weight of 0 stays 0.  Host arrays."""
+    b = np.asarray(b, np.float64)
+    K, N = b.shape
+    groups = -(-K // group)
+    padded = np.zeros((groups * group, N))
+    padded[:K] = b
+    padded = padded.reshape(groups, group, N)
+    lo, hi = np.minimum(padded.min(1), 0), np.maximum(padded.max(1), 0)
+    scales = ((hi - lo) / 15).astype(np.float16)
+    scales = np.where(scales > 0, scales, np.float16(2.0 ** -24))
+    s = scales.astype(np.float64)
+    zeros = np.clip(np.rint(-lo / s), 0, 15)
+    codes = np.clip(np.rint(padded / s[:, None]) + zeros[:, None], 0, 15)
+    return (codes.reshape(-1, N)[:K].astype(np.uint8), scales, zeros.astype(np.uint8))
+
+
+def launch_gemv_w4(stream, dtype, a, w, scales, zeros, c, M, N, K, group, alpha=1.0, beta=0.0,
+                   lda=0, ldc=0):
+    """C = alpha*A@W + beta*C, up to 64 rows, 4-bit weights (phx_gemv_w4);
+    zeros 0 for zero points of 8."""
+    e, g = _ESZ.get(dtype, 4), -(-K // group) if group > 0 else 0
+    check(lib().phx_gemv_w4(_sh(stream), dtype, _addr(a, _span(M, lda, K, e), "A"),
+                            _addr(w, w4_packed_bytes(N, K), "W"), _addr(scales, 2 * g * N, "scales"),
+                            _addr(zeros, g * N, "zeros"), _addr(c, _span(M, ldc, N, e), "C"),
+                            M, N, K, group, alpha, beta, lda, ldc))
+
+
+def kv4_page_bytes(heads, head_dim, page_tokens):
+    return lib().phx_kv4_page_bytes(heads, head_dim, page_tokens)
+
+
+def launch_kv4_append(stream, cache, batch, dtype, k, v, ldk=0, ldv=0):
+    """The rows' K and V [rows][heads][head_dim], quantised, into the cache
+    (phx_kv4_append)."""
+    e, w = _ESZ.get(dtype, 4), cache.heads * cache.head_dim
+    check(lib().phx_kv4_append(_sh(stream), cache, batch, dtype,
+                               _addr(k, _span(batch.rows, ldk, w, e), "K"),
+                               _addr(v, _span(batch.rows, ldv, w, e), "V"), ldk, ldv))
+
+
+def launch_kv4_read(stream, cache, batch, dtype, k, v, ldk=0, ldv=0):
+    """The rows' K and V as the cache holds them (phx_kv4_read)."""
+    e, w = _ESZ.get(dtype, 4), cache.heads * cache.head_dim
+    check(lib().phx_kv4_read(_sh(stream), cache, batch, dtype,
+                             _addr(k, _span(batch.rows, ldk, w, e), "K"),
+                             _addr(v, _span(batch.rows, ldv, w, e), "V"), ldk, ldv))
+
+
+def launch_kv4_attention(stream, cache, batch, dtype, q, o, q_heads, scale, causal=True, ldq=0,
+                         ldo=0):
+    """Attention of the rows' queries over their sequences in the cache
+    (phx_kv4_attention)."""
+    e, w = _ESZ.get(dtype, 4), q_heads * cache.head_dim
+    check(lib().phx_kv4_attention(_sh(stream), cache, batch, dtype,
+                                  _addr(q, _span(batch.rows, ldq, w, e), "Q"),
+                                  _addr(o, _span(batch.rows, ldo, w, e), "O"), q_heads, scale,
+                                  1 if causal else 0, ldq, ldo))
+
+
+def kv4_split_plan(cache, batch, q_heads):
+    """(splits, workspace bytes) of such an attention (phx_kv4_split_plan)."""
+    sp, ws = ctypes.c_int(), _sz()
+    check(lib().phx_kv4_split_plan(cache, batch, q_heads, ctypes.byref(sp), ctypes.byref(ws)))
+    return sp.value, ws.value
+
+
+def pages_copy(stream, pool, pages, page_bytes, src, dst, layers=1, layer_stride=0):
+    """Copies page src[i] to page dst[i] in each layer's pool (phx_pages_copy)."""
+    src, dst = (np.ascontiguousarray(x, np.int32) for x in (src, dst))
+    if src.shape != dst.shape or src.ndim != 1:
+        raise PhxError(PHX_E_INVALID, "pages_copy: src and dst are lists of one length")
+    whole = (layers - 1) * layer_stride + pages * page_bytes if layers > 0 else 0
+    check(lib().phx_pages_copy(_sh(stream), _addr(pool, whole, "pool"), pages, page_bytes,
+                               src.ctypes.data, dst.ctypes.data, src.size, layers, layer_stride))
+
+
+class Pages:
+    """Which page of a cache belongs to which sequence (phx_pages_*)."""
+
+    def __init__(self, pages, page_tokens):
+        self.handle = None
+        h = _vp()
+        check(lib().phx_pages_create(ctypes.byref(h), pages, page_tokens))
+        self.handle = h.value
+
+    def new(self):
+        seq = _i64()
+        check(lib().phx_pages_new(self.handle, ctypes.byref(seq)))
+        return seq.value
+
+    def resize(self, seq, tokens):
+        check(lib().phx_pages_resize(self.handle, seq, tokens))
+
+    def fork(self, seq):
+        child = _i64()
+        check(lib().phx_pages_fork(self.handle, seq, ctypes.byref(child)))
+        return child.value
+
+    def free(self, seq):
+        check(lib().phx_pages_free(self.handle, seq))
+
+    def compact(self):
+        check(lib().phx_pages_compact(self.handle))
+
+    def table(self, seq):
+        n = _i64()
+        check(lib().phx_pages_table(self.handle, seq, None, 0, ctypes.byref(n)))
+        out = np.empty(n.value, np.int32)
+        check(lib().phx_pages_table(self.handle, seq,
+                                    out.ctypes.data_as(ctypes.POINTER(ctypes.c_int32)), out.size,
+                                    ctypes.byref(n)))
+        return out
+
+    def stats(self):
+        """(pages in use, one past the highest of them, pending copies)."""
+        v = [_i64() for _ in range(3)]
+        check(lib().phx_pages_stats(self.handle, *(ctypes.byref(x) for x in v)))
+        return tuple(x.value for x in v)
+
+    def pending(self, clear=False):
+        """The pending copies as (src, dst) arrays; with clear the caller runs
+        them and they are no longer pending."""
+        n = self.stats()[2]
+        out = [np.empty(n, np.int32) for _ in range(2)]
+        ptr = [x.ctypes.data_as(ctypes.POINTER(ctypes.c_int32)) for x in out]
+        check(lib().phx_pages_pending(self.handle, *ptr, n, None, 1 if clear else 0))
+        return tuple(out)
+
+    def apply(self, stream, pool, page_bytes, layers=1, layer_stride=0):
+        """Launches the pending copies in the layers' pools and clears them."""
+        check(lib().phx_pages_apply(self.handle, _sh(stream), _addr(pool, 0, "pool"), page_bytes,
+                                    layers, layer_stride))
+
+    def destroy(self):
+        if self.handle:
+            check(lib().phx_pages_destroy(self.handle))
+            self.handle = None
+
+    def __del__(self):
+        try:
+            if self.handle and _LIB is not None:
+                _LIB.phx_pages_destroy(self.handle)
+                self.handle = None
+        except Exception:
+            pass
 
 
 def grid_for(kernel, dims):
