@@ -27,6 +27,8 @@ struct PhxKv4 {
     float scale;
 };
 
+#define PHX_KV4_SPLITS 128  // the most parts of a sequence's keys
+
 // A call's copies of pages, by value: a launch carries its lists itself.
 #define PHX_PAGES_PER_LAUNCH 448
 struct PhxPagesCopy {

@@ -15,6 +15,7 @@ namespace {
 
 const char *const kW4File = "gemv_w4.hsaco";
 const char *const kKv4File = "kv4.hsaco";
+const char *const kAttendFile = "kv4_attend.hsaco";
 const char *const kPagesFile = "pages.hsaco";
 
 int launch(const char *file, const char *entry, dim3 grid, uint32_t threads, hipStream_t s,
@@ -209,6 +210,33 @@ int phx_kv4_read(phx_stream s, const phx_kv4_cache *cache, const phx_kv4_batch *
     return move_rows(s, cache, batch, t, k, v, ldk, ldv, "kv4_read", names);
 }
 
+// How an attention runs: tiles of 16 columns per wave (column_tiles), and the
+// split of the keys that brings the launch to kAttendGroups workgroups, of
+// parts of at least kAttendPart keys each (of the longest sequence there can
+// be) and at most PHX_KV4_SPLITS of them.
+static const int64_t kAttendGroups = 512, kAttendPart = 512;
+
+static int column_tiles(phx_dtype t, int64_t columns) {
+    return columns <= 16 ? 1 : columns <= 32 || t == PHX_F32 ? 2 : 4;
+}
+
+static int64_t attend_groups(const phx_kv4_cache *c, const phx_kv4_batch *b, int64_t ratio,
+                             int tiles) {
+    return b->batch * c->heads * ((b->max_q * ratio + 16 * tiles - 1) / (16 * tiles));
+}
+
+static size_t split_bytes(const phx_kv4_cache *c, const phx_kv4_batch *b, int64_t q_heads) {
+    return (size_t)b->rows * (size_t)q_heads * (size_t)(c->head_dim + 2) * sizeof(float);
+}
+
+static int64_t attend_splits(const phx_kv4_cache *c, const phx_kv4_batch *b, int64_t q_heads) {
+    const int64_t ratio = q_heads / c->heads;
+    const int64_t groups = attend_groups(c, b, ratio, column_tiles(PHX_F16, b->max_q * ratio));
+    const int64_t keys = std::min(b->max_len, b->table_stride * c->page_tokens);
+    if (!has_work(b) || groups * 2 > kAttendGroups) return 1;
+    return std::max<int64_t>(1, std::min({kAttendGroups / groups, keys / kAttendPart, (int64_t)PHX_KV4_SPLITS}));
+}
+
 static int check_heads(const phx_kv4_cache *c, int64_t q_heads, const char *who) {
     if (q_heads < 1 || q_heads % c->heads || q_heads > 65535)
         return set_error(PHX_E_INVALID, "%s: %lld query heads over %d KV heads", who,
@@ -221,16 +249,23 @@ int phx_kv4_split_plan(const phx_kv4_cache *cache, const phx_kv4_batch *batch, i
     if (int rc = check_cache(cache, "kv4_split_plan")) return rc;
     if (int rc = check_batch(batch, "kv4_split_plan")) return rc;
     if (int rc = check_heads(cache, q_heads, "kv4_split_plan")) return rc;
-    if (splits) *splits = 1;
-    if (workspace_bytes) *workspace_bytes = 0;
+    const int64_t sp = attend_splits(cache, batch, q_heads);
+    if (splits) *splits = (int)sp;
+    if (workspace_bytes) *workspace_bytes = sp > 1 ? (size_t)sp * split_bytes(cache, batch, q_heads) : 0;
     return PHX_OK;
 }
 
 int phx_kv4_attention(phx_stream s, const phx_kv4_cache *cache, const phx_kv4_batch *batch,
                       phx_dtype t, uint64_t q, uint64_t o, int64_t q_heads, float scale,
                       int causal, int64_t ldq, int64_t ldo) {
-    static const char *const names[4] = {"kv4_attend_f16_d64", "kv4_attend_f16_d128",
-                                         "kv4_attend_f32_d64", "kv4_attend_f32_d128"};
+    static const char *const names[3][4] = {
+        {"kv4_attend_f16_d64_c1", "kv4_attend_f16_d128_c1", "kv4_attend_f32_d64_c1",
+         "kv4_attend_f32_d128_c1"},
+        {"kv4_attend_f16_d64_c2", "kv4_attend_f16_d128_c2", "kv4_attend_f32_d64_c2",
+         "kv4_attend_f32_d128_c2"},
+        {"kv4_attend_f16_d64_c4", "kv4_attend_f16_d128_c4", nullptr, nullptr}};
+    static const char *const combine[4] = {"kv4_combine_f16_d64", "kv4_combine_f16_d128",
+                                           "kv4_combine_f32_d64", "kv4_combine_f32_d128"};
     const char *who = "kv4_attention";
     if (!known(t)) return set_error(PHX_E_INVALID, "%s: unknown type %d", who, (int)t);
     if (int rc = check_cache(cache, who)) return rc;
@@ -251,9 +286,23 @@ int phx_kv4_attention(phx_stream s, const phx_kv4_cache *cache, const phx_kv4_ba
     p.ratio = (int32_t)(q_heads / cache->heads);
     p.causal = causal != 0;
     p.scale = scale;
-    return launch(kKv4File, entry_of(names, t, cache->head_dim),
-                  dim3((uint32_t)batch->max_q, (uint32_t)q_heads, (uint32_t)batch->batch), 64,
-                  (hipStream_t)s, &p);
+    const int tiles = column_tiles(t, batch->max_q * p.ratio);
+    const int64_t groups = attend_groups(cache, batch, p.ratio, tiles);
+    const int64_t units = batch->batch * batch->max_q * q_heads;
+    size_t room = 0;
+    if (int rc = phx_stream_get_workspace(s, &p.ws, &room)) return rc;
+    const size_t part = split_bytes(cache, batch, q_heads);
+    p.splits = (int32_t)std::max<int64_t>(
+        1, std::min<int64_t>(attend_splits(cache, batch, q_heads), (int64_t)(room / part)));
+    if (groups * p.splits > INT32_MAX || units > INT32_MAX)
+        return set_error(PHX_E_INVALID, "%s: %lld sequences of up to %lld rows are too many", who,
+                         (long long)batch->batch, (long long)batch->max_q);
+    if (int rc = launch(kAttendFile, entry_of(names[tiles / 2], t, cache->head_dim),
+                        dim3((uint32_t)(groups * p.splits)), 256, (hipStream_t)s, &p))
+        return rc;
+    if (p.splits == 1) return PHX_OK;
+    return launch(kAttendFile, entry_of(combine, t, cache->head_dim),
+                  dim3((uint32_t)units), 256, (hipStream_t)s, &p);
 }
 
 // ------------------------------------------------------------------ pages

@@ -46,7 +46,8 @@ KERNEL_NAMES = {
 
 CODE_OBJECTS = ["saxpy_fp32.hsaco", "gemm_fp32.hsaco", "gemm_fp16tc_fp32acc.hsaco",
                 "gemm_fp16.hsaco", "flash_attention_fp32.hsaco", "flash_attention_fp16.hsaco",
-                "matmul_cluster_fp32.hsaco", "gemv_w4.hsaco", "kv4.hsaco", "pages.hsaco"]
+                "matmul_cluster_fp32.hsaco", "gemv_w4.hsaco", "kv4.hsaco",
+                "kv4_attend.hsaco", "pages.hsaco"]
 
 # phx_dtype of the decode operators
 F32 = 0
