@@ -4,6 +4,10 @@
 #include "phx_common.h"
 #include "phx_decode.h"
 
+// Addresses arrive as integers: without their address space they would be
+// accessed with flat instructions, which also take the LDS path.
+#define PHX_GLOBAL __attribute__((address_space(1)))
+
 namespace {
 
 // A sequence of the call: its tokens, and its rows' first index and count.
@@ -15,12 +19,12 @@ __device__ __forceinline__ Seq kv4_seq(const PhxKv4 &p, int64_t b) {
     Seq s;
     int64_t most = p.table_stride * p.page_tokens;
     if (p.max_len < most) most = p.max_len;
-    s.tokens = ((const int32_t *)p.lens)[b];
+    s.tokens = ((const PHX_GLOBAL int32_t *)p.lens)[b];
     s.tokens = s.tokens < 0 ? 0 : s.tokens > most ? most : s.tokens;
     s.row0 = b * p.max_q;
     s.count = p.max_q;
     if (p.q_starts) {
-        const int32_t *q = (const int32_t *)p.q_starts + b;
+        const PHX_GLOBAL int32_t *q = (const PHX_GLOBAL int32_t *)p.q_starts + b;
         s.row0 = q[0];
         const int64_t n = (int64_t)q[1] - q[0];
         s.count = n < 0 ? 0 : n > p.max_q ? p.max_q : n;
@@ -30,14 +34,14 @@ __device__ __forceinline__ Seq kv4_seq(const PhxKv4 &p, int64_t b) {
 
 // The page of a sequence's token, or -1.
 __device__ __forceinline__ int64_t kv4_page(const PhxKv4 &p, int64_t b, int64_t token) {
-    const int64_t page = ((const int32_t *)p.table)[b * p.table_stride + token / p.page_tokens];
+    const int64_t page = ((const PHX_GLOBAL int32_t *)p.table)[b * p.table_stride + token / p.page_tokens];
     return page >= 0 && page < p.pages ? page : -1;
 }
 
 // A page's bytes of one head.
 template <int D>
-__device__ __forceinline__ char *kv4_head(const PhxKv4 &p, int64_t page, int head) {
-    return (char *)p.pool + (page * p.heads + head) * ((int64_t)p.page_tokens * (D + 8));
+__device__ __forceinline__ PHX_GLOBAL char *kv4_head(const PhxKv4 &p, int64_t page, int head) {
+    return (PHX_GLOBAL char *)p.pool + (page * p.heads + head) * ((int64_t)p.page_tokens * (D + 8));
 }
 
 // Byte offset of the dword with elements 8e .. 8e+7 of a token, in a head's

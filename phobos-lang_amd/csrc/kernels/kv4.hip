@@ -32,7 +32,7 @@ __device__ __forceinline__ Unit kv4_unit(const PhxKv4 &p, int64_t u) {
 }
 
 template <typename T>
-__device__ __forceinline__ void load8(const T *src, float *x) {
+__device__ __forceinline__ void load8(const PHX_GLOBAL T *src, float *x) {
     for (int i = 0; i < 8; ++i) x[i] = (float)src[i];
 }
 
@@ -44,7 +44,8 @@ __device__ __forceinline__ void append(const PhxKv4 &p) {
     if (!u.live || u.token < 0) return;
     const int64_t page = kv4_page(p, u.b, u.token);
     if (page < 0) return;
-    const T *src = u.v ? (const T *)p.y + u.row * p.ldy : (const T *)p.x + u.row * p.ldx;
+    const PHX_GLOBAL T *src = u.v ? (const PHX_GLOBAL T *)p.y + u.row * p.ldy
+                                  : (const PHX_GLOBAL T *)p.x + u.row * p.ldx;
     float x[8];
     load8(src + u.head * D + e * 8, x);
     float lo = x[0], hi = x[0];
@@ -62,14 +63,14 @@ __device__ __forceinline__ void append(const PhxKv4 &p) {
         const double c = rint(((double)x[i] - (double)(float)m) / (double)(float)sc);
         word |= (c > 0.0 ? c < 15.0 ? (uint32_t)c : 15u : 0u) << (4 * i);
     }
-    char *head = kv4_head<D>(p, page, u.head);
+    PHX_GLOBAL char *head = kv4_head<D>(p, page, u.head);
     const uint32_t slot = (uint32_t)(u.token % p.page_tokens);
-    *(uint32_t *)(head + kv4_word<D>(p.page_tokens, u.v, slot, e)) = word;
+    *(PHX_GLOBAL uint32_t *)(head + kv4_word<D>(p.page_tokens, u.v, slot, e)) = word;
     if (e == 0) {
         phx_h2 pair;
         pair.x = sc;
         pair.y = m;
-        *(phx_h2 *)(head + kv4_param<D>(p.page_tokens, u.v, slot)) = pair;
+        *(PHX_GLOBAL phx_h2 *)(head + kv4_param<D>(p.page_tokens, u.v, slot)) = pair;
     }
 }
 
@@ -79,14 +80,15 @@ __device__ __forceinline__ void read(const PhxKv4 &p) {
     const int e = threadIdx.x % L;
     const Unit u = kv4_unit<D>(p, (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L);
     if (!u.live) return;
-    T *dst = (u.v ? (T *)p.y + u.row * p.ldy : (T *)p.x + u.row * p.ldx) + u.head * D + e * 8;
+    PHX_GLOBAL T *dst = (u.v ? (PHX_GLOBAL T *)p.y + u.row * p.ldy
+                             : (PHX_GLOBAL T *)p.x + u.row * p.ldx) + u.head * D + e * 8;
     const int64_t page = u.token < 0 ? -1 : kv4_page(p, u.b, u.token);
     float x[8] = {};
     if (page >= 0) {
-        const char *head = kv4_head<D>(p, page, u.head);
+        const PHX_GLOBAL char *head = kv4_head<D>(p, page, u.head);
         const uint32_t slot = (uint32_t)(u.token % p.page_tokens);
-        const uint32_t word = *(const uint32_t *)(head + kv4_word<D>(p.page_tokens, u.v, slot, e));
-        const phx_h2 pair = *(const phx_h2 *)(head + kv4_param<D>(p.page_tokens, u.v, slot));
+        const uint32_t word = *(const PHX_GLOBAL uint32_t *)(head + kv4_word<D>(p.page_tokens, u.v, slot, e));
+        const phx_h2 pair = *(const PHX_GLOBAL phx_h2 *)(head + kv4_param<D>(p.page_tokens, u.v, slot));
         for (int i = 0; i < 8; ++i)
             x[i] = (float)((word >> (4 * i)) & 15) * (float)pair.x + (float)pair.y;
     }

@@ -17,10 +17,13 @@
 // the second's operand as they stand, and V is stored so that one 16-byte load
 // brings the same lane's keys (four tokens' dwords).
 //
-// A code enters as the f16 with its bits: 0x000c is c 2^-24, 0x00c0 is c 2^-20,
-// both exact (the matrix instructions keep f16 subnormals).  So unpacking is a
-// mask (and for half of them a shift or a byte permute) per pair of codes, and
-// no subtraction; the powers of two go into the queries and the last scaling.
+// A code enters exactly, as an f16 whose mantissa its bits are put into: K's as
+// 16 + c (a shift and a mask per pair of codes), the product starting from
+// -24 sum_d q_d; V's as 64 + c or 1024 + c less as much and 8 (its sums run over
+// all keys: with sizes of 0 .. 15 they would be many times what they leave
+// after the minima's term).  Codes as subnormals, 0x000c, would need neither,
+// but the matrix instructions keep only about 20 bits of a sum of those
+// (measured: errors of 2^-20 of the largest product, 2^-25 with these).
 //
 // The waves of a workgroup take the key blocks of its share in turns and merge
 // at the end in LDS; with too few workgroups for the GPU the keys are split
@@ -33,16 +36,19 @@
 
 namespace {
 
-constexpr uint32_t kLow = 0x000f000f, kHigh = 0x00f000f0, kBias = 0x64006400;
+// Constants kept in registers: with both of its constants as literals, a mask
+// and the bits set behind it are two instructions instead of one.
+__device__ __forceinline__ uint32_t in_sgpr(uint32_t x) {
+    asm("" : "+s"(x));
+    return x;
+}
+__device__ __forceinline__ uint32_t in_vgpr(uint32_t x) {
+    asm("" : "+v"(x));
+    return x;
+}
 
 __device__ __forceinline__ phx_h8 h8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     return __builtin_bit_cast(phx_h8, (phx_u4){a, b, c, d});
-}
-// Halves of 1024 + x, less `off`: exact, as every whole number up to 2048 is.
-__device__ __forceinline__ phx_h8 centred(uint32_t a, uint32_t b, uint32_t c, uint32_t d,
-                                          int off) {
-    const phx_h8 v = h8(a | kBias, b | kBias, c | kBias, d | kBias);
-    return v - (_Float16)off;
 }
 __device__ __forceinline__ phx_f4 mfma(phx_h8 a, phx_h8 b, phx_f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -51,61 +57,93 @@ __device__ __forceinline__ _Float16 half_of(uint32_t w, int i) {
     const phx_h2 h = __builtin_bit_cast(phx_h2, w);
     return i ? h.y : h.x;
 }
+// What code 8 stands for.
+__device__ __forceinline__ float middle(uint32_t w) {
+    return fmaf(8.0f, (float)half_of(w, 0), (float)half_of(w, 1));
+}
+// (scale, minimum) with a scale that is not positive, as of a page never
+// written, made the smallest: it stands for the same where codes are 0.
+__device__ __forceinline__ uint32_t positive(uint32_t w) {
+    const phx_h2 least = {(_Float16)0x1p-24f, (_Float16)-INFINITY};
+    return __builtin_bit_cast(
+        uint32_t, __builtin_elementwise_max(__builtin_bit_cast(phx_h2, w), least));
+}
 
-// 32 keys as loaded: codes, and (scale, minimum) of the lane's keys
-// 16 t + 4 quad + i.
-template <int D>
-struct Raw {
-    uint32_t k[2][D / 32];
-    phx_u4 v[2], kp[2], vp[2];
+// How a wave's 16 columns are used.  G 1: 16 columns over 32 keys, two products
+// of 16 keys.  With at most 16/G columns in the call, G copies of them: copy g
+// takes the g-th 16 keys alone.  All copies' scores come out of one chain of
+// products, in which the queries of the other copies are zeros, so the softmax
+// has 4 scores per lane and none of a column that does not exist, where G 1
+// would have 8 per 32 keys.
+template <int G>
+struct Shape {
+    static constexpr int TILES = G == 4 ? 4 : 2;   // of 16 keys, in a step
+    static constexpr int UNITS = TILES / 2;        // of 32 keys: what a page holds whole
+    static constexpr int SETS = TILES / G;         // of 4 scores per lane
+    static constexpr int COLS = 16 / G;
 };
 
-template <int D>
-__device__ __forceinline__ void load_block(Raw<D> &r, const char *head, uint32_t P, uint32_t slot,
-                                           uint32_t lane) {
+// A step's keys as loaded: codes, and (scale, minimum) of the lane's own keys
+// 16 t + 4 quad + i, t being its copy's tile (G 1: both).
+template <int D, int G>
+struct Raw {
+    uint32_t k[Shape<G>::TILES][D / 32];
+    phx_u4 v[Shape<G>::TILES], kp[Shape<G>::SETS], vp[Shape<G>::SETS];
+};
+
+template <typename T>
+__device__ __forceinline__ T fetch(const PHX_GLOBAL char *base, uint32_t off) {
+    return *(const PHX_GLOBAL T *)(base + off);
+}
+
+// The tiles of one unit; its place in the step is u.
+template <int D, int G>
+__device__ __forceinline__ void load_unit(Raw<D, G> &r, int u, const PHX_GLOBAL char *head,
+                                          uint32_t P, uint32_t slot, uint32_t lane) {
     const uint32_t c = lane & 15, quad = lane >> 4;
-    const char *k = head + slot * (D / 2), *v = k + P * (D / 2);
-    const char *kp = head + P * D + slot * 4, *vp = kp + P * 4;
+    const PHX_GLOBAL char *k = head + slot * (D / 2), *v = k + P * (D / 2);
     const uint32_t ko = c * (D / 2) + quad * (D / 8);
     const uint32_t vo = (quad * (D / 8) + (c & (D / 8 - 1))) * 16;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
+        uint32_t *to = r.k[2 * u + t];
         if constexpr (D == 128) {
-            const phx_u4 w = *(const phx_u4 *)(k + ko + t * 8 * D);
-            r.k[t][0] = w.x, r.k[t][1] = w.y, r.k[t][2] = w.z, r.k[t][3] = w.w;
+            const phx_u4 w = fetch<phx_u4>(k, ko + t * 8 * D);
+            to[0] = w.x, to[1] = w.y, to[2] = w.z, to[3] = w.w;
         } else {
-            const phx_u2 w = *(const phx_u2 *)(k + ko + t * 8 * D);
-            r.k[t][0] = w.x, r.k[t][1] = w.y;
+            const phx_u2 w = fetch<phx_u2>(k, ko + t * 8 * D);
+            to[0] = w.x, to[1] = w.y;
         }
-        r.v[t] = *(const phx_u4 *)(v + vo + t * 8 * D);
-        r.kp[t] = *(const phx_u4 *)(kp + quad * 16 + t * 64);
-        r.vp[t] = *(const phx_u4 *)(vp + quad * 16 + t * 64);
+        r.v[2 * u + t] = fetch<phx_u4>(v, vo + t * 8 * D);
     }
 }
 
 // The columns' queries as matrix operands, and what turns a product into a
-// score in log2 units: t = s_j x S x a + m_j x b.
+// score in log2 units: t = s_j S a + (m_j + 8 s_j) b, S being the product with
+// c_j - 8, as it starts at c: with a code's own size 0 .. 15 the
+// two terms are larger than their sum and lose its last bits.
 template <int D, int TERMS>
 struct Query {
     phx_h8 q[TERMS][D / 32];
-    float a, b;
+    float a, b, c;
     int32_t limit;  // keys the column sees
 };
 
 template <typename T, int D, int TERMS>
 __device__ __forceinline__ void load_query(Query<D, TERMS> &r, const PhxKv4 &p, const Seq &s,
-                                           int head, int64_t col, uint32_t quad) {
+                                           int head, uint32_t col, uint32_t quad) {
     constexpr int N = D / 4;  // elements of a lane: D/4 of a row, from quad D/4 on
-    const int64_t i = col / p.ratio, row = s.row0 + i;
+    const uint32_t ratio = p.ratio, i = col / ratio;
+    const int64_t row = s.row0 + i;
     const bool live = i < s.count && row >= 0 && row < p.rows;
     r.limit = (int32_t)(!live ? 0 : p.causal ? s.tokens - s.count + i + 1 : s.tokens);
     float x[N];
-    const T *src = (const T *)p.x + row * p.ldx +
-                   ((int64_t)head * p.ratio + col % p.ratio) * D + quad * N;
+    const PHX_GLOBAL T *src = (const PHX_GLOBAL T *)p.x + row * p.ldx +
+                              ((int64_t)head * ratio + col % ratio) * D + quad * N;
 #pragma unroll
     for (int u = 0; u < N; u += 16 / sizeof(T)) {
         phx_u4 w = {0, 0, 0, 0};
-        if (live) w = *(const phx_u4 *)(src + u);
+        if (live) w = *(const PHX_GLOBAL phx_u4 *)(src + u);
 #pragma unroll
         for (int i = 0; i < (int)(16 / sizeof(T)); ++i)
             x[u + i] = sizeof(T) == 4 ? __builtin_bit_cast(float, (uint32_t)w[i & 3])
@@ -125,16 +163,14 @@ __device__ __forceinline__ void load_query(Query<D, TERMS> &r, const PhxKv4 &p, 
     for (int j = 0; j < D / 32; ++j)
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-            // element of the pair of dwords: nibbles 0 4 2 6 (the even operand,
-            // 16 below the odd one, 1 5 3 7)
-            constexpr int order[4] = {0, 4, 2, 6};
-            const int d = (j / 2) * 16 + (u / 4) * 8 + order[u % 4] + (j & 1);
-            const float v = ldexpf(x[d], 9 - e + (j & 1 ? 0 : 4));
+            // a dword's pairs of nibbles: 0 4, 1 5, 2 6, 3 7
+            const float v = ldexpf(x[j * 8 + u / 2 + u % 2 * 4], 9 - e);
             const _Float16 hi = (_Float16)v;
             r.q[0][j][u] = hi;
             if constexpr (TERMS == 2) r.q[1][j][u] = (_Float16)(v - (float)hi);
         }
-    r.a = ldexpf(p.scale * KV4_LOG2E, 11 + e);
+    r.a = ldexpf(p.scale * KV4_LOG2E, e - 9);
+    r.c = -24.0f * ldexpf(sum, 9 - e);
     // a row with an infinity has no scores, as its weights would be inf / inf
     r.b = top < INFINITY ? sum * (p.scale * KV4_LOG2E) : NAN;
 }
@@ -146,93 +182,125 @@ struct State {
     float m, l, pm;
 };
 
-template <int D, int TERMS, int NC, bool MASK>
-__device__ __forceinline__ void attend_block(const Raw<D> &r, const Query<D, TERMS> (&q)[NC],
-                                             State<D> (&st)[NC], uint32_t key0, uint32_t lane) {
-    const uint32_t quad = lane >> 4;
-    phx_h8 k[2][D / 32], v[D / 16];
+template <bool B>
+struct Flag {
+    static constexpr bool value = B;
+};
+
+// What a lane knows of its copy.
+template <int D, int G>
+struct Lane {
+    uint32_t lane, quad, tile;                   // G 1: tile 0 of each set
+    uint32_t keep[G == 1 ? 1 : Shape<G>::TILES]; // all ones for its own tile, else 0
+    const phx_h8 *q[G == 1 ? 1 : Shape<G>::TILES]; // queries in LDS, or zeros
+};
+
+// A step of keys for NC tiles of columns.  masked: some keys are past what a
+// column sees, or in a unit without a page (a bit of `absent`).
+template <int D, int TERMS, int NC, int G>
+__device__ __forceinline__ void attend_step(const Raw<D, G> &r, const Query<D, TERMS> (&q)[NC],
+                                            State<D> (&st)[NC], const Lane<D, G> &ln, uint32_t key0,
+                                            bool masked, uint32_t absent) {
+    using Sh = Shape<G>;
+    constexpr int W = 4 * Sh::SETS;  // scores per lane
+    const uint32_t kmask = in_sgpr(0x03c003c0), kone = in_vgpr(0x4c004c00);
+    const uint32_t vmask[2] = {in_sgpr(0x000f000f), in_sgpr(0x00f000f0)};
+    const uint32_t vone[2] = {in_vgpr(0x64006400), in_vgpr(0x54005400)};
+    phx_f4 s[NC][Sh::SETS];
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int c = 0; c < NC; ++c)
 #pragma unroll
-        for (int u = 0; u < D / 64; ++u) {
-            const uint32_t a = r.k[t][2 * u], b = r.k[t][2 * u + 1];
-            k[t][2 * u] = h8(a & kLow, (a >> 8) & kLow, b & kLow, (b >> 8) & kLow);
-            k[t][2 * u + 1] = h8(a & kHigh, (a >> 8) & kHigh, b & kHigh, (b >> 8) & kHigh);
+        for (int a = 0; a < Sh::SETS; ++a) s[c][a] = (phx_f4){q[c].c, q[c].c, q[c].c, q[c].c};
+#pragma unroll
+    for (int t = 0; t < Sh::TILES; ++t)
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) {
+            // 16 and the code behind it
+            const uint32_t w = r.k[t][j];
+            const phx_h8 k = h8((w << 6 & kmask) | kone, (w << 2 & kmask) | kone,
+                                (w >> 2 & kmask) | kone, (w >> 6 & kmask) | kone);
+#pragma unroll
+            for (int x = 0; x < TERMS; ++x)
+                if constexpr (G == 1) {
+#pragma unroll
+                    for (int c = 0; c < NC; ++c) s[c][t] = mfma(k, q[c].q[x][j], s[c][t]);
+                } else {
+                    s[0][0] = mfma(k, ln.q[t][(x * (D / 32) + j) * 64], s[0][0]);
+                }
         }
-    // an octet of elements per row of the operand; at D 64 the upper eight rows
-    // are the same octets' other half
-    const uint32_t first = D == 64 && (lane & 8) ? 0x0c060c02 : 0x0c040c00;
+    uint32_t vp[W];
+    float km[W], vm[W];
 #pragma unroll
-    for (int b = 0; b < D / 32; ++b) {
-        const uint32_t sel = first + b * 0x00010001;
-        uint32_t x[4];
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            x[2 * t] = __builtin_amdgcn_perm(r.v[t].y, r.v[t].x, sel);
-            x[2 * t + 1] = __builtin_amdgcn_perm(r.v[t].w, r.v[t].z, sel);
-        }
-        v[2 * b] = centred(x[0] & kLow, x[1] & kLow, x[2] & kLow, x[3] & kLow, 1032);
-        v[2 * b + 1] = centred(x[0] & kHigh, x[1] & kHigh, x[2] & kHigh, x[3] & kHigh, 1152);
+    for (int u = 0; u < W; ++u) {
+        vp[u] = positive(r.vp[u / 4][u % 4]);
+        km[u] = middle(r.kp[u / 4][u % 4]);
+        vm[u] = middle(vp[u]);
     }
+    uint32_t hi[NC][W / 2], lo[NC][W / 2];  // pairs of halves
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-        const int32_t left = q[c].limit - (int32_t)(key0 + 4 * quad);
-        phx_f4 s[2];
+        const int32_t left = q[c].limit - (int32_t)(key0 + 16 * ln.tile + 4 * ln.quad);
+        auto in = [&](int u) {
+            return 16 * (u / 4) + u % 4 < left && !(absent >> (ln.tile / 2) & 1);
+        };
+        float sum, pm;
+        bool over;
+        // weights against the reference m, in two f16 terms (22 bits): w as f16
+        // and what that leaves of the exact product; `over`: m does not hold
+        auto weigh = [&](auto mask) {
+            constexpr bool MASK = decltype(mask)::value;
+            sum = pm = 0.0f;
+            phx_h2 h, top = {(_Float16)0.0f, (_Float16)0.0f}, l;
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            s[t] = (phx_f4){0, 0, 0, 0};
-#pragma unroll
-            for (int j = 0; j < D / 32; ++j)
-#pragma unroll
-                for (int x = 0; x < TERMS; ++x) s[t] = mfma(k[t][j], q[c].q[x][j], s[t]);
-        }
-        float w[8], low[8], sum = 0.0f, pm = 0.0f, top = 0.0f;
-        // weights against the reference m; their largest tells whether it holds
-        auto weigh = [&]() {
-            sum = pm = top = 0.0f;
-#pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const int t = u / 4, i = u % 4;
-                const float x = (float)half_of(r.kp[t][i], 0) * s[t][i];
-                const float y = fmaf((float)half_of(r.kp[t][i], 1), q[c].b, -st[c].m);
-                float e = fmaf(x, q[c].a, y);
-                float sv = fmaxf((float)half_of(r.vp[t][i], 0), 0x1p-24f);
-                float mv = fmaf(8.0f, sv, (float)half_of(r.vp[t][i], 1));
+            for (int u = 0; u < W; ++u) {
+                const float y = fmaf(km[u], q[c].b, -st[c].m);
+                float e = fmaf((float)half_of(r.kp[u / 4][u % 4], 0), s[c][u / 4][u % 4] * q[c].a, y);
+                _Float16 sv = half_of(vp[u], 0);
+                float mv = vm[u];
                 if (MASK) {
-                    const bool in = 16 * t + i < left;
-                    e = in ? e : -INFINITY;
-                    sv = in ? sv : 0.0f;
-                    mv = in ? mv : 0.0f;
+                    e = in(u) ? e : -INFINITY;
+                    sv = in(u) ? sv : (_Float16)0.0f;
+                    mv = in(u) ? mv : 0.0f;
                 }
                 const float pr = __builtin_amdgcn_exp2f(e);
-                w[u] = pr * sv;
                 sum += pr;
                 pm = fmaf(pr, mv, pm);
-                top = fmaxf(top, w[u] == w[u] ? w[u] : INFINITY);
+                h[u % 2] = (_Float16)fmaf(pr, (float)sv, 0.0f);
+                l[u % 2] = (_Float16)fmaf(pr, (float)sv, -(float)h[u % 2]);
+                if (u % 2) {
+                    top = __builtin_elementwise_max(top, h);
+                    hi[c][u / 2] = __builtin_bit_cast(uint32_t, h);
+                    lo[c][u / 2] = __builtin_bit_cast(uint32_t, l);
+                }
             }
+            over = fmaxf((float)top.x, (float)top.y) > 32768.0f;
         };
-        weigh();
+        if (masked)
+            weigh(Flag<true>());
+        else
+            weigh(Flag<false>());
         // The reference m is of score + log2 s_V, and stays while no weight
-        // passes 2^15: rarely raised after the first block, and then to 2^7
-        // below the block's largest.  (p itself is at most w 2^24 in f32.)
-        if (__any(!(top <= 32768.0f))) {
+        // passes 2^15: rarely raised after the first step, and then to 2^7
+        // below the step's largest.  (p itself is at most w 2^24 in f32.  A row
+        // with a NaN is NaN whatever its reference.)
+        if (__any(over)) {
             float most = -INFINITY;
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const int t = u / 4, i = u % 4;
-                const float x = (float)half_of(r.kp[t][i], 0) * s[t][i];
-                const float e = fmaf(x, q[c].a, (float)half_of(r.kp[t][i], 1) * q[c].b);
-                const float sv = fmaxf((float)half_of(r.vp[t][i], 0), 0x1p-24f);
-                const bool in = !MASK || 16 * t + i < left;
-                most = fmaxf(most, in ? e + __builtin_amdgcn_logf(sv) : -INFINITY);
+            for (int u = 0; u < W; ++u) {
+                const float e = fmaf((float)half_of(r.kp[u / 4][u % 4], 0),
+                                     s[c][u / 4][u % 4] * q[c].a, km[u] * q[c].b);
+                most = fmaxf(most, !masked || in(u)
+                                       ? e + __builtin_amdgcn_logf((float)half_of(vp[u], 0))
+                                       : -INFINITY);
             }
             most = fmaxf(most, __shfl_xor(most, 16));
             most = fmaxf(most, __shfl_xor(most, 32));
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
             // by the column's own weights alone: no row's result depends on
             // the rows next to it
-            if (top > 32768.0f && most - 7.0f > st[c].m) {
+            uint32_t any = over;
+            any |= __shfl_xor(any, 16);
+            any |= __shfl_xor(any, 32);
+            if (any && most - 7.0f > st[c].m) {
                 const float f = __builtin_amdgcn_exp2f(st[c].m - (most - 7.0f));
                 st[c].m = most - 7.0f;
                 st[c].l *= f;
@@ -240,54 +308,90 @@ __device__ __forceinline__ void attend_block(const Raw<D> &r, const Query<D, TER
 #pragma unroll
                 for (int j = 0; j < D / 16; ++j) st[c].o[j] = st[c].o[j] * f;
             }
-            weigh();
+            if (masked)
+                weigh(Flag<true>());
+            else
+                weigh(Flag<false>());
         }
         st[c].l += sum;
         st[c].pm += pm;
-        // weights in two f16 terms: 22 bits
-        phx_h8 hi, lo;
+    }
+    // an octet of elements per row of the operand; at D 64 the upper eight rows
+    // are the same octets' other half
+    const uint32_t first = D == 64 && (ln.lane & 8) ? 0x0c060c02 : 0x0c040c00;
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            hi[u] = (_Float16)w[u];
-            lo[u] = (_Float16)(w[u] - (float)hi[u]);
-        }
+    for (int n = 0; n < Sh::UNITS; ++n) {
+        // the unit's weights: a copy's are zeros but for its own tile
+        phx_h8 wh[NC], wl[NC];
 #pragma unroll
-        for (int j = 0; j < D / 16; ++j) {
-            st[c].o[j] = mfma(v[j], hi, st[c].o[j]);
-            st[c].o[j] = mfma(v[j], lo, st[c].o[j]);
+        for (int c = 0; c < NC; ++c)
+            if constexpr (G == 1) {
+                wh[c] = h8(hi[c][0], hi[c][1], hi[c][2], hi[c][3]);
+                wl[c] = h8(lo[c][0], lo[c][1], lo[c][2], lo[c][3]);
+            } else {
+                const uint32_t k0 = ln.keep[2 * n], k1 = ln.keep[2 * n + 1];
+                wh[c] = h8(hi[c][0] & k0, hi[c][1] & k0, hi[c][0] & k1, hi[c][1] & k1);
+                wl[c] = h8(lo[c][0] & k0, lo[c][1] & k0, lo[c][0] & k1, lo[c][1] & k1);
+            }
+#pragma unroll
+        for (int b = 0; b < D / 32; ++b) {
+            const uint32_t sel = first + b * 0x00010001;
+            uint32_t x[4];  // a byte of the lane's eight keys, in halves
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const phx_u4 v = r.v[2 * n + t];
+                x[2 * t] = __builtin_amdgcn_perm(v.y, v.x, sel);
+                x[2 * t + 1] = __builtin_amdgcn_perm(v.w, v.z, sel);
+            }
+#pragma unroll
+            for (int odd = 0; odd < 2; ++odd) {
+                const uint32_t mask = vmask[odd], one = vone[odd];
+                const phx_h8 v = h8((x[0] & mask) | one, (x[1] & mask) | one, (x[2] & mask) | one,
+                                    (x[3] & mask) | one) - (_Float16)(odd ? 72 : 1032);
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    st[c].o[2 * b + odd] = mfma(v, wh[c], st[c].o[2 * b + odd]);
+                    st[c].o[2 * b + odd] = mfma(v, wl[c], st[c].o[2 * b + odd]);
+                }
+            }
         }
     }
 }
 
-// N outputs from their sums, zeros without a key.
-template <typename T, int N>
-__device__ __forceinline__ void store(T *dst, const float (&o)[N], float sum) {
-    T out[N];
+// Four outputs from their sums, zeros without a key.
+template <typename T>
+__device__ __forceinline__ void store(PHX_GLOBAL T *dst, phx_f4 o, float sum) {
+    typedef T four __attribute__((ext_vector_type(4)));
+    four out;
 #pragma unroll
-    for (int u = 0; u < N; ++u) out[u] = (T)(sum == 0.0f ? 0.0f : o[u] / sum);
-    __builtin_memcpy(__builtin_assume_aligned(dst, N * sizeof(T) < 16 ? N * sizeof(T) : 16), out,
-                     sizeof out);
+    for (int i = 0; i < 4; ++i) out[i] = (T)(sum == 0.0f ? 0.0f : o[i] / sum);
+    *(PHX_GLOBAL four *)dst = out;
 }
 
-template <typename T, int D, int NC>
+template <typename T, int D, int NC, int G>
 __device__ __forceinline__ void attend(const PhxKv4 &p) {
-    constexpr int TERMS = sizeof(T) == 4 ? 2 : 1, PITCH = D + 4;
+    using Sh = Shape<G>;
+    constexpr int TERMS = sizeof(T) == 4 ? 2 : 1, PITCH = D + 4, COLS = NC * Sh::COLS;
     __shared__ float merged[KV4_WAVES * 16 * PITCH];
     __shared__ float stats[KV4_WAVES * 16 * 2];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, quad = lane >> 4;
+    __shared__ phx_h8 queries[G == 1 ? 1 : TERMS * (D / 32) * 64 * 2];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    Lane<D, G> ln;
+    ln.lane = lane;
+    ln.quad = lane >> 4;
+    ln.tile = G == 1 ? 0 : (lane & 15) / Sh::COLS;
     // column groups of one KV head next to each other, and so on one XCD
-    int64_t item = phx_xcd_swizzle_any(blockIdx.x, gridDim.x);
-    const int64_t groups = (p.max_q * p.ratio + 16 * NC - 1) / (16 * NC);
-    const int64_t cg = groups - 1 - item % groups;  // the longest rows first
+    uint32_t item = phx_xcd_swizzle_any(blockIdx.x, gridDim.x);
+    const uint32_t groups = p.groups, cg = groups - 1 - item % groups;  // the longest rows first
     item /= groups;
-    const uint32_t split = (uint32_t)(item % p.splits);
+    const uint32_t split = item % p.splits;
     item /= p.splits;
-    const int head = (int)(item % p.heads);
+    const int head = item % p.heads;
     const int64_t b = item / p.heads;
     const Seq s = kv4_seq(p, b);
-    const int64_t col0 = cg * 16 * NC, first = col0 / p.ratio;
+    const uint32_t ratio = p.ratio, col0 = cg * COLS, first = col0 / ratio;
     if (first >= s.count) return;
-    int64_t last = (col0 + 16 * NC - 1) / p.ratio;
+    int64_t last = (col0 + COLS - 1) / ratio;
     if (last >= s.count) last = s.count - 1;
     // keys that some column sees, and that all columns with a row see
     int64_t most = p.causal ? s.tokens - s.count + last + 1 : s.tokens;
@@ -299,46 +403,92 @@ __device__ __forceinline__ void attend(const PhxKv4 &p) {
     State<D> st[NC];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-        load_query<T, D, TERMS>(q[c], p, s, head, col0 + c * 16 + (lane & 15), quad);
+        load_query<T, D, TERMS>(q[c], p, s, head, col0 + c * 16 + (lane & 15) % Sh::COLS, ln.quad);
         st[c].m = KV4_NONE;
         st[c].l = st[c].pm = 0.0f;
 #pragma unroll
         for (int j = 0; j < D / 16; ++j) st[c].o[j] = (phx_f4){0, 0, 0, 0};
     }
-    const uint32_t blocks = (uint32_t)(most + 31) / 32;  // fewer than 2^26
-    const uint32_t per = (blocks + p.splits - 1) / p.splits;
-    const uint32_t end = min((split + 1) * per, blocks);
+    if constexpr (G > 1) {
+        // the queries, and as many zeros behind them
+        constexpr int N = TERMS * (D / 32);
+        if (wave == 0) {
+#pragma unroll
+            for (int x = 0; x < N; ++x) {
+                queries[x * 64 + lane] = q[0].q[x / (D / 32)][x % (D / 32)];
+                queries[(N + x) * 64 + lane] = h8(0, 0, 0, 0);
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < Sh::TILES; ++t) {
+            const bool own = (uint32_t)t == ln.tile;
+            ln.keep[t] = own ? ~0u : 0;
+            ln.q[t] = queries + (own ? 0 : N * 64) + lane;
+        }
+    }
+    constexpr uint32_t KEYS = 16 * Sh::TILES, PER = 64 / Sh::UNITS;  // steps of whose pages the lanes hold
+    const uint32_t steps = (uint32_t)(most + KEYS - 1) / KEYS;
+    const uint32_t per = (steps + p.splits - 1) / p.splits;
+    const uint32_t end = min((split + 1) * per, steps), seen = (uint32_t)least / KEYS;
+    const uint32_t units = (uint32_t)(most + 31) / 32;
     const uint32_t P = p.page_tokens, shift = __builtin_ctz(P / 32);
-    const int32_t *table = (const int32_t *)p.table + b * p.table_stride;
-    // the wave's blocks are begin + KV4_WAVES i; the lanes hold the pages of 64
+    const PHX_GLOBAL int32_t *table =
+        (const PHX_GLOBAL int32_t *)p.table + b * p.table_stride;
+    // the wave's steps are begin + KV4_WAVES i; the lanes hold the pages of PER
     // of them
     const uint32_t begin = split * per + __builtin_amdgcn_readfirstlane(wave);
-    for (uint32_t base = begin; base < end; base += 64 * KV4_WAVES) {
+    for (uint32_t base = begin; base < end; base += PER * KV4_WAVES) {
         int32_t ids = -1;
-        const uint32_t mine = base + KV4_WAVES * lane;
-        if (mine < end) ids = table[mine >> shift];
+        const uint32_t mine = (base + lane / Sh::UNITS * KV4_WAVES) * Sh::UNITS + lane % Sh::UNITS;
+        if (mine < units) ids = table[mine >> shift];
         if (ids >= p.pages) ids = -1;
-        const int n = min((end - base + KV4_WAVES - 1) / KV4_WAVES, 64u);
-        auto where = [&](int i) {
-            const int id = __builtin_amdgcn_readlane(ids, i);
-            return kv4_head<D>(p, id < 0 ? 0 : id, head);
+        const int n = min((end - base + KV4_WAVES - 1) / KV4_WAVES, PER);
+        auto load = [&](Raw<D, G> &r, int i) {
+            const PHX_GLOBAL char *own = nullptr;
+#pragma unroll
+            for (int u = 0; u < Sh::UNITS; ++u) {
+                const int id = __builtin_amdgcn_readlane(ids, i * Sh::UNITS + u);
+                const uint32_t unit = (base + KV4_WAVES * i) * Sh::UNITS + u;
+                const uint32_t slot = (unit & ((1u << shift) - 1)) * 32;
+                const PHX_GLOBAL char *at = kv4_head<D>(p, id < 0 ? 0 : id, head);
+                load_unit<D, G>(r, u, at, P, slot, lane);
+                at += P * D + slot * 4;
+                own = Sh::UNITS == 1 || ln.tile / 2 == (uint32_t)u ? at : own;
+            }
+#pragma unroll
+            for (int a = 0; a < Sh::SETS; ++a) {
+                const uint32_t off = (ln.tile % 2 + a) * 64 + ln.quad * 16;
+                r.kp[a] = fetch<phx_u4>(own, off);
+                r.vp[a] = fetch<phx_u4>(own, off + P * 4);
+            }
         };
-        auto slot = [&](int i) { return ((base + KV4_WAVES * i) & ((1u << shift) - 1)) * 32; };
-        Raw<D> next;
-        load_block<D>(next, where(0), P, slot(0), lane);
-        for (int i = 0; i < n; ++i) {
-            const Raw<D> now = next;
-            if (i + 1 < n) load_block<D>(next, where(i + 1), P, slot(i + 1), lane);
-            if (__builtin_amdgcn_readlane(ids, i) < 0) continue;
-            const uint32_t key0 = (base + KV4_WAVES * i) * 32;
-            if (key0 + 32 <= (uint32_t)least)
-                attend_block<D, TERMS, NC, false>(now, q, st, key0, lane);
-            else
-                attend_block<D, TERMS, NC, true>(now, q, st, key0, lane);
+        auto absent = [&](int i) {
+            uint32_t bits = 0;
+#pragma unroll
+            for (int u = 0; u < Sh::UNITS; ++u)
+                bits |= (__builtin_amdgcn_readlane(ids, i * Sh::UNITS + u) < 0 ? 1u : 0u) << u;
+            return bits;
+        };
+        auto step = [&](const Raw<D, G> &r, int i, bool whole) {
+            const uint32_t no = absent(i), key0 = (base + KV4_WAVES * i) * KEYS;
+            if (no == (1u << Sh::UNITS) - 1) return;
+            attend_step<D, TERMS, NC, G>(r, q, st, ln, key0, !whole || no, no);
+        };
+        // two steps' loads under way
+        const int whole = base >= seen ? 0 : (int)((seen - base + KV4_WAVES - 1) / KV4_WAVES);
+        Raw<D, G> r, r2;
+        load(r, 0);
+        if (n > 1) load(r2, 1);
+        for (int i = 0; i < n; i += 2) {
+            step(r, i, i < whole);
+            if (i + 2 < n) load(r, i + 2);
+            if (i + 1 < n) step(r2, i + 1, i + 1 < whole);
+            if (i + 3 < n) load(r2, i + 3);
         }
     }
 
-    // the waves' results of one tile of columns after the other
+    // the results of the waves and copies, one tile of columns after the other
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
         float l = st[c].l, pm = st[c].pm;
@@ -350,48 +500,47 @@ __device__ __forceinline__ void attend(const PhxKv4 &p) {
         float *out = merged + (wave * 16 + (lane & 15)) * PITCH;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t row = 4 * quad + i;
+            const uint32_t row = 4 * ln.quad + i;
             const uint32_t d = D == 128 ? 8 * row : 8 * (row & 7) + 4 * (row >> 3);
 #pragma unroll
-            for (int j = 0; j < D / 16; ++j)
-                out[d + j] = fmaf(st[c].o[j][i], j & 1 ? 0x1p-4f : 1.0f, pm);
+            for (int j = 0; j < D / 16; ++j) out[d + j] = st[c].o[j][i] + pm;
         }
-        if (quad == 0) {
+        if (ln.quad == 0) {
             stats[(wave * 16 + lane) * 2] = st[c].m;
             stats[(wave * 16 + lane) * 2 + 1] = l;
         }
         __syncthreads();
-        // 16 threads per column, D/16 elements each
-        constexpr int N = D / 16;
-        const uint32_t col = threadIdx.x >> 4, d = (threadIdx.x & 15) * N;
-        float m = stats[col * 2], sum = 0.0f, o[N] = {};
+        for (uint32_t x = threadIdx.x; x < Sh::COLS * (D / 4); x += 64 * KV4_WAVES) {
+            const uint32_t col = x / (D / 4), d = x % (D / 4) * 4;
+            float m = KV4_NONE, sum = 0.0f;
+            phx_f4 o = {0, 0, 0, 0};
 #pragma unroll
-        for (int w = 1; w < KV4_WAVES; ++w) m = fmaxf(m, stats[(w * 16 + col) * 2]);
+            for (int w = 0; w < KV4_WAVES * G; ++w) m = fmaxf(m, stats[(w * Sh::COLS + col) * 2]);
 #pragma unroll
-        for (int w = 0; w < KV4_WAVES; ++w) {
-            const float f = __builtin_amdgcn_exp2f(stats[(w * 16 + col) * 2] - m);
-            sum = fmaf(f, stats[(w * 16 + col) * 2 + 1], sum);
+            for (int w = 0; w < KV4_WAVES * G; ++w) {
+                const uint32_t at = w * Sh::COLS + col;
+                const float f = __builtin_amdgcn_exp2f(stats[at * 2] - m);
+                sum = fmaf(f, stats[at * 2 + 1], sum);
+                const phx_f4 v = *(const phx_f4 *)(merged + at * PITCH + d);
 #pragma unroll
-            for (int u = 0; u < N; ++u)
-                o[u] = fmaf(f, merged[(w * 16 + col) * PITCH + d + u], o[u]);
-        }
-        const int64_t at = col0 + c * 16 + col, i = at / p.ratio, row = s.row0 + i;
-        if (i >= s.count || row < 0 || row >= p.rows) continue;
-        const int64_t qh = (int64_t)head * p.ratio + at % p.ratio;
-        if (p.splits == 1) {
-            T *dst = (T *)p.y + row * p.ldy + qh * D + d;
-            store<T, N>(dst, o, sum);
-        } else {
-            const int64_t units = p.rows * p.heads * p.ratio;
-            const int64_t unit = split * units + row * p.heads * p.ratio + qh;
-            float *dst = (float *)p.ws + unit * D + d;
-            if (sum != 0.0f)
-#pragma unroll
-                for (int u = 0; u < N; ++u) dst[u] = o[u];
-            if (d == 0) {
-                float *ml = (float *)p.ws + units * p.splits * D + unit * 2;
-                ml[0] = m;
-                ml[1] = sum;
+                for (int u = 0; u < 4; ++u) o[u] = fmaf(f, v[u], o[u]);
+            }
+            const uint32_t at = col0 + c * 16 + col, i = at / ratio;
+            const int64_t row = s.row0 + i;
+            if (i >= s.count || row < 0 || row >= p.rows) continue;
+            const int64_t qh = (int64_t)head * ratio + at % ratio;
+            if (p.splits == 1) {
+                store<T>((PHX_GLOBAL T *)p.y + row * p.ldy + qh * D + d, o, sum);
+            } else {
+                const int64_t rows = p.rows * p.heads * ratio;
+                const int64_t unit = split * rows + row * p.heads * ratio + qh;
+                if (sum != 0.0f) *(PHX_GLOBAL phx_f4 *)((PHX_GLOBAL float *)p.ws + unit * D + d) = o;
+                if (d == 0) {
+                    PHX_GLOBAL float *ml =
+                        (PHX_GLOBAL float *)p.ws + rows * p.splits * D + unit * 2;
+                    ml[0] = m;
+                    ml[1] = sum;
+                }
             }
         }
     }
@@ -408,19 +557,19 @@ __device__ __forceinline__ void combine(const PhxKv4 &p) {
     __shared__ float factor[PHX_KV4_SPLITS];
     __shared__ float wave_m[4], wave_l[4];
     __shared__ phx_f4 sums[G][L];
-    const int64_t heads = p.heads * p.ratio;
-    const int64_t qh = blockIdx.x % heads, i = blockIdx.x / heads % p.max_q;
-    const Seq s = kv4_seq(p, blockIdx.x / heads / p.max_q);
+    const uint32_t heads = p.heads * p.ratio, max_q = (uint32_t)p.max_q;
+    const uint32_t qh = blockIdx.x % heads, i = blockIdx.x / heads % max_q;
+    const Seq s = kv4_seq(p, blockIdx.x / heads / max_q);
     const int64_t row = s.row0 + i;
     if (i >= s.count || row < 0 || row >= p.rows) return;
     const int64_t units = p.rows * heads, unit = row * heads + qh;
-    const float *ml = (const float *)p.ws + units * p.splits * D;
+    const PHX_GLOBAL float *ml = (const PHX_GLOBAL float *)p.ws + units * p.splits * D;
     const int t = threadIdx.x;
     float m = KV4_NONE, l = 0.0f;
     if (t < p.splits) {
-        const float2 w = *(const float2 *)(ml + (t * units + unit) * 2);
-        l = w.y;
-        if (l != 0.0f) m = w.x;
+        const PHX_GLOBAL float *w = ml + (t * units + unit) * 2;
+        l = w[1];
+        if (l != 0.0f) m = w[0];
     }
     float top = m;
     for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
@@ -435,13 +584,13 @@ __device__ __forceinline__ void combine(const PhxKv4 &p) {
     if ((t & 63) == 0) wave_l[t >> 6] = sum;
     __syncthreads();
     const int g = t / L, lane = t % L;
-    const float *part = (const float *)p.ws + unit * D + lane * 4;
+    const PHX_GLOBAL float *part = (const PHX_GLOBAL float *)p.ws + unit * D + lane * 4;
     phx_f4 o = {0, 0, 0, 0};
 #pragma unroll 4
     for (int x = g; x < p.splits; x += G) {
         const float w = factor[x];
         if (w == 0.0f) continue;
-        const phx_f4 v = *(const phx_f4 *)(part + x * units * D);
+        const phx_f4 v = *(const PHX_GLOBAL phx_f4 *)(part + x * units * D);
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = fmaf(w, v[e], o[e]);
     }
@@ -450,33 +599,33 @@ __device__ __forceinline__ void combine(const PhxKv4 &p) {
     if (g) return;
 #pragma unroll
     for (int x = 1; x < G; ++x) o = o + sums[x][lane];
-    const float out[4] = {o[0], o[1], o[2], o[3]};
-    store<T, 4>((T *)p.y + row * p.ldy + qh * D + lane * 4, out,
-                (wave_l[0] + wave_l[1]) + (wave_l[2] + wave_l[3]));
+    store<T>((PHX_GLOBAL T *)p.y + row * p.ldy + qh * D + lane * 4, o,
+             (wave_l[0] + wave_l[1]) + (wave_l[2] + wave_l[3]));
 }
 
 }  // namespace
 
-#define ATTEND(T, D, suffix, NC, WAVES)                                                         \
-    extern "C" __global__ __launch_bounds__(64 * KV4_WAVES, WAVES) void kv4_attend_##suffix##_c##NC( \
-        PhxKv4 p) {                                                                             \
-        attend<T, D, NC>(p);                                                                    \
+#define ATTEND(T, D, suffix, NC, G, WAVES)                                                      \
+    extern "C" __global__ __launch_bounds__(64 * KV4_WAVES, WAVES) void                         \
+        kv4_attend_##suffix##_c##NC##_g##G(PhxKv4 p) {                                          \
+        attend<T, D, NC, G>(p);                                                                 \
     }
 #define COMBINE(T, D, suffix)                                                                   \
     extern "C" __global__ __launch_bounds__(256) void kv4_combine_##suffix(PhxKv4 p) {          \
         combine<T, D>(p);                                                                       \
     }
-ATTEND(_Float16, 64, f16_d64, 1, 2)
-ATTEND(_Float16, 128, f16_d128, 1, 2)
-ATTEND(float, 64, f32_d64, 1, 2)
-ATTEND(float, 128, f32_d128, 1, 2)
-ATTEND(_Float16, 64, f16_d64, 2, 2)
-ATTEND(_Float16, 128, f16_d128, 2, 2)
-ATTEND(float, 64, f32_d64, 2, 2)
-ATTEND(float, 128, f32_d128, 2, 1)
-ATTEND(_Float16, 64, f16_d64, 4, 1)
-ATTEND(_Float16, 128, f16_d128, 4, 1)
-COMBINE(_Float16, 64, f16_d64)
-COMBINE(_Float16, 128, f16_d128)
-COMBINE(float, 64, f32_d64)
-COMBINE(float, 128, f32_d128)
+#define ALL(T, D, suffix)                                                                       \
+    ATTEND(T, D, suffix, 1, 4, 2)                                                               \
+    ATTEND(T, D, suffix, 1, 2, 2)                                                               \
+    ATTEND(T, D, suffix, 1, 1, 2)                                                               \
+    COMBINE(T, D, suffix)
+ALL(_Float16, 64, f16_d64)
+ALL(_Float16, 128, f16_d128)
+ALL(float, 64, f32_d64)
+ALL(float, 128, f32_d128)
+ATTEND(_Float16, 64, f16_d64, 2, 1, 2)
+ATTEND(_Float16, 128, f16_d128, 2, 1, 2)
+ATTEND(float, 64, f32_d64, 2, 1, 2)
+ATTEND(float, 128, f32_d128, 2, 1, 1)
+ATTEND(_Float16, 64, f16_d64, 4, 1, 1)
+ATTEND(_Float16, 128, f16_d128, 4, 1, 1)

@@ -23,7 +23,7 @@ struct PhxKv4 {
     uint64_t x, y;  // append, read: K and V; attention: Q and O
     int64_t ldx, ldy;
     uint64_t ws;
-    int32_t ratio, splits, causal;
+    int32_t ratio, splits, causal, groups;  // groups: of columns, per KV head
     float scale;
 };
 

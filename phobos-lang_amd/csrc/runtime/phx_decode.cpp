@@ -210,19 +210,32 @@ int phx_kv4_read(phx_stream s, const phx_kv4_cache *cache, const phx_kv4_batch *
     return move_rows(s, cache, batch, t, k, v, ldk, ldv, "kv4_read", names);
 }
 
-// How an attention runs: tiles of 16 columns per wave (column_tiles), and the
-// split of the keys that brings the launch to kAttendGroups workgroups, of
-// parts of at least kAttendPart keys each (of the longest sequence there can
-// be) and at most PHX_KV4_SPLITS of them.
+// How an attention runs.  A workgroup takes 4, 8, 16, 32 or 64 columns, a
+// column being a row and query head of one KV head: the fewest that hold them
+// all (kv4_attend.hip; f32 queries, twice the registers, at most 32).  The keys
+// are split to bring the launch to kAttendGroups workgroups, into parts of at
+// least kAttendPart keys (of the longest sequence there can be) and at most
+// PHX_KV4_SPLITS of them.
 static const int64_t kAttendGroups = 512, kAttendPart = 512;
+struct AttendForm {
+    int64_t columns;
+    const char *entry[4];
+};
+#define FORM(columns, tail)                                                                  \
+    {columns, {"kv4_attend_f16_d64_" tail, "kv4_attend_f16_d128_" tail,                      \
+               "kv4_attend_f32_d64_" tail, "kv4_attend_f32_d128_" tail}}
+static const AttendForm kAttendForms[] = {FORM(4, "c1_g4"), FORM(8, "c1_g2"), FORM(16, "c1_g1"),
+                                          FORM(32, "c2_g1"), FORM(64, "c4_g1")};
+#undef FORM
 
-static int column_tiles(phx_dtype t, int64_t columns) {
-    return columns <= 16 ? 1 : columns <= 32 || t == PHX_F32 ? 2 : 4;
+static const AttendForm &attend_form(phx_dtype t, int64_t columns) {
+    int i = 0;
+    while (i < (t == PHX_F32 ? 3 : 4) && kAttendForms[i].columns < columns) ++i;
+    return kAttendForms[i];
 }
 
-static int64_t attend_groups(const phx_kv4_cache *c, const phx_kv4_batch *b, int64_t ratio,
-                             int tiles) {
-    return b->batch * c->heads * ((b->max_q * ratio + 16 * tiles - 1) / (16 * tiles));
+static int64_t attend_groups(const phx_kv4_batch *b, int64_t ratio, const AttendForm &f) {
+    return (b->max_q * ratio + f.columns - 1) / f.columns;
 }
 
 static size_t split_bytes(const phx_kv4_cache *c, const phx_kv4_batch *b, int64_t q_heads) {
@@ -231,7 +244,8 @@ static size_t split_bytes(const phx_kv4_cache *c, const phx_kv4_batch *b, int64_
 
 static int64_t attend_splits(const phx_kv4_cache *c, const phx_kv4_batch *b, int64_t q_heads) {
     const int64_t ratio = q_heads / c->heads;
-    const int64_t groups = attend_groups(c, b, ratio, column_tiles(PHX_F16, b->max_q * ratio));
+    const int64_t groups = b->batch * c->heads *
+                           attend_groups(b, ratio, attend_form(PHX_F16, b->max_q * ratio));
     const int64_t keys = std::min(b->max_len, b->table_stride * c->page_tokens);
     if (!has_work(b) || groups * 2 > kAttendGroups) return 1;
     return std::max<int64_t>(1, std::min({kAttendGroups / groups, keys / kAttendPart, (int64_t)PHX_KV4_SPLITS}));
@@ -258,12 +272,6 @@ int phx_kv4_split_plan(const phx_kv4_cache *cache, const phx_kv4_batch *batch, i
 int phx_kv4_attention(phx_stream s, const phx_kv4_cache *cache, const phx_kv4_batch *batch,
                       phx_dtype t, uint64_t q, uint64_t o, int64_t q_heads, float scale,
                       int causal, int64_t ldq, int64_t ldo) {
-    static const char *const names[3][4] = {
-        {"kv4_attend_f16_d64_c1", "kv4_attend_f16_d128_c1", "kv4_attend_f32_d64_c1",
-         "kv4_attend_f32_d128_c1"},
-        {"kv4_attend_f16_d64_c2", "kv4_attend_f16_d128_c2", "kv4_attend_f32_d64_c2",
-         "kv4_attend_f32_d128_c2"},
-        {"kv4_attend_f16_d64_c4", "kv4_attend_f16_d128_c4", nullptr, nullptr}};
     static const char *const combine[4] = {"kv4_combine_f16_d64", "kv4_combine_f16_d128",
                                            "kv4_combine_f32_d64", "kv4_combine_f32_d128"};
     const char *who = "kv4_attention";
@@ -286,8 +294,10 @@ int phx_kv4_attention(phx_stream s, const phx_kv4_cache *cache, const phx_kv4_ba
     p.ratio = (int32_t)(q_heads / cache->heads);
     p.causal = causal != 0;
     p.scale = scale;
-    const int tiles = column_tiles(t, batch->max_q * p.ratio);
-    const int64_t groups = attend_groups(cache, batch, p.ratio, tiles);
+    const AttendForm &form = attend_form(t, batch->max_q * p.ratio);
+    const int64_t each = attend_groups(batch, p.ratio, form);
+    const int64_t groups = batch->batch * cache->heads * each;
+    p.groups = (int32_t)each;
     const int64_t units = batch->batch * batch->max_q * q_heads;
     size_t room = 0;
     if (int rc = phx_stream_get_workspace(s, &p.ws, &room)) return rc;
@@ -297,7 +307,7 @@ int phx_kv4_attention(phx_stream s, const phx_kv4_cache *cache, const phx_kv4_ba
     if (groups * p.splits > INT32_MAX || units > INT32_MAX)
         return set_error(PHX_E_INVALID, "%s: %lld sequences of up to %lld rows are too many", who,
                          (long long)batch->batch, (long long)batch->max_q);
-    if (int rc = launch(kAttendFile, entry_of(names[tiles / 2], t, cache->head_dim),
+    if (int rc = launch(kAttendFile, entry_of(form.entry, t, cache->head_dim),
                         dim3((uint32_t)(groups * p.splits)), 256, (hipStream_t)s, &p))
         return rc;
     if (p.splits == 1) return PHX_OK;
