@@ -30,7 +30,6 @@
 // further over workgroups, whose results kv4_combine merges.
 #include "kv4.h"
 
-#define KV4_WAVES 4
 #define KV4_LOG2E 1.44269504088896340736f
 #define KV4_NONE -3e38f  // a reference below every score: no key yet
 
@@ -61,12 +60,15 @@ __device__ __forceinline__ _Float16 half_of(uint32_t w, int i) {
 __device__ __forceinline__ float middle(uint32_t w) {
     return fmaf(8.0f, (float)half_of(w, 0), (float)half_of(w, 1));
 }
-// (scale, minimum) with a scale that is not positive, as of a page never
-// written, made the smallest: it stands for the same where codes are 0.
+// (scale, minimum) as finite numbers, whatever is in a slot without a token,
+// and a scale that is not positive, as of a page never written, as the
+// smallest: it stands for the same where codes are 0.
 __device__ __forceinline__ uint32_t positive(uint32_t w) {
-    const phx_h2 least = {(_Float16)0x1p-24f, (_Float16)-INFINITY};
+    const phx_h2 least = {(_Float16)0x1p-24f, (_Float16)-65504.0f};
+    const phx_h2 most = {(_Float16)65504.0f, (_Float16)65504.0f};
     return __builtin_bit_cast(
-        uint32_t, __builtin_elementwise_max(__builtin_bit_cast(phx_h2, w), least));
+        uint32_t, __builtin_elementwise_min(
+                      __builtin_elementwise_max(__builtin_bit_cast(phx_h2, w), least), most));
 }
 
 // How a wave's 16 columns are used.  G 1: 16 columns over 32 keys, two products
@@ -96,26 +98,27 @@ __device__ __forceinline__ T fetch(const PHX_GLOBAL char *base, uint32_t off) {
     return *(const PHX_GLOBAL T *)(base + off);
 }
 
-// The tiles of one unit; its place in the step is u.
-template <int D, int G>
-__device__ __forceinline__ void load_unit(Raw<D, G> &r, int u, const PHX_GLOBAL char *head,
-                                          uint32_t P, uint32_t slot, uint32_t lane) {
-    const uint32_t c = lane & 15, quad = lane >> 4;
-    const PHX_GLOBAL char *k = head + slot * (D / 2), *v = k + P * (D / 2);
-    const uint32_t ko = c * (D / 2) + quad * (D / 8);
-    const uint32_t vo = (quad * (D / 8) + (c & (D / 8 - 1))) * 16;
+// Codes of the two tiles of a unit whose head's part of the page is at `head`.
+template <int D>
+__device__ __forceinline__ void load_k(uint32_t (*to)[D / 32], const PHX_GLOBAL char *head,
+                                       uint32_t slot, uint32_t lane) {
+    const uint32_t off = (lane & 15) * (D / 2) + (lane >> 4) * (D / 8);
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        uint32_t *to = r.k[2 * u + t];
+    for (int t = 0; t < 2; ++t)
         if constexpr (D == 128) {
-            const phx_u4 w = fetch<phx_u4>(k, ko + t * 8 * D);
-            to[0] = w.x, to[1] = w.y, to[2] = w.z, to[3] = w.w;
+            const phx_u4 w = fetch<phx_u4>(head + slot * (D / 2), off + t * 8 * D);
+            to[t][0] = w.x, to[t][1] = w.y, to[t][2] = w.z, to[t][3] = w.w;
         } else {
-            const phx_u2 w = fetch<phx_u2>(k, ko + t * 8 * D);
-            to[0] = w.x, to[1] = w.y;
+            const phx_u2 w = fetch<phx_u2>(head + slot * (D / 2), off + t * 8 * D);
+            to[t][0] = w.x, to[t][1] = w.y;
         }
-        r.v[2 * u + t] = fetch<phx_u4>(v, vo + t * 8 * D);
-    }
+}
+template <int D>
+__device__ __forceinline__ void load_v(phx_u4 *to, const PHX_GLOBAL char *head, uint32_t P,
+                                       uint32_t slot, uint32_t lane) {
+    const uint32_t off = ((lane >> 4) * (D / 8) + (lane & (D / 8 - 1))) * 16;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) to[t] = fetch<phx_u4>(head + (P + slot) * (D / 2), off + t * 8 * D);
 }
 
 // The columns' queries as matrix operands, and what turns a product into a
@@ -182,52 +185,78 @@ struct State {
     float m, l, pm;
 };
 
-template <bool B>
-struct Flag {
-    static constexpr bool value = B;
-};
-
 // What a lane knows of its copy.
 template <int D, int G>
 struct Lane {
-    uint32_t lane, quad, tile;                   // G 1: tile 0 of each set
-    uint32_t keep[G == 1 ? 1 : Shape<G>::TILES]; // all ones for its own tile, else 0
+    uint32_t lane, quad, tile;                     // G 1: tile 0 of each set
+    uint32_t keep[G == 1 ? 1 : Shape<G>::TILES];   // all ones for its own tile, else 0
     const phx_h8 *q[G == 1 ? 1 : Shape<G>::TILES]; // queries in LDS, or zeros
 };
 
-// A step of keys for NC tiles of columns.  masked: some keys are past what a
-// column sees, or in a unit without a page (a bit of `absent`).
+// x of the lane n columns on, in the same 16.
+template <int N>
+__device__ __forceinline__ float turned(float x) {
+    return __builtin_bit_cast(
+        float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x120 + N, 0xf, 0xf, true));
+}
+// Over a column's copies.
+template <int G>
+__device__ __forceinline__ float copies_sum(float x) {
+    if constexpr (G >= 2) x += turned<8>(x);
+    if constexpr (G == 4) x += turned<4>(x);
+    return x;
+}
+template <int G>
+__device__ __forceinline__ float copies_max(float x) {
+    if constexpr (G >= 2) x = fmaxf(x, turned<8>(x));
+    if constexpr (G == 4) x = fmaxf(x, turned<4>(x));
+    return x;
+}
+
+// The scores' products of a step.
 template <int D, int TERMS, int NC, int G>
-__device__ __forceinline__ void attend_step(const Raw<D, G> &r, const Query<D, TERMS> (&q)[NC],
-                                            State<D> (&st)[NC], const Lane<D, G> &ln, uint32_t key0,
-                                            bool masked, uint32_t absent) {
+__device__ __forceinline__ void scores(const Raw<D, G> &r, const Query<D, TERMS> (&q)[NC],
+                                       const Lane<D, G> &ln, phx_f4 (&s)[NC][Shape<G>::SETS]) {
     using Sh = Shape<G>;
-    constexpr int W = 4 * Sh::SETS;  // scores per lane
-    const uint32_t kmask = in_sgpr(0x03c003c0), kone = in_vgpr(0x4c004c00);
-    const uint32_t vmask[2] = {in_sgpr(0x000f000f), in_sgpr(0x00f000f0)};
-    const uint32_t vone[2] = {in_vgpr(0x64006400), in_vgpr(0x54005400)};
-    phx_f4 s[NC][Sh::SETS];
+    const uint32_t mask = in_sgpr(0x03c003c0), one = in_vgpr(0x4c004c00);
+    phx_f4 odd = {0, 0, 0, 0};  // G 2, 4: two chains, as one would wait for itself
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
         for (int a = 0; a < Sh::SETS; ++a) s[c][a] = (phx_f4){q[c].c, q[c].c, q[c].c, q[c].c};
 #pragma unroll
-    for (int t = 0; t < Sh::TILES; ++t)
+    for (int j = 0; j < D / 32; ++j)
 #pragma unroll
-        for (int j = 0; j < D / 32; ++j) {
+        for (int t = 0; t < Sh::TILES; ++t) {
             // 16 and the code behind it
             const uint32_t w = r.k[t][j];
-            const phx_h8 k = h8((w << 6 & kmask) | kone, (w << 2 & kmask) | kone,
-                                (w >> 2 & kmask) | kone, (w >> 6 & kmask) | kone);
+            const phx_h8 k = h8((w << 6 & mask) | one, (w << 2 & mask) | one, (w >> 2 & mask) | one,
+                                (w >> 6 & mask) | one);
 #pragma unroll
             for (int x = 0; x < TERMS; ++x)
                 if constexpr (G == 1) {
 #pragma unroll
                     for (int c = 0; c < NC; ++c) s[c][t] = mfma(k, q[c].q[x][j], s[c][t]);
                 } else {
-                    s[0][0] = mfma(k, ln.q[t][(x * (D / 32) + j) * 64], s[0][0]);
+                    phx_f4 &to = t % 2 ? odd : s[0][0];
+                    to = mfma(k, ln.q[t][(x * (D / 32) + j) * 64], to);
                 }
         }
+    if constexpr (G > 1) s[0][0] = s[0][0] + odd;
+}
+
+// The weights p_j s_j of a step's scores, in two f16 terms (22 bits): pairs of
+// halves, the f16 of the exact product and of what that leaves.  Keys past what
+// a column sees, or in a unit without a page (a bit of `absent`), get zeros
+// (without MASK there are none such).
+template <int D, int TERMS, int NC, int G, bool MASK>
+__device__ __forceinline__ void weights(const Raw<D, G> &r, const Query<D, TERMS> (&q)[NC],
+                                        State<D> (&st)[NC], const Lane<D, G> &ln,
+                                        const phx_f4 (&s)[NC][Shape<G>::SETS],
+                                        uint32_t (&hi)[NC][2 * Shape<G>::SETS],
+                                        uint32_t (&lo)[NC][2 * Shape<G>::SETS], uint32_t key0,
+                                        uint32_t absent, bool fresh) {
+    constexpr int W = 4 * Shape<G>::SETS;  // scores per lane
     uint32_t vp[W];
     float km[W], vm[W];
 #pragma unroll
@@ -236,35 +265,56 @@ __device__ __forceinline__ void attend_step(const Raw<D, G> &r, const Query<D, T
         km[u] = middle(r.kp[u / 4][u % 4]);
         vm[u] = middle(vp[u]);
     }
-    uint32_t hi[NC][W / 2], lo[NC][W / 2];  // pairs of halves
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-        const int32_t left = q[c].limit - (int32_t)(key0 + 16 * ln.tile + 4 * ln.quad);
-        auto in = [&](int u) {
-            return 16 * (u / 4) + u % 4 < left && !(absent >> (ln.tile / 2) & 1);
+        int32_t left = q[c].limit - (int32_t)(key0 + 16 * ln.tile + 4 * ln.quad);
+        if (absent >> (ln.tile / 2) & 1) left = 0;
+        float e[W];
+#pragma unroll
+        for (int u = 0; u < W; ++u) e[u] = s[c][u / 4][u % 4] * q[c].a;
+        // the score in log2 units, less m
+        auto score = [&](int u, float m) {
+            const float x = fmaf((float)half_of(r.kp[u / 4][u % 4], 0), e[u], fmaf(km[u], q[c].b, -m));
+            return !MASK || 16 * (u / 4) + u % 4 < left ? x : -INFINITY;
         };
-        float sum, pm;
-        bool over;
-        // weights against the reference m, in two f16 terms (22 bits): w as f16
-        // and what that leaves of the exact product; `over`: m does not hold
-        auto weigh = [&](auto mask) {
-            constexpr bool MASK = decltype(mask)::value;
+        // The reference m is of score + log2 s_V, and stays while no weight
+        // passes 40000: rarely raised after the first step, and then to 2^7
+        // below the step's largest.  (p itself is at most w 2^24 in f32.  A row
+        // with a NaN is NaN whatever its reference.)
+        float sum, pm, need = fresh ? INFINITY : 0.0f;
+        bool raise = fresh;
+        for (int pass = 0; pass < 2; ++pass) {
+            if (raise) {
+                float most = -INFINITY;
+#pragma unroll
+                for (int u = 0; u < W; ++u)
+                    most = fmaxf(most, score(u, 0.0f) +
+                                           __builtin_amdgcn_logf((float)half_of(vp[u], 0)));
+                most = copies_max<G>(most);
+                most = fmaxf(most, __shfl_xor(most, 16));
+                most = fmaxf(most, __shfl_xor(most, 32));
+                need = copies_max<G>(need);
+                need = fmaxf(need, __shfl_xor(need, 16));
+                need = fmaxf(need, __shfl_xor(need, 32));
+                // by the column's own weights alone: no row's result depends
+                // on the rows next to it
+                if (need > 40000.0f && most - 7.0f > st[c].m) {
+                    const float f = __builtin_amdgcn_exp2f(st[c].m - (most - 7.0f));
+                    st[c].m = most - 7.0f;
+                    st[c].l *= f;
+                    st[c].pm *= f;
+#pragma unroll
+                    for (int j = 0; j < D / 16; ++j) st[c].o[j] = st[c].o[j] * f;
+                }
+            }
             sum = pm = 0.0f;
-            phx_h2 h, top = {(_Float16)0.0f, (_Float16)0.0f}, l;
+            phx_h2 h, l, top = {(_Float16)0.0f, (_Float16)0.0f};
 #pragma unroll
             for (int u = 0; u < W; ++u) {
-                const float y = fmaf(km[u], q[c].b, -st[c].m);
-                float e = fmaf((float)half_of(r.kp[u / 4][u % 4], 0), s[c][u / 4][u % 4] * q[c].a, y);
-                _Float16 sv = half_of(vp[u], 0);
-                float mv = vm[u];
-                if (MASK) {
-                    e = in(u) ? e : -INFINITY;
-                    sv = in(u) ? sv : (_Float16)0.0f;
-                    mv = in(u) ? mv : 0.0f;
-                }
-                const float pr = __builtin_amdgcn_exp2f(e);
+                const float pr = __builtin_amdgcn_exp2f(score(u, st[c].m));
+                const _Float16 sv = half_of(vp[u], 0);
                 sum += pr;
-                pm = fmaf(pr, mv, pm);
+                pm = fmaf(pr, vm[u], pm);
                 h[u % 2] = (_Float16)fmaf(pr, (float)sv, 0.0f);
                 l[u % 2] = (_Float16)fmaf(pr, (float)sv, -(float)h[u % 2]);
                 if (u % 2) {
@@ -273,54 +323,27 @@ __device__ __forceinline__ void attend_step(const Raw<D, G> &r, const Query<D, T
                     lo[c][u / 2] = __builtin_bit_cast(uint32_t, l);
                 }
             }
-            over = fmaxf((float)top.x, (float)top.y) > 32768.0f;
-        };
-        if (masked)
-            weigh(Flag<true>());
-        else
-            weigh(Flag<false>());
-        // The reference m is of score + log2 s_V, and stays while no weight
-        // passes 2^15: rarely raised after the first step, and then to 2^7
-        // below the step's largest.  (p itself is at most w 2^24 in f32.  A row
-        // with a NaN is NaN whatever its reference.)
-        if (__any(over)) {
-            float most = -INFINITY;
-#pragma unroll
-            for (int u = 0; u < W; ++u) {
-                const float e = fmaf((float)half_of(r.kp[u / 4][u % 4], 0),
-                                     s[c][u / 4][u % 4] * q[c].a, km[u] * q[c].b);
-                most = fmaxf(most, !masked || in(u)
-                                       ? e + __builtin_amdgcn_logf((float)half_of(vp[u], 0))
-                                       : -INFINITY);
-            }
-            most = fmaxf(most, __shfl_xor(most, 16));
-            most = fmaxf(most, __shfl_xor(most, 32));
-            // by the column's own weights alone: no row's result depends on
-            // the rows next to it
-            uint32_t any = over;
-            any |= __shfl_xor(any, 16);
-            any |= __shfl_xor(any, 32);
-            if (any && most - 7.0f > st[c].m) {
-                const float f = __builtin_amdgcn_exp2f(st[c].m - (most - 7.0f));
-                st[c].m = most - 7.0f;
-                st[c].l *= f;
-                st[c].pm *= f;
-#pragma unroll
-                for (int j = 0; j < D / 16; ++j) st[c].o[j] = st[c].o[j] * f;
-            }
-            if (masked)
-                weigh(Flag<true>());
-            else
-                weigh(Flag<false>());
+            need = fmaxf((float)top.x, (float)top.y);
+            raise = __any(need > 40000.0f);
+            if (!raise) break;
         }
         st[c].l += sum;
         st[c].pm += pm;
     }
+}
+
+// The weights' product with a step's values.
+template <int D, int NC, int G>
+__device__ __forceinline__ void sums(const Raw<D, G> &r, State<D> (&st)[NC], const Lane<D, G> &ln,
+                                     const uint32_t (&hi)[NC][2 * Shape<G>::SETS],
+                                     const uint32_t (&lo)[NC][2 * Shape<G>::SETS]) {
+    const uint32_t mask[2] = {in_sgpr(0x000f000f), in_sgpr(0x00f000f0)};
+    const uint32_t one[2] = {in_vgpr(0x64006400), in_vgpr(0x54005400)};
     // an octet of elements per row of the operand; at D 64 the upper eight rows
     // are the same octets' other half
     const uint32_t first = D == 64 && (ln.lane & 8) ? 0x0c060c02 : 0x0c040c00;
 #pragma unroll
-    for (int n = 0; n < Sh::UNITS; ++n) {
+    for (int n = 0; n < Shape<G>::UNITS; ++n) {
         // the unit's weights: a copy's are zeros but for its own tile
         phx_h8 wh[NC], wl[NC];
 #pragma unroll
@@ -345,9 +368,9 @@ __device__ __forceinline__ void attend_step(const Raw<D, G> &r, const Query<D, T
             }
 #pragma unroll
             for (int odd = 0; odd < 2; ++odd) {
-                const uint32_t mask = vmask[odd], one = vone[odd];
-                const phx_h8 v = h8((x[0] & mask) | one, (x[1] & mask) | one, (x[2] & mask) | one,
-                                    (x[3] & mask) | one) - (_Float16)(odd ? 72 : 1032);
+                const phx_h8 v = h8((x[0] & mask[odd]) | one[odd], (x[1] & mask[odd]) | one[odd],
+                                    (x[2] & mask[odd]) | one[odd], (x[3] & mask[odd]) | one[odd]) -
+                                 (_Float16)(odd ? 72 : 1032);
 #pragma unroll
                 for (int c = 0; c < NC; ++c) {
                     st[c].o[2 * b + odd] = mfma(v, wh[c], st[c].o[2 * b + odd]);
@@ -368,26 +391,31 @@ __device__ __forceinline__ void store(PHX_GLOBAL T *dst, phx_f4 o, float sum) {
     *(PHX_GLOBAL four *)dst = out;
 }
 
-template <typename T, int D, int NC, int G>
+template <typename T, int D, int NC, int G, int WAVES>
 __device__ __forceinline__ void attend(const PhxKv4 &p) {
     using Sh = Shape<G>;
     constexpr int TERMS = sizeof(T) == 4 ? 2 : 1, PITCH = D + 4, COLS = NC * Sh::COLS;
-    __shared__ float merged[KV4_WAVES * 16 * PITCH];
-    __shared__ float stats[KV4_WAVES * 16 * 2];
+    __shared__ float merged[WAVES * Sh::COLS * PITCH];
+    __shared__ float stats[WAVES * Sh::COLS * 2];
     __shared__ phx_h8 queries[G == 1 ? 1 : TERMS * (D / 32) * 64 * 2];
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     Lane<D, G> ln;
     ln.lane = lane;
     ln.quad = lane >> 4;
     ln.tile = G == 1 ? 0 : (lane & 15) / Sh::COLS;
-    // column groups of one KV head next to each other, and so on one XCD
-    uint32_t item = phx_xcd_swizzle_any(blockIdx.x, gridDim.x);
-    const uint32_t groups = p.groups, cg = groups - 1 - item % groups;  // the longest rows first
-    item /= groups;
-    const uint32_t split = item % p.splits;
-    item /= p.splits;
-    const int head = item % p.heads;
-    const int64_t b = item / p.heads;
+    uint32_t cg = 0, split = blockIdx.x, head = blockIdx.y, b = blockIdx.z;
+    if (p.groups > 1) {
+        // column groups of one KV head next to each other on one XCD, the
+        // longest rows first
+        const uint32_t groups = p.groups, splits = p.splits;
+        uint32_t item = phx_xcd_swizzle_any(phx_block_linear(), phx_block_count());
+        cg = groups - 1 - item % groups;
+        item /= groups;
+        split = item % splits;
+        item /= splits;
+        head = item % p.heads;
+        b = item / p.heads;
+    }
     const Seq s = kv4_seq(p, b);
     const uint32_t ratio = p.ratio, col0 = cg * COLS, first = col0 / ratio;
     if (first >= s.count) return;
@@ -398,6 +426,65 @@ __device__ __forceinline__ void attend(const PhxKv4 &p) {
     int64_t least = p.causal ? s.tokens - s.count + first + 1 : s.tokens;
     if (most < 0) most = 0;
     if (least < 0) least = 0;
+
+    constexpr uint32_t KEYS = 16 * Sh::TILES, PER = 64 / Sh::UNITS;  // steps of whose pages the lanes hold
+    const uint32_t steps = (uint32_t)(most + KEYS - 1) / KEYS;
+    const uint32_t per = (steps + p.splits - 1) / p.splits;
+    const uint32_t end = min((split + 1) * per, steps), seen = (uint32_t)least / KEYS;
+    const uint32_t units = (uint32_t)(most + 31) / 32;
+    const uint32_t P = p.page_tokens, shift = __builtin_ctz(P / 32);
+    const PHX_GLOBAL int32_t *table =
+        (const PHX_GLOBAL int32_t *)p.table + b * p.table_stride;
+    // the wave's steps are base + WAVES i, and the lanes hold the pages of PER
+    // of them
+    uint32_t base = split * per + __builtin_amdgcn_readfirstlane(wave);
+    int32_t ids;
+    int n;
+    auto pages = [&]() {
+        ids = -1;
+        const uint32_t mine = (base + lane / Sh::UNITS * WAVES) * Sh::UNITS + lane % Sh::UNITS;
+        if (base < end && mine < units) ids = table[mine >> shift];
+        if (ids >= p.pages) ids = -1;
+        n = base < end ? min((end - base + WAVES - 1) / WAVES, PER) : 0;
+    };
+    // a step's page of unit u, and its slot there
+    auto slot = [&](int i, int u) {
+        return (((base + WAVES * i) * Sh::UNITS + u) & ((1u << shift) - 1)) * 32;
+    };
+    auto page = [&](int i, int u) {
+        const int id = __builtin_amdgcn_readlane(ids, i * Sh::UNITS + u);
+        return kv4_head<D>(p, id < 0 ? 0 : id, head);
+    };
+    Raw<D, G> r;
+    auto next_k = [&](int i) {
+#pragma unroll
+        for (int u = 0; u < Sh::UNITS; ++u) load_k<D>(r.k + 2 * u, page(i, u), slot(i, u), lane);
+    };
+    auto next_v = [&](int i) {
+#pragma unroll
+        for (int u = 0; u < Sh::UNITS; ++u)
+            load_v<D>(r.v + 2 * u, page(i, u), P, slot(i, u), lane);
+    };
+    auto next_p = [&](int i) {
+        const PHX_GLOBAL char *own = page(i, 0) + slot(i, 0) * 4;
+        if (Sh::UNITS == 2 && ln.tile >= 2) own = page(i, 1) + slot(i, 1) * 4;
+#pragma unroll
+        for (int a = 0; a < Sh::SETS; ++a) {
+            const uint32_t off = P * D + (ln.tile % 2 + a) * 64 + ln.quad * 16;
+            r.kp[a] = fetch<phx_u4>(own, off);
+            r.vp[a] = fetch<phx_u4>(own, off + P * 4);
+        }
+    };
+    // a step's loads go out as the one before is done with their registers, the
+    // first step's before the queries are looked at
+    auto start = [&]() {
+        pages();
+        if (n == 0) return;
+        next_k(0);
+        next_p(0);
+        next_v(0);
+    };
+    start();
 
     Query<D, TERMS> q[NC];
     State<D> st[NC];
@@ -427,97 +514,65 @@ __device__ __forceinline__ void attend(const PhxKv4 &p) {
             ln.q[t] = queries + (own ? 0 : N * 64) + lane;
         }
     }
-    constexpr uint32_t KEYS = 16 * Sh::TILES, PER = 64 / Sh::UNITS;  // steps of whose pages the lanes hold
-    const uint32_t steps = (uint32_t)(most + KEYS - 1) / KEYS;
-    const uint32_t per = (steps + p.splits - 1) / p.splits;
-    const uint32_t end = min((split + 1) * per, steps), seen = (uint32_t)least / KEYS;
-    const uint32_t units = (uint32_t)(most + 31) / 32;
-    const uint32_t P = p.page_tokens, shift = __builtin_ctz(P / 32);
-    const PHX_GLOBAL int32_t *table =
-        (const PHX_GLOBAL int32_t *)p.table + b * p.table_stride;
-    // the wave's steps are begin + KV4_WAVES i; the lanes hold the pages of PER
-    // of them
-    const uint32_t begin = split * per + __builtin_amdgcn_readfirstlane(wave);
-    for (uint32_t base = begin; base < end; base += PER * KV4_WAVES) {
-        int32_t ids = -1;
-        const uint32_t mine = (base + lane / Sh::UNITS * KV4_WAVES) * Sh::UNITS + lane % Sh::UNITS;
-        if (mine < units) ids = table[mine >> shift];
-        if (ids >= p.pages) ids = -1;
-        const int n = min((end - base + KV4_WAVES - 1) / KV4_WAVES, PER);
-        auto load = [&](Raw<D, G> &r, int i) {
-            const PHX_GLOBAL char *own = nullptr;
-#pragma unroll
-            for (int u = 0; u < Sh::UNITS; ++u) {
-                const int id = __builtin_amdgcn_readlane(ids, i * Sh::UNITS + u);
-                const uint32_t unit = (base + KV4_WAVES * i) * Sh::UNITS + u;
-                const uint32_t slot = (unit & ((1u << shift) - 1)) * 32;
-                const PHX_GLOBAL char *at = kv4_head<D>(p, id < 0 ? 0 : id, head);
-                load_unit<D, G>(r, u, at, P, slot, lane);
-                at += P * D + slot * 4;
-                own = Sh::UNITS == 1 || ln.tile / 2 == (uint32_t)u ? at : own;
-            }
-#pragma unroll
-            for (int a = 0; a < Sh::SETS; ++a) {
-                const uint32_t off = (ln.tile % 2 + a) * 64 + ln.quad * 16;
-                r.kp[a] = fetch<phx_u4>(own, off);
-                r.vp[a] = fetch<phx_u4>(own, off + P * 4);
-            }
-        };
-        auto absent = [&](int i) {
-            uint32_t bits = 0;
+    bool fresh = true;
+    while (n > 0) {
+        for (int i = 0; i < n; ++i) {
+            const uint32_t at = base + WAVES * i;
+            uint32_t absent = 0;
 #pragma unroll
             for (int u = 0; u < Sh::UNITS; ++u)
-                bits |= (__builtin_amdgcn_readlane(ids, i * Sh::UNITS + u) < 0 ? 1u : 0u) << u;
-            return bits;
-        };
-        auto step = [&](const Raw<D, G> &r, int i, bool whole) {
-            const uint32_t no = absent(i), key0 = (base + KV4_WAVES * i) * KEYS;
-            if (no == (1u << Sh::UNITS) - 1) return;
-            attend_step<D, TERMS, NC, G>(r, q, st, ln, key0, !whole || no, no);
-        };
-        // two steps' loads under way
-        const int whole = base >= seen ? 0 : (int)((seen - base + KV4_WAVES - 1) / KV4_WAVES);
-        Raw<D, G> r, r2;
-        load(r, 0);
-        if (n > 1) load(r2, 1);
-        for (int i = 0; i < n; i += 2) {
-            step(r, i, i < whole);
-            if (i + 2 < n) load(r, i + 2);
-            if (i + 1 < n) step(r2, i + 1, i + 1 < whole);
-            if (i + 3 < n) load(r2, i + 3);
+                absent |= (__builtin_amdgcn_readlane(ids, i * Sh::UNITS + u) < 0 ? 1u : 0u) << u;
+            phx_f4 x[NC][Sh::SETS];
+            uint32_t hi[NC][2 * Sh::SETS], lo[NC][2 * Sh::SETS];
+            scores<D, TERMS, NC, G>(r, q, ln, x);
+            if (i + 1 < n) next_k(i + 1);
+            weights<D, TERMS, NC, G, true>(r, q, st, ln, x, hi, lo, at * KEYS, absent, fresh);
+            fresh = false;
+            if (i + 1 < n) next_p(i + 1);
+            sums<D, NC, G>(r, st, ln, hi, lo);
+            if (i + 1 < n) next_v(i + 1);
         }
+        base += PER * WAVES;
+        start();
     }
 
-    // the results of the waves and copies, one tile of columns after the other
+    // the results of the waves, one tile of columns after the other; a column's
+    // copies have one reference
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-        float l = st[c].l, pm = st[c].pm;
+        float l = copies_sum<G>(st[c].l), pm = copies_sum<G>(st[c].pm);
         l += __shfl_xor(l, 16);
         l += __shfl_xor(l, 32);
         pm += __shfl_xor(pm, 16);
         pm += __shfl_xor(pm, 32);
         if (c) __syncthreads();
-        float *out = merged + (wave * 16 + (lane & 15)) * PITCH;
+        const uint32_t col = lane & 15, entry = wave * Sh::COLS + col;
+        float *out = merged + entry * PITCH;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const uint32_t row = 4 * ln.quad + i;
             const uint32_t d = D == 128 ? 8 * row : 8 * (row & 7) + 4 * (row >> 3);
 #pragma unroll
-            for (int j = 0; j < D / 16; ++j) out[d + j] = st[c].o[j][i] + pm;
+            for (int j = 0; j < D / 16; j += 4) {
+                phx_f4 o;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[k] = copies_sum<G>(st[c].o[j + k][i]) + pm;
+                if (G == 1 || col < Sh::COLS) *(phx_f4 *)(out + d + j) = o;
+            }
         }
-        if (ln.quad == 0) {
-            stats[(wave * 16 + lane) * 2] = st[c].m;
-            stats[(wave * 16 + lane) * 2 + 1] = l;
+        if (lane < Sh::COLS) {
+            stats[entry * 2] = st[c].m;
+            stats[entry * 2 + 1] = l;
         }
         __syncthreads();
-        for (uint32_t x = threadIdx.x; x < Sh::COLS * (D / 4); x += 64 * KV4_WAVES) {
+        for (uint32_t x = threadIdx.x; x < Sh::COLS * (D / 4); x += 64 * WAVES) {
             const uint32_t col = x / (D / 4), d = x % (D / 4) * 4;
             float m = KV4_NONE, sum = 0.0f;
             phx_f4 o = {0, 0, 0, 0};
 #pragma unroll
-            for (int w = 0; w < KV4_WAVES * G; ++w) m = fmaxf(m, stats[(w * Sh::COLS + col) * 2]);
+            for (int w = 0; w < WAVES; ++w) m = fmaxf(m, stats[(w * Sh::COLS + col) * 2]);
 #pragma unroll
-            for (int w = 0; w < KV4_WAVES * G; ++w) {
+            for (int w = 0; w < WAVES; ++w) {
                 const uint32_t at = w * Sh::COLS + col;
                 const float f = __builtin_amdgcn_exp2f(stats[at * 2] - m);
                 sum = fmaf(f, stats[at * 2 + 1], sum);
@@ -605,27 +660,30 @@ __device__ __forceinline__ void combine(const PhxKv4 &p) {
 
 }  // namespace
 
-#define ATTEND(T, D, suffix, NC, G, WAVES)                                                      \
-    extern "C" __global__ __launch_bounds__(64 * KV4_WAVES, WAVES) void                         \
-        kv4_attend_##suffix##_c##NC##_g##G(PhxKv4 p) {                                          \
-        attend<T, D, NC, G>(p);                                                                 \
+#define ATTEND(T, D, suffix, NC, G, WAVES, PER_SIMD)                                            \
+    extern "C" __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void                          \
+        kv4_attend_##suffix##_c##NC##_g##G##_w##WAVES(PhxKv4 p) {                               \
+        attend<T, D, NC, G, WAVES>(p);                                                          \
     }
 #define COMBINE(T, D, suffix)                                                                   \
     extern "C" __global__ __launch_bounds__(256) void kv4_combine_##suffix(PhxKv4 p) {          \
         combine<T, D>(p);                                                                       \
     }
 #define ALL(T, D, suffix)                                                                       \
-    ATTEND(T, D, suffix, 1, 4, 2)                                                               \
-    ATTEND(T, D, suffix, 1, 2, 2)                                                               \
-    ATTEND(T, D, suffix, 1, 1, 2)                                                               \
+    ATTEND(T, D, suffix, 1, 4, 4, 2)                                                            \
+    ATTEND(T, D, suffix, 1, 2, 4, 2)                                                            \
+    ATTEND(T, D, suffix, 1, 1, 4, 2)                                                            \
+    ATTEND(T, D, suffix, 1, 4, 12, 3)                                                           \
+    ATTEND(T, D, suffix, 1, 2, 16, 4)                                                           \
+    ATTEND(T, D, suffix, 1, 1, 8, 2)                                                            \
     COMBINE(T, D, suffix)
 ALL(_Float16, 64, f16_d64)
 ALL(_Float16, 128, f16_d128)
 ALL(float, 64, f32_d64)
 ALL(float, 128, f32_d128)
-ATTEND(_Float16, 64, f16_d64, 2, 1, 2)
-ATTEND(_Float16, 128, f16_d128, 2, 1, 2)
-ATTEND(float, 64, f32_d64, 2, 1, 2)
-ATTEND(float, 128, f32_d128, 2, 1, 1)
-ATTEND(_Float16, 64, f16_d64, 4, 1, 1)
-ATTEND(_Float16, 128, f16_d128, 4, 1, 1)
+ATTEND(_Float16, 64, f16_d64, 2, 1, 4, 2)
+ATTEND(_Float16, 128, f16_d128, 2, 1, 4, 2)
+ATTEND(float, 64, f32_d64, 2, 1, 4, 2)
+ATTEND(float, 128, f32_d128, 2, 1, 4, 1)
+ATTEND(_Float16, 64, f16_d64, 4, 1, 4, 1)
+ATTEND(_Float16, 128, f16_d128, 4, 1, 4, 1)

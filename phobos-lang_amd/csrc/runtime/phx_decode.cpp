@@ -212,21 +212,27 @@ int phx_kv4_read(phx_stream s, const phx_kv4_cache *cache, const phx_kv4_batch *
 
 // How an attention runs.  A workgroup takes 4, 8, 16, 32 or 64 columns, a
 // column being a row and query head of one KV head: the fewest that hold them
-// all (kv4_attend.hip; f32 queries, twice the registers, at most 32).  The keys
-// are split to bring the launch to kAttendGroups workgroups, into parts of at
-// least kAttendPart keys (of the longest sequence there can be) and at most
-// PHX_KV4_SPLITS of them.
-static const int64_t kAttendGroups = 512, kAttendPart = 512;
+// all (kv4_attend.hip; f32 queries, twice the registers, at most 32).  Up to 16
+// columns a workgroup has eight waves where as many cannot fill the GPU
+// (kAttendFull), and the keys are split further to bring the launch to
+// kAttendGroups workgroups, into parts of at least kAttendPart keys (of the
+// longest sequence there can be) and at most PHX_KV4_SPLITS of them.
+static const int64_t kAttendFull = 512, kAttendGroups = 256, kAttendPart = 1024;
 struct AttendForm {
     int64_t columns;
-    const char *entry[4];
+    uint32_t waves;  // of the wide form
+    const char *entry[2][4];
 };
-#define FORM(columns, tail)                                                                  \
-    {columns, {"kv4_attend_f16_d64_" tail, "kv4_attend_f16_d128_" tail,                      \
-               "kv4_attend_f32_d64_" tail, "kv4_attend_f32_d128_" tail}}
-static const AttendForm kAttendForms[] = {FORM(4, "c1_g4"), FORM(8, "c1_g2"), FORM(16, "c1_g1"),
-                                          FORM(32, "c2_g1"), FORM(64, "c4_g1")};
-#undef FORM
+#define ENTRIES(tail)                                                          \
+    {"kv4_attend_f16_d64_" tail, "kv4_attend_f16_d128_" tail,                  \
+     "kv4_attend_f32_d64_" tail, "kv4_attend_f32_d128_" tail}
+static const AttendForm kAttendForms[] = {
+    {4, 12, {ENTRIES("c1_g4_w4"), ENTRIES("c1_g4_w12")}},
+    {8, 16, {ENTRIES("c1_g2_w4"), ENTRIES("c1_g2_w16")}},
+    {16, 8, {ENTRIES("c1_g1_w4"), ENTRIES("c1_g1_w8")}},
+    {32, 4, {ENTRIES("c2_g1_w4"), ENTRIES("c2_g1_w4")}},
+    {64, 4, {ENTRIES("c4_g1_w4"), ENTRIES("c4_g1_w4")}}};
+#undef ENTRIES
 
 static const AttendForm &attend_form(phx_dtype t, int64_t columns) {
     int i = 0;
@@ -247,7 +253,7 @@ static int64_t attend_splits(const phx_kv4_cache *c, const phx_kv4_batch *b, int
     const int64_t groups = b->batch * c->heads *
                            attend_groups(b, ratio, attend_form(PHX_F16, b->max_q * ratio));
     const int64_t keys = std::min(b->max_len, b->table_stride * c->page_tokens);
-    if (!has_work(b) || groups * 2 > kAttendGroups) return 1;
+    if (!has_work(b)) return 1;
     return std::max<int64_t>(1, std::min({kAttendGroups / groups, keys / kAttendPart, (int64_t)PHX_KV4_SPLITS}));
 }
 
@@ -304,11 +310,14 @@ int phx_kv4_attention(phx_stream s, const phx_kv4_cache *cache, const phx_kv4_ba
     const size_t part = split_bytes(cache, batch, q_heads);
     p.splits = (int32_t)std::max<int64_t>(
         1, std::min<int64_t>(attend_splits(cache, batch, q_heads), (int64_t)(room / part)));
-    if (groups * p.splits > INT32_MAX || units > INT32_MAX)
+    if (units > INT32_MAX || each * p.splits > INT32_MAX || groups * p.splits > INT32_MAX)
         return set_error(PHX_E_INVALID, "%s: %lld sequences of up to %lld rows are too many", who,
                          (long long)batch->batch, (long long)batch->max_q);
-    if (int rc = launch(kAttendFile, entry_of(form.entry, t, cache->head_dim),
-                        dim3((uint32_t)(groups * p.splits)), 256, (hipStream_t)s, &p))
+    const bool wide = form.columns <= 16 && groups < kAttendFull;
+    if (int rc = launch(kAttendFile, entry_of(form.entry[wide], t, cache->head_dim),
+                        dim3((uint32_t)(each * p.splits), (uint32_t)cache->heads,
+                             (uint32_t)batch->batch),
+                        64 * (wide ? form.waves : 4), (hipStream_t)s, &p))
         return rc;
     if (p.splits == 1) return PHX_OK;
     return launch(kAttendFile, entry_of(combine, t, cache->head_dim),
