@@ -9,8 +9,7 @@
 
 struct PhxGemvW4 {
     uint64_t a, w, scales, zeros, c;
-    int64_t M, N, K, lda, ldc;
-    int32_t group;
+    int64_t M, N, K, lda, ldc, groups;
     float alpha, beta;
 };
 

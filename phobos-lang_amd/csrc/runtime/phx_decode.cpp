@@ -18,6 +18,7 @@ const char *const kKv4File = "kv4.hsaco";
 const char *const kAttendFile = "kv4_attend.hsaco";
 const char *const kPagesFile = "pages.hsaco";
 
+// (file and entry are literals: aux_function knows them by address)
 int launch(const char *file, const char *entry, dim3 grid, uint32_t threads, hipStream_t s,
            void *record) {
     hipFunction_t f;
@@ -184,9 +185,15 @@ int phx_gemv_w4(phx_stream s, phx_dtype t, uint64_t a, uint64_t w, uint64_t scal
                          "gemv_w4: A and the codes must be 16-byte aligned, scales and C by element");
     if (int rc = on_device((hipStream_t)s)) return rc;
     if (M == 0) return PHX_OK;
-    PhxGemvW4 p = {a, w, scales, zeros, c, M, N, K, lda, ldc, (int32_t)group, alpha, beta};
-    return launch(kW4File, t == PHX_F16 ? "gemv_w4_f16" : "gemv_w4_f32",
-                  dim3((uint32_t)((N + 3) / 4), (uint32_t)M), 256, (hipStream_t)s, &p);
+    PhxGemvW4 p = {a, w, scales, zeros, c, M, N, K, lda, ldc, (K + group - 1) / group, alpha, beta};
+#define GROUPS(form) {"gemv_w4_" form "_g1", "gemv_w4_" form "_g2", "gemv_w4_" form "_g4"}
+    static const char *const entries[2][3][3] = {
+        {GROUPS("f32_m1_n1"), GROUPS("f32_m2_n1"), GROUPS("f32_m4_n1")},
+        {GROUPS("f16_m1_n1"), GROUPS("f16_m2_n1"), GROUPS("f16_m4_n1")}};
+#undef GROUPS
+    const char *entry = entries[t == PHX_F16][M <= 16 ? 0 : M <= 32 ? 1 : 2]
+                               [group == 128 ? 0 : group == 64 ? 1 : 2];
+    return launch(kW4File, entry, dim3((uint32_t)((N + 15) / 16)), 512, (hipStream_t)s, &p);
 }
 
 // ------------------------------------------------------------------ 4-bit cache
@@ -213,11 +220,14 @@ int phx_kv4_read(phx_stream s, const phx_kv4_cache *cache, const phx_kv4_batch *
 // How an attention runs.  A workgroup takes 4, 8, 16, 32 or 64 columns, a
 // column being a row and query head of one KV head: the fewest that hold them
 // all (kv4_attend.hip; f32 queries, twice the registers, at most 32).  Up to 16
-// columns a workgroup has eight waves where as many cannot fill the GPU
-// (kAttendFull), and the keys are split further to bring the launch to
+// columns a workgroup has 8 to 16 waves instead of four where there are fewer
+// than kAttendFull like it and kAttendWide keys or more to share out (32
+// sequences, 8 x 4 heads of 128: 512 keys 9.4 us with 4 waves, 10.0 with 12; 2048
+// keys 23.7 and 19.3).  The keys are split further to bring the launch to
 // kAttendGroups workgroups, into parts of at least kAttendPart keys (of the
 // longest sequence there can be) and at most PHX_KV4_SPLITS of them.
-static const int64_t kAttendFull = 512, kAttendGroups = 256, kAttendPart = 1024;
+static const int64_t kAttendFull = 512, kAttendWide = 1024, kAttendGroups = 256,
+                     kAttendPart = 1024;
 struct AttendForm {
     int64_t columns;
     uint32_t waves;  // of the wide form
@@ -313,7 +323,8 @@ int phx_kv4_attention(phx_stream s, const phx_kv4_cache *cache, const phx_kv4_ba
     if (units > INT32_MAX || each * p.splits > INT32_MAX || groups * p.splits > INT32_MAX)
         return set_error(PHX_E_INVALID, "%s: %lld sequences of up to %lld rows are too many", who,
                          (long long)batch->batch, (long long)batch->max_q);
-    const bool wide = form.columns <= 16 && groups < kAttendFull;
+    const bool wide = form.columns <= 16 && groups < kAttendFull &&
+                      std::min(batch->max_len, batch->table_stride * cache->page_tokens) >= kAttendWide;
     if (int rc = launch(kAttendFile, entry_of(form.entry[wide], t, cache->head_dim),
                         dim3((uint32_t)(each * p.splits), (uint32_t)cache->heads,
                              (uint32_t)batch->batch),
