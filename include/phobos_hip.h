@@ -341,7 +341,10 @@ int phx_w4_pack(phx_stream s, uint64_t codes, uint64_t packed, int64_t N, int64_
  * f16 operands enter the products exactly, f32 operands with all their bits;
  * products, sums and scales are f32, and C is rounded once from
  * fl(fl(alpha*acc) + fl(beta*c)), not read when beta == 0.  C overlaps no
- * other operand. */
+ * other operand.  An infinity in an f32 row makes the row NaN.  A launch of
+ * more than 16 rows that cannot fill the GPU is split over K where s has a
+ * workspace bound that holds two or four parts of M*N f32 (so at most 16*M*N
+ * bytes are used; see phx_kv4_attention on graphs), else it runs unsplit. */
 int phx_gemv_w4(phx_stream s, phx_dtype t, uint64_t a, uint64_t w, uint64_t scales,
                 uint64_t zeros, uint64_t c, int64_t M, int64_t N, int64_t K, int64_t group,
                 float alpha, float beta, int64_t lda, int64_t ldc);

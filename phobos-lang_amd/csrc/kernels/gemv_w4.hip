@@ -10,6 +10,17 @@
 // f32 rows in three bf16 terms): a tile's dword is a lane's eight k of
 // v_mfma_f32_16x16x32, so 16 bytes of a lane are four products' operands, and a
 // group is one to four of them, whose sum is scaled once.
+//
+// Few rows are bound by the codes' bytes, and by latency where those are few:
+// every code is read once, two blocks of a wave ahead. 16384 x 8192 in groups of
+// 128, f16: 1 row 16.7 us (4.2 TB/s), 16 rows 19.4 us; f32: 27.1 and 35.9 us.
+// 64 rows of 16384 x 8192 take 34.1 us (504 TFLOP/s; f32 77 us): unpacking costs
+// as many cycles as the products, and the rows pass through LDS in every
+// workgroup.
+// A split of N in tiles leaves CUs idle below 4096 columns; there 8 or 16 waves
+// share a tile's K. A scale and a zero point are loaded by a quarter of a wave
+// for the groups of a block and handed around by the lanes (groups of 32, 64 rows,
+// 16384 x 8192: 47.4 us; every lane loading all of them 64.1).
 #include "phx_common.h"
 #include "phx_decode.h"
 
@@ -41,59 +52,99 @@ __device__ __forceinline__ uint32_t in_vgpr(uint32_t x) {
     return x;
 }
 
-// 16 rows by 32 k of A as a matrix operand (a lane: row lane % 16, eight k from
-// 8 (lane / 16) on), rows and k that do not exist as zeros: one f16 term, or
-// three bf16 terms of an f32, which hold its 24 bits.
+// Rows of A as matrix operands: of each k one f16 term, or three bf16 terms of an
+// f32, which hold its 24 bits.
 template <typename T>
 struct Rows;
 template <>
 struct Rows<_Float16> {
-    phx_h8 v;
+    static constexpr int TERMS = 1;
+    phx_h8 v[1];
 };
 template <>
 struct Rows<float> {
+    static constexpr int TERMS = 3;
     b8 v[3];
 };
 
-__device__ __forceinline__ void load(Rows<_Float16> &r, __amdgpu_buffer_rsrc_t a, uint32_t off) {
-    r.v = __builtin_bit_cast(phx_h8, __builtin_amdgcn_raw_buffer_load_b128(a, off, 0, 0));
-}
-__device__ __forceinline__ void load(Rows<float> &r, __amdgpu_buffer_rsrc_t a, uint32_t off) {
-    const phx_u4 x = __builtin_amdgcn_raw_buffer_load_b128(a, off, 0, 0);
-    const phx_u4 y = __builtin_amdgcn_raw_buffer_load_b128(a, off, 16, 0);
+// 16 rows of a block of 128 k go through LDS: in memory a lane's neighbours have
+// the next k of the same row (a wave's load of 16 rows by 64 bytes, as the
+// operands have them, takes 64 cycles of the CU's vector memory path, one a
+// lane, where whole rows take 16), in the operands the same k of the next.
+// A term's 16 bytes of row r and k 8c .. 8c+7 are at 256 c + 16 (r ^ c): writes
+// and reads of 16 lanes touch every bank once.
+constexpr uint32_t kTile = 4096;  // bytes of 16 rows of one term
+
+template <typename T>
+struct Staged {
+    static constexpr uint32_t ROWS = sizeof(T) == 2 ? 4 : 2;  // of a wave's load
+    static constexpr uint32_t LOADS = 16 / ROWS;              // for 16 rows
+    static constexpr uint32_t BYTES = kTile * Rows<T>::TERMS;
+
+    // the lane's row and first k in a block in load f of its rows
+    static __device__ __forceinline__ uint32_t row(uint32_t f, uint32_t lane) {
+        return f * ROWS + lane / (64 / ROWS);
+    }
+    static __device__ __forceinline__ uint32_t k(uint32_t lane) {
+        return lane % (64 / ROWS) * (16 / sizeof(T));
+    }
+    static __device__ __forceinline__ uint32_t at(uint32_t row, uint32_t c) {
+        return c * 256 + ((row ^ c) & 15) * 16;
+    }
+    // `lds`: the 16 rows' part
+    static __device__ __forceinline__ void put(char *lds, phx_u4 x, uint32_t row, uint32_t lane) {
+        if constexpr (sizeof(T) == 2) {
+            *(phx_u4 *)(lds + at(row, lane % 16)) = x;
+        } else {
+            phx_u2 out[3];
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-        // the top 16 bits, what they leave, and what that leaves: each exact
-        uint32_t t[3][2];
+            for (int i = 0; i < 2; ++i) {
+                // the top 16 bits, what they leave, and what that leaves: each exact
+                uint32_t t[3][2];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const uint32_t w = i < 4 ? x[(i + k) & 3] : y[(i + k) & 3];
-            const uint32_t hi = w & 0xffff0000u;
-            const float rest = __builtin_bit_cast(float, w) - __builtin_bit_cast(float, hi);
-            const uint32_t mid = __builtin_bit_cast(uint32_t, rest) & 0xffff0000u;
-            t[0][k] = hi;
-            t[1][k] = mid;
-            t[2][k] = __builtin_bit_cast(uint32_t, rest - __builtin_bit_cast(float, mid));
-        }
+                for (int k = 0; k < 2; ++k) {
+                    const uint32_t w = x[2 * i + k], hi = w & 0xffff0000u;
+                    const float rest = __builtin_bit_cast(float, w) - __builtin_bit_cast(float, hi);
+                    const uint32_t mid = __builtin_bit_cast(uint32_t, rest) & 0xffff0000u;
+                    t[0][k] = hi;
+                    t[1][k] = mid;
+                    t[2][k] = __builtin_bit_cast(uint32_t, rest - __builtin_bit_cast(float, mid));
+                }
 #pragma unroll
-        for (int n = 0; n < 3; ++n) {
-            const uint32_t pair = __builtin_amdgcn_perm(t[n][1], t[n][0], 0x07060302);
-            const phx_u2 both = {pair, 0};
-            r.v[n][i] = __builtin_bit_cast(__bf16, (uint16_t)both.x);
-            r.v[n][i + 1] = __builtin_bit_cast(__bf16, (uint16_t)(both.x >> 16));
+                for (int n = 0; n < 3; ++n)
+                    out[n][i] = __builtin_amdgcn_perm(t[n][1], t[n][0], 0x07060302);
+            }
+#pragma unroll
+            for (int n = 0; n < 3; ++n)
+                *(phx_u2 *)(lds + n * kTile + at(row, lane % 32 / 2) + lane % 2 * 8) = out[n];
         }
     }
-}
+    // the operand of the block's j-th 32 k
+    static __device__ __forceinline__ Rows<T> get(const char *lds, int j, uint32_t lane) {
+        Rows<T> r;
+#pragma unroll
+        for (int n = 0; n < Rows<T>::TERMS; ++n)
+            r.v[n] = __builtin_bit_cast(
+                __typeof__(r.v[n]), *(const phx_u4 *)(lds + n * kTile + at(lane & 15, 4 * j + lane / 16)));
+        return r;
+    }
+};
 
 // Eight codes less their zero point, exactly.
-__device__ __forceinline__ phx_h8 codes(uint32_t w, int zero, uint32_t one, _Float16) {
-    const uint32_t mask = 0x000f000f;
-    const phx_u4 x = {(w & mask) | one, (w >> 4 & mask) | one, (w >> 8 & mask) | one,
-                      (w >> 12 & mask) | one};  // 1024 + code
-    const _Float16 z = __builtin_bit_cast(_Float16, (uint16_t)(0x6400 + zero));
-    return __builtin_bit_cast(phx_h8, x) - (phx_h8){z, z, z, z, z, z, z, z};
+__device__ __forceinline__ phx_h8 codes(uint32_t w, int zero, const uint32_t (&one)[2], _Float16) {
+    const uint32_t low = 0x000f000f, high = 0x00f000f0;
+    // 1024 + code in the low nibbles of a half's byte, 64 + code in the high
+    const _Float16 z = (_Float16)(1024 + zero), y = (_Float16)(64 + zero);
+    const phx_h2 zz = {z, z}, yy = {y, y};
+    auto less = [](uint32_t x, phx_h2 y) {
+        return __builtin_bit_cast(uint32_t, __builtin_bit_cast(phx_h2, x) - y);
+    };
+    const uint32_t v = w >> 8;
+    const phx_u4 x = {less((w & low) | one[0], zz), less((w & high) | one[1], yy),
+                      less((v & low) | one[0], zz), less((v & high) | one[1], yy)};
+    return __builtin_bit_cast(phx_h8, x);
 }
-__device__ __forceinline__ b8 codes(uint32_t w, int zero, uint32_t, float) {
+__device__ __forceinline__ b8 codes(uint32_t w, int zero, const uint32_t (&)[2], float) {
     const float z = (float)zero;
     const uint32_t lo = w & 0x0f0f0f0f, hi = w >> 4 & 0x0f0f0f0f;
     phx_u4 x;
@@ -110,7 +161,7 @@ __device__ __forceinline__ b8 codes(uint32_t w, int zero, uint32_t, float) {
 }
 
 __device__ __forceinline__ phx_f4 product(const Rows<_Float16> &a, phx_h8 w, phx_f4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a.v, w, c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a.v[0], w, c, 0, 0, 0);
 }
 __device__ __forceinline__ phx_f4 product(const Rows<float> &a, b8 w, phx_f4 c) {
     // the small terms first
@@ -119,125 +170,303 @@ __device__ __forceinline__ phx_f4 product(const Rows<float> &a, b8 w, phx_f4 c) 
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[0], w, c, 0, 0, 0);
 }
 
-// A workgroup: NT tiles of 16 columns, MT tiles of 16 rows, its waves over the
-// tiles of K in turns; they add up in LDS.  PER groups in a tile.
-template <typename T, int MT, int NT, int WAVES, int PER>
+// The weights of a 128-row block of NT tiles of columns, as loaded: of its PER
+// groups a lane has the scale and the zero point of the (lane / 16 % PER)-th.
+template <int NT>
+struct Block {
+    phx_u4 w[NT];
+    uint16_t s[NT];
+    uint8_t z[NT];
+};
+
+// A lane's columns, 16 n + lane % 16 from n0 on, in the codes and the groups.
+template <int NT, int PER>
+struct Columns {
+    uint32_t col[NT];
+    const PHX_GLOBAL char *w[NT];
+
+    __device__ __forceinline__ void start(const PhxGemvW4 &p, int64_t n0, int64_t kb, uint32_t lane) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            // columns past N read the last one's, and are not stored
+            const int64_t c = n0 + 16 * n + (lane & 15);
+            col[n] = (uint32_t)(c < p.N ? c : p.N - 1);
+            w[n] = (const PHX_GLOBAL char *)p.w + (int64_t)(col[n] / 16) * kb * 1024 +
+                   (lane >> 4) * 256 + col[n] % 16 * 16;
+        }
+    }
+    __device__ __forceinline__ void fetch(const PhxGemvW4 &p, Block<NT> &t, int64_t b,
+                                          uint32_t lane) const {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) t.w[n] = *(const PHX_GLOBAL phx_u4 *)(w[n] + b * 1024);
+        int64_t group = b * PER + lane / 16 % PER;
+        if (group >= p.groups) group = p.groups - 1;
+        const PHX_GLOBAL uint16_t *s = (const PHX_GLOBAL uint16_t *)p.scales + group * p.N;
+        const PHX_GLOBAL uint8_t *z = (const PHX_GLOBAL uint8_t *)p.zeros + group * p.N;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            t.s[n] = s[col[n]];
+            t.z[n] = p.zeros ? z[col[n]] : 8;
+        }
+    }
+};
+
+// The j-th 32 rows of a block: its products, and at the end of a group their
+// sum, scaled.
+template <typename T, int MT, int NT, int PER>
+__device__ __forceinline__ void step(const Block<NT> &t, const Rows<T> (&rows)[MT], int j,
+                                     uint32_t lane, const uint32_t (&one)[2],
+                                     uint32_t (&group)[NT], phx_f4 (&sum)[NT][MT],
+                                     phx_f4 (&acc)[NT][MT]) {
+    constexpr int EACH = 4 / PER;  // of a group
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        if (j % EACH == 0) {
+            group[n] = (uint32_t)t.z[n] << 16 | t.s[n];
+            if (PER > 1)
+                group[n] = __builtin_amdgcn_ds_bpermute(
+                    (int)((lane & 15) + 16 * (j / EACH)) * 4, (int)group[n]);
+        }
+        const auto w = codes(t.w[n][j], (int)(group[n] >> 16), one, T());
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            sum[n][m] = product(rows[m], w, j % EACH ? sum[n][m] : (phx_f4){0, 0, 0, 0});
+            if (j % EACH == EACH - 1) {
+                const float s = (float)__builtin_bit_cast(_Float16, (uint16_t)group[n]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[n][m][i] = fmaf(s, sum[n][m][i], acc[n][m][i]);
+            }
+        }
+    }
+}
+
+// Stores a lane's four sums: column c, rows row .. row + 3; to C, or a part of a
+// split as it is.
+template <typename T>
+__device__ __forceinline__ void store(const PhxGemvW4 &p, phx_f4 sum, int64_t c, uint32_t row) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (c < p.N && row + i < p.M) {
+            if (p.splits > 1) {
+                ((PHX_GLOBAL float *)p.ws)[((int64_t)blockIdx.z * p.M + row + i) * p.N + c] = sum[i];
+                continue;
+            }
+            PHX_GLOBAL T *to = (PHX_GLOBAL T *)p.c + (row + i) * p.ldc + c;
+            float o = p.alpha * sum[i];
+            if (p.beta != 0.0f) o = o + p.beta * (float)*to;
+            *to = (T)o;
+        }
+}
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const PhxGemvW4 &p, size_t size) {
+    return __builtin_amdgcn_make_buffer_rsrc((void *)p.a, 0,
+                                             (int)(((p.M - 1) * p.lda + p.K) * size), 0x00020000);
+}
+
+// Up to 16 rows: a workgroup takes NT tiles of 16 columns, its waves the blocks
+// of K in turns, each with the rows it needs in its own part of LDS; they add up
+// at the end.
+template <typename T, int NT, int WAVES, int PER>
 __device__ __forceinline__ void gemv_w4(const PhxGemvW4 &p) {
-    __shared__ phx_f4 part[WAVES * MT * NT * 64];
+    using St = Staged<T>;
+    __shared__ phx_u4 lds[WAVES * St::BYTES / 16];
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint32_t r = lane & 15, quad = lane >> 4;
     const int64_t kb = (p.K + 127) / 128, n0 = (int64_t)blockIdx.x * (16 * NT);
-    const uint32_t one = in_vgpr(0x64006400);
-    const __amdgpu_buffer_rsrc_t a = __builtin_amdgcn_make_buffer_rsrc(
-        (void *)p.a, 0, (int)(((p.M - 1) * p.lda + p.K) * sizeof(T)), 0x00020000);
+    const uint32_t one[2] = {in_vgpr(0x64006400), in_vgpr(0x54005400)};
+    const __amdgpu_buffer_rsrc_t a = rows_of(p, sizeof(T));
+    char *own = (char *)lds + wave * St::BYTES;
+    phx_f4 acc[NT][1];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[n][0] = (phx_f4){0, 0, 0, 0};
+    Columns<NT, PER> columns;
+    columns.start(p, n0, kb, lane);
+    // rows and k that do not exist lie past the resource's end: zeros; loads of
+    // none but such rows are left out, and their part of LDS keeps its zeros
+    const uint32_t loads = ((uint32_t)p.M + St::ROWS - 1) / St::ROWS;
+    struct Share {
+        phx_u4 x[St::LOADS];
+    };
+    auto fetch = [&](Share &x, Block<NT> &t, uint32_t b) {
+        const uint32_t k = b * 128 + St::k(lane);
+#pragma unroll
+        for (uint32_t f = 0; f < St::LOADS; ++f)
+            if (f < loads) {
+                const uint32_t row = St::row(f, lane);
+                x.x[f] = __builtin_amdgcn_raw_buffer_load_b128(
+                    a, row < p.M && k < p.K ? (uint32_t)((row * p.lda + k) * sizeof(T)) : 0x80000000u,
+                    0, 0);
+            }
+        columns.fetch(p, t, b, lane);
+    };
+    auto multiply = [&](const Share &x, const Block<NT> &t) {
+#pragma unroll
+        for (uint32_t f = 0; f < St::LOADS; ++f)
+            if (f < loads) St::put(own, x.x[f], St::row(f, lane), lane);
+        uint32_t group[NT];
+        phx_f4 sum[NT][1];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const Rows<T> rows[1] = {St::get(own, j, lane)};
+            step<T, 1, NT, PER>(t, rows, j, lane, one, group, sum, acc);
+        }
+    };
+    Share x, x2;
+    Block<NT> t, t2;
+    const uint32_t first = __builtin_amdgcn_readfirstlane(wave), end = (uint32_t)kb;
+    if (first < end) fetch(x, t, first);
+    if (first + WAVES < end) fetch(x2, t2, first + WAVES);
+    for (uint32_t i = lane; i < St::BYTES / 16; i += 64) ((phx_u4 *)own)[i] = (phx_u4){0, 0, 0, 0};
+    for (uint32_t b = first; b < end; b += 2 * WAVES) {
+        multiply(x, t);
+        if (b + 2 * WAVES < end) fetch(x, t, b + 2 * WAVES);
+        if (b + WAVES < end) multiply(x2, t2);
+        if (b + 3 * WAVES < end) fetch(x2, t2, b + 3 * WAVES);
+    }
+    // a lane's four sums: column lane % 16, rows 4 (lane / 16) .. + 3
+    phx_f4 *part = (phx_f4 *)lds;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        __syncthreads();
+        part[wave * 64 + lane] = acc[n][0];
+        __syncthreads();
+        if (wave) continue;
+        phx_f4 sum = part[lane];
+#pragma unroll
+        for (int v = 1; v < WAVES; ++v) sum = sum + part[v * 64 + lane];
+        store<T>(p, sum, n0 + 16 * n + (lane & 15), lane / 16 * 4);
+    }
+}
+
+// More rows: a workgroup takes WN x NT tiles of columns and MT of rows, and its
+// WN x WK waves share the rows through LDS: WK blocks of K at a time, split into
+// their matrix terms once, each read by the WN waves of a block for NT tiles.
+// One barrier for every WK blocks: the next ones are loaded into registers
+// while these are multiplied, and written to the other half of LDS.
+template <typename T, int MT, int NT, int WN, int WK, int PER>
+__device__ __forceinline__ void gemm_w4(const PhxGemvW4 &p) {
+    using St = Staged<T>;
+    constexpr uint32_t EACH = MT * St::LOADS / WN;       // a wave's loads of its block
+    constexpr uint32_t STAGE = WK * MT * St::BYTES;
+    constexpr uint32_t SUMS = WK * WN * NT * MT * 1024;
+    __shared__ phx_u4 lds[(2 * STAGE > SUMS ? 2 * STAGE : SUMS) / 16];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t wn = __builtin_amdgcn_readfirstlane(wave % WN);
+    const uint32_t wk = __builtin_amdgcn_readfirstlane(wave / WN);
+    const int64_t kb = (p.K + 127) / 128, n0 = ((int64_t)blockIdx.x * WN + wn) * (16 * NT);
+    const uint32_t m0 = blockIdx.y * (16 * MT);
+    const uint32_t per = ((uint32_t)kb + p.splits - 1) / p.splits;
+    const uint32_t begin = blockIdx.z * per, end = min(begin + per, (uint32_t)kb);
+    const uint32_t one[2] = {in_vgpr(0x64006400), in_vgpr(0x54005400)};
+    const __amdgpu_buffer_rsrc_t a = rows_of(p, sizeof(T));
+    Columns<NT, PER> columns;
+    columns.start(p, n0, kb, lane);
+    phx_u4 x[EACH];
+    // a wave with no block left multiplies zero rows with the last block's codes
+    auto fetch = [&](Block<NT> &t, uint32_t b) {
+        const uint32_t k = b * 128 + St::k(lane);
+#pragma unroll
+        for (uint32_t e = 0; e < EACH; ++e) {
+            const uint32_t row = m0 + St::row(wn * EACH + e, lane);
+            x[e] = __builtin_amdgcn_raw_buffer_load_b128(
+                a, row < p.M && k < p.K && b < end ? (uint32_t)((row * p.lda + k) * sizeof(T))
+                                                   : 0x80000000u, 0, 0);
+        }
+        columns.fetch(p, t, min(b, (uint32_t)kb - 1), lane);
+    };
     phx_f4 acc[NT][MT];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int m = 0; m < MT; ++m) acc[n][m] = (phx_f4){0, 0, 0, 0};
-
-    struct Block {
-        phx_u4 w[NT];
-        _Float16 s[NT][PER];
-        int z[NT][PER];
-    };
-    auto fetch = [&](Block &t, int64_t b) {
+    Block<NT> t, next;
+    fetch(next, begin + wk);
+    for (uint32_t b = begin, half = 0; b < end; b += WK, half ^= 1) {
+        char *block = (char *)lds + half * STAGE + wk * (MT * St::BYTES);
+        t = next;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            // (columns past N read the last one's, and are not stored)
-            int64_t col = n0 + 16 * n + r;
-            if (col >= p.N) col = p.N - 1;
-            t.w[n] = *(const PHX_GLOBAL phx_u4 *)((const PHX_GLOBAL char *)p.w +
-                                                 ((col / 16 * kb + b) * 64 + quad * 16 + col % 16) * 16);
-#pragma unroll
-            for (int g = 0; g < PER; ++g) {
-                int64_t group = b * PER + g;
-                if (group >= p.groups) group = p.groups - 1;
-                t.s[n][g] = ((const PHX_GLOBAL _Float16 *)p.scales)[group * p.N + col];
-                t.z[n][g] = p.zeros ? ((const PHX_GLOBAL uint8_t *)p.zeros)[group * p.N + col] : 8;
-            }
+        for (uint32_t e = 0; e < EACH; ++e) {
+            const uint32_t row = St::row(wn * EACH + e, lane);
+            St::put(block + row / 16 * St::BYTES, x[e], row, lane);
         }
-    };
-    auto multiply = [&](const Block &t, int64_t b) {
+        __syncthreads();
+        if (b + WK < end) fetch(next, b + WK + wk);
+        uint32_t group[NT];
+        phx_f4 sum[NT][MT];
 #pragma unroll
-        for (int g = 0; g < PER; ++g) {
-            phx_f4 sum[NT][MT];
+        for (int j = 0; j < 4; ++j) {
+            Rows<T> rows[MT];
 #pragma unroll
-            for (int j = g * (4 / PER); j < (g + 1) * (4 / PER); ++j) {
-                const uint32_t k = (uint32_t)b * 128 + 32 * j + 8 * quad;
-                Rows<T> x[MT];
-#pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    const uint32_t row = 16 * m + r;
-                    // past the resource's end: zeros
-                    load(x[m], a, row < p.M && k < p.K ? (uint32_t)((row * p.lda + k) * sizeof(T))
-                                                       : 0x80000000u);
-                }
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const auto w = codes(t.w[n][j], t.z[n][g], one, T());
-#pragma unroll
-                    for (int m = 0; m < MT; ++m)
-                        sum[n][m] = product(x[m], w, j == g * (4 / PER) ? (phx_f4){0, 0, 0, 0}
-                                                                        : sum[n][m]);
-                }
-            }
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int m = 0; m < MT; ++m)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        acc[n][m][i] = fmaf((float)t.s[n][g], sum[n][m][i], acc[n][m][i]);
+            for (int m = 0; m < MT; ++m) rows[m] = St::get(block + m * St::BYTES, j, lane);
+            step<T, MT, NT, PER>(t, rows, j, lane, one, group, sum, acc);
         }
-    };
-    Block t, t2;
-    const int64_t first = __builtin_amdgcn_readfirstlane(wave);
-    if (first < kb) fetch(t, first);
-    if (first + WAVES < kb) fetch(t2, first + WAVES);
-    for (int64_t b = first; b < kb; b += 2 * WAVES) {
-        multiply(t, b);
-        if (b + 2 * WAVES < kb) fetch(t, b + 2 * WAVES);
-        if (b + WAVES < kb) multiply(t2, b + WAVES);
-        if (b + 3 * WAVES < kb) fetch(t2, b + 3 * WAVES);
     }
+    __syncthreads();
+    phx_f4 *part = (phx_f4 *)lds;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int m = 0; m < MT; ++m) part[((wave * NT + n) * MT + m) * 64 + lane] = acc[n][m];
+        for (int m = 0; m < MT; ++m)
+            part[(((wk * WN + wn) * NT + n) * MT + m) * 64 + lane] = acc[n][m];
     __syncthreads();
-    // a lane's four sums: column r, rows 4 quad .. 4 quad + 3 of the tile
-    for (uint32_t x = threadIdx.x; x < NT * MT * 64; x += 64 * WAVES) {
-        phx_f4 sum = part[x];
+    constexpr uint32_t EVERY = WN * NT * MT * 64;
+    for (uint32_t i = threadIdx.x; i < EVERY; i += 64 * WN * WK) {
+        phx_f4 sum = part[i];
 #pragma unroll
-        for (int w = 1; w < WAVES; ++w) sum = sum + part[w * (NT * MT * 64) + x];
-        const int64_t col = n0 + x / (MT * 64) * 16 + (x & 15);
-        const uint32_t row = x / 64 % MT * 16 + (x >> 4 & 3) * 4;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (col < p.N && row + i < p.M) {
-                PHX_GLOBAL T *c = (PHX_GLOBAL T *)p.c + (row + i) * p.ldc + col;
-                float o = p.alpha * sum[i];
-                if (p.beta != 0.0f) o = o + p.beta * (float)*c;
-                *c = (T)o;
-            }
+        for (int v = 1; v < WK; ++v) sum = sum + part[v * EVERY + i];
+        const uint32_t m = i / 64 % MT, tile = i / (64 * MT);
+        store<T>(p, sum, ((int64_t)blockIdx.x * (WN * NT) + tile) * 16 + (i & 15),
+                 m0 + 16 * m + (i >> 4 & 3) * 4);
     }
 }
 
 }  // namespace
 
-#define GEMV(T, suffix, MT, NT, WAVES, PER)                                                     \
+#define GEMV(T, suffix, NT, WAVES, PER)                                                         \
     extern "C" __global__ __launch_bounds__(64 * WAVES) void                                    \
-        gemv_w4_##suffix##_m##MT##_n##NT##_g##PER(PhxGemvW4 p) {                                \
-        gemv_w4<T, MT, NT, WAVES, PER>(p);                                                      \
+        gemv_w4_##suffix##_n##NT##_w##WAVES##_g##PER(PhxGemvW4 p) {                             \
+        gemv_w4<T, NT, WAVES, PER>(p);                                                          \
     }
-#define GROUPS(T, suffix, MT, NT, WAVES)                                                        \
-    GEMV(T, suffix, MT, NT, WAVES, 1)                                                           \
-    GEMV(T, suffix, MT, NT, WAVES, 2)                                                           \
-    GEMV(T, suffix, MT, NT, WAVES, 4)
-GROUPS(_Float16, f16, 1, 1, 8)
-GROUPS(_Float16, f16, 2, 1, 8)
-GROUPS(_Float16, f16, 4, 1, 8)
-GROUPS(float, f32, 1, 1, 8)
-GROUPS(float, f32, 2, 1, 8)
-GROUPS(float, f32, 4, 1, 8)
+#define GROUPS(T, suffix, NT, WAVES)                                                            \
+    GEMV(T, suffix, NT, WAVES, 1)                                                               \
+    GEMV(T, suffix, NT, WAVES, 2)                                                               \
+    GEMV(T, suffix, NT, WAVES, 4)
+#define GEMM(T, suffix, MT, NT, WN, WK, PER)                                                    \
+    extern "C" __global__ __launch_bounds__(64 * WN * WK) void                                  \
+        gemm_w4_##suffix##_m##MT##_n##NT##_##WN##x##WK##_g##PER(PhxGemvW4 p) {                  \
+        gemm_w4<T, MT, NT, WN, WK, PER>(p);                                                     \
+    }
+#define GEMM_GROUPS(T, suffix, MT, NT, WN, WK)                                                  \
+    GEMM(T, suffix, MT, NT, WN, WK, 1)                                                          \
+    GEMM(T, suffix, MT, NT, WN, WK, 2)                                                          \
+    GEMM(T, suffix, MT, NT, WN, WK, 4)
+GROUPS(_Float16, f16, 1, 8)
+GROUPS(_Float16, f16, 1, 16)
+GROUPS(_Float16, f16, 4, 8)
+GROUPS(float, f32, 1, 8)
+GROUPS(float, f32, 4, 8)
+GEMM_GROUPS(_Float16, f16, 2, 2, 2, 4)
+GEMM_GROUPS(_Float16, f16, 2, 1, 1, 8)
+GEMM_GROUPS(float, f32, 2, 2, 4, 2)
+GEMM_GROUPS(float, f32, 2, 1, 4, 2)
+
+// C from the parts of a split, in order.
+template <typename T>
+__device__ __forceinline__ void reduce(const PhxGemvW4 &p) {
+    const int64_t plane = p.M * p.N;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < plane;
+         i += (int64_t)gridDim.x * 256) {
+        const PHX_GLOBAL float *part = (const PHX_GLOBAL float *)p.ws + i;
+        float sum = part[0];
+        for (int v = 1; v < p.splits; ++v) sum += part[v * plane];
+        PHX_GLOBAL T *to = (PHX_GLOBAL T *)p.c + i / p.N * p.ldc + i % p.N;
+        float o = p.alpha * sum;
+        if (p.beta != 0.0f) o = o + p.beta * (float)*to;
+        *to = (T)o;
+    }
+}
+extern "C" __global__ __launch_bounds__(256) void gemm_w4_reduce_f16(PhxGemvW4 p) {
+    reduce<_Float16>(p);
+}
+extern "C" __global__ __launch_bounds__(256) void gemm_w4_reduce_f32(PhxGemvW4 p) {
+    reduce<float>(p);
+}

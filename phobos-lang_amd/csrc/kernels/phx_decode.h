@@ -11,6 +11,8 @@ struct PhxGemvW4 {
     uint64_t a, w, scales, zeros, c;
     int64_t M, N, K, lda, ldc, groups;
     float alpha, beta;
+    uint64_t ws;
+    int32_t splits;
 };
 
 // A kv4 call: the cache, its sequences, and the tensors of their rows.

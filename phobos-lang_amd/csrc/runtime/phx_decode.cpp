@@ -35,6 +35,63 @@ int64_t size_of(phx_dtype t) { return t == PHX_F16 ? 2 : 4; }
 constexpr int64_t kMost = INT64_C(1) << 40;  // of any extent: products of two stay in 64 bits
 bool extent(int64_t v) { return v >= 0 && v <= INT32_MAX; }
 
+// ------------------------------------------------------------------ 4-bit weights
+// A kernel of gemv_w4.hip: the columns and rows of a workgroup, and the blocks
+// of 128 k it takes at a time, in so many nanoseconds (measured; more than 16
+// rows).
+struct W4Form {
+    int64_t columns, rows;
+    uint32_t threads;
+    int64_t blocks, ns;
+    const char *entry[3];  // groups of 128, 64 and 32
+};
+#define GROUPS(name) {name "_g1", name "_g2", name "_g4"}
+const W4Form kW4F16[] = {{16, 16, 512, 8, 0, GROUPS("gemv_w4_f16_n1_w8")},
+                         {16, 16, 1024, 16, 0, GROUPS("gemv_w4_f16_n1_w16")},
+                         {64, 16, 512, 8, 0, GROUPS("gemv_w4_f16_n4_w8")},
+                         {64, 32, 512, 4, 1130, GROUPS("gemm_w4_f16_m2_n2_2x4")},
+                         {16, 32, 512, 8, 1350, GROUPS("gemm_w4_f16_m2_n1_1x8")}};
+const W4Form kW4F32[] = {{16, 16, 512, 8, 0, GROUPS("gemv_w4_f32_n1_w8")},
+                         {64, 16, 512, 8, 0, GROUPS("gemv_w4_f32_n4_w8")},
+                         {128, 32, 512, 2, 2250, GROUPS("gemm_w4_f32_m2_n2_4x2")},
+                         {64, 32, 512, 2, 1600, GROUPS("gemm_w4_f32_m2_n1_4x2")}};
+#undef GROUPS
+
+// The kernel for a product, and the K chunks it runs in, at most `most`.
+//   Up to 16 rows: 16 columns a workgroup while the CUs are not all several
+// times occupied, in f16 with 16 waves over long K (4096 x 16384: 9.3 us against
+// 10.6 with 8), else 64 columns (16 rows, 16384 x 8192: f16 19.9 us against 22.0,
+// f32 33.8 against 66.0).
+//   More: the one that is estimated fastest: its rounds of workgroups on the
+// CUs, each K chunk's blocks; a split in 2 or 4 chunks costs its reduction
+// (f16, 32 x 4096 x 16384: 18.1 us in 4, 23.5 in none of the other form).
+const W4Form &w4_form(phx_dtype t, int64_t M, int64_t N, int64_t K, int64_t most,
+                      int64_t *splits) {
+    const W4Form *forms = t == PHX_F16 ? kW4F16 : kW4F32;
+    const int64_t tiles = (N + 15) / 16;
+    *splits = 1;
+    if (M <= 16) {
+        if (t == PHX_F32) return forms[tiles > 512];
+        return forms[tiles >= 1024 ? 2 : tiles <= 256 && K >= 8192 ? 1 : 0];
+    }
+    const W4Form *best = nullptr;
+    int64_t least = 0;
+    for (const W4Form *f = forms + (t == PHX_F16 ? 3 : 2), *e = f + 2; f != e; ++f)
+        for (int64_t sp = 1; sp <= 4 && sp <= std::max<int64_t>(most, 1); sp *= 2) {
+            const int64_t groups = ((N + f->columns - 1) / f->columns) *
+                                   ((M + f->rows - 1) / f->rows) * sp;
+            const int64_t blocks = ((K + 127) / 128 + sp - 1) / sp;
+            int64_t ns = (groups + 255) / 256 * ((blocks + f->blocks - 1) / f->blocks) * f->ns;
+            if (sp > 1) ns += 3300 + (sp + 1) * M * N / 1000;
+            if (!best || ns < least) {
+                best = f;
+                least = ns;
+                *splits = sp;
+            }
+        }
+    return *best;
+}
+
 // ------------------------------------------------------------------ 4-bit cache
 int check_cache(const phx_kv4_cache *c, const char *who) {
     if (!c) return set_error(PHX_E_INVALID, "%s: null cache", who);
@@ -185,15 +242,22 @@ int phx_gemv_w4(phx_stream s, phx_dtype t, uint64_t a, uint64_t w, uint64_t scal
                          "gemv_w4: A and the codes must be 16-byte aligned, scales and C by element");
     if (int rc = on_device((hipStream_t)s)) return rc;
     if (M == 0) return PHX_OK;
-    PhxGemvW4 p = {a, w, scales, zeros, c, M, N, K, lda, ldc, (K + group - 1) / group, alpha, beta};
-#define GROUPS(form) {"gemv_w4_" form "_g1", "gemv_w4_" form "_g2", "gemv_w4_" form "_g4"}
-    static const char *const entries[2][3][3] = {
-        {GROUPS("f32_m1_n1"), GROUPS("f32_m2_n1"), GROUPS("f32_m4_n1")},
-        {GROUPS("f16_m1_n1"), GROUPS("f16_m2_n1"), GROUPS("f16_m4_n1")}};
-#undef GROUPS
-    const char *entry = entries[t == PHX_F16][M <= 16 ? 0 : M <= 32 ? 1 : 2]
-                               [group == 128 ? 0 : group == 64 ? 1 : 2];
-    return launch(kW4File, entry, dim3((uint32_t)((N + 15) / 16)), 512, (hipStream_t)s, &p);
+    PhxGemvW4 p = {a,   w,   scales, zeros, c,    M, N, K, lda, ldc, (K + group - 1) / group,
+                   alpha, beta, 0, 1};
+    int64_t splits = 1;
+    size_t room = 0;
+    if (int rc = phx_stream_get_workspace(s, &p.ws, &room)) return rc;
+    const W4Form &f = w4_form(t, M, N, K, (int64_t)(room / sizeof(float)) / (M * N), &splits);
+    p.splits = (int32_t)splits;
+    if (int rc = launch(kW4File, f.entry[group == 128 ? 0 : group == 64 ? 1 : 2],
+                        dim3((uint32_t)((N + f.columns - 1) / f.columns),
+                             (uint32_t)((M + f.rows - 1) / f.rows), (uint32_t)splits),
+                        f.threads, (hipStream_t)s, &p))
+        return rc;
+    if (splits == 1) return PHX_OK;
+    return launch(kW4File, t == PHX_F16 ? "gemm_w4_reduce_f16" : "gemm_w4_reduce_f32",
+                  dim3((uint32_t)std::min<int64_t>((M * N + 255) / 256, 2048)), 256, (hipStream_t)s,
+                  &p);
 }
 
 // ------------------------------------------------------------------ 4-bit cache

@@ -6,6 +6,8 @@ the output."""
 import numpy as np
 import pytest
 
+from hip_graph import Graph
+
 pytestmark = pytest.mark.gpu
 
 GUARD = 64  # elements around every output
@@ -180,3 +182,68 @@ def test_quantised_weights_stand_for_the_weights(px_gpu, stream):
     a = a.astype(np.float64)
     assert (np.abs(got - a @ w) <= _bound(a @ w, np.abs(a) @ np.abs(w), 200, np.float16)).all()
     assert np.abs(w - b).max() <= scales.astype(np.float64).max() * (1 + 15 * 2.0 ** -11)
+
+
+# M at the edges of the row tiles; K that splits in 2 and in 4 chunks, the last
+# of them short
+SPLIT = [(17, 1000, 4136), (32, 33, 2056), (33, 1000, 4136), (48, 65, 1160), (64, 2500, 2048),
+         (64, 16, 16384), (24, 130, 9000)]
+
+
+@pytest.mark.parametrize("M,N,K", SPLIT)
+@pytest.mark.parametrize("bits", [16, 32])
+@pytest.mark.parametrize("parts", [0, 1.9, 2, 3.9, 4, 9])
+def test_split_over_k(px_gpu, bits, M, N, K, parts):
+    # a workspace of so many parts: what lies behind it has to stay
+    px = px_gpu
+    rng = np.random.default_rng(M + N + K)
+    dtype = px.F16 if bits == 16 else px.F32
+    t = _np(px, dtype)
+    codes = rng.integers(0, 16, (K, N)).astype(np.uint8)
+    scales = (rng.random((-(-K // 64), N)) * 0.01).astype(np.float16)
+    a, c = rng.standard_normal((M, K)).astype(t), rng.standard_normal((M, N)).astype(t)
+    w = _weights(codes, scales, None, 64)
+    want = 0.5 * (a.astype(np.float64) @ w) + c
+    mag = np.abs(a.astype(np.float64)) @ np.abs(w)
+    room = int(parts * M * N) * 4
+    ws = px.DeviceBuffer.from_array(np.full(room + 4096, 0xAB, np.uint8))
+    s = px.Stream()
+    if room:
+        px.set_workspace(s, ws.ptr, room)
+    got = _run(px, s, dtype, a, codes, scales, None, 64, 0.5, 1.0, c)
+    px.set_workspace(s, 0, 0)
+    s.destroy()
+    assert (np.abs(got - want) <= _bound(want, mag, K, t, 0.5, np.abs(c))).all()
+    assert (ws.download(np.uint8, room + 4096)[room:] == 0xAB).all()
+
+
+def test_captured_and_replayed(px_gpu):
+    px = px_gpu
+    rng = np.random.default_rng(2)
+    M, N, K = 40, 600, 4136
+    codes = rng.integers(0, 16, (K, N)).astype(np.uint8)
+    scales = (rng.random((-(-K // 32), N)) * 0.01).astype(np.float16)
+    s = px.Stream()
+    px.bind_workspace(s, 16 * M * N)
+    w, ds = _pack(px, s, codes), px.DeviceBuffer.from_array(scales)
+    da, dc = px.DeviceBuffer(2 * M * K), px.DeviceBuffer(2 * M * N)
+
+    def step(m):
+        px.launch_gemv_w4(s, px.F16, da, w, ds, 0, dc, m, N, K, 32)
+    step(M)
+    s.synchronize()
+    graphs = [Graph(s, lambda: step(M)), Graph(s, lambda: step(20))]
+    for _ in range(4):
+        da.upload(rng.standard_normal((M, K)).astype(np.float16))
+        for g, m in zip(graphs, (M, 20)):
+            step(m)
+            s.synchronize()
+            want = dc.download(np.float16, (m, N)).copy()
+            dc.upload(np.full((M, N), 9, np.float16))
+            g.replay()
+            s.synchronize()
+            assert np.array_equal(dc.download(np.float16, (M, N))[:m], want)
+    for g in graphs:
+        g.destroy()
+    px.bind_workspace(s, 0)
+    s.destroy()
