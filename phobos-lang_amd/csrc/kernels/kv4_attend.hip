@@ -121,6 +121,17 @@ __device__ __forceinline__ void load_v(phx_u4 *to, const PHX_GLOBAL char *head, 
     for (int t = 0; t < 2; ++t) to[t] = fetch<phx_u4>(head + (P + slot) * (D / 2), off + t * 8 * D);
 }
 
+// Eight codes of a key as f16: 16 and the code behind it, and for queries of two
+// terms 24 less, the middle.  (Sums of 16 + c from -24 sum_d q_d on pass through
+// several times their result: f32 outputs were 2.4e-6 off, 0.6e-6 without.  For f16
+// queries, whose outputs round at 2^-11, that saves the subtraction.)
+template <int TERMS>
+__device__ __forceinline__ phx_h8 keys(uint32_t w, uint32_t mask, uint32_t one) {
+    const phx_h8 k = h8((w << 6 & mask) | one, (w << 2 & mask) | one, (w >> 2 & mask) | one,
+                        (w >> 6 & mask) | one);
+    return TERMS == 2 ? k - (_Float16)24 : k;
+}
+
 // The columns' queries as matrix operands, and what turns a product into a
 // score in log2 units: t = s_j S a + (m_j + 8 s_j) b, S being the product with
 // c_j - 8, as it starts at c: with a code's own size 0 .. 15 the
@@ -173,7 +184,7 @@ __device__ __forceinline__ void load_query(Query<D, TERMS> &r, const PhxKv4 &p, 
             if constexpr (TERMS == 2) r.q[1][j][u] = (_Float16)(v - (float)hi);
         }
     r.a = ldexpf(p.scale * KV4_LOG2E, e - 9);
-    r.c = -24.0f * ldexpf(sum, 9 - e);
+    r.c = TERMS == 2 ? 0.0f : -24.0f * ldexpf(sum, 9 - e);
     // a row with an infinity has no scores, as its weights would be inf / inf
     r.b = top < INFINITY ? sum * (p.scale * KV4_LOG2E) : NAN;
 }
@@ -228,10 +239,8 @@ __device__ __forceinline__ void scores(const Raw<D, G> &r, const Query<D, TERMS>
     for (int j = 0; j < D / 32; ++j)
 #pragma unroll
         for (int t = 0; t < Sh::TILES; ++t) {
-            // 16 and the code behind it
             const uint32_t w = r.k[t][j];
-            const phx_h8 k = h8((w << 6 & mask) | one, (w << 2 & mask) | one, (w >> 2 & mask) | one,
-                                (w >> 6 & mask) | one);
+            const phx_h8 k = keys<TERMS>(w, mask, one);
 #pragma unroll
             for (int x = 0; x < TERMS; ++x)
                 if constexpr (G == 1) {
@@ -247,9 +256,8 @@ __device__ __forceinline__ void scores(const Raw<D, G> &r, const Query<D, TERMS>
 
 // The weights p_j s_j of a step's scores, in two f16 terms (22 bits): pairs of
 // halves, the f16 of the exact product and of what that leaves.  Keys past what
-// a column sees, or in a unit without a page (a bit of `absent`), get zeros
-// (without MASK there are none such).
-template <int D, int TERMS, int NC, int G, bool MASK>
+// a column sees, or in a unit without a page (a bit of `absent`), get zeros.
+template <int D, int TERMS, int NC, int G>
 __device__ __forceinline__ void weights(const Raw<D, G> &r, const Query<D, TERMS> (&q)[NC],
                                         State<D> (&st)[NC], const Lane<D, G> &ln,
                                         const phx_f4 (&s)[NC][Shape<G>::SETS],
@@ -275,7 +283,7 @@ __device__ __forceinline__ void weights(const Raw<D, G> &r, const Query<D, TERMS
         // the score in log2 units, less m
         auto score = [&](int u, float m) {
             const float x = fmaf((float)half_of(r.kp[u / 4][u % 4], 0), e[u], fmaf(km[u], q[c].b, -m));
-            return !MASK || 16 * (u / 4) + u % 4 < left ? x : -INFINITY;
+            return 16 * (u / 4) + u % 4 < left ? x : -INFINITY;
         };
         // The reference m is of score + log2 s_V, and stays while no weight
         // passes 40000: rarely raised after the first step, and then to 2^7
@@ -526,7 +534,7 @@ __device__ __forceinline__ void attend(const PhxKv4 &p) {
             uint32_t hi[NC][2 * Sh::SETS], lo[NC][2 * Sh::SETS];
             scores<D, TERMS, NC, G>(r, q, ln, x);
             if (i + 1 < n) next_k(i + 1);
-            weights<D, TERMS, NC, G, true>(r, q, st, ln, x, hi, lo, at * KEYS, absent, fresh);
+            weights<D, TERMS, NC, G>(r, q, st, ln, x, hi, lo, at * KEYS, absent, fresh);
             fresh = false;
             if (i + 1 < n) next_p(i + 1);
             sums<D, NC, G>(r, st, ln, hi, lo);
@@ -601,6 +609,297 @@ __device__ __forceinline__ void attend(const PhxKv4 &p) {
     }
 }
 
+// Many columns, as of a prompt's chunk: the work on a key that every column
+// repeats, its codes to f16 and its parameters to f32, is done once for a
+// workgroup's 128 columns and shared through LDS. Four waves take 32 columns
+// each and all of the keys, KEYS at a time; the next ones are loaded while these
+// are multiplied, and LDS has two halves, so that there is one barrier in
+// between. Bound by the vector instructions: for 32 keys and 32 columns about 220
+// of a wave, 110 of them the softmax, next to 48 matrix instructions (2 x 1000
+// rows over 4133 keys, 8 x 4 heads of 128: 211 us, 565 TFLOP/s of the products
+// without the weights' second term; a wave unpacking for its own 64 columns
+// alone 425).
+template <int D>
+struct Chunk {
+    static constexpr int KEYS = 8192 / D;     // 16 KiB of f16 each for K and V
+    static constexpr int UNITS = KEYS / 32;
+    // K: chunk c of eight elements of key r of tile t at (t D/8 + c) 256 +
+    // 16 (r ^ c): reads and writes of 16 lanes touch every bank once (D 64: writes
+    // twice).  V: the operand of 16 rows of elements for 32 keys as a wave
+    // reads it.
+    phx_h8 k[KEYS * D / 8], v[KEYS * D / 8];
+    float par[4][KEYS];  // scale and middle of K, of V
+};
+
+template <typename T, int D>
+__device__ __forceinline__ void chunk(const PhxKv4 &p) {
+    using Ch = Chunk<D>;
+    constexpr int TERMS = sizeof(T) == 4 ? 2 : 1, NC = 2, COLS = 64 * NC;
+    constexpr int UNROLL = sizeof(T) == 4 ? 1 : 2;  // as many as fit the registers
+    constexpr uint32_t KEYS = Ch::KEYS, UNITS = Ch::UNITS, PER = 64 / UNITS;
+    __shared__ Ch lds[2];
+    const uint32_t lane = threadIdx.x & 63, quad = lane >> 4;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // column groups of one KV head next to each other on one XCD, in turns the
+    // longest rows first and last, so that two on a CU differ
+    const uint32_t groups = p.groups;
+    uint32_t item = phx_xcd_swizzle_any(phx_block_linear(), phx_block_count());
+    uint32_t cg = item % groups;
+    item /= groups;
+    if (item % 2 == 0) cg = groups - 1 - cg;
+    const uint32_t head = item % p.heads, b = item / p.heads;
+    const Seq s = kv4_seq(p, b);
+    const uint32_t ratio = p.ratio, col0 = cg * COLS + wave * (16 * NC);
+    if (cg * COLS / ratio >= s.count) return;
+    int64_t last = (cg * COLS + COLS - 1) / ratio;
+    if (last >= s.count) last = s.count - 1;
+    // keys that some column sees, and that all of the wave's columns see
+    int64_t most = p.causal ? s.tokens - s.count + last + 1 : s.tokens;
+    int64_t least = p.causal ? s.tokens - s.count + col0 / ratio + 1 : s.tokens;
+    if (most < 0) most = 0;
+    if (least < 0) least = 0;
+    const uint32_t steps = (uint32_t)(most + KEYS - 1) / KEYS;
+    const uint32_t seen = (uint32_t)least / KEYS;
+    const uint32_t units = (uint32_t)(most + 31) / 32;
+    const uint32_t P = p.page_tokens, shift = __builtin_ctz(P / 32);
+    const PHX_GLOBAL int32_t *table =
+        (const PHX_GLOBAL int32_t *)p.table + b * p.table_stride;
+    // the lanes hold the pages of PER steps from `base` on
+    int32_t ids;
+    uint32_t base;
+    auto pages = [&](uint32_t from) {
+        base = from;
+        ids = -1;
+        const uint32_t mine = base * UNITS + lane;
+        if (mine < units) ids = table[mine >> shift];
+        if (ids >= p.pages) ids = -1;
+    };
+    // the wave's share of a step, all of one unit: 16 bytes of K and of V a
+    // lane, and the parameters of 64 / UNITS ... keys
+    const uint32_t unit = wave * UNITS / 4;
+    const uint32_t own = threadIdx.x % (256 / UNITS);  // in the unit
+    constexpr uint32_t PARAMS = KEYS / 4;              // keys of a wave's parameters
+    phx_u4 raw_k, raw_v;
+    uint32_t raw_p;
+    auto fetch_step = [&](uint32_t i) {
+        const int id = __builtin_amdgcn_readlane(ids, (i - base) * UNITS + unit);
+        const uint32_t slot = ((i * UNITS + unit) & ((1u << shift) - 1)) * 32;
+        const PHX_GLOBAL char *part = kv4_head<D>(p, id < 0 ? 0 : id, head);
+        raw_k = fetch<phx_u4>(part + slot * (D / 2), own * 16);
+        raw_v = fetch<phx_u4>(part + (P + slot) * (D / 2), own * 16);
+        if (lane < 2 * PARAMS)
+            raw_p = fetch<uint32_t>(part, P * D + (lane < PARAMS ? 0 : 4 * P) +
+                                              4 * (slot + wave * PARAMS % 32 + lane % PARAMS));
+    };
+    auto stage = [&](Ch &to) {
+        const uint32_t mask = in_sgpr(0x03c003c0), one = in_vgpr(0x4c004c00);
+        constexpr uint32_t LANES = D / 32;  // of a key
+        const uint32_t key = threadIdx.x / LANES, r = key & 15;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            const uint32_t w = raw_k[i], c = threadIdx.x % LANES * 4 + i;
+            to.k[(key / 16 * (D / 8) + c) * 16 + ((r ^ c) & 15)] =
+                keys<TERMS>(w, mask, one);
+        }
+        // four keys' dwords of octet e: halves of the operands' 16 bytes
+        const uint32_t low[2] = {in_sgpr(0x000f000f), in_sgpr(0x00f000f0)};
+        const uint32_t bits[2] = {in_vgpr(0x64006400), in_vgpr(0x54005400)};
+        const uint32_t four = threadIdx.x / (D / 8), e = threadIdx.x % (D / 8);
+        phx_u2 *dst = (phx_u2 *)to.v + ((four / 8 * (D / 16)) * 64 + four % 4 * 16 + e) * 2 + four / 4 % 2;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+            const uint32_t sel = 0x0c040c00 + x / 2 * 0x00010001;
+            const uint32_t a = __builtin_amdgcn_perm(raw_v.y, raw_v.x, sel);
+            const uint32_t c = __builtin_amdgcn_perm(raw_v.w, raw_v.z, sel);
+            typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+            const h4 v = __builtin_bit_cast(h4, (phx_u2){(a & low[x % 2]) | bits[x % 2],
+                                                         (c & low[x % 2]) | bits[x % 2]}) -
+                         (_Float16)(x % 2 ? 72 : 1032);
+            dst[D == 128 ? x * 128 : (x % 4 * 64 + x / 4 * 8) * 2] = __builtin_bit_cast(phx_u2, v);
+        }
+        if (lane < 2 * PARAMS) {
+            const bool values = lane >= PARAMS;
+            const uint32_t w = values ? positive(raw_p) : raw_p;
+            const uint32_t key = wave * PARAMS + lane % PARAMS;
+            to.par[values ? 2 : 0][key] = (float)half_of(w, 0);
+            to.par[values ? 3 : 1][key] = middle(w);
+        }
+    };
+    pages(0);
+    if (steps > 0) fetch_step(0);
+
+    Query<D, TERMS> q[NC];
+    State<D> st[NC];
+    phx_f4 zero[NC];
+    bool none[NC];  // the column sees keys, but none so far
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        load_query<T, D, TERMS>(q[c], p, s, head, col0 + c * 16 + (lane & 15), quad);
+        zero[c] = (phx_f4){q[c].c, q[c].c, q[c].c, q[c].c};
+        none[c] = q[c].limit > 0;
+        st[c].m = st[c].l = st[c].pm = 0.0f;
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) st[c].o[j] = (phx_f4){0, 0, 0, 0};
+    }
+    for (uint32_t at = 0; at < steps; ++at) {
+        Ch &now = lds[at % 2];
+        uint32_t absent = 0;  // units without a page
+#pragma unroll
+        for (uint32_t u = 0; u < UNITS; ++u)
+            absent |= (__builtin_amdgcn_readlane(ids, (at - base) * UNITS + u) < 0 ? 1u : 0u) << u;
+        stage(now);
+        __syncthreads();
+        if (at + 1 < steps) {
+            if (at + 1 - base == PER) pages(at + 1);
+            fetch_step(at + 1);
+        }
+#pragma unroll UNROLL
+        for (uint32_t n = 0; n < UNITS; ++n) {
+            // a lane's scores: columns 16 c + lane % 16, keys 16 t + 4 quad + i
+            phx_f4 x[NC][2], ks[2], km[2], vs[2], vm[2];
+#pragma unroll
+            for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const uint32_t o = quad * (D / 32) + j;
+                    const phx_h8 k = now.k[((2 * n + t) * (D / 8) + o) * 16 + ((lane ^ o) & 15)];
+#pragma unroll
+                    for (int y = 0; y < TERMS; ++y)
+#pragma unroll
+                        for (int c = 0; c < NC; ++c)
+                            x[c][t] = mfma(k, q[c].q[y][j], j || y ? x[c][t] : zero[c]);
+                }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const uint32_t key = n * 32 + t * 16 + quad * 4;
+                ks[t] = *(const phx_f4 *)&now.par[0][key];
+                km[t] = *(const phx_f4 *)&now.par[1][key];
+                vs[t] = *(const phx_f4 *)&now.par[2][key];
+                vm[t] = *(const phx_f4 *)&now.par[3][key];
+            }
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+                    x[c][u / 4][u % 4] = fmaf(ks[u / 4][u % 4], x[c][u / 4][u % 4] * q[c].a,
+                                              fmaf(km[u / 4][u % 4], q[c].b, -st[c].m));
+            if (at >= seen || absent) {
+                const int32_t key0 = (int32_t)(at * KEYS + n * 32 + quad * 4);
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    const int32_t left = absent >> n & 1 ? 0 : q[c].limit - key0;
+#pragma unroll
+                    for (int u = 0; u < 8; ++u)
+                        x[c][u / 4][u % 4] =
+                            16 * (u / 4) + u % 4 < left ? x[c][u / 4][u % 4] : -INFINITY;
+                }
+            }
+            // as weights() has it, with the scores kept less m
+            __builtin_amdgcn_s_setprio(1);  // before the products of the wave next to it
+            uint32_t hi[NC][4], lo[NC][4];
+            float sum[NC], pm[NC], need[NC];
+            auto weigh = [&]() {
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    phx_h2 h, l, top = {(_Float16)0.0f, (_Float16)0.0f};
+                    sum[c] = pm[c] = 0.0f;
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) {
+                        const float pr = __builtin_amdgcn_exp2f(x[c][u / 4][u % 4]);
+                        const float sv = vs[u / 4][u % 4];
+                        sum[c] += pr;
+                        pm[c] = fmaf(pr, vm[u / 4][u % 4], pm[c]);
+                        h[u % 2] = (_Float16)fmaf(pr, sv, 0.0f);
+                        l[u % 2] = (_Float16)fmaf(pr, sv, -(float)h[u % 2]);
+                        if (u % 2) {
+                            top = __builtin_elementwise_max(top, h);
+                            hi[c][u / 2] = __builtin_bit_cast(uint32_t, h);
+                            lo[c][u / 2] = __builtin_bit_cast(uint32_t, l);
+                        }
+                    }
+                    need[c] = none[c] ? INFINITY : fmaxf((float)top.x, (float)top.y);
+                }
+            };
+            weigh();
+            bool raise = false;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) raise |= need[c] > 40000.0f;
+            if (__any(raise)) {
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    float most = -INFINITY;
+#pragma unroll
+                    for (int u = 0; u < 8; ++u)
+                        most = fmaxf(most,
+                                     x[c][u / 4][u % 4] + __builtin_amdgcn_logf(vs[u / 4][u % 4]));
+                    most = fmaxf(most, __shfl_xor(most, 16));
+                    most = fmaxf(most, __shfl_xor(most, 32));
+                    need[c] = fmaxf(need[c], __shfl_xor(need[c], 16));
+                    need[c] = fmaxf(need[c], __shfl_xor(need[c], 32));
+                    if (need[c] > 40000.0f && most > (none[c] ? -INFINITY : 7.0f)) {
+                        const float up = most - 7.0f;
+                        const float f = none[c] ? 0.0f : __builtin_amdgcn_exp2f(-up);
+                        none[c] = false;
+                        st[c].m += up;
+                        st[c].l *= f;
+                        st[c].pm *= f;
+#pragma unroll
+                        for (int j = 0; j < D / 16; ++j) st[c].o[j] = st[c].o[j] * f;
+#pragma unroll
+                        for (int t = 0; t < 2; ++t) x[c][t] = x[c][t] - up;
+                    }
+                }
+                weigh();
+            }
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                st[c].l += sum[c];
+                st[c].pm += pm[c];
+            }
+            __builtin_amdgcn_s_setprio(0);
+            const phx_h8 *v = now.v + n * (D / 16) * 64 + lane;
+#pragma unroll
+            for (int j = 0; j < D / 16; j += 2) {
+                // a sum's two products apart, as the second waits for the first
+                const phx_h8 w[2] = {v[j * 64], v[(j + 1) * 64]};
+#pragma unroll
+                for (int y = 0; y < 2; ++y)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int c = 0; c < NC; ++c) {
+                            const uint32_t(&r)[4] = y ? lo[c] : hi[c];
+                            st[c].o[j + k] = mfma(w[k], h8(r[0], r[1], r[2], r[3]), st[c].o[j + k]);
+                        }
+            }
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        float l = st[c].l, pm = st[c].pm;
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+        pm += __shfl_xor(pm, 16);
+        pm += __shfl_xor(pm, 32);
+        const uint32_t col = col0 + c * 16 + (lane & 15), i = col / ratio;
+        const int64_t row = s.row0 + i;
+        if (i >= s.count || row < 0 || row >= p.rows) continue;
+        const int64_t qh = (int64_t)head * ratio + col % ratio;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t r = 4 * quad + i;
+            const uint32_t d = D == 128 ? 8 * r : 8 * (r & 7) + 4 * (r >> 3);
+#pragma unroll
+            for (int j = 0; j < D / 16; j += 4) {
+                phx_f4 o;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[k] = st[c].o[j + k][i] + pm;
+                store<T>((PHX_GLOBAL T *)p.y + row * p.ldy + qh * D + d + j, o, l);
+            }
+        }
+    }
+}
+
 // The parts of a split launch: a workgroup per row and query head.  Its lanes
 // first share the parts' statistics out, then D/4 lanes by 1024/D of them take
 // parts in turns; sums are in a fixed order.  (One group of lanes walking the
@@ -665,6 +964,10 @@ __device__ __forceinline__ void combine(const PhxKv4 &p) {
         kv4_attend_##suffix##_c##NC##_g##G##_w##WAVES(PhxKv4 p) {                               \
         attend<T, D, NC, G, WAVES>(p);                                                          \
     }
+#define CHUNK(T, D, suffix)                                                                     \
+    extern "C" __global__ __launch_bounds__(256, 2) void kv4_attend_##suffix##_chunk(PhxKv4 p) {\
+        chunk<T, D>(p);                                                                         \
+    }
 #define COMBINE(T, D, suffix)                                                                   \
     extern "C" __global__ __launch_bounds__(256) void kv4_combine_##suffix(PhxKv4 p) {          \
         combine<T, D>(p);                                                                       \
@@ -676,6 +979,7 @@ __device__ __forceinline__ void combine(const PhxKv4 &p) {
     ATTEND(T, D, suffix, 1, 4, 12, 3)                                                           \
     ATTEND(T, D, suffix, 1, 2, 16, 4)                                                           \
     ATTEND(T, D, suffix, 1, 1, 8, 2)                                                            \
+    CHUNK(T, D, suffix)                                                                         \
     COMBINE(T, D, suffix)
 ALL(_Float16, 64, f16_d64)
 ALL(_Float16, 128, f16_d128)
@@ -685,5 +989,3 @@ ATTEND(_Float16, 64, f16_d64, 2, 1, 4, 2)
 ATTEND(_Float16, 128, f16_d128, 2, 1, 4, 2)
 ATTEND(float, 64, f32_d64, 2, 1, 4, 2)
 ATTEND(float, 128, f32_d128, 2, 1, 4, 1)
-ATTEND(_Float16, 64, f16_d64, 4, 1, 4, 1)
-ATTEND(_Float16, 128, f16_d128, 4, 1, 4, 1)

@@ -281,17 +281,20 @@ int phx_kv4_read(phx_stream s, const phx_kv4_cache *cache, const phx_kv4_batch *
     return move_rows(s, cache, batch, t, k, v, ldk, ldv, "kv4_read", names);
 }
 
-// How an attention runs.  A workgroup takes 4, 8, 16, 32 or 64 columns, a
-// column being a row and query head of one KV head: the fewest that hold them
-// all (kv4_attend.hip; f32 queries, twice the registers, at most 32).  Up to 16
-// columns a workgroup has 8 to 16 waves instead of four where there are fewer
-// than kAttendFull like it and kAttendWide keys or more to share out (32
-// sequences, 8 x 4 heads of 128: 512 keys 9.4 us with 4 waves, 10.0 with 12; 2048
-// keys 23.7 and 19.3).  The keys are split further to bring the launch to
+// How an attention runs.  A workgroup takes 4, 8, 16 or 32 columns, a column
+// being a row and query head of one KV head: the fewest that hold them all
+// (kv4_attend.hip).  Up to 16 columns a workgroup has 8 to 16 waves instead of
+// four where there are fewer than kAttendFull like it and kAttendWide keys or
+// more to share out (32 sequences, 8 x 4 heads of 128: 512 keys 9.4 us with 4
+// waves, 10.0 with 12; 2048 keys 23.7 and 19.3).  Above 64 columns it takes 128
+// of them, with no wave of its own for a share of the keys, where that gives
+// kAttendChunks workgroups (16 KV heads of 128 x 1000 columns over 4133 keys:
+// 211 us against 353; 64 x 256 columns over 4000: 113 against 104; 24 x 800 over
+// 1000: 49 against 53).  The keys are split further to bring the launch to
 // kAttendGroups workgroups, into parts of at least kAttendPart keys (of the
 // longest sequence there can be) and at most PHX_KV4_SPLITS of them.
-static const int64_t kAttendFull = 512, kAttendWide = 1024, kAttendGroups = 256,
-                     kAttendPart = 1024;
+static const int64_t kAttendFull = 512, kAttendWide = 1024, kAttendChunks = 160,
+                     kAttendGroups = 256, kAttendPart = 1024;
 struct AttendForm {
     int64_t columns;
     uint32_t waves;  // of the wide form
@@ -305,17 +308,22 @@ static const AttendForm kAttendForms[] = {
     {8, 16, {ENTRIES("c1_g2_w4"), ENTRIES("c1_g2_w16")}},
     {16, 8, {ENTRIES("c1_g1_w4"), ENTRIES("c1_g1_w8")}},
     {32, 4, {ENTRIES("c2_g1_w4"), ENTRIES("c2_g1_w4")}},
-    {64, 4, {ENTRIES("c4_g1_w4"), ENTRIES("c4_g1_w4")}}};
+    {128, 4, {ENTRIES("chunk"), ENTRIES("chunk")}}};
 #undef ENTRIES
-
-static const AttendForm &attend_form(phx_dtype t, int64_t columns) {
-    int i = 0;
-    while (i < (t == PHX_F32 ? 3 : 4) && kAttendForms[i].columns < columns) ++i;
-    return kAttendForms[i];
-}
 
 static int64_t attend_groups(const phx_kv4_batch *b, int64_t ratio, const AttendForm &f) {
     return (b->max_q * ratio + f.columns - 1) / f.columns;
+}
+
+static const AttendForm &attend_form(const phx_kv4_cache *c, const phx_kv4_batch *b,
+                                     int64_t ratio) {
+    const int64_t columns = b->max_q * ratio;
+    const AttendForm &chunk = kAttendForms[4];
+    if (columns > 64 && b->batch * c->heads * attend_groups(b, ratio, chunk) >= kAttendChunks)
+        return chunk;
+    int i = 0;
+    while (i < 3 && kAttendForms[i].columns < columns) ++i;
+    return kAttendForms[i];
 }
 
 static size_t split_bytes(const phx_kv4_cache *c, const phx_kv4_batch *b, int64_t q_heads) {
@@ -325,7 +333,7 @@ static size_t split_bytes(const phx_kv4_cache *c, const phx_kv4_batch *b, int64_
 static int64_t attend_splits(const phx_kv4_cache *c, const phx_kv4_batch *b, int64_t q_heads) {
     const int64_t ratio = q_heads / c->heads;
     const int64_t groups = b->batch * c->heads *
-                           attend_groups(b, ratio, attend_form(PHX_F16, b->max_q * ratio));
+                           attend_groups(b, ratio, attend_form(c, b, ratio));
     const int64_t keys = std::min(b->max_len, b->table_stride * c->page_tokens);
     if (!has_work(b)) return 1;
     return std::max<int64_t>(1, std::min({kAttendGroups / groups, keys / kAttendPart, (int64_t)PHX_KV4_SPLITS}));
@@ -374,7 +382,7 @@ int phx_kv4_attention(phx_stream s, const phx_kv4_cache *cache, const phx_kv4_ba
     p.ratio = (int32_t)(q_heads / cache->heads);
     p.causal = causal != 0;
     p.scale = scale;
-    const AttendForm &form = attend_form(t, batch->max_q * p.ratio);
+    const AttendForm &form = attend_form(cache, batch, p.ratio);
     const int64_t each = attend_groups(batch, p.ratio, form);
     const int64_t groups = batch->batch * cache->heads * each;
     p.groups = (int32_t)each;

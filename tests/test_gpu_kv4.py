@@ -524,3 +524,32 @@ def test_threads_on_streams_of_their_own(px_gpu):
     [t.start() for t in threads]
     [t.join() for t in threads]
     assert not wrong
+
+
+# Enough columns and sequences for whole workgroups of columns
+@pytest.mark.parametrize("bits", [16, 32])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("size", [1.0, 40.0])
+@pytest.mark.parametrize("D,heads,R,P,max_q", [(128, 4, 6, 32, 13), (64, 2, 33, 64, 4),
+                                               (128, 4, 70, 64, 1), (64, 4, 1, 32, 65)])
+def test_many_columns(px_gpu, stream, bits, causal, size, D, heads, R, P, max_q):
+    rng = np.random.default_rng(max_q)
+    lens = [2200, 0, 1, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 257] + list(rng.integers(1, 200, 26))
+    counts = rng.integers(0, 4 if max_q > 3 else max_q + 1, 40)
+    counts[[0, 9]] = max_q
+    counts[2] = min(max_q, 3)  # rows before the first key, in a causal call
+    starts = np.concatenate([[0], counts.cumsum()])
+    c = Call(px_gpu, heads, D, P, lens, starts, max_q, seed=max_q)
+    c.table[20, 0], c.table[21, 1:], c.table[22, :] = -1, c.pool.pages, -5
+    c.table[0, 3], c.table[0, 40 // (P // 32)] = 1 << 30, -1
+    c.fill().upload()
+    q = c.rng.standard_normal((c.rows, heads * R, D)) * size
+    q[-1] = 0
+    q[-2, 0] *= 2.0 ** -16
+    got = c.check(stream, bits, q, D ** -0.5, causal, pad=8, extra=2)
+    # a row that is no number stays in its row
+    q[-3, 1, 5] = np.inf
+    again = c.attend(stream, bits, q.astype(_t(bits)), D ** -0.5, causal)
+    assert not np.isfinite(again[-3, 1]).any() or c.lens[np.searchsorted(starts, len(q) - 3, "right") - 1] < 1
+    again[-3, 1] = got[-3, 1]
+    assert np.array_equal(again, got.astype(_t(bits)))
