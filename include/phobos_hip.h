@@ -408,8 +408,11 @@ int phx_kv4_read(phx_stream s, const phx_kv4_cache *cache, const phx_kv4_batch *
  * head h / (q_heads / heads).  A row without keys gets zeros.  Q and O are of
  * type t, rows ldq and ldo elements apart (0: q_heads*head_dim), and start
  * 16-byte aligned (ldq, ldo % 8 == 0 for f16, % 4 for f32).  Codes and f16
- * queries enter the products exactly, f32 queries and the softmax's weights as
- * two f16 terms (22 bits); scores, statistics and sums are f32.
+ * queries enter the products exactly (of a row what is below 2^-32 of its
+ * largest is rounded), f32 queries and the softmax's weights as two f16 terms
+ * (22 bits); scores, statistics and sums are f32.  A query that is infinite or
+ * NaN makes its row and head NaN.  A scale of V that is not positive counts as
+ * 2^-24.
  * A launch too small to fill the GPU is split over the keys when s has a
  * workspace bound that holds the parts (phx_stream_set_workspace,
  * phx_kv4_split_plan), else it runs unsplit.  A captured launch keeps the

@@ -32,12 +32,6 @@ __device__ __forceinline__ Seq kv4_seq(const PhxKv4 &p, int64_t b) {
     return s;
 }
 
-// The page of a sequence's token, or -1.
-__device__ __forceinline__ int64_t kv4_page(const PhxKv4 &p, int64_t b, int64_t token) {
-    const int64_t page = ((const PHX_GLOBAL int32_t *)p.table)[b * p.table_stride + token / p.page_tokens];
-    return page >= 0 && page < p.pages ? page : -1;
-}
-
 // A page's bytes of one head.
 template <int D>
 __device__ __forceinline__ PHX_GLOBAL char *kv4_head(const PhxKv4 &p, int64_t page, int head) {

@@ -181,7 +181,7 @@ int move_rows(phx_stream s, const phx_kv4_cache *c, const phx_kv4_batch *b, phx_
     p.ldy = ldv;
     const int64_t units = b->batch * 2 * c->heads * b->max_q, per = 256 / (c->head_dim / 8);
     const int64_t groups = (units + per - 1) / per;
-    if (groups > INT32_MAX)
+    if (units > INT32_MAX)  // the kernels' indices
         return set_error(PHX_E_INVALID, "%s: %lld sequences of up to %lld rows are too many", who,
                          (long long)b->batch, (long long)b->max_q);
     return launch(kKv4File, entry_of(names, t, c->head_dim), dim3((uint32_t)groups), 256,

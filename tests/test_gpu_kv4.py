@@ -171,6 +171,45 @@ def test_append_bit_for_bit(px_gpu, stream, bits, D, heads, P, lens, starts, max
                     assert np.abs(got - x).max() <= step / 2 + slack
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_append_next_to_every_tie(px_gpu, stream, D):
+    # f32 elements on ties between two codes and 1, 2 and 40 steps beside them,
+    # and ranges whose f16 scale is such a tie or next to one
+    px, heads, rows, P = px_gpu, 2, 300, 64
+    c = Call(px, heads, D, P, [rows], None, rows, seed=1).upload()
+    r = c.rng
+    steps = np.array([-40, -2, -1, 0, 1, 2, 40])
+    x = np.empty((2, rows, heads, D), np.float32)
+    for i in np.ndindex(2, rows, heads):
+        low = np.float64(np.float16(r.standard_normal() * 2.0 ** r.integers(-6, 6)))
+        s = np.float64(np.float16(r.uniform(1, 2) * 2.0 ** r.integers(-8, 4)))
+        tie = (low + s * (r.integers(0, 15, D) + 0.5)).astype(np.float32)
+        row = (tie.view(np.int32) + r.choice(steps, D).astype(np.int32)).view(np.float32)
+        row[0] = low
+        # the largest: 15 scales, or 15 times the middle of two f16 and beside it
+        mid = (s + np.float64(np.nextafter(np.float16(s), np.float16(9e4)))) / 2
+        row[1] = low + 15 * s if r.random() < 0.5 else \
+            (np.float32(low + 15 * mid).view(np.int32) + np.int32(r.choice(steps))).view(np.float32)
+        x[i] = np.clip(row, row[0], row[1])
+    dk, dv = (px.DeviceBuffer.from_array(y.reshape(rows, -1)) for y in x)
+    px.launch_kv4_append(stream, c.cache, c.batch, px.F32, dk, dv)
+    stream.synchronize()
+    got = Pool(c.pool.pages, heads, D, P)
+    got.data = c.d_pool.download(np.uint8, c.pool.data.shape)
+    checked = 0
+    for row in range(rows):
+        for h in range(heads):
+            for v in (False, True):
+                # a step below 0.0 is a NaN, which is no value to append
+                if not np.isfinite(x[int(v), row, h]).all():
+                    continue
+                mine = got.raw(page_of(c.pool, c.table, 0, row), h, row % P, v)
+                for y, z in zip(mine, quantise(x[int(v), row, h])):
+                    assert np.array_equal(y, z), (row, h, v)
+                checked += 1
+    assert checked > 1100
+
+
 @pytest.mark.parametrize("bits", [16, 32])
 @pytest.mark.parametrize("D", [64, 128])
 def test_append_and_read_skip_what_is_no_page(px_gpu, stream, bits, D):
