@@ -424,6 +424,16 @@ __device__ __forceinline__ void attend(const PhxKv4 &p) {
         head = item % p.heads;
         b = item / p.heads;
     }
+    constexpr uint32_t KEYS = 16 * Sh::TILES, PER = 64 / Sh::UNITS;  // steps of whose pages the lanes hold
+    const uint32_t P = p.page_tokens, shift = __builtin_ctz(P / 32);
+    const PHX_GLOBAL int32_t *table =
+        (const PHX_GLOBAL int32_t *)p.table + b * p.table_stride;
+    // the wave's steps are base + WAVES i, and the lanes hold the pages of PER
+    // of them; unsplit the first ones are known, and loaded, before the length is
+    uint32_t base = __builtin_amdgcn_readfirstlane(wave);
+    auto unit_of = [&]() { return (base + lane / Sh::UNITS * WAVES) * Sh::UNITS + lane % Sh::UNITS; };
+    int32_t early = -1;
+    if (p.splits == 1 && (unit_of() >> shift) < p.table_stride) early = table[unit_of() >> shift];
     const Seq s = kv4_seq(p, b);
     const uint32_t ratio = p.ratio, col0 = cg * COLS, first = col0 / ratio;
     if (first >= s.count) return;
@@ -435,23 +445,17 @@ __device__ __forceinline__ void attend(const PhxKv4 &p) {
     if (most < 0) most = 0;
     if (least < 0) least = 0;
 
-    constexpr uint32_t KEYS = 16 * Sh::TILES, PER = 64 / Sh::UNITS;  // steps of whose pages the lanes hold
     const uint32_t steps = (uint32_t)(most + KEYS - 1) / KEYS;
     const uint32_t per = (steps + p.splits - 1) / p.splits;
     const uint32_t end = min((split + 1) * per, steps), seen = (uint32_t)least / KEYS;
     const uint32_t units = (uint32_t)(most + 31) / 32;
-    const uint32_t P = p.page_tokens, shift = __builtin_ctz(P / 32);
-    const PHX_GLOBAL int32_t *table =
-        (const PHX_GLOBAL int32_t *)p.table + b * p.table_stride;
-    // the wave's steps are base + WAVES i, and the lanes hold the pages of PER
-    // of them
-    uint32_t base = split * per + __builtin_amdgcn_readfirstlane(wave);
+    base += split * per;
     int32_t ids;
     int n;
-    auto pages = [&]() {
+    auto pages = [&](bool first) {
         ids = -1;
-        const uint32_t mine = (base + lane / Sh::UNITS * WAVES) * Sh::UNITS + lane % Sh::UNITS;
-        if (base < end && mine < units) ids = table[mine >> shift];
+        const uint32_t mine = unit_of();
+        if (base < end && mine < units) ids = first && p.splits == 1 ? early : table[mine >> shift];
         if (ids >= p.pages) ids = -1;
         n = base < end ? min((end - base + WAVES - 1) / WAVES, PER) : 0;
     };
@@ -485,14 +489,14 @@ __device__ __forceinline__ void attend(const PhxKv4 &p) {
     };
     // a step's loads go out as the one before is done with their registers, the
     // first step's before the queries are looked at
-    auto start = [&]() {
-        pages();
+    auto start = [&](bool first) {
+        pages(first);
         if (n == 0) return;
         next_k(0);
         next_p(0);
         next_v(0);
     };
-    start();
+    start(true);
 
     Query<D, TERMS> q[NC];
     State<D> st[NC];
@@ -541,7 +545,7 @@ __device__ __forceinline__ void attend(const PhxKv4 &p) {
             if (i + 1 < n) next_v(i + 1);
         }
         base += PER * WAVES;
-        start();
+        start(false);
     }
 
     // the results of the waves, one tile of columns after the other; a column's
@@ -900,16 +904,16 @@ __device__ __forceinline__ void chunk(const PhxKv4 &p) {
     }
 }
 
-// The parts of a split launch: a workgroup per row and query head.  Its lanes
-// first share the parts' statistics out, then D/4 lanes by 1024/D of them take
-// parts in turns; sums are in a fixed order.  (One group of lanes walking the
-// parts in a chain waits for memory at every part: 102 us for 32 rows of 128
-// parts.)
+// The parts of a split launch: a workgroup per row and query head, D/4 lanes by
+// 2048/D, each of which takes up to PARTS parts, in a fixed order. All parts are
+// loaded before the statistics that weigh them have come: latency is all that
+// this costs (32 rows of 64 parts TODO us; with the statistics first and four
+// parts at a time 5.4).
 template <typename T, int D>
 __device__ __forceinline__ void combine(const PhxKv4 &p) {
-    constexpr int L = D / 4, G = 256 / L;
+    constexpr int L = D / 4, G = 512 / L, PARTS = PHX_KV4_SPLITS / G;
     __shared__ float factor[PHX_KV4_SPLITS];
-    __shared__ float wave_m[4], wave_l[4];
+    __shared__ float part_m[2], part_l[2];
     __shared__ phx_f4 sums[G][L];
     const uint32_t heads = p.heads * p.ratio, max_q = (uint32_t)p.max_q;
     const uint32_t qh = blockIdx.x % heads, i = blockIdx.x / heads % max_q;
@@ -917,44 +921,46 @@ __device__ __forceinline__ void combine(const PhxKv4 &p) {
     const int64_t row = s.row0 + i;
     if (i >= s.count || row < 0 || row >= p.rows) return;
     const int64_t units = p.rows * heads, unit = row * heads + qh;
-    const PHX_GLOBAL float *ml = (const PHX_GLOBAL float *)p.ws + units * p.splits * D;
-    const int t = threadIdx.x;
+    const int t = threadIdx.x, g = t / L, lane = t % L;
+    const PHX_GLOBAL float *part = (const PHX_GLOBAL float *)p.ws + unit * D + lane * 4;
+    phx_f4 v[PARTS];
+#pragma unroll
+    for (int x = 0; x < PARTS; ++x)
+        if (g + x * G < p.splits) v[x] = *(const PHX_GLOBAL phx_f4 *)(part + (g + x * G) * units * D);
     float m = KV4_NONE, l = 0.0f;
     if (t < p.splits) {
-        const PHX_GLOBAL float *w = ml + (t * units + unit) * 2;
+        const PHX_GLOBAL float *w =
+            (const PHX_GLOBAL float *)p.ws + units * p.splits * D + (t * units + unit) * 2;
         l = w[1];
         if (l != 0.0f) m = w[0];
     }
     float top = m;
     for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
-    if ((t & 63) == 0) wave_m[t >> 6] = top;
+    if (t < PHX_KV4_SPLITS && (t & 63) == 0) part_m[t >> 6] = top;
     __syncthreads();
-    top = fmaxf(fmaxf(wave_m[0], wave_m[1]), fmaxf(wave_m[2], wave_m[3]));
-    // a part without keys has stored no sums: its factor of 0 skips them
+    top = fmaxf(part_m[0], part_m[1]);
+    // a part without keys has stored no sums: its factor of 0 leaves them out
     const float f = l != 0.0f ? __builtin_amdgcn_exp2f(m - top) : 0.0f;
-    if (t < p.splits) factor[t] = f;
+    if (t < PHX_KV4_SPLITS) factor[t] = f;
     float sum = f * l;
     for (int x = 32; x; x >>= 1) sum += __shfl_xor(sum, x);
-    if ((t & 63) == 0) wave_l[t >> 6] = sum;
+    if (t < PHX_KV4_SPLITS && (t & 63) == 0) part_l[t >> 6] = sum;
     __syncthreads();
-    const int g = t / L, lane = t % L;
-    const PHX_GLOBAL float *part = (const PHX_GLOBAL float *)p.ws + unit * D + lane * 4;
     phx_f4 o = {0, 0, 0, 0};
-#pragma unroll 4
-    for (int x = g; x < p.splits; x += G) {
-        const float w = factor[x];
-        if (w == 0.0f) continue;
-        const phx_f4 v = *(const PHX_GLOBAL phx_f4 *)(part + x * units * D);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = fmaf(w, v[e], o[e]);
+    for (int x = 0; x < PARTS; ++x) {
+        if (g + x * G >= p.splits) continue;
+        const float w = factor[g + x * G];
+        if (w == 0.0f) continue;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = fmaf(w, v[x][e], o[e]);
     }
     sums[g][lane] = o;
     __syncthreads();
     if (g) return;
 #pragma unroll
     for (int x = 1; x < G; ++x) o = o + sums[x][lane];
-    store<T>((PHX_GLOBAL T *)p.y + row * p.ldy + qh * D + lane * 4, o,
-             (wave_l[0] + wave_l[1]) + (wave_l[2] + wave_l[3]));
+    store<T>((PHX_GLOBAL T *)p.y + row * p.ldy + qh * D + lane * 4, o, part_l[0] + part_l[1]);
 }
 
 }  // namespace
@@ -969,7 +975,7 @@ __device__ __forceinline__ void combine(const PhxKv4 &p) {
         chunk<T, D>(p);                                                                         \
     }
 #define COMBINE(T, D, suffix)                                                                   \
-    extern "C" __global__ __launch_bounds__(256) void kv4_combine_##suffix(PhxKv4 p) {          \
+    extern "C" __global__ __launch_bounds__(512) void kv4_combine_##suffix(PhxKv4 p) {          \
         combine<T, D>(p);                                                                       \
     }
 #define ALL(T, D, suffix)                                                                       \

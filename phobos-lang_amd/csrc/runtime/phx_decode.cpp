@@ -404,7 +404,7 @@ int phx_kv4_attention(phx_stream s, const phx_kv4_cache *cache, const phx_kv4_ba
         return rc;
     if (p.splits == 1) return PHX_OK;
     return launch(kAttendFile, entry_of(combine, t, cache->head_dim),
-                  dim3((uint32_t)units), 256, (hipStream_t)s, &p);
+                  dim3((uint32_t)units), 512, (hipStream_t)s, &p);
 }
 
 // ------------------------------------------------------------------ pages
