@@ -17,7 +17,7 @@
 // 64 rows of 16384 x 8192 take 34.1 us (504 TFLOP/s; f32 77 us): unpacking costs
 // as many cycles as the products, and the rows pass through LDS in every
 // workgroup.
-// A split of N in tiles leaves CUs idle below 4096 columns; there 8 or 16 waves
+// A split of N in tiles leaves CUs idle below 4096 columns; there 8 to 16 waves
 // share a tile's K. A scale and a zero point are loaded by a quarter of a wave
 // for the groups of a block and handed around by the lanes (groups of 32, 64 rows,
 // 16384 x 8192: 47.4 us; every lane loading all of them 64.1).
@@ -442,7 +442,7 @@ __device__ __forceinline__ void gemm_w4(const PhxGemvW4 &p) {
 GROUPS(_Float16, f16, 1, 8)
 GROUPS(_Float16, f16, 1, 16)
 GROUPS(_Float16, f16, 4, 8)
-GROUPS(float, f32, 1, 8)
+GROUPS(float, f32, 1, 12)
 GROUPS(float, f32, 4, 8)
 GEMM_GROUPS(_Float16, f16, 2, 2, 2, 4)
 GEMM_GROUPS(_Float16, f16, 2, 1, 1, 8)

@@ -51,7 +51,7 @@ const W4Form kW4F16[] = {{16, 16, 512, 8, 0, GROUPS("gemv_w4_f16_n1_w8")},
                          {64, 16, 512, 8, 0, GROUPS("gemv_w4_f16_n4_w8")},
                          {64, 32, 512, 4, 1130, GROUPS("gemm_w4_f16_m2_n2_2x4")},
                          {16, 32, 512, 8, 1350, GROUPS("gemm_w4_f16_m2_n1_1x8")}};
-const W4Form kW4F32[] = {{16, 16, 512, 8, 0, GROUPS("gemv_w4_f32_n1_w8")},
+const W4Form kW4F32[] = {{16, 16, 768, 12, 0, GROUPS("gemv_w4_f32_n1_w12")},
                          {64, 16, 512, 8, 0, GROUPS("gemv_w4_f32_n4_w8")},
                          {128, 32, 512, 2, 2250, GROUPS("gemm_w4_f32_m2_n2_4x2")},
                          {64, 32, 512, 2, 1600, GROUPS("gemm_w4_f32_m2_n1_4x2")}};
@@ -60,7 +60,8 @@ const W4Form kW4F32[] = {{16, 16, 512, 8, 0, GROUPS("gemv_w4_f32_n1_w8")},
 // The kernel for a product, and the K chunks it runs in, at most `most`.
 //   Up to 16 rows: 16 columns a workgroup while the CUs are not all several
 // times occupied, in f16 with 16 waves over long K (4096 x 16384: 9.3 us against
-// 10.6 with 8), else 64 columns (16 rows, 16384 x 8192: f16 19.9 us against 22.0,
+// 10.6 with 8), in f32 with the 12 whose rows LDS holds (16.9 us against 18.9 with
+// 8), else 64 columns (16 rows, 16384 x 8192: f16 19.9 us against 22.0,
 // f32 33.8 against 66.0).
 //   More: the one that is estimated fastest: its rounds of workgroups on the
 // CUs, each K chunk's blocks; a split in 2 or 4 chunks costs its reduction
