@@ -336,7 +336,7 @@ size_t phx_w4_packed_bytes(int64_t N, int64_t K);
 int phx_w4_pack(phx_stream s, uint64_t codes, uint64_t packed, int64_t N, int64_t K);
 /* C = alpha*A@W + beta*C over 0 <= M <= 64 rows (more is a GEMM's work), A
  * [M, K] and C [M, N] of type t with rows lda and ldc elements apart (0: K
- * and N).  K % 8 == 0, any N; A's rows and the packed codes start 16-byte
+ * and N).  K % 8 == 0, N below 2^25; A's rows and the packed codes start 16-byte
  * aligned (lda % 8 == 0 for f16, % 4 for f32).  Codes less zero points and
  * f16 operands enter the products exactly, f32 operands with all their bits;
  * products, sums and scales are f32, and C is rounded once from

@@ -275,7 +275,7 @@ __device__ __forceinline__ void weights(const Raw<D, G> &r, const Query<D, TERMS
     }
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-        int32_t left = q[c].limit - (int32_t)(key0 + 16 * ln.tile + 4 * ln.quad);
+        int32_t left = (int32_t)((uint32_t)q[c].limit - (key0 + 16 * ln.tile + 4 * ln.quad));
         if (absent >> (ln.tile / 2) & 1) left = 0;
         float e[W];
 #pragma unroll
@@ -788,10 +788,11 @@ __device__ __forceinline__ void chunk(const PhxKv4 &p) {
                     x[c][u / 4][u % 4] = fmaf(ks[u / 4][u % 4], x[c][u / 4][u % 4] * q[c].a,
                                               fmaf(km[u / 4][u % 4], q[c].b, -st[c].m));
             if (at >= seen || absent) {
-                const int32_t key0 = (int32_t)(at * KEYS + n * 32 + quad * 4);
+                const uint32_t key0 = at * KEYS + n * 32 + quad * 4;
 #pragma unroll
                 for (int c = 0; c < NC; ++c) {
-                    const int32_t left = absent >> n & 1 ? 0 : q[c].limit - key0;
+                    const int32_t left =
+                        absent >> n & 1 ? 0 : (int32_t)((uint32_t)q[c].limit - key0);
 #pragma unroll
                     for (int u = 0; u < 8; ++u)
                         x[c][u / 4][u % 4] =

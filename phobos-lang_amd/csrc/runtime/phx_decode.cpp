@@ -33,6 +33,7 @@ bool known(phx_dtype t) { return t == PHX_F32 || t == PHX_F16; }
 int64_t size_of(phx_dtype t) { return t == PHX_F16 ? 2 : 4; }
 
 constexpr int64_t kMost = INT64_C(1) << 40;  // of any extent: products of two stay in 64 bits
+constexpr int64_t kMostThreads = UINT32_MAX;  // of a launch along one axis
 bool extent(int64_t v) { return v >= 0 && v <= INT32_MAX; }
 
 // ------------------------------------------------------------------ 4-bit weights
@@ -173,6 +174,11 @@ int move_rows(phx_stream s, const phx_kv4_cache *c, const phx_kv4_batch *b, phx_
         if (int rc = check_rows(c, t, k, c->heads, &ldk, who, "K")) return rc;
     if (work)
         if (int rc = check_rows(c, t, v, c->heads, &ldv, who, "V")) return rc;
+    const int64_t units = b->batch * 2 * c->heads * b->max_q, per = 256 / (c->head_dim / 8);
+    const int64_t groups = (units + per - 1) / per;
+    if (work && groups > kMostThreads / 256)
+        return set_error(PHX_E_INVALID, "%s: %lld sequences of up to %lld rows are too many", who,
+                         (long long)b->batch, (long long)b->max_q);
     if (int rc = on_device((hipStream_t)s)) return rc;
     if (!work) return PHX_OK;
     PhxKv4 p = record(c, b);
@@ -180,11 +186,6 @@ int move_rows(phx_stream s, const phx_kv4_cache *c, const phx_kv4_batch *b, phx_
     p.y = v;
     p.ldx = ldk;
     p.ldy = ldv;
-    const int64_t units = b->batch * 2 * c->heads * b->max_q, per = 256 / (c->head_dim / 8);
-    const int64_t groups = (units + per - 1) / per;
-    if (units > INT32_MAX)  // the kernels' indices
-        return set_error(PHX_E_INVALID, "%s: %lld sequences of up to %lld rows are too many", who,
-                         (long long)b->batch, (long long)b->max_q);
     return launch(kKv4File, entry_of(names, t, c->head_dim), dim3((uint32_t)groups), 256,
                   (hipStream_t)s, &p);
 }
@@ -224,6 +225,8 @@ int phx_gemv_w4(phx_stream s, phx_dtype t, uint64_t a, uint64_t w, uint64_t scal
         return set_error(PHX_E_INVALID,
                          "gemv_w4 needs 0 <= M <= %d, N > 0 and K > 0 with K%%8==0 (got %lld,%lld,%lld)",
                          PHX_W4_MAX_ROWS, (long long)M, (long long)N, (long long)K);
+    if (N >> 25)  // up to 1024 threads for 16 columns: a launch's 2^32 along an axis
+        return set_error(PHX_E_INVALID, "gemv_w4: %lld columns are too many", (long long)N);
     if (group != 32 && group != 64 && group != 128)
         return set_error(PHX_E_INVALID, "gemv_w4: groups of 32, 64 or 128 (got %lld)",
                          (long long)group);
@@ -373,6 +376,16 @@ int phx_kv4_attention(phx_stream s, const phx_kv4_cache *cache, const phx_kv4_ba
         if (int rc = check_rows(cache, t, q, q_heads, &ldq, who, "Q")) return rc;
     if (work)
         if (int rc = check_rows(cache, t, o, q_heads, &ldo, who, "O")) return rc;
+    const int64_t ratio = q_heads / cache->heads;
+    const AttendForm &form = attend_form(cache, batch, ratio);
+    const int64_t each = attend_groups(batch, ratio, form);
+    const int64_t groups = batch->batch * cache->heads * each;
+    const int64_t units = batch->batch * batch->max_q * q_heads;
+    // (the workgroups of a form, and of the one that joins the parts of a split)
+    const int64_t planned = attend_splits(cache, batch, q_heads);
+    if (work && (groups > kMostThreads / 1024 / planned || (planned > 1 && units > kMostThreads / 512)))
+        return set_error(PHX_E_INVALID, "%s: %lld sequences of up to %lld rows are too many", who,
+                         (long long)batch->batch, (long long)batch->max_q);
     if (int rc = on_device((hipStream_t)s)) return rc;
     if (!work) return PHX_OK;
     PhxKv4 p = record(cache, batch);
@@ -380,22 +393,14 @@ int phx_kv4_attention(phx_stream s, const phx_kv4_cache *cache, const phx_kv4_ba
     p.y = o;
     p.ldx = ldq;
     p.ldy = ldo;
-    p.ratio = (int32_t)(q_heads / cache->heads);
+    p.ratio = (int32_t)ratio;
     p.causal = causal != 0;
     p.scale = scale;
-    const AttendForm &form = attend_form(cache, batch, p.ratio);
-    const int64_t each = attend_groups(batch, p.ratio, form);
-    const int64_t groups = batch->batch * cache->heads * each;
     p.groups = (int32_t)each;
-    const int64_t units = batch->batch * batch->max_q * q_heads;
     size_t room = 0;
     if (int rc = phx_stream_get_workspace(s, &p.ws, &room)) return rc;
     const size_t part = split_bytes(cache, batch, q_heads);
-    p.splits = (int32_t)std::max<int64_t>(
-        1, std::min<int64_t>(attend_splits(cache, batch, q_heads), (int64_t)(room / part)));
-    if (units > INT32_MAX || each * p.splits > INT32_MAX || groups * p.splits > INT32_MAX)
-        return set_error(PHX_E_INVALID, "%s: %lld sequences of up to %lld rows are too many", who,
-                         (long long)batch->batch, (long long)batch->max_q);
+    p.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>(planned, (int64_t)(room / part)));
     const bool wide = form.columns <= 16 && groups < kAttendFull &&
                       std::min(batch->max_len, batch->table_stride * cache->page_tokens) >= kAttendWide;
     if (int rc = launch(kAttendFile, entry_of(form.entry[wide], t, cache->head_dim),

@@ -34,7 +34,7 @@ def _gemv(**kw):
 
 
 @pytest.mark.parametrize("ok", [{}, {"M": 64}, {"M": 0, "a": 0, "c": 0}, {"K": 8}, {"group": 64},
-                                {"group": 128}, {"lda": 48, "ldc": 7}, {"dtype": px.F32, "lda": 44},
+                                {"group": 128}, {"lda": 48, "ldc": 7}, {"N": (1 << 25) - 1}, {"dtype": px.F32, "lda": 44},
                                 {"scales": A + 2, "zeros": A + 1, "c": A + 2}])
 def test_gemv_takes(ok):
     assert _gemv(**ok) == px.PHX_E_NOT_INIT
@@ -42,7 +42,7 @@ def test_gemv_takes(ok):
 
 @pytest.mark.parametrize("bad", [
     {"dtype": 2}, {"dtype": -1}, {"M": -1}, {"M": 65}, {"N": 0}, {"N": -5}, {"K": 0}, {"K": 4},
-    {"K": 44}, {"K": -8}, {"N": 1 << 31}, {"K": 1 << 31}, {"group": 0}, {"group": 16}, {"group": -32},
+    {"K": 44}, {"K": -8}, {"N": 1 << 31}, {"N": 1 << 25}, {"K": 1 << 31}, {"group": 0}, {"group": 16}, {"group": -32},
     {"group": 256}, {"lda": 32}, {"lda": 44}, {"ldc": 4}, {"lda": -40}, {"dtype": px.F32, "lda": 42},
     {"lda": 1 << 40}, {"lda": 1 << 62}, {"ldc": 1 << 62}, {"a": 0}, {"w": 0}, {"scales": 0}, {"c": 0},
     {"a": A + 8}, {"w": A + 4}, {"scales": A + 1}, {"c": A + 1}, {"dtype": px.F32, "c": A + 2}])
@@ -107,6 +107,15 @@ def test_kv4_refuses(op, what, bad):
     kw = dict(bad) if what == "args" else {what: bad}
     assert _kv4(op, **kw) == px.PHX_E_INVALID
     assert "kv4_" in px.lib().phx_last_error().decode()
+
+
+@pytest.mark.parametrize("op", OPS)
+def test_more_rows_than_a_launch_takes(op):
+    # with q_starts max_q is a bound that no tensor has to hold
+    few = dict(q_starts=A, batch=100, rows=3)
+    assert _kv4(op, batch=dict(few, max_q=1000)) == px.PHX_E_NOT_INIT
+    assert _kv4(op, batch=dict(few, batch=65535, max_q=(1 << 31) - 1)) == px.PHX_E_INVALID
+    assert "too many" in px.lib().phx_last_error().decode()
 
 
 def test_kv4_attention_heads():

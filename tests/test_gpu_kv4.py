@@ -187,7 +187,7 @@ def test_append_next_to_every_tie(px_gpu, stream, D):
         row = (tie.view(np.int32) + r.choice(steps, D).astype(np.int32)).view(np.float32)
         row[0] = low
         # the largest: 15 scales, or 15 times the middle of two f16 and beside it
-        mid = (s + np.float64(np.nextafter(np.float16(s), np.float16(9e4)))) / 2
+        mid = (s + np.float64(np.nextafter(np.float16(s), np.float16(np.inf)))) / 2
         row[1] = low + 15 * s if r.random() < 0.5 else \
             (np.float32(low + 15 * mid).view(np.int32) + np.int32(r.choice(steps))).view(np.float32)
         x[i] = np.clip(row, row[0], row[1])
