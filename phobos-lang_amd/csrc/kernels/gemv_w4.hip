@@ -180,33 +180,38 @@ struct Block {
 };
 
 // A lane's columns, 16 n + lane % 16 from n0 on, in the codes and the groups.
+// Addresses are a scalar base and a lane's 32-bit offset.
 template <int NT, int PER>
 struct Columns {
-    uint32_t col[NT];
-    const PHX_GLOBAL char *w[NT];
+    uint32_t col[NT], lane_w, group;
+    int64_t tile[NT];  // its first block
 
     __device__ __forceinline__ void start(const PhxGemvW4 &p, int64_t n0, int64_t kb, uint32_t lane) {
+        lane_w = (lane >> 4) * 256 + (lane & 15) * 16;
+        group = lane / 16 % PER;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            // columns past N read the last one's, and are not stored
-            const int64_t c = n0 + 16 * n + (lane & 15);
+            // columns past N read the last one's, and tiles past it the last
+            // one, and are not stored
+            const int64_t c = n0 + 16 * n + (lane & 15), last = (p.N - 1) / 16;
             col[n] = (uint32_t)(c < p.N ? c : p.N - 1);
-            w[n] = (const PHX_GLOBAL char *)p.w + (int64_t)(col[n] / 16) * kb * 1024 +
-                   (lane >> 4) * 256 + col[n] % 16 * 16;
+            tile[n] = (n0 / 16 + n < last ? n0 / 16 + n : last) * kb;
         }
     }
-    __device__ __forceinline__ void fetch(const PhxGemvW4 &p, Block<NT> &t, int64_t b,
-                                          uint32_t lane) const {
+    __device__ __forceinline__ void fetch(const PhxGemvW4 &p, Block<NT> &t, uint32_t b) const {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) t.w[n] = *(const PHX_GLOBAL phx_u4 *)(w[n] + b * 1024);
-        int64_t group = b * PER + lane / 16 % PER;
-        if (group >= p.groups) group = p.groups - 1;
-        const PHX_GLOBAL uint16_t *s = (const PHX_GLOBAL uint16_t *)p.scales + group * p.N;
-        const PHX_GLOBAL uint8_t *z = (const PHX_GLOBAL uint8_t *)p.zeros + group * p.N;
+        for (int n = 0; n < NT; ++n)
+            t.w[n] = *(const PHX_GLOBAL phx_u4 *)((const PHX_GLOBAL char *)p.w +
+                                                  (tile[n] + b) * 1024 + lane_w);
+        const int64_t first = (int64_t)b * PER * p.N;
+        const uint32_t left = (uint32_t)p.groups - 1 - b * PER;  // groups behind the first
+        const uint32_t at = (PER == 1 ? 0 : min(group, left)) * (uint32_t)p.N;
+        const PHX_GLOBAL uint16_t *s = (const PHX_GLOBAL uint16_t *)p.scales + first;
+        const PHX_GLOBAL uint8_t *z = (const PHX_GLOBAL uint8_t *)p.zeros + first;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            t.s[n] = s[col[n]];
-            t.z[n] = p.zeros ? z[col[n]] : 8;
+            t.s[n] = s[at + col[n]];
+            t.z[n] = p.zeros ? z[at + col[n]] : 8;
         }
     }
 };
@@ -296,7 +301,7 @@ __device__ __forceinline__ void gemv_w4(const PhxGemvW4 &p) {
                     a, row < p.M && k < p.K ? (uint32_t)((row * p.lda + k) * sizeof(T)) : 0x80000000u,
                     0, 0);
             }
-        columns.fetch(p, t, b, lane);
+        columns.fetch(p, t, b);
     };
     auto multiply = [&](const Share &x, const Block<NT> &t) {
 #pragma unroll
@@ -371,7 +376,7 @@ __device__ __forceinline__ void gemm_w4(const PhxGemvW4 &p) {
                 a, row < p.M && k < p.K && b < end ? (uint32_t)((row * p.lda + k) * sizeof(T))
                                                    : 0x80000000u, 0, 0);
         }
-        columns.fetch(p, t, min(b, (uint32_t)kb - 1), lane);
+        columns.fetch(p, t, min(b, (uint32_t)kb - 1));
     };
     phx_f4 acc[NT][MT];
 #pragma unroll
