@@ -1,6 +1,7 @@
 // Copies of pages within pools (phx_pages_copy): a stream of 16-byte loads and
 // stores, bound by HBM.  A workgroup moves 16 KiB of one page of one layer,
-// four loads of a thread in flight.
+// four loads of a thread in flight. 200 pages of 68 KiB in 16 layers: 88 us (5.1
+// TB/s); 3 pages of 9 KiB: 1.8 us.
 #include "phx_common.h"
 #include "phx_decode.h"
 
