@@ -316,7 +316,8 @@ int phx_flash_attention_bh_noalloc(phx_stream s, phx_kernel k, uint64_t q, uint6
  * allocates or waits, so it can be captured into a graph (the first use of a
  * kernel loads its code object, in a capture too).  The device given to
  * phx_init has to be the calling thread's current one and the stream's
- * (PHX_E_INVALID otherwise).  Arguments are checked before anything is
+ * (PHX_E_INVALID otherwise).  Several threads may launch them, on one stream
+ * too.  Arguments are checked before anything is
  * launched; what lies in device memory (lengths, tables, row starts) is
  * checked by the kernels, which read and write nothing outside the pool, the
  * tables and the rows they were given, whatever it holds. */

@@ -268,8 +268,8 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const PhxGemvW4 &p, si
                                              (int)(((p.M - 1) * p.lda + p.K) * size), 0x00020000);
 }
 
-// Up to 16 rows: a workgroup takes NT tiles of 16 columns, its waves the blocks
-// of K in turns, each with the rows it needs in its own part of LDS; they add up
+// 16 rows: a workgroup takes NT tiles of 16 columns, its waves the blocks of K in
+// turns, each with the rows it needs in its own part of LDS; they add up
 // at the end.
 template <typename T, int NT, int WAVES, int PER>
 __device__ __forceinline__ void gemv_w4(const PhxGemvW4 &p) {
@@ -287,7 +287,8 @@ __device__ __forceinline__ void gemv_w4(const PhxGemvW4 &p) {
     columns.start(p, n0, kb, lane);
     // rows and k that do not exist lie past the resource's end: zeros; loads of
     // none but such rows are left out, and their part of LDS keeps its zeros
-    const uint32_t loads = ((uint32_t)p.M + St::ROWS - 1) / St::ROWS;
+    const uint32_t m0 = blockIdx.y * 16;
+    const uint32_t loads = (min((uint32_t)p.M - m0, 16u) + St::ROWS - 1) / St::ROWS;
     struct Share {
         phx_u4 x[St::LOADS];
     };
@@ -296,7 +297,7 @@ __device__ __forceinline__ void gemv_w4(const PhxGemvW4 &p) {
 #pragma unroll
         for (uint32_t f = 0; f < St::LOADS; ++f)
             if (f < loads) {
-                const uint32_t row = St::row(f, lane);
+                const uint32_t row = m0 + St::row(f, lane);
                 x.x[f] = __builtin_amdgcn_raw_buffer_load_b128(
                     a, row < p.M && k < p.K ? (uint32_t)((row * p.lda + k) * sizeof(T)) : 0x80000000u,
                     0, 0);
@@ -338,7 +339,7 @@ __device__ __forceinline__ void gemv_w4(const PhxGemvW4 &p) {
         phx_f4 sum = part[lane];
 #pragma unroll
         for (int v = 1; v < WAVES; ++v) sum = sum + part[v * 64 + lane];
-        store<T>(p, sum, n0 + 16 * n + (lane & 15), lane / 16 * 4);
+        store<T>(p, sum, n0 + 16 * n + (lane & 15), m0 + lane / 16 * 4);
     }
 }
 

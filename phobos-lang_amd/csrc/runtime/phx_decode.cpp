@@ -4,6 +4,7 @@
 // check themselves (kv4.hip).
 #include <algorithm>
 #include <exception>
+#include <mutex>
 #include <vector>
 
 #include "../kernels/phx_decode.h"
@@ -29,6 +30,10 @@ int launch(const char *file, const char *entry, dim3 grid, uint32_t threads, hip
     return e == hipSuccess ? PHX_OK : hip_error(e, entry);
 }
 
+// Held over the two launches of a split call: no other thread's parts come
+// between them in the stream's workspace.
+std::mutex g_pair;
+
 bool known(phx_dtype t) { return t == PHX_F32 || t == PHX_F16; }
 int64_t size_of(phx_dtype t) { return t == PHX_F16 ? 2 : 4; }
 
@@ -38,7 +43,7 @@ bool extent(int64_t v) { return v >= 0 && v <= INT32_MAX; }
 
 // ------------------------------------------------------------------ 4-bit weights
 // A kernel of gemv_w4.hip: the columns and rows of a workgroup, and the blocks
-// of 128 k it takes at a time, in so many nanoseconds (measured; more than 16
+// of 128 k it takes at a time, in so many nanoseconds (measured; 0: only up to 16
 // rows).
 struct W4Form {
     int64_t columns, rows;
@@ -47,12 +52,12 @@ struct W4Form {
     const char *entry[3];  // groups of 128, 64 and 32
 };
 #define GROUPS(name) {name "_g1", name "_g2", name "_g4"}
-const W4Form kW4F16[] = {{16, 16, 512, 8, 0, GROUPS("gemv_w4_f16_n1_w8")},
-                         {16, 16, 1024, 16, 0, GROUPS("gemv_w4_f16_n1_w16")},
+const W4Form kW4F16[] = {{16, 16, 512, 8, 670, GROUPS("gemv_w4_f16_n1_w8")},
+                         {16, 16, 1024, 16, 1150, GROUPS("gemv_w4_f16_n1_w16")},
                          {64, 16, 512, 8, 0, GROUPS("gemv_w4_f16_n4_w8")},
                          {64, 32, 512, 4, 1130, GROUPS("gemm_w4_f16_m2_n2_2x4")},
                          {16, 32, 512, 8, 1350, GROUPS("gemm_w4_f16_m2_n1_1x8")}};
-const W4Form kW4F32[] = {{16, 16, 768, 12, 0, GROUPS("gemv_w4_f32_n1_w12")},
+const W4Form kW4F32[] = {{16, 16, 768, 12, 2000, GROUPS("gemv_w4_f32_n1_w12")},
                          {64, 16, 512, 8, 0, GROUPS("gemv_w4_f32_n4_w8")},
                          {128, 32, 512, 2, 2250, GROUPS("gemm_w4_f32_m2_n2_4x2")},
                          {64, 32, 512, 2, 1600, GROUPS("gemm_w4_f32_m2_n1_4x2")}};
@@ -66,7 +71,10 @@ const W4Form kW4F32[] = {{16, 16, 768, 12, 0, GROUPS("gemv_w4_f32_n1_w12")},
 // f32 33.8 against 66.0).
 //   More: the one that is estimated fastest: its rounds of workgroups on the
 // CUs, each K chunk's blocks; a split in 2 or 4 chunks costs its reduction
-// (f16, 32 x 4096 x 16384: 18.1 us in 4, 23.5 in none of the other form).
+// (f16, 32 x 4096 x 16384: 18.1 us in 4, 23.5 in none of the other form).  Tiles of
+// 16 rows that share nothing are taken while each has a CU of its own (64 x 1000
+// x 4136: f16 6.6 us against 9.3, f32 11.7 against 14.0; 48 x 4096 x 4096 f16, on 768
+// of them, 15.2 against 11.5).
 const W4Form &w4_form(phx_dtype t, int64_t M, int64_t N, int64_t K, int64_t most,
                       int64_t *splits) {
     const W4Form *forms = t == PHX_F16 ? kW4F16 : kW4F32;
@@ -78,19 +86,24 @@ const W4Form &w4_form(phx_dtype t, int64_t M, int64_t N, int64_t K, int64_t most
     }
     const W4Form *best = nullptr;
     int64_t least = 0;
-    for (const W4Form *f = forms + (t == PHX_F16 ? 3 : 2), *e = f + 2; f != e; ++f)
-        for (int64_t sp = 1; sp <= 4 && sp <= std::max<int64_t>(most, 1); sp *= 2) {
-            const int64_t groups = ((N + f->columns - 1) / f->columns) *
-                                   ((M + f->rows - 1) / f->rows) * sp;
+    for (int i = 0; i < 5 - (t == PHX_F32); ++i) {
+        const W4Form &f = forms[i];
+        if (!f.ns) continue;
+        const bool shared = f.rows > 16;  // the others have no split
+        for (int64_t sp = 1; sp <= (shared ? 4 : 1) && sp <= std::max<int64_t>(most, 1); sp *= 2) {
+            const int64_t groups =
+                ((N + f.columns - 1) / f.columns) * ((M + f.rows - 1) / f.rows) * sp;
+            if (!shared && groups > 256) break;
             const int64_t blocks = ((K + 127) / 128 + sp - 1) / sp;
-            int64_t ns = (groups + 255) / 256 * ((blocks + f->blocks - 1) / f->blocks) * f->ns;
+            int64_t ns = (groups + 255) / 256 * ((blocks + f.blocks - 1) / f.blocks) * f.ns;
             if (sp > 1) ns += 3300 + (sp + 1) * M * N / 1000;
             if (!best || ns < least) {
-                best = f;
+                best = &f;
                 least = ns;
                 *splits = sp;
             }
         }
+    }
     return *best;
 }
 
@@ -253,6 +266,8 @@ int phx_gemv_w4(phx_stream s, phx_dtype t, uint64_t a, uint64_t w, uint64_t scal
     if (int rc = phx_stream_get_workspace(s, &p.ws, &room)) return rc;
     const W4Form &f = w4_form(t, M, N, K, (int64_t)(room / sizeof(float)) / (M * N), &splits);
     p.splits = (int32_t)splits;
+    std::unique_lock<std::mutex> pair(g_pair, std::defer_lock);
+    if (splits > 1) pair.lock();
     if (int rc = launch(kW4File, f.entry[group == 128 ? 0 : group == 64 ? 1 : 2],
                         dim3((uint32_t)((N + f.columns - 1) / f.columns),
                              (uint32_t)((M + f.rows - 1) / f.rows), (uint32_t)splits),
@@ -403,6 +418,8 @@ int phx_kv4_attention(phx_stream s, const phx_kv4_cache *cache, const phx_kv4_ba
     p.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>(planned, (int64_t)(room / part)));
     const bool wide = form.columns <= 16 && groups < kAttendFull &&
                       std::min(batch->max_len, batch->table_stride * cache->page_tokens) >= kAttendWide;
+    std::unique_lock<std::mutex> pair(g_pair, std::defer_lock);
+    if (p.splits > 1) pair.lock();
     if (int rc = launch(kAttendFile, entry_of(form.entry[wide], t, cache->head_dim),
                         dim3((uint32_t)(each * p.splits), (uint32_t)cache->heads,
                              (uint32_t)batch->batch),

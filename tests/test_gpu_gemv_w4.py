@@ -187,7 +187,7 @@ def test_quantised_weights_stand_for_the_weights(px_gpu, stream):
 # M at the edges of the row tiles; K that splits in 2 and in 4 chunks, the last
 # of them short
 SPLIT = [(17, 1000, 4136), (32, 33, 2056), (33, 1000, 4136), (48, 65, 1160), (64, 2500, 2048),
-         (64, 16, 16384), (24, 130, 9000)]
+         (64, 16, 16384), (24, 130, 9000), (33, 1500, 8192), (64, 1290, 4400), (47, 2600, 16384)]
 
 
 @pytest.mark.parametrize("M,N,K", SPLIT)
@@ -217,10 +217,10 @@ def test_split_over_k(px_gpu, bits, M, N, K, parts):
     assert (ws.download(np.uint8, room + 4096)[room:] == 0xAB).all()
 
 
-def test_captured_and_replayed(px_gpu):
+@pytest.mark.parametrize("M,N,K", [(40, 600, 4136), (40, 1500, 8192)])
+def test_captured_and_replayed(px_gpu, M, N, K):
     px = px_gpu
     rng = np.random.default_rng(2)
-    M, N, K = 40, 600, 4136
     codes = rng.integers(0, 16, (K, N)).astype(np.uint8)
     scales = (rng.random((-(-K // 32), N)) * 0.01).astype(np.float16)
     s = px.Stream()

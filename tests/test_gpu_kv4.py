@@ -565,6 +565,49 @@ def test_threads_on_streams_of_their_own(px_gpu):
     assert not wrong
 
 
+def test_threads_on_one_stream(px_gpu):
+    # split launches, whose parts share the stream's workspace
+    import threading
+    px = px_gpu
+    s = px.Stream()
+    px.bind_workspace(s, 8 << 20)
+    calls = [Call(px, 1, 64, 64, [6000 + 64 * i], seed=50 + i, spare=2) for i in range(3)]
+    work = []
+    for c in calls:
+        c.pool.data[:] = c.rng.integers(0, 256, c.pool.data.shape)
+        par = np.empty((c.pool.pages, 1, 2, 64, 2), np.float16)
+        par[..., 0], par[..., 1] = 0.1, -0.7
+        c.pool.data[:, :, 64 * 64:] = par.reshape(c.pool.pages, 1, -1).view(np.uint8)
+        c.upload()
+        assert px.kv4_split_plan(c.cache, c.batch, 4)[0] > 1
+        q = px.DeviceBuffer.from_array(c.rng.standard_normal((1, 4, 64)).astype(np.float16))
+        outs = [px.DeviceBuffer(2 * 4 * 64) for _ in range(20)]
+        work.append([lambda o, c=c, q=q: px.launch_kv4_attention(
+            s, c.cache, c.batch, px.F16, q, o, 4, 0.125), outs])
+    rng = np.random.default_rng(1)
+    M, N, K = 40, 1500, 8192
+    w = px.DeviceBuffer.from_array(rng.integers(0, 256, px.w4_packed_bytes(N, K)).astype(np.uint8))
+    sc = px.DeviceBuffer.from_array((rng.random((256, N)) * 0.01).astype(np.float16))
+    a = px.DeviceBuffer.from_array(rng.standard_normal((M, K)).astype(np.float16))
+    work.append([lambda o: px.launch_gemv_w4(s, px.F16, a, w, sc, 0, o, M, N, K, 32),
+                 [px.DeviceBuffer(2 * M * N) for _ in range(20)]])
+    want = []
+    for f, outs in work:
+        f(outs[0])
+        s.synchronize()
+        want.append(outs[0].download(np.uint16, outs[0].nbytes // 2).copy())
+    threads = [threading.Thread(target=lambda f=f, outs=outs: [f(o) for o in outs])
+               for f, outs in work]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    s.synchronize()
+    for (f, outs), x in zip(work, want):
+        for o in outs:
+            assert np.array_equal(o.download(np.uint16, o.nbytes // 2), x)
+    px.bind_workspace(s, 0)
+    s.destroy()
+
+
 # Enough columns and sequences for whole workgroups of columns
 @pytest.mark.parametrize("bits", [16, 32])
 @pytest.mark.parametrize("causal", [True, False])
