@@ -14,13 +14,13 @@
 // Few rows are bound by the codes' bytes, and by latency where those are few:
 // every code is read once, two blocks of a wave ahead. 16384 x 8192 in groups of
 // 128, f16: 1 row 16.7 us (4.2 TB/s), 16 rows 19.4 us; f32: 27.1 and 35.9 us.
-// 64 rows of 16384 x 8192 take 34.1 us (504 TFLOP/s; f32 77 us): unpacking costs
+// 64 rows of 16384 x 8192 take 30.2 us (570 TFLOP/s; f32 60.8 us): unpacking costs
 // as many cycles as the products, and the rows pass through LDS in every
 // workgroup.
 // A split of N in tiles leaves CUs idle below 4096 columns; there 8 to 16 waves
 // share a tile's K. A scale and a zero point are loaded by a quarter of a wave
 // for the groups of a block and handed around by the lanes (groups of 32, 64 rows,
-// 16384 x 8192: 47.4 us; every lane loading all of them 64.1).
+// 16384 x 8192, in another tile: 47.4 us; every lane loading all of them 64.1).
 #include "phx_common.h"
 #include "phx_decode.h"
 
@@ -343,32 +343,34 @@ __device__ __forceinline__ void gemv_w4(const PhxGemvW4 &p) {
     }
 }
 
-// More rows: a workgroup takes WN x NT tiles of columns and MT of rows, and its
-// WN x WK waves share the rows through LDS: WK blocks of K at a time, split into
-// their matrix terms once, each read by the WN waves of a block for NT tiles.
+// More rows: a workgroup takes WN tiles of columns and MT of rows, and its WN x WK
+// waves share the rows through LDS: WK blocks of K at a time, split into their
+// matrix terms once, each read by the WN waves of a block.  (16 waves with a tile
+// of columns each: 64 x 16384 x 8192 f16 30.2 us, with 8 waves of two 36.5 and of
+// four rows' tiles as well 33.8, however far ahead they load.)
 // One barrier for every WK blocks: the next ones are loaded into registers
 // while these are multiplied, and written to the other half of LDS.
-template <typename T, int MT, int NT, int WN, int WK, int PER>
+template <typename T, int MT, int WN, int WK, int PER>
 __device__ __forceinline__ void gemm_w4(const PhxGemvW4 &p) {
     using St = Staged<T>;
     constexpr uint32_t EACH = MT * St::LOADS / WN;       // a wave's loads of its block
     constexpr uint32_t STAGE = WK * MT * St::BYTES;
-    constexpr uint32_t SUMS = WK * WN * NT * MT * 1024;
+    constexpr uint32_t SUMS = WK * WN * MT * 1024;
     __shared__ phx_u4 lds[(2 * STAGE > SUMS ? 2 * STAGE : SUMS) / 16];
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint32_t wn = __builtin_amdgcn_readfirstlane(wave % WN);
     const uint32_t wk = __builtin_amdgcn_readfirstlane(wave / WN);
-    const int64_t kb = (p.K + 127) / 128, n0 = ((int64_t)blockIdx.x * WN + wn) * (16 * NT);
+    const int64_t kb = (p.K + 127) / 128, n0 = ((int64_t)blockIdx.x * WN + wn) * 16;
     const uint32_t m0 = blockIdx.y * (16 * MT);
     const uint32_t per = ((uint32_t)kb + p.splits - 1) / p.splits;
     const uint32_t begin = blockIdx.z * per, end = min(begin + per, (uint32_t)kb);
     const uint32_t one[2] = {in_vgpr(0x64006400), in_vgpr(0x54005400)};
     const __amdgpu_buffer_rsrc_t a = rows_of(p, sizeof(T));
-    Columns<NT, PER> columns;
+    Columns<1, PER> columns;
     columns.start(p, n0, kb, lane);
     phx_u4 x[EACH];
     // a wave with no block left multiplies zero rows with the last block's codes
-    auto fetch = [&](Block<NT> &t, uint32_t b) {
+    auto fetch = [&](Block<1> &t, uint32_t b) {
         const uint32_t k = b * 128 + St::k(lane);
 #pragma unroll
         for (uint32_t e = 0; e < EACH; ++e) {
@@ -379,12 +381,10 @@ __device__ __forceinline__ void gemm_w4(const PhxGemvW4 &p) {
         }
         columns.fetch(p, t, min(b, (uint32_t)kb - 1));
     };
-    phx_f4 acc[NT][MT];
+    phx_f4 acc[1][MT];
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int m = 0; m < MT; ++m) acc[n][m] = (phx_f4){0, 0, 0, 0};
-    Block<NT> t, next;
+    for (int m = 0; m < MT; ++m) acc[0][m] = (phx_f4){0, 0, 0, 0};
+    Block<1> t, next;
     fetch(next, begin + wk);
     for (uint32_t b = begin, half = 0; b < end; b += WK, half ^= 1) {
         char *block = (char *)lds + half * STAGE + wk * (MT * St::BYTES);
@@ -396,31 +396,28 @@ __device__ __forceinline__ void gemm_w4(const PhxGemvW4 &p) {
         }
         __syncthreads();
         if (b + WK < end) fetch(next, b + WK + wk);
-        uint32_t group[NT];
-        phx_f4 sum[NT][MT];
+        uint32_t group[1];
+        phx_f4 sum[1][MT];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             Rows<T> rows[MT];
 #pragma unroll
             for (int m = 0; m < MT; ++m) rows[m] = St::get(block + m * St::BYTES, j, lane);
-            step<T, MT, NT, PER>(t, rows, j, lane, one, group, sum, acc);
+            step<T, MT, 1, PER>(t, rows, j, lane, one, group, sum, acc);
         }
     }
     __syncthreads();
     phx_f4 *part = (phx_f4 *)lds;
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-            part[(((wk * WN + wn) * NT + n) * MT + m) * 64 + lane] = acc[n][m];
+    for (int m = 0; m < MT; ++m) part[((wk * WN + wn) * MT + m) * 64 + lane] = acc[0][m];
     __syncthreads();
-    constexpr uint32_t EVERY = WN * NT * MT * 64;
+    constexpr uint32_t EVERY = WN * MT * 64;
     for (uint32_t i = threadIdx.x; i < EVERY; i += 64 * WN * WK) {
         phx_f4 sum = part[i];
 #pragma unroll
         for (int v = 1; v < WK; ++v) sum = sum + part[v * EVERY + i];
         const uint32_t m = i / 64 % MT, tile = i / (64 * MT);
-        store<T>(p, sum, ((int64_t)blockIdx.x * (WN * NT) + tile) * 16 + (i & 15),
+        store<T>(p, sum, ((int64_t)blockIdx.x * WN + tile) * 16 + (i & 15),
                  m0 + 16 * m + (i >> 4 & 3) * 4);
     }
 }
@@ -436,24 +433,26 @@ __device__ __forceinline__ void gemm_w4(const PhxGemvW4 &p) {
     GEMV(T, suffix, NT, WAVES, 1)                                                               \
     GEMV(T, suffix, NT, WAVES, 2)                                                               \
     GEMV(T, suffix, NT, WAVES, 4)
-#define GEMM(T, suffix, MT, NT, WN, WK, PER)                                                    \
+#define GEMM(T, suffix, MT, WN, WK, PER)                                                        \
     extern "C" __global__ __launch_bounds__(64 * WN * WK) void                                  \
-        gemm_w4_##suffix##_m##MT##_n##NT##_##WN##x##WK##_g##PER(PhxGemvW4 p) {                  \
-        gemm_w4<T, MT, NT, WN, WK, PER>(p);                                                     \
+        gemm_w4_##suffix##_m##MT##_##WN##x##WK##_g##PER(PhxGemvW4 p) {                          \
+        gemm_w4<T, MT, WN, WK, PER>(p);                                                         \
     }
-#define GEMM_GROUPS(T, suffix, MT, NT, WN, WK)                                                  \
-    GEMM(T, suffix, MT, NT, WN, WK, 1)                                                          \
-    GEMM(T, suffix, MT, NT, WN, WK, 2)                                                          \
-    GEMM(T, suffix, MT, NT, WN, WK, 4)
+#define GEMM_GROUPS(T, suffix, MT, WN, WK)                                                      \
+    GEMM(T, suffix, MT, WN, WK, 1)                                                              \
+    GEMM(T, suffix, MT, WN, WK, 2)                                                              \
+    GEMM(T, suffix, MT, WN, WK, 4)
 GROUPS(_Float16, f16, 1, 8)
 GROUPS(_Float16, f16, 1, 16)
 GROUPS(_Float16, f16, 4, 8)
 GROUPS(float, f32, 1, 12)
 GROUPS(float, f32, 4, 8)
-GEMM_GROUPS(_Float16, f16, 2, 2, 2, 4)
-GEMM_GROUPS(_Float16, f16, 2, 1, 1, 8)
-GEMM_GROUPS(float, f32, 2, 2, 4, 2)
-GEMM_GROUPS(float, f32, 2, 1, 4, 2)
+GEMM_GROUPS(_Float16, f16, 4, 4, 4)
+GEMM_GROUPS(_Float16, f16, 2, 4, 4)
+GEMM_GROUPS(_Float16, f16, 2, 2, 8)
+GEMM_GROUPS(float, f32, 4, 16, 1)
+GEMM_GROUPS(float, f32, 2, 8, 2)
+GEMM_GROUPS(float, f32, 2, 4, 2)
 
 // C from the parts of a split, in order.
 template <typename T>

@@ -55,12 +55,14 @@ struct W4Form {
 const W4Form kW4F16[] = {{16, 16, 512, 8, 670, GROUPS("gemv_w4_f16_n1_w8")},
                          {16, 16, 1024, 16, 1150, GROUPS("gemv_w4_f16_n1_w16")},
                          {64, 16, 512, 8, 0, GROUPS("gemv_w4_f16_n4_w8")},
-                         {64, 32, 512, 4, 1130, GROUPS("gemm_w4_f16_m2_n2_2x4")},
-                         {16, 32, 512, 8, 1350, GROUPS("gemm_w4_f16_m2_n1_1x8")}};
+                         {64, 64, 1024, 4, 1600, GROUPS("gemm_w4_f16_m4_4x4")},
+                         {64, 32, 1024, 4, 1050, GROUPS("gemm_w4_f16_m2_4x4")},
+                         {32, 32, 1024, 8, 1300, GROUPS("gemm_w4_f16_m2_2x8")}};
 const W4Form kW4F32[] = {{16, 16, 768, 12, 2000, GROUPS("gemv_w4_f32_n1_w12")},
                          {64, 16, 512, 8, 0, GROUPS("gemv_w4_f32_n4_w8")},
-                         {128, 32, 512, 2, 2250, GROUPS("gemm_w4_f32_m2_n2_4x2")},
-                         {64, 32, 512, 2, 1600, GROUPS("gemm_w4_f32_m2_n1_4x2")}};
+                         {256, 64, 1024, 1, 2700, GROUPS("gemm_w4_f32_m4_16x1")},
+                         {128, 32, 1024, 2, 2100, GROUPS("gemm_w4_f32_m2_8x2")},
+                         {64, 32, 512, 2, 1600, GROUPS("gemm_w4_f32_m2_4x2")}};
 #undef GROUPS
 
 // The kernel for a product, and the K chunks it runs in, at most `most`.
@@ -71,7 +73,8 @@ const W4Form kW4F32[] = {{16, 16, 768, 12, 2000, GROUPS("gemv_w4_f32_n1_w12")},
 // f32 33.8 against 66.0).
 //   More: the one that is estimated fastest: its rounds of workgroups on the
 // CUs, each K chunk's blocks; a split in 2 or 4 chunks costs its reduction
-// (f16, 32 x 4096 x 16384: 18.1 us in 4, 23.5 in none of the other form).  Tiles of
+// (64 x 4096 x 16384: f16 20.9 us in 4 on tiles of 64 x 64, 24.5 in none on 32 x 32;
+// 64 x 16384 x 8192: f32 60.8 in 4 on 256 x 64, 73.2 in none on 128 x 32).  Tiles of
 // 16 rows that share nothing are taken while each has a CU of its own (64 x 1000
 // x 4136: f16 6.6 us against 9.3, f32 11.7 against 14.0; 48 x 4096 x 4096 f16, on 768
 // of them, 15.2 against 11.5).
@@ -86,7 +89,7 @@ const W4Form &w4_form(phx_dtype t, int64_t M, int64_t N, int64_t K, int64_t most
     }
     const W4Form *best = nullptr;
     int64_t least = 0;
-    for (int i = 0; i < 5 - (t == PHX_F32); ++i) {
+    for (int i = 0; i < (t == PHX_F16 ? 6 : 5); ++i) {
         const W4Form &f = forms[i];
         if (!f.ns) continue;
         const bool shared = f.rows > 16;  // the others have no split
