@@ -446,6 +446,7 @@ GROUPS(_Float16, f16, 1, 8)
 GROUPS(_Float16, f16, 1, 16)
 GROUPS(_Float16, f16, 4, 8)
 GROUPS(float, f32, 1, 12)
+GROUPS(float, f32, 2, 12)
 GROUPS(float, f32, 4, 8)
 GEMM_GROUPS(_Float16, f16, 4, 4, 4)
 GEMM_GROUPS(_Float16, f16, 2, 4, 4)

@@ -59,6 +59,7 @@ const W4Form kW4F16[] = {{16, 16, 512, 8, 670, GROUPS("gemv_w4_f16_n1_w8")},
                          {64, 32, 1024, 4, 1050, GROUPS("gemm_w4_f16_m2_4x4")},
                          {32, 32, 1024, 8, 1300, GROUPS("gemm_w4_f16_m2_2x8")}};
 const W4Form kW4F32[] = {{16, 16, 768, 12, 2000, GROUPS("gemv_w4_f32_n1_w12")},
+                         {32, 16, 768, 12, 0, GROUPS("gemv_w4_f32_n2_w12")},
                          {64, 16, 512, 8, 0, GROUPS("gemv_w4_f32_n4_w8")},
                          {256, 64, 1024, 1, 2700, GROUPS("gemm_w4_f32_m4_16x1")},
                          {128, 32, 1024, 2, 2100, GROUPS("gemm_w4_f32_m2_8x2")},
@@ -69,8 +70,9 @@ const W4Form kW4F32[] = {{16, 16, 768, 12, 2000, GROUPS("gemv_w4_f32_n1_w12")},
 //   Up to 16 rows: 16 columns a workgroup while the CUs are not all several
 // times occupied, in f16 with 16 waves over long K (4096 x 16384: 9.3 us against
 // 10.6 with 8), in f32 with the 12 whose rows LDS holds (16.9 us against 18.9 with
-// 8), else 64 columns (16 rows, 16384 x 8192: f16 19.9 us against 22.0,
-// f32 33.8 against 66.0).
+// 8), else 64 columns (16 rows, 16384 x 8192: f16 19.5 us against 21.7,
+// f32 35.0 against 61.7), in f32 32 between (8192 x 4096: 13.3 us, 16 columns 19.0,
+// 64 19.1).
 //   More: the one that is estimated fastest: its rounds of workgroups on the
 // CUs, each K chunk's blocks; a split in 2 or 4 chunks costs its reduction
 // (64 x 4096 x 16384: f16 20.9 us in 4 on tiles of 64 x 64, 24.5 in none on 32 x 32;
@@ -84,12 +86,12 @@ const W4Form &w4_form(phx_dtype t, int64_t M, int64_t N, int64_t K, int64_t most
     const int64_t tiles = (N + 15) / 16;
     *splits = 1;
     if (M <= 16) {
-        if (t == PHX_F32) return forms[tiles > 512];
+        if (t == PHX_F32) return forms[tiles > 512 ? 2 : tiles > 256 ? 1 : 0];
         return forms[tiles >= 1024 ? 2 : tiles <= 256 && K >= 8192 ? 1 : 0];
     }
     const W4Form *best = nullptr;
     int64_t least = 0;
-    for (int i = 0; i < (t == PHX_F16 ? 6 : 5); ++i) {
+    for (int i = 0; i < 6; ++i) {
         const W4Form &f = forms[i];
         if (!f.ns) continue;
         const bool shared = f.rows > 16;  // the others have no split

@@ -247,3 +247,23 @@ def test_captured_and_replayed(px_gpu, M, N, K):
         g.destroy()
     px.bind_workspace(s, 0)
     s.destroy()
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 8190, 392), (16, 5000, 264), (7, 20001, 136), (16, 4111, 2056),
+                                   (3, 16400, 8)])
+@pytest.mark.parametrize("bits", [16, 32])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_many_columns(px_gpu, stream, bits, M, N, K, group):
+    # the tiles of 32 and 64 columns, the last of them short
+    px = px_gpu
+    rng = np.random.default_rng(N)
+    dtype = px.F16 if bits == 16 else px.F32
+    t = _np(px, dtype)
+    codes = rng.integers(0, 16, (K, N)).astype(np.uint8)
+    scales = (rng.random((-(-K // group), N)) * 0.01).astype(np.float16)
+    zeros = rng.integers(0, 16, scales.shape).astype(np.uint8)
+    a = rng.standard_normal((M, K)).astype(t)
+    w = _weights(codes, scales, zeros, group)
+    want, mag = a.astype(np.float64) @ w, np.abs(a.astype(np.float64)) @ np.abs(w)
+    got = _run(px, stream, dtype, a, codes, scales, zeros, group)
+    assert (np.abs(got - want) <= _bound(want, mag, K, t)).all()
