@@ -309,16 +309,21 @@ int phx_kv4_read(phx_stream s, const phx_kv4_cache *cache, const phx_kv4_batch *
 // being a row and query head of one KV head: the fewest that hold them all
 // (kv4_attend.hip).  Up to 16 columns a workgroup has 8 to 16 waves instead of
 // four where there are fewer than kAttendFull like it and kAttendWide keys or
-// more to share out (32 sequences, 8 x 4 heads of 128: 512 keys 9.4 us with 4
-// waves, 10.0 with 12; 2048 keys 23.7 and 19.3).  Above 64 columns it takes 128
+// more to share out, half of them in a part of a split (32 sequences, 8 x 4 heads
+// of 128: 512 keys 9.4 us with 4 waves, 10.0 with 12; 2048 keys 23.7 and 19.3; one
+// sequence of 4096 in 16 parts 9.9 and 11.1).  Above 64 columns it takes 128
 // of them, with no wave of its own for a share of the keys, where that gives
 // kAttendChunks workgroups (16 KV heads of 128 x 1000 columns over 4133 keys:
 // 211 us against 353; 64 x 256 columns over 4000: 113 against 104; 24 x 800 over
-// 1000: 49 against 53).  The keys are split further to bring the launch to
-// kAttendGroups workgroups, into parts of at least kAttendPart keys (of the
-// longest sequence there can be) and at most PHX_KV4_SPLITS of them.
+// 1000: 49 against 53).  The keys are split further (those of the longest
+// sequence there can be) to bring the launch to kAttendGroups workgroups, into
+// parts of at least kAttendPart keys and at most PHX_KV4_SPLITS of them, where that
+// spares a workgroup kAttendSaved keys, as joining the parts is a launch more (one
+// sequence, 8 x 4 heads of 128: 4096 keys in parts of 256 9.9 us, of 512 12.4, of
+// 1024 14.3; 512 keys whole 8.1, in two 9.9; 24 sequences of 1024, 4 heads, f32: whole
+// 11.2, in two 12.8).
 static const int64_t kAttendFull = 512, kAttendWide = 1024, kAttendChunks = 160,
-                     kAttendGroups = 256, kAttendPart = 1024;
+                     kAttendGroups = 256, kAttendPart = 256, kAttendSaved = 768;
 struct AttendForm {
     int64_t columns;
     uint32_t waves;  // of the wide form
@@ -354,13 +359,20 @@ static size_t split_bytes(const phx_kv4_cache *c, const phx_kv4_batch *b, int64_
     return (size_t)b->rows * (size_t)q_heads * (size_t)(c->head_dim + 2) * sizeof(float);
 }
 
+// The most keys that a sequence can have.
+static int64_t longest(const phx_kv4_cache *c, const phx_kv4_batch *b) {
+    return std::min(b->max_len, b->table_stride * c->page_tokens);
+}
+
 static int64_t attend_splits(const phx_kv4_cache *c, const phx_kv4_batch *b, int64_t q_heads) {
     const int64_t ratio = q_heads / c->heads;
     const int64_t groups = b->batch * c->heads *
                            attend_groups(b, ratio, attend_form(c, b, ratio));
-    const int64_t keys = std::min(b->max_len, b->table_stride * c->page_tokens);
+    const int64_t keys = longest(c, b);
     if (!has_work(b)) return 1;
-    return std::max<int64_t>(1, std::min({kAttendGroups / groups, keys / kAttendPart, (int64_t)PHX_KV4_SPLITS}));
+    const int64_t splits = std::max<int64_t>(
+        1, std::min({kAttendGroups / groups, keys / kAttendPart, (int64_t)PHX_KV4_SPLITS}));
+    return keys - keys / splits < kAttendSaved ? 1 : splits;
 }
 
 static int check_heads(const phx_kv4_cache *c, int64_t q_heads, const char *who) {
@@ -422,7 +434,8 @@ int phx_kv4_attention(phx_stream s, const phx_kv4_cache *cache, const phx_kv4_ba
     const size_t part = split_bytes(cache, batch, q_heads);
     p.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>(planned, (int64_t)(room / part)));
     const bool wide = form.columns <= 16 && groups < kAttendFull &&
-                      std::min(batch->max_len, batch->table_stride * cache->page_tokens) >= kAttendWide;
+                      longest(cache, batch) / p.splits >=
+                          (p.splits > 1 ? kAttendWide / 2 : kAttendWide);
     std::unique_lock<std::mutex> pair(g_pair, std::defer_lock);
     if (p.splits > 1) pair.lock();
     if (int rc = launch(kAttendFile, entry_of(form.entry[wide], t, cache->head_dim),
