@@ -318,10 +318,11 @@ int phx_kv4_read(phx_stream s, const phx_kv4_cache *cache, const phx_kv4_batch *
 // 1000: 49 against 53).  The keys are split further (those of the longest
 // sequence there can be) to bring the launch to kAttendGroups workgroups, into
 // parts of at least kAttendPart keys and at most PHX_KV4_SPLITS of them, where that
-// spares a workgroup kAttendSaved keys, as joining the parts is a launch more (one
-// sequence, 8 x 4 heads of 128: 4096 keys in parts of 256 9.9 us, of 512 12.4, of
-// 1024 14.3; 512 keys whole 8.1, in two 9.9; 24 sequences of 1024, 4 heads, f32: whole
-// 11.2, in two 12.8).
+// spares a workgroup kAttendSaved keys, and one more for 32 rows' and heads' parts,
+// as joining the parts is a launch more (one sequence, 8 x 4 heads of 128: 4096
+// keys in parts of 256 9.9 us, of 512 12.4, of 1024 14.3; 512 keys whole 8.1, in two
+// 9.9; 24 sequences of 1024, 4 heads, f32: whole 11.2, in two 12.8; 2 x 300 rows over
+// 1200 keys, 2 x 2 heads: whole 28.3, in three 35.5).
 static const int64_t kAttendFull = 512, kAttendWide = 1024, kAttendChunks = 160,
                      kAttendGroups = 256, kAttendPart = 256, kAttendSaved = 768;
 struct AttendForm {
@@ -372,7 +373,9 @@ static int64_t attend_splits(const phx_kv4_cache *c, const phx_kv4_batch *b, int
     if (!has_work(b)) return 1;
     const int64_t splits = std::max<int64_t>(
         1, std::min({kAttendGroups / groups, keys / kAttendPart, (int64_t)PHX_KV4_SPLITS}));
-    return keys - keys / splits < kAttendSaved ? 1 : splits;
+    if (splits == 1) return 1;  // (else there are few rows)
+    const int64_t parts = b->batch * b->max_q * q_heads * splits;
+    return keys - keys / splits < kAttendSaved + parts / 32 ? 1 : splits;
 }
 
 static int check_heads(const phx_kv4_cache *c, int64_t q_heads, const char *who) {
