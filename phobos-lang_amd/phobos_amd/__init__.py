@@ -535,14 +535,30 @@ def kv4_split_plan(cache, batch, q_heads):
     return sp.value, ws.value
 
 
+def _page_list(x):
+    """x as an i32 array of its own.  (By way of Python's numbers, as a cast of
+    wider ones would wrap around; and a tensor's tolist() is what is fast.)"""
+    if hasattr(x, "tolist") and getattr(x, "dtype", None) != np.int32:
+        x = x.tolist()
+    try:
+        x = np.array(x, np.int32)
+    except OverflowError as e:
+        raise PhxError(PHX_E_INVALID, f"pages_copy: {e}") from None
+    if x.ndim != 1:
+        raise PhxError(PHX_E_INVALID, "pages_copy: src and dst are lists of page numbers")
+    return x
+
+
 def pages_copy(stream, pool, pages, page_bytes, src, dst, layers=1, layer_stride=0):
     """Copies page src[i] to page dst[i] in each layer's pool (phx_pages_copy)."""
-    src, dst = (np.ascontiguousarray(x, np.int32) for x in (src, dst))
-    if src.shape != dst.shape or src.ndim != 1:
+    src, dst = _page_list(src), _page_list(dst)
+    if src.size != dst.size:
         raise PhxError(PHX_E_INVALID, "pages_copy: src and dst are lists of one length")
     whole = (layers - 1) * layer_stride + pages * page_bytes if layers > 0 else 0
-    check(lib().phx_pages_copy(_sh(stream), _addr(pool, whole, "pool"), pages, page_bytes,
-                               src.ctypes.data, dst.ctypes.data, src.size, layers, layer_stride))
+    # (x.ctypes.data takes four times as long)
+    at = [ctypes.byref(ctypes.c_int32.from_buffer(x)) if x.size else None for x in (src, dst)]
+    check(lib().phx_pages_copy(_sh(stream), _addr(pool, whole, "pool"), pages, page_bytes, *at,
+                               src.size, layers, layer_stride))
 
 
 class Pages:

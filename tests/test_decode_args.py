@@ -164,6 +164,18 @@ def test_pages_copy():
     assert _rc(lambda: px.pages_copy(None, A, 8, 4096, [0, 1], [2])) == px.PHX_E_INVALID
 
 
+def test_page_lists():
+    # numbers that would wrap around to a page, arrays of every kind
+    for bad in ([1 << 32], np.array([1 << 32]), np.array([(1 << 32) + 1], np.uint64), [-(1 << 40)],
+                [[0]], 0, np.int64(0)):
+        assert _copy(bad, [1]) == px.PHX_E_INVALID, bad
+        assert _copy([1], bad) == px.PHX_E_INVALID, bad
+    held = np.array([0, 3], np.int32)
+    held.flags.writeable = False
+    for ok in (held, held.astype(np.int64), (0, 3), np.array([0, 9, 3, 9])[::2], held.astype(np.uint8)):
+        assert _copy(ok, [1, 2]) == px.PHX_E_NOT_INIT
+
+
 def test_a_copy_onto_a_kept_page_is_still_one_destination():
     # 2 -> 2 is left out, and then 2 is the destination of one copy only
     assert _copy([2, 0], [2, 2]) == px.PHX_E_NOT_INIT
