@@ -105,7 +105,8 @@ int phx_stream_synchronize(phx_stream s);
  * split whose workspace fits in the bound bytes, and unsplit when none fits
  * or nothing is bound; it never allocates.  The buffer must stay valid until
  * every launch on s that may use it has completed; launches on one stream
- * run in order, so they can share it.  Unbinding (or phx_stream_destroy)
+ * run in order, so they can share it, from several threads too (a split
+ * call's launches are enqueued together).  Unbinding (or phx_stream_destroy)
  * forgets it; the caller frees it. */
 int phx_stream_set_workspace(phx_stream s, uint64_t dptr, size_t bytes);
 int phx_stream_get_workspace(phx_stream s, uint64_t *dptr, size_t *bytes);

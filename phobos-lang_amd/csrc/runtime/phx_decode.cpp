@@ -30,10 +30,6 @@ int launch(const char *file, const char *entry, dim3 grid, uint32_t threads, hip
     return e == hipSuccess ? PHX_OK : hip_error(e, entry);
 }
 
-// Held over the two launches of a split call: no other thread's parts come
-// between them in the stream's workspace.
-std::mutex g_pair;
-
 bool known(phx_dtype t) { return t == PHX_F32 || t == PHX_F16; }
 int64_t size_of(phx_dtype t) { return t == PHX_F16 ? 2 : 4; }
 
@@ -271,8 +267,8 @@ int phx_gemv_w4(phx_stream s, phx_dtype t, uint64_t a, uint64_t w, uint64_t scal
     if (int rc = phx_stream_get_workspace(s, &p.ws, &room)) return rc;
     const W4Form &f = w4_form(t, M, N, K, (int64_t)(room / sizeof(float)) / (M * N), &splits);
     p.splits = (int32_t)splits;
-    std::unique_lock<std::mutex> pair(g_pair, std::defer_lock);
-    if (splits > 1) pair.lock();
+    std::unique_lock<std::mutex> together(split_mutex((hipStream_t)s), std::defer_lock);
+    if (splits > 1) together.lock();
     if (int rc = launch(kW4File, f.entry[group == 128 ? 0 : group == 64 ? 1 : 2],
                         dim3((uint32_t)((N + f.columns - 1) / f.columns),
                              (uint32_t)((M + f.rows - 1) / f.rows), (uint32_t)splits),
@@ -439,8 +435,8 @@ int phx_kv4_attention(phx_stream s, const phx_kv4_cache *cache, const phx_kv4_ba
     const bool wide = form.columns <= 16 && groups < kAttendFull &&
                       longest(cache, batch) / p.splits >=
                           (p.splits > 1 ? kAttendWide / 2 : kAttendWide);
-    std::unique_lock<std::mutex> pair(g_pair, std::defer_lock);
-    if (p.splits > 1) pair.lock();
+    std::unique_lock<std::mutex> together(split_mutex((hipStream_t)s), std::defer_lock);
+    if (p.splits > 1) together.lock();
     if (int rc = launch(kAttendFile, entry_of(form.entry[wide], t, cache->head_dim),
                         dim3((uint32_t)(each * p.splits), (uint32_t)cache->heads,
                              (uint32_t)batch->batch),

@@ -2,6 +2,8 @@
 #pragma once
 #include <hip/hip_runtime.h>
 
+#include <mutex>
+
 #include "../kernels/phx_geometry.h"
 #include "phobos_hip.h"
 
@@ -26,6 +28,9 @@ int aux_function(const char *file, const char *entry, hipFunction_t *out);
 // PHX_OK if the device given to phx_init is the calling thread's current one
 // and the stream's
 int on_device(hipStream_t s);
+// Locked from a split launch's first kernel to its last, which share the
+// workspace of stream s: launches of another thread on s come before or after.
+std::mutex &split_mutex(hipStream_t s);
 // split-key flash attention (phx_runtime.cpp)
 int flash_split(phx_kernel k, int64_t BH, int64_t Nq, int64_t Nk);
 size_t flash_split_bytes(int64_t BH, int64_t Nq, int sp);

@@ -462,6 +462,16 @@ Workspace stream_workspace(hipStream_t s) {
     return it == g_ws.end() ? Workspace{} : it->second;
 }
 
+}  // namespace
+
+// One of 64 locks by the stream's handle: streams that share one only wait for
+// each other's two enqueues.
+std::mutex &split_mutex(hipStream_t s) {
+    static std::mutex locks[64];
+    return locks[(uint64_t)(uintptr_t)s * 0x9e3779b97f4a7c15u >> 58];
+}
+
+namespace {
 // Chunks a split of `units` (K steps or key blocks) into at most sp chunks of
 // whole units really makes: ceil(units / ceil(units / sp)), so no chunk is
 // empty.
@@ -599,6 +609,7 @@ static int launch_gemm_split_ws(phx_kernel k, const char *entry, int64_t tm, int
     int64_t lda = t[0].stride[0], ldb = t[1].stride[0], ldc = t[2].stride[0];
     int64_t kchunk = split_chunk(K, sp);
     void *ka[] = {&a, &b, &ws, &lda, &ldb, &M, &N, &K, &kchunk};
+    std::lock_guard<std::mutex> together(split_mutex(s));
     hipError_t e = hipModuleLaunchKernel(fk, (uint32_t)tiles, (uint32_t)sp, 1, threads, 1, 1, 0,
                                          s, ka, nullptr);
     if (e != hipSuccess) return hip_error(e, "hipModuleLaunchKernel(gemm_splitk)");
@@ -872,6 +883,7 @@ int launch_flash_split_ws(phx_kernel k, const Desc *t, int rank, int64_t BH, int
     int32_t nsplit = sp;
     void *sa[] = {&q, &kk, &v, &ws, &BH, &Nq, &Nk, &ldq, &ldk, &ldv, &hq, &hk, &hv, &kchunk,
                   &nsplit, &scale};
+    std::lock_guard<std::mutex> together(split_mutex(s));
     hipError_t e = hipModuleLaunchKernel(fs, (uint32_t)items, (uint32_t)sp, 1, kSpecs[k].block, 1,
                                          1, 0, s, sa, nullptr);
     if (e != hipSuccess) return hip_error(e, "hipModuleLaunchKernel(flash_attention_split)");
@@ -980,6 +992,8 @@ int launch_flash_small(phx_kernel k, const Desc *t, int rank, int64_t BH, int64_
     void *a[] = {&q,   &kk,  &v,  &o,  &ws, &BH, &Nq,     &Nk, &ldq, &ldk,
                  &ldv, &ldo, &hq, &hk, &hv, &ho, &kchunk, &sp, &scale};
     const int64_t items = (Nq + best->q - 1) / best->q * BH;
+    std::unique_lock<std::mutex> together(split_mutex(s), std::defer_lock);
+    if (sp > 1) together.lock();
     hipError_t e = hipModuleLaunchKernel(f, (uint32_t)items, (uint32_t)sp, 1, best->threads, 1, 1, 0,
                                          s, a, nullptr);
     if (e != hipSuccess) return hip_error(e, "hipModuleLaunchKernel(flash_w)");

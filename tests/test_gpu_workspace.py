@@ -339,3 +339,57 @@ def test_pod_concurrent_split_computes_each_take_a_slab(px_gpu, tmp_path, slabs)
         rel = np.abs(got - want) / np.maximum(np.abs(want), 1e-2 * np.sqrt(np.mean(want ** 2)))
         assert rel.max() < 1e-4, (slabs, i, rel.max())
     pod.close()
+
+
+def test_threads_with_split_launches_of_every_kind_on_one_stream(px_gpu):
+    # each call's parts lie in the one workspace until its second launch joins
+    # them: every result is the one that the call has alone
+    import threading
+    px = px_gpu
+    rng = np.random.default_rng(3)
+    s = px.Stream()
+    px.bind_workspace(s, 64 << 20)
+    f32 = lambda *n: px.DeviceBuffer.from_array(rng.standard_normal(n).astype(np.float32))  # noqa: E731
+    f16 = lambda *n: px.DeviceBuffer.from_array(rng.standard_normal(n).astype(np.float16))  # noqa: E731
+    work = []  # (call, bytes of its result)
+    a, b = f32(256, 8192), f32(8192, 256)
+    for k, n in ((px.GEMM_FP16TC_FP32ACC, 256), (px.GEMM_FP32, 64)):
+        assert px.split_plan(k, (n, n, 8192))[0] > 1
+        work.append((lambda o, k=k, n=n: px.launch_gemm(s, k, a, b, o, n, n, 8192, 1.0, 0.0),
+                     4 * n * n))
+    q, kv, v = f16(2048, 64), f16(4096, 64), f16(4096, 64)
+    assert px.split_plan(px.FLASH_FP16, (2048, 4096, 64))[0] > 1
+    work.append((lambda o: px.launch_flash(s, px.FLASH_FP16, q, kv, v, o, 2048, 4096, 64, 0.125),
+                 2 * 2048 * 64))
+    pool = rng.integers(0, 256, (100, 64 * 72)).astype(np.uint8)
+    par = np.empty((100, 2, 64, 2), np.float16)
+    par[..., 0], par[..., 1] = 0.1, -0.7
+    pool[:, 64 * 64:] = par.reshape(100, -1).view(np.uint8)
+    held = [px.DeviceBuffer.from_array(x) for x in
+            (pool, np.arange(100, dtype=np.int32), np.array([6400], np.int32))]
+    cache = px.Kv4Cache(held[0].ptr, 100, 1, 64, 64)
+    batch = px.Kv4Batch(held[1].ptr, 100, held[2].ptr, 0, 1, 1, 6400, 1)
+    assert px.kv4_split_plan(cache, batch, 4)[0] > 1
+    work.append((lambda o: px.launch_kv4_attention(s, cache, batch, px.F16, q, o, 4, 0.125),
+                 2 * 4 * 64))
+    w = px.DeviceBuffer.from_array(rng.integers(0, 256, px.w4_packed_bytes(1500, 8192)).astype(np.uint8))
+    sc = px.DeviceBuffer.from_array((rng.random((256, 1500)) * 0.01).astype(np.float16))
+    work.append((lambda o: px.launch_gemv_w4(s, px.F32, a, w, sc, 0, o, 40, 1500, 8192, 32),
+                 4 * 40 * 1500))
+    jobs = []
+    for f, size in work:
+        alone, outs = px.DeviceBuffer(size), [px.DeviceBuffer(size) for _ in range(20)]
+        f(alone)
+        s.synchronize()
+        jobs.append((f, alone.download(np.uint16, size // 2), outs))
+        assert jobs[-1][1].any()
+    threads = [threading.Thread(target=lambda f=f, outs=outs: [f(o) for o in outs])
+               for f, _, outs in jobs]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    s.synchronize()
+    for i, (f, want, outs) in enumerate(jobs):
+        for o in outs:
+            assert np.array_equal(o.download(np.uint16, want.size), want), i
+    px.bind_workspace(s, 0)
+    s.destroy()
