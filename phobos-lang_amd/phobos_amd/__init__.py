@@ -549,16 +549,21 @@ def _page_list(x):
     return x
 
 
+def _layers(pool, pages, page_bytes, layers, layer_stride):
+    """The address of `layers` pools of pages."""
+    whole = (layers - 1) * layer_stride + pages * page_bytes if layers > 0 else 0
+    return _addr(pool, whole, "pool")
+
+
 def pages_copy(stream, pool, pages, page_bytes, src, dst, layers=1, layer_stride=0):
     """Copies page src[i] to page dst[i] in each layer's pool (phx_pages_copy)."""
     src, dst = _page_list(src), _page_list(dst)
     if src.size != dst.size:
         raise PhxError(PHX_E_INVALID, "pages_copy: src and dst are lists of one length")
-    whole = (layers - 1) * layer_stride + pages * page_bytes if layers > 0 else 0
     # (x.ctypes.data takes four times as long)
     at = [ctypes.byref(ctypes.c_int32.from_buffer(x)) if x.size else None for x in (src, dst)]
-    check(lib().phx_pages_copy(_sh(stream), _addr(pool, whole, "pool"), pages, page_bytes, *at,
-                               src.size, layers, layer_stride))
+    check(lib().phx_pages_copy(_sh(stream), _layers(pool, pages, page_bytes, layers, layer_stride),
+                               pages, page_bytes, *at, src.size, layers, layer_stride))
 
 
 class Pages:
@@ -568,7 +573,7 @@ class Pages:
         self.handle = None
         h = _vp()
         check(lib().phx_pages_create(ctypes.byref(h), pages, page_tokens))
-        self.handle = h.value
+        self.handle, self.pages = h.value, pages
 
     def new(self):
         seq = _i64()
@@ -615,8 +620,9 @@ class Pages:
 
     def apply(self, stream, pool, page_bytes, layers=1, layer_stride=0):
         """Launches the pending copies in the layers' pools and clears them."""
-        check(lib().phx_pages_apply(self.handle, _sh(stream), _addr(pool, 0, "pool"), page_bytes,
-                                    layers, layer_stride))
+        check(lib().phx_pages_apply(self.handle, _sh(stream),
+                                    _layers(pool, self.pages, page_bytes, layers, layer_stride),
+                                    page_bytes, layers, layer_stride))
 
     def destroy(self):
         if self.handle:

@@ -226,3 +226,20 @@ def test_an_uninitialised_process_is_refused():
     out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
     assert out.stdout.strip() == str(px.PHX_E_NOT_INIT), out.stderr
     assert ctypes.sizeof(px.Kv4Cache) == 32 and ctypes.sizeof(px.Kv4Batch) == 64
+
+
+def test_pages_apply_measures_its_pool():
+    # every page of every layer has to lie in the buffer, whichever are copied
+    pool = px.Pages(8, 4)
+    a = pool.new()
+    pool.resize(a, 2)
+    pool.resize(pool.fork(a), 3)
+    buf = px.DeviceBuffer.__new__(px.DeviceBuffer)
+    buf.ptr = A
+    for nbytes, layers, stride, rc in [(8 * 64, 1, 0, px.PHX_E_NOT_INIT), (8 * 64 - 1, 1, 0, px.PHX_E_INVALID),
+                                       (9 * 64 + 8 * 64, 2, 9 * 64, px.PHX_E_NOT_INIT),
+                                       (9 * 64 + 8 * 64 - 1, 2, 9 * 64, px.PHX_E_INVALID)]:
+        buf.nbytes = nbytes
+        assert _rc(lambda: pool.apply(None, buf, 64, layers, stride)) == rc, (nbytes, layers)
+        assert pool.stats()[2] == 1
+    buf.ptr = 0  # nothing of it is freed
