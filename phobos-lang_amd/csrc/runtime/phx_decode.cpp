@@ -462,6 +462,11 @@ int phx_pages_copy(phx_stream s, uint64_t pool, int64_t pages, size_t page_bytes
         return set_error(PHX_E_INVALID, "pages_copy: null list");
     if (n && layers && (!pool || (pool & 15)))
         return set_error(PHX_E_INVALID, "pages_copy: the pool must be 16-byte aligned");
+    // (one layer is below 2^61 bytes)
+    const uint64_t last = layers ? UINT64_MAX - (uint64_t)pages * page_bytes : 0;
+    if (n && layers && (pool > last || (layers > 1 && layer_stride > (last - pool) / (uint64_t)(layers - 1))))
+        return set_error(PHX_E_INVALID, "pages_copy: %lld layers %llu bytes apart end past the address space",
+                         (long long)layers, (unsigned long long)layer_stride);
     try {
         std::vector<int32_t> from, to;
         from.reserve((size_t)n);

@@ -243,3 +243,17 @@ def test_pages_apply_measures_its_pool():
         assert _rc(lambda: pool.apply(None, buf, 64, layers, stride)) == rc, (nbytes, layers)
         assert pool.stats()[2] == 1
     buf.ptr = 0  # nothing of it is freed
+
+
+def test_layers_that_wrap_around():
+    # (a negative distance arrives as one of nearly 2^64 bytes)
+    buf = px.DeviceBuffer.__new__(px.DeviceBuffer)
+    buf.ptr, buf.nbytes = 1 << 40, 16 * 4096
+    for pool in (1 << 40, buf):
+        for layers, stride in [(2, -8 * 4096), (2, (1 << 64) - 8 * 4096), (3, 1 << 63), (65535, 1 << 49),
+                               (2, -(1 << 30)), (5, -(1 << 62))]:
+            assert _copy([0], [1], pool=pool, layers=layers, stride=stride) == px.PHX_E_INVALID, stride
+    assert _copy([0], [1], pool=(1 << 64) - 16 * 4096, layers=2) == px.PHX_E_INVALID
+    assert _copy([0], [1], pool=(1 << 64) - 17 * 4096, layers=2) == px.PHX_E_NOT_INIT
+    assert _copy([0], [1], pool=(1 << 64) - 8 * 4096, layers=1) == px.PHX_E_INVALID
+    buf.ptr = 0  # nothing of it is freed
