@@ -12,6 +12,7 @@ Every call goes to the gfx950 code objects through hipModuleLaunchKernel.
 There is no CPU fallback: if the library or a code object is missing, or no
 GPU is present, the call raises.
 """
+import array
 import ctypes
 import os
 import re
@@ -536,14 +537,18 @@ def kv4_split_plan(cache, batch, q_heads):
 
 
 def _page_list(x):
-    """x as an i32 array of its own.  (By way of Python's numbers, as a cast of
-    wider ones would wrap around; and a tensor's tolist() is what is fast.)"""
-    if hasattr(x, "tolist") and getattr(x, "dtype", None) != np.int32:
-        x = x.tolist()
-    try:
+    """x, whole numbers of any kind, as an i32 array of its own."""
+    if getattr(x, "dtype", None) == np.int32:
         x = np.array(x, np.int32)
-    except OverflowError as e:
-        raise PhxError(PHX_E_INVALID, f"pages_copy: {e}") from None
+    else:
+        try:
+            x = list(x.tolist() if hasattr(x, "tolist") else x)
+            if x and isinstance(x[0], bool):
+                raise TypeError("a mask is no list of page numbers")
+            # array() takes whole numbers alone, and those that fit
+            x = np.frombuffer(array.array("i", x), np.int32) if x else np.empty(0, np.int32)
+        except (TypeError, OverflowError) as e:
+            raise PhxError(PHX_E_INVALID, f"pages_copy: {e}") from None
     if x.ndim != 1:
         raise PhxError(PHX_E_INVALID, "pages_copy: src and dst are lists of page numbers")
     return x

@@ -257,3 +257,23 @@ def test_layers_that_wrap_around():
     assert _copy([0], [1], pool=(1 << 64) - 17 * 4096, layers=2) == px.PHX_E_NOT_INIT
     assert _copy([0], [1], pool=(1 << 64) - 8 * 4096, layers=1) == px.PHX_E_INVALID
     buf.ptr = 0  # nothing of it is freed
+
+
+def test_page_numbers_are_whole():
+    nan = float("nan")
+    for bad in ([1.7], [1.0], np.array([0.7]), np.array([3.0], np.float32), [nan], ["1"], [None], [True],
+                np.array([True]), [1 + 0j], [1 << 70], [-(1 << 63) - 1], [(1 << 31)], [-(1 << 31) - 1],
+                None, "1", [[1], [2, 3]]):
+        assert _copy(bad, [1]) == px.PHX_E_INVALID, bad
+        assert _copy([0], bad) == px.PHX_E_INVALID, bad
+    for ok in (np.array([0], t) for t in (np.int8, np.uint16, np.uint32, np.uint64, ">i4", ">i8")):
+        assert _copy(ok, [1]) == px.PHX_E_NOT_INIT, ok.dtype
+    torch = pytest.importorskip("torch")
+    for ok in (torch.tensor([0, 3]), torch.tensor([0, 3], dtype=torch.int32), torch.arange(4)[::3]):
+        assert _copy(ok, [1, 2]) == px.PHX_E_NOT_INIT
+    for bad in (torch.tensor([0.5]), torch.tensor([True]), torch.tensor(0), torch.tensor([1 << 32])):
+        assert _copy(bad, [1]) == px.PHX_E_INVALID
+    for none in (np.int64(0), torch.tensor(0), 0):
+        assert _copy(none, []) == px.PHX_E_INVALID
+    # an empty list has no kind
+    assert _copy([], np.empty(0)) == _copy((), torch.empty(0)) == px.PHX_E_NOT_INIT
