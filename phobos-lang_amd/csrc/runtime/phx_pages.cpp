@@ -271,6 +271,9 @@ int phx_pages_pending(phx_pages p, int32_t *src, int32_t *dst, int64_t cap, int6
 int phx_pages_apply(phx_pages p, phx_stream s, uint64_t pool, size_t page_bytes, int64_t layers,
                     uint64_t layer_stride) {
     return with_pool(p, "pages_apply", [&](phx_pages_s &p) {
+        if (layers < 1 && !p.pending.empty())
+            return set_error(PHX_E_INVALID, "pages_apply: %zu copies are pending in %lld layers",
+                             p.pending.size(), (long long)layers);
         std::vector<int32_t> src, dst;
         for (const Copy &c : p.pending) {
             src.push_back(c.src);

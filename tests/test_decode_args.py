@@ -277,3 +277,13 @@ def test_page_numbers_are_whole():
         assert _copy(none, []) == px.PHX_E_INVALID
     # an empty list has no kind
     assert _copy([], np.empty(0)) == _copy((), torch.empty(0)) == px.PHX_E_NOT_INIT
+
+
+def test_pages_apply_of_no_layers_keeps_its_copies():
+    pool = px.Pages(8, 4)
+    a = pool.new()
+    pool.resize(a, 2)
+    pool.resize(pool.fork(a), 3)
+    for layers in (0, -1, 65536):
+        assert _rc(lambda: pool.apply(None, A, 4096, layers, 8 * 4096)) == px.PHX_E_INVALID
+        assert pool.stats()[2] == 1
