@@ -600,13 +600,15 @@ class Pages:
         check(lib().phx_pages_compact(self.handle))
 
     def table(self, seq):
-        n = _i64()
-        check(lib().phx_pages_table(self.handle, seq, None, 0, ctypes.byref(n)))
-        out = np.empty(n.value, np.int32)
-        check(lib().phx_pages_table(self.handle, seq,
-                                    out.ctypes.data_as(ctypes.POINTER(ctypes.c_int32)), out.size,
-                                    ctypes.byref(n)))
-        return out
+        n, cap = _i64(), 0
+        while True:  # other threads may change it between its size and its contents
+            out = np.empty(cap, np.int32)
+            check(lib().phx_pages_table(self.handle, seq,
+                                        out.ctypes.data_as(ctypes.POINTER(ctypes.c_int32)), cap,
+                                        ctypes.byref(n)))
+            if n.value <= cap:
+                return out[:n.value]
+            cap = n.value
 
     def stats(self):
         """(pages in use, one past the highest of them, pending copies)."""
@@ -617,11 +619,15 @@ class Pages:
     def pending(self, clear=False):
         """The pending copies as (src, dst) arrays; with clear the caller runs
         them and they are no longer pending."""
-        n = self.stats()[2]
-        out = [np.empty(n, np.int32) for _ in range(2)]
-        ptr = [x.ctypes.data_as(ctypes.POINTER(ctypes.c_int32)) for x in out]
-        check(lib().phx_pages_pending(self.handle, *ptr, n, None, 1 if clear else 0))
-        return tuple(out)
+        n, cap = _i64(), self.stats()[2]
+        while True:  # as table()
+            out = [np.empty(cap, np.int32) for _ in range(2)]
+            ptr = [x.ctypes.data_as(ctypes.POINTER(ctypes.c_int32)) for x in out]
+            rc = lib().phx_pages_pending(self.handle, *ptr, cap, ctypes.byref(n), 1 if clear else 0)
+            if n.value <= cap:
+                check(rc)
+                return tuple(x[:n.value] for x in out)
+            cap = n.value
 
     def apply(self, stream, pool, page_bytes, layers=1, layer_stride=0):
         """Launches the pending copies in the layers' pools and clears them."""

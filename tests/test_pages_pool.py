@@ -197,3 +197,44 @@ def test_refusals():
     assert L.phx_pages_new(None, None) == px.PHX_E_INVALID
     assert L.phx_pages_table(pool.handle, pool.new(), None, 3, None) == px.PHX_E_INVALID
     assert L.phx_pages_destroy(None) == 0
+
+
+def test_lists_that_change_between_their_size_and_their_contents(monkeypatch):
+    # calls on one pool may come from several threads
+    pool = px.Pages(16, 4)
+    a = pool.new()
+    pool.resize(a, 10)
+    pool.resize(pool.fork(a), 11)
+    L = px.lib()
+
+    def between(name, act):
+        """The first call of `name` that asks for a size, then act()."""
+        real, left = getattr(L, name), [1]
+
+        def call(*args):
+            rc = real(*args)
+            if left and left.pop():
+                act()
+            return rc
+        monkeypatch.setattr(L, name, call)
+
+    between("phx_pages_table", lambda: pool.resize(a, 3))
+    assert list(pool.table(a)) == [0]
+    monkeypatch.undo()
+    between("phx_pages_table", lambda: pool.resize(a, 30))
+    t = list(pool.table(a))
+    assert len(t) == 8 and len(set(t)) == 8
+    monkeypatch.undo()
+    n = pool.stats()[2]
+    assert n >= 1
+    between("phx_pages_stats", lambda: pool.pending(clear=True))
+    src, dst = pool.pending(clear=True)
+    assert len(src) == len(dst) == 0
+    monkeypatch.undo()
+
+    def more():
+        pool.resize(pool.fork(a), 31)
+
+    between("phx_pages_stats", more)
+    src, dst = pool.pending(clear=True)
+    assert len(src) == len(dst) == 1 and pool.stats()[2] == 0
