@@ -75,10 +75,20 @@ class ScalarArg(ctypes.Structure):
     _fields_ = [("pos", ctypes.c_uint32), ("bytes", ctypes.c_uint32), ("bits", ctypes.c_uint64)]
 
 
+def _fit32(*sizes):
+    """Whether none would wrap around as an int32."""
+    return all(-(1 << 31) <= x < 1 << 31 for x in sizes)
+
+
 class Kv4Cache(ctypes.Structure):
     """phx_kv4_cache: a pool of 4-bit key and value pages (device address)."""
     _fields_ = [("pool", ctypes.c_uint64), ("pages", ctypes.c_int64), ("heads", ctypes.c_int32),
                 ("head_dim", ctypes.c_int32), ("page_tokens", ctypes.c_int32)]
+
+    def __init__(self, pool=0, pages=0, heads=0, head_dim=0, page_tokens=0):
+        if not _fit32(heads, head_dim, page_tokens):
+            raise PhxError(PHX_E_INVALID, f"cache of {heads} heads of {head_dim}, {page_tokens} tokens a page")
+        super().__init__(pool, pages, heads, head_dim, page_tokens)
 
 
 class Kv4Batch(ctypes.Structure):
@@ -498,6 +508,8 @@ def launch_gemv_w4(stream, dtype, a, w, scales, zeros, c, M, N, K, group, alpha=
 
 
 def kv4_page_bytes(heads, head_dim, page_tokens):
+    if not _fit32(heads, head_dim, page_tokens):
+        return 0
     return lib().phx_kv4_page_bytes(heads, head_dim, page_tokens)
 
 
@@ -577,6 +589,8 @@ class Pages:
     def __init__(self, pages, page_tokens):
         self.handle = None
         h = _vp()
+        if not _fit32(pages, page_tokens):
+            raise PhxError(PHX_E_INVALID, f"pages_create: {pages} pages of {page_tokens} tokens")
         check(lib().phx_pages_create(ctypes.byref(h), pages, page_tokens))
         self.handle, self.pages = h.value, pages
 

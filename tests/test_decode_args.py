@@ -287,3 +287,18 @@ def test_pages_apply_of_no_layers_keeps_its_copies():
     for layers in (0, -1, 65536):
         assert _rc(lambda: pool.apply(None, A, 4096, layers, 8 * 4096)) == px.PHX_E_INVALID
         assert pool.stats()[2] == 1
+
+
+def test_sizes_that_would_wrap_around():
+    for far in (1 << 32, 1 << 31, -(1 << 32), 1 << 64):
+        assert _rc(lambda: px.Pages(8 + far, 4)) == px.PHX_E_INVALID
+        assert _rc(lambda: px.Pages(8, 4 + far)) == px.PHX_E_INVALID
+        for i in range(3):
+            sizes = [2, 64, 32]
+            sizes[i] += far
+            assert _rc(lambda: px.Kv4Cache(A, 9, *sizes)) == px.PHX_E_INVALID
+            assert px.kv4_page_bytes(*sizes) == 0
+    assert _rc(lambda: px.Kv4Cache(A, 9, 2, head_dim=64 + (1 << 32), page_tokens=32)) == px.PHX_E_INVALID
+    c = px.Kv4Cache(A, 9, 2, head_dim=64, page_tokens=32)
+    assert (c.pool, c.pages, c.heads, c.head_dim, c.page_tokens) == (A, 9, 2, 64, 32)
+    assert px.Kv4Cache().heads == 0
