@@ -488,7 +488,11 @@ def w4_quantize(b, group):
     padded[:K] = b
     padded = padded.reshape(groups, group, N)
     lo, hi = np.minimum(padded.min(1), 0), np.maximum(padded.max(1), 0)
-    scales = ((hi - lo) / 15).astype(np.float16)
+    with np.errstate(over="ignore", invalid="ignore"):
+        scales = ((hi - lo) / 15).astype(np.float16)
+    if not np.isfinite(scales).all():
+        raise PhxError(PHX_E_INVALID, "w4_quantize: weights that are infinite or NaN, or a range of more "
+                       "than 15 * 65504")
     scales = np.where(scales > 0, scales, np.float16(2.0 ** -24))
     s = scales.astype(np.float64)
     zeros = np.clip(np.rint(-lo / s), 0, 15)

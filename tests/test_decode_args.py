@@ -302,3 +302,13 @@ def test_sizes_that_would_wrap_around():
     c = px.Kv4Cache(A, 9, 2, head_dim=64, page_tokens=32)
     assert (c.pool, c.pages, c.heads, c.head_dim, c.page_tokens) == (A, 9, 2, 64, 32)
     assert px.Kv4Cache().heads == 0
+
+
+def test_w4_quantize_refuses_what_no_scale_holds():
+    b = np.zeros((64, 3))
+    b[40, 1] = 15 * 65504.0
+    codes, scales, zeros = px.w4_quantize(b, 32)
+    assert scales[1, 1] == 65504 and codes[40, 1] == 15
+    for bad in (15.1 * 65504 * 1.001, -1e300, np.nan, np.inf, -np.inf):
+        b[40, 1] = bad
+        assert _rc(lambda: px.w4_quantize(b, 32)) == px.PHX_E_INVALID, bad
