@@ -493,6 +493,9 @@ def w4_quantize(b, group):
     if not np.isfinite(scales).all():
         raise PhxError(PHX_E_INVALID, "w4_quantize: weights that are infinite or NaN, or a range of more "
                        "than 15 * 65504")
+    # below 2^-14 f16 numbers are 2^-24 apart: one too small leaves a weight out of reach
+    short = (scales < np.float16(2.0 ** -14)) & (scales.astype(np.float64) < (hi - lo) / 15)
+    scales = np.where(short, np.nextafter(scales, np.float16(1)), scales)
     scales = np.where(scales > 0, scales, np.float16(2.0 ** -24))
     s = scales.astype(np.float64)
     zeros = np.clip(np.rint(-lo / s), 0, 15)

@@ -312,3 +312,18 @@ def test_w4_quantize_refuses_what_no_scale_holds():
     for bad in (15.1 * 65504 * 1.001, -1e300, np.nan, np.inf, -np.inf):
         b[40, 1] = bad
         assert _rc(lambda: px.w4_quantize(b, 32)) == px.PHX_E_INVALID, bad
+
+
+def test_w4_quantize_of_tiny_weights():
+    # scales below f16's normal numbers are up to half of themselves off when
+    # rounded to the nearest, which left the largest weights out of reach
+    rng = np.random.default_rng(6)
+    for size in 2.0 ** -np.arange(8.0, 24.0):
+        b = (rng.random((64, 40)) - 0.3) * size
+        codes, scales, zeros = px.w4_quantize(b, 32)
+        s = scales.astype(np.float64)[np.arange(64) // 32]
+        back = (codes.astype(np.float64) - zeros[np.arange(64) // 32]) * s
+        assert (np.abs(back - b) <= s * (1.0 + 15 * 2.0 ** -11)).all(), size
+        # no step is wider than the range takes, but for the f16 it is rounded to
+        want = np.stack([np.ptp(np.concatenate([b[g:g + 32], b[:1] * 0]), axis=0) for g in (0, 32)]) / 15
+        assert (scales <= want * (1 + 2.0 ** -11) + 2.0 ** -24).all(), size
