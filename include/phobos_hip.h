@@ -340,7 +340,8 @@ int phx_w4_pack(phx_stream s, uint64_t codes, uint64_t packed, int64_t N, int64_
  * [M, K] and C [M, N] of type t with rows lda and ldc elements apart (0: K
  * and N).  K % 8 == 0, N below 2^25; A's rows and the packed codes start 16-byte
  * aligned (lda % 8 == 0 for f16, % 4 for f32).  Codes less zero points and
- * f16 operands enter the products exactly, f32 operands with all their bits;
+ * f16 operands enter the products exactly, f32 operands with all their bits
+ * (but for what an element has below 2^-126, which counts as 0);
  * products, sums and scales are f32, and C is rounded once from
  * fl(fl(alpha*acc) + fl(beta*c)), not read when beta == 0.  C overlaps no
  * other operand.  An infinity in an f32 row makes the row NaN.  A launch of

@@ -53,7 +53,8 @@ __device__ __forceinline__ uint32_t in_vgpr(uint32_t x) {
 }
 
 // Rows of A as matrix operands: of each k one f16 term, or three bf16 terms of an
-// f32, which hold its 24 bits.
+// f32, which hold its 24 bits (those from 2^-126 up: the matrix instructions
+// take a bf16 below its normal numbers as 0).
 template <typename T>
 struct Rows;
 template <>

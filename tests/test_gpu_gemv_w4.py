@@ -267,3 +267,26 @@ def test_many_columns(px_gpu, stream, bits, M, N, K, group):
     want, mag = a.astype(np.float64) @ w, np.abs(a.astype(np.float64)) @ np.abs(w)
     got = _run(px, stream, dtype, a, codes, scales, zeros, group)
     assert (np.abs(got - want) <= _bound(want, mag, K, t)).all()
+
+
+@pytest.mark.parametrize("M,N,K", [(3, 40, 520), (40, 300, 1032)])
+@pytest.mark.parametrize("bits,exponent", [(16, -8), (16, -14), (16, -17), (16, -20), (32, 40), (32, -104),
+                                           (32, -112), (32, -120), (32, -126), (32, -135)])
+def test_rows_of_tiny_and_large_elements(px_gpu, stream, bits, exponent, M, N, K):
+    # what an f32 element has below 2^-126 counts as 0; f16 elements enter whole,
+    # subnormal ones too
+    px = px_gpu
+    rng = np.random.default_rng(M + 200 - exponent)
+    dtype = px.F16 if bits == 16 else px.F32
+    t = _np(px, dtype)
+    codes = rng.integers(0, 16, (K, N)).astype(np.uint8)
+    scales = np.full((-(-K // 32), N), 64.0)
+    a = np.ldexp(rng.standard_normal((M, K)), exponent).astype(t)
+    w = _weights(codes, scales, None, 32)
+    want, mag = a.astype(np.float64) @ w, np.abs(a.astype(np.float64)) @ np.abs(w)
+    got = _run(px, stream, dtype, a, codes, scales, None, 32)
+    lost = np.abs(w).sum(0) * 2.0 ** -126 if bits == 32 else 0.0
+    # (of a sum of f16 subnormals the matrix instructions keep 20 bits: one
+    # rounding in every 32 products)
+    lost = lost + (mag * 2.0 ** -20 if bits == 16 else 0.0)
+    assert (np.abs(got - want) <= _bound(want, mag, K, t) + lost).all()
