@@ -464,8 +464,10 @@ int phx_pages_pending(phx_pages p, int32_t *src, int32_t *dst, int64_t cap, int6
 /* Launches the pending copies in the pool at `pool` and clears them: to be
  * called on the stream of the cache's work after resizes and compactions and
  * before the cache is read or written with the new tables.  Arguments as
- * phx_pages_copy; copies that are pending take at least one layer.  If it
- * fails they stay pending. */
+ * phx_pages_copy; copies that are pending take at least one layer, and are
+ * refused on a stream that is being captured, as each replay would copy the
+ * pages once more, over what was written since (phx_pages_copy can be
+ * captured).  If it fails they stay pending. */
 int phx_pages_apply(phx_pages p, phx_stream s, uint64_t pool, size_t page_bytes, int64_t layers,
                     uint64_t layer_stride);
 /* Copies page src[i] to page dst[i], i < n, in each of `layers` pools

@@ -274,6 +274,15 @@ int phx_pages_apply(phx_pages p, phx_stream s, uint64_t pool, size_t page_bytes,
         if (layers < 1 && !p.pending.empty())
             return set_error(PHX_E_INVALID, "pages_apply: %zu copies are pending in %lld layers",
                              p.pending.size(), (long long)layers);
+        // captured, they would not have run, and every replay would run them again
+        hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+        if (s && !p.pending.empty()) {
+            hipError_t e = hipStreamIsCapturing((hipStream_t)s, &capture);
+            if (e != hipSuccess) return hip_error(e, "hipStreamIsCapturing");
+        }
+        if (capture != hipStreamCaptureStatusNone)
+            return set_error(PHX_E_INVALID, "pages_apply: %zu copies are pending on a stream that is "
+                             "being captured", p.pending.size());
         std::vector<int32_t> src, dst;
         for (const Copy &c : p.pending) {
             src.push_back(c.src);

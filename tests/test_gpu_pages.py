@@ -96,3 +96,39 @@ def test_copies_in_a_captured_graph(px_gpu):
         assert (got[[0, 3, 5]] == 1000 + i).all() and np.array_equal(got[[1, 2, 4]], host[[1, 2, 4]])
     g.destroy()
     s.destroy()
+
+
+def test_apply_is_no_part_of_a_graph(px_gpu):
+    # replayed, it would copy the old pages over what was written since
+    px = px_gpu
+    host = np.arange(6 * 64, dtype=np.uint32).reshape(6, 64)
+    buf, s = px.DeviceBuffer.from_array(host), px.Stream()
+    pool = px.Pages(6, 4)
+    a = pool.new()
+    pool.resize(a, 2)
+    b = pool.fork(a)
+    pool.resize(b, 3)
+    refused = []
+
+    def body():
+        px.pages_copy(s, buf, 6, 256, [3], [4])
+        try:
+            pool.apply(s, buf, 256)
+        except px.PhxError as e:
+            refused.append(e.code)
+
+    g = Graph(s, body)
+    assert refused == [px.PHX_E_INVALID] and pool.stats()[2] == 1
+    pool.apply(s, buf, 256)
+    assert pool.stats()[2] == 0
+    g.replay()
+    # with nothing pending there is nothing to launch, captured or not
+    quiet = Graph(s, lambda: (pool.apply(s, buf, 256), px.pages_copy(s, buf, 6, 256, [3], [5])))
+    quiet.replay()
+    s.synchronize()
+    got = buf.download(np.uint32, host.shape)
+    assert np.array_equal(got[pool.table(b)[0]], host[0])
+    assert np.array_equal(got[[4, 5]], host[[3, 3]])
+    g.destroy()
+    quiet.destroy()
+    s.destroy()
