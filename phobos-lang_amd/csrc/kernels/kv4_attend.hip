@@ -446,15 +446,12 @@ __device__ __forceinline__ void attend(const PhxKv4 &p) {
     if (first >= s.count) return;
     int64_t last = (col0 + COLS - 1) / ratio;
     if (last >= s.count) last = s.count - 1;
-    // keys that some column sees, and that all columns with a row see
-    int64_t most = p.causal ? s.tokens - s.count + last + 1 : s.tokens;
-    int64_t least = p.causal ? s.tokens - s.count + first + 1 : s.tokens;
+    int64_t most = p.causal ? s.tokens - s.count + last + 1 : s.tokens;  // keys that some column sees
     if (most < 0) most = 0;
-    if (least < 0) least = 0;
 
     const uint32_t steps = (uint32_t)(most + KEYS - 1) / KEYS;
     const uint32_t per = (steps + p.splits - 1) / p.splits;
-    const uint32_t end = min((split + 1) * per, steps), seen = (uint32_t)least / KEYS;
+    const uint32_t end = min((split + 1) * per, steps);
     const uint32_t units = (uint32_t)(most + 31) / 32;
     base += split * per;
     int32_t ids;
