@@ -14,13 +14,15 @@
 // Few rows are bound by the codes' bytes, and by latency where those are few:
 // every code is read once, two blocks of a wave ahead. 16384 x 8192 in groups of
 // 128, f16: 1 row 16.7 us (4.2 TB/s), 16 rows 19.4 us; f32: 27.1 and 35.9 us.
-// 64 rows of 16384 x 8192 take 30.2 us (570 TFLOP/s; f32 60.8 us): unpacking costs
-// as many cycles as the products, and the rows pass through LDS in every
-// workgroup.
+// 64 rows of 16384 x 8192 take 30.2 us (570 TFLOP/s; f32 60.8 us). Of a CU's cycles
+// the vector instructions are busy 48 %, LDS 41 % (a row's operand read from
+// it serves one product) and the matrix cores 26 %, which four waves a SIMD
+// overlap in part.
 // A split of N in tiles leaves CUs idle below 4096 columns; there 8 to 16 waves
 // share a tile's K. A scale and a zero point are loaded by a quarter of a wave
-// for the groups of a block and handed around by the lanes (groups of 32, 64 rows,
-// 16384 x 8192, in another tile: 47.4 us; every lane loading all of them 64.1).
+// for the groups of a block and handed around by the lanes. Groups of 32 cost
+// more than their bytes (zero points, 16384 x 8192, f16: 1 row 21.5 us against 16.6
+// in groups of 128, 64 rows 40.1 against 31.8).
 #include "phx_common.h"
 #include "phx_decode.h"
 
@@ -443,6 +445,9 @@ __device__ __forceinline__ void gemm_w4(const PhxGemvW4 &p) {
     GEMM(T, suffix, MT, WN, WK, 1)                                                              \
     GEMM(T, suffix, MT, WN, WK, 2)                                                              \
     GEMM(T, suffix, MT, WN, WK, 4)
+// (Three f32 forms are past their registers, by what the compiler spills, and are
+// slower for it: n2_w12 in groups of 64 and 32 by 8 and 42, n4_w8 in groups of 32 by
+// 32.  16 rows, 16384 x 8192: 45.6 us in groups of 32, 36.9 of 64, 35.7 of 128.)
 GROUPS(_Float16, f16, 1, 8)
 GROUPS(_Float16, f16, 1, 16)
 GROUPS(_Float16, f16, 4, 8)

@@ -130,7 +130,8 @@ __device__ __forceinline__ void load_v(phx_u4 *to, const PHX_GLOBAL char *head, 
 
 // Eight codes of a key as f16: 16 and the code behind it, and for queries of two
 // terms 24 less, the middle.  (Sums of 16 + c from -24 sum_d q_d on pass through
-// several times their result: f32 outputs were 2.4e-6 off, 0.6e-6 without.  For f16
+// several times their result: f32 outputs of a prompt's chunk were 2.4e-6 off,
+// 0.6e-6 without.  For f16
 // queries, whose outputs round at 2^-11, that saves the subtraction.)
 template <int TERMS>
 __device__ __forceinline__ phx_h8 keys(uint32_t w, uint32_t mask, uint32_t one) {
@@ -625,8 +626,8 @@ __device__ __forceinline__ void attend(const PhxKv4 &p) {
 // between. Bound by the vector instructions: for 32 keys and 32 columns about 220
 // of a wave, 110 of them the softmax, next to 48 matrix instructions (2 x 1000
 // rows over 4133 keys, 8 x 4 heads of 128: 211 us, 565 TFLOP/s of the products
-// without the weights' second term; a wave unpacking for its own 64 columns
-// alone 425).
+// without the weights' second term; vector instructions are busy 69 % of the
+// cycles, LDS 40 % and the matrix cores 39 %, at two waves a SIMD).
 template <int D>
 struct Chunk {
     static constexpr int KEYS = 8192 / D;     // 16 KiB of f16 each for K and V
@@ -983,6 +984,7 @@ __device__ __forceinline__ void combine(const PhxKv4 &p) {
     extern "C" __global__ __launch_bounds__(512) void kv4_combine_##suffix(PhxKv4 p) {          \
         combine<T, D>(p);                                                                       \
     }
+// (f32, D 64, c1_g2_w16 spills 7 of its 128 registers, no other one any.)
 #define ALL(T, D, suffix)                                                                       \
     ATTEND(T, D, suffix, 1, 4, 4, 2)                                                            \
     ATTEND(T, D, suffix, 1, 2, 4, 2)                                                            \
