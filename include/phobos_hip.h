@@ -416,6 +416,9 @@ int phx_kv4_read(phx_stream s, const phx_kv4_cache *cache, const phx_kv4_batch *
  * (22 bits); scores, statistics and sums are f32.  A query that is infinite or
  * NaN makes its row and head NaN.  A scale of V that is not positive counts as
  * 2^-24.
+ * A launch's form goes by max_q and q_heads / heads for every sequence: where
+ * some have a chunk of rows and others one, a call for each kind is faster
+ * (512 rows and 31 single tokens: 222 us in two calls, 1490 in one).
  * A launch too small to fill the GPU is split over the keys when s has a
  * workspace bound that holds the parts (phx_stream_set_workspace,
  * phx_kv4_split_plan), else it runs unsplit.  A captured launch keeps the

@@ -131,8 +131,8 @@ __device__ __forceinline__ void load_v(phx_u4 *to, const PHX_GLOBAL char *head, 
 // Eight codes of a key as f16: 16 and the code behind it, and for queries of two
 // terms 24 less, the middle.  (Sums of 16 + c from -24 sum_d q_d on pass through
 // several times their result: f32 outputs of a prompt's chunk were 2.4e-6 off,
-// 0.6e-6 without.  For f16
-// queries, whose outputs round at 2^-11, that saves the subtraction.)
+// 0.6e-6 without.  For f16 queries, whose outputs round at 2^-11, that saves the
+// subtraction.)
 template <int TERMS>
 __device__ __forceinline__ phx_h8 keys(uint32_t w, uint32_t mask, uint32_t one) {
     const phx_h8 k = h8((w << 6 & mask) | one, (w << 2 & mask) | one, (w >> 2 & mask) | one,
