@@ -445,9 +445,10 @@ __device__ __forceinline__ void gemm_w4(const PhxGemvW4 &p) {
     GEMM(T, suffix, MT, WN, WK, 1)                                                              \
     GEMM(T, suffix, MT, WN, WK, 2)                                                              \
     GEMM(T, suffix, MT, WN, WK, 4)
-// (Three f32 forms are past their registers, by what the compiler spills, and are
-// slower for it: n2_w12 in groups of 64 and 32 by 8 and 42, n4_w8 in groups of 32 by
-// 32.  16 rows, 16384 x 8192: 45.6 us in groups of 32, 36.9 of 64, 35.7 of 128.)
+// (Three f32 forms spill registers: n2_w12 in groups of 64 and 32 8 and 42 of 168,
+// n4_w8 in groups of 32 32 of 256.  16 rows in groups of 128, 64 and 32: 8192 x 4096
+// in the first 13.5, 14.5 and 19.1 us, 16384 x 8192 in the second 35.7, 36.9 and 45.6;
+// 1 row 26.8, 27.7 and 29.3.)
 GROUPS(_Float16, f16, 1, 8)
 GROUPS(_Float16, f16, 1, 16)
 GROUPS(_Float16, f16, 4, 8)
