@@ -483,6 +483,71 @@ int phx_pages_copy(phx_stream s, uint64_t pool, int64_t pages, size_t page_bytes
                    const int32_t *src, const int32_t *dst, int64_t n, int64_t layers,
                    uint64_t layer_stride);
 
+/* ------------------------------------------------------------ rows and weights in 8 bits */
+/* What lies between two attentions when a layer's weights are held in 8 bits:
+ * the norm that turns rows into 8-bit ones, products of those with the weights,
+ * dense or grouped by expert, and the gated activation between two products.
+ * No counterparts in the reference, whose GEMMs read f32 and f16
+ * (examples/gemm_fp16.ph:1-40).  Launches, streams, threads, checks and graphs
+ * are as of the decode operators above.
+ *
+ * Codes are e4m3 (1 sign, 4 exponent and 3 mantissa bits, largest 448, no
+ * infinities, NaN 0x7f and 0xff).  Each 128 of a row, counted from its start, and
+ * each 128 x 128 of a weight, counted from its corner, the last ones as far as
+ * they go, have a scale (f32): a code c stands for c * scale.
+ *
+ * To write a block of a row, with t its values in f32 and a the largest magnitude
+ * among them, code = e4m3(448 t / a) of the exact quotient, ties to even, and 0
+ * for a block of zeros; its scale is given with each operator.  A block with an
+ * infinity or a NaN has codes of NaN and a scale of NaN.  K % 16 == 0. */
+typedef struct {
+    uint64_t codes;  /* [rows][ld], 16-byte aligned */
+    uint64_t scales; /* f32 [rows][lds], 16-byte aligned, the first ceil(k/128) of each */
+    int64_t rows;
+    int64_t k;   /* at most 2^22, as ld and lds */
+    int64_t ld;  /* bytes from row to row, ld % 16 == 0 (0: k) */
+    int64_t lds; /* scales from row to row, lds % 4 == 0 (0: ceil(k/512)*4) */
+} phx_f8_rows;
+typedef struct {
+    uint64_t codes;  /* [experts][n][k], 16-byte aligned: k next to each other */
+    uint64_t scales; /* f32 [experts][ceil(n/128)][ceil(k/128)] */
+    int64_t experts; /* 1 for a dense product, at most 65535 */
+    int64_t n;
+    int64_t k;
+} phx_f8_weights;
+
+/* The root-mean-square norm of M rows of K (at most 32768) elements of type t:
+ * H = round(X + R), or X where r is 0, stored where h is not 0 (it may be x or r);
+ * f = 1/sqrt(mean(H^2) + eps); of t = H * gain (f32 products) the codes go to q,
+ * with the scales a * f / 448 (nullable), and round(f * t) to Y (0: not wanted).
+ * The squares are summed in 64 bits.  gain is [K] of type t.  Rows are ldx, ldr,
+ * ldh and ldy elements apart (0: K), start 16-byte aligned and in whole 16-byte
+ * chunks.  q has M rows of K.  Outputs overlap nothing else. */
+int phx_norm_f8(phx_stream s, phx_dtype t, uint64_t x, uint64_t r, uint64_t gain, uint64_t h,
+                uint64_t y, const phx_f8_rows *q, int64_t M, int64_t K, float eps, int64_t ldx,
+                int64_t ldr, int64_t ldh, int64_t ldy);
+/* The gated activation: of each row of U, the gates [0, K) and the values
+ * [K, 2K) next to them, gate / (1 + exp(-gate)) * value in f32 (within 2^-20)
+ * into the rows q, with the scales a / 448.  Rows of U (type t) are ldu elements
+ * apart (0: 2K), start 16-byte aligned and in whole 16-byte chunks. */
+int phx_glu_f8(phx_stream s, phx_dtype t, uint64_t u, const phx_f8_rows *q, int64_t ldu);
+/* C = alpha * A @ W^T + beta * C of type t, [A's rows, n], rows ldc elements apart
+ * (0: n): the products of a row's and a weight's codes in a block of 128 of K are
+ * summed, then scaled by both scales and added in f32; C is rounded once from
+ * fl(fl(alpha*acc) + fl(beta*c)), not read when beta == 0.  C overlaps no other
+ * operand. */
+int phx_gemm_f8(phx_stream s, const phx_f8_rows *a, const phx_f8_weights *w, phx_dtype t, uint64_t c,
+                float alpha, float beta, int64_t ldc);
+/* The same for M rows of C sorted by expert: row i, starts[e] <= i < starts[e+1],
+ * is A's row list[i] (i where list is 0) times the weights of expert e.  starts is
+ * i32 [experts+1] and list i32 [M], both in device memory.  starts ascend from 0
+ * up to at most M (cut to 0 .. M; one below an earlier one counts as that one); rows of C
+ * before the first and from the last on are left as they are.  A row may be
+ * listed any number of times; an entry that is no row of A is a row of zeros. */
+int phx_gemm_f8_grouped(phx_stream s, const phx_f8_rows *a, const phx_f8_weights *w,
+                        uint64_t starts, uint64_t list, int64_t M, phx_dtype t, uint64_t c,
+                        float alpha, float beta, int64_t ldc);
+
 /* ------------------------------------------------------------ inputs */
 /* Lcg::unit_f32s (phobos-base/src/rng.rs:9-25) into host memory. */
 int phx_lcg_fill_f32(uint64_t seed, size_t n, float *out);

@@ -1,0 +1,191 @@
+// Kernels that write rows in 8 bits: the root-mean-square norm with the
+// residual's addition, and the gated activation (the layout and the arithmetic:
+// include/phobos_hip.h, phx_norm_f8 and phx_glu_f8).
+#include "f8.h"
+
+namespace {
+
+template <typename T>
+struct Chunk {  // 16 bytes of a row
+    static constexpr int N = 16 / sizeof(T);
+    static constexpr int LANES = PHX_F8_BLOCK / N;  // of a scale's block
+    float v[N];
+
+    __device__ __forceinline__ void load(const PHX_GLOBAL T *p) {
+        const phx_u4 w = *(const PHX_GLOBAL phx_u4 *)p;
+        if constexpr (sizeof(T) == 2) {
+            const phx_h8 h = __builtin_bit_cast(phx_h8, w);
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = (float)h[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = __builtin_bit_cast(float, (uint32_t)w[i]);
+        }
+    }
+    __device__ __forceinline__ void store(PHX_GLOBAL T *p) const {
+        if constexpr (sizeof(T) == 2) {
+            phx_h8 h;
+#pragma unroll
+            for (int i = 0; i < N; ++i) h[i] = (_Float16)v[i];
+            *(PHX_GLOBAL phx_h8 *)p = h;
+        } else {
+            *(PHX_GLOBAL phx_f4 *)p = (phx_f4){v[0], v[1], v[2], v[3]};
+        }
+    }
+};
+
+// The largest magnitude of a block, in all its lanes.
+template <int LANES>
+__device__ __forceinline__ uint32_t block_largest(uint32_t a) {
+#pragma unroll
+    for (int s = 1; s < LANES; s <<= 1) a = max(a, (uint32_t)__shfl_xor((int)a, s));
+    return a;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_codes(const PhxF8Rows &p, int64_t row, uint32_t k,
+                                            const float (&t)[Chunk<T>::N], uint32_t a) {
+    uint32_t out[Chunk<T>::N / 4];
+    f8_codes(t, a, out);
+    PHX_GLOBAL char *to = (PHX_GLOBAL char *)p.q + row * p.ldq + k;
+    if constexpr (sizeof(T) == 2)
+        *(PHX_GLOBAL phx_u2 *)to = (phx_u2){out[0], out[1]};
+    else
+        *(PHX_GLOBAL uint32_t *)to = out[0];
+}
+
+// R threads (waves of one workgroup) take a row, chunks of 16 bytes next to their
+// neighbours', up to C chunks a thread, which stay in registers between the sum and
+// what follows it: every byte is read once and written once.
+template <typename T, int R, int C>
+__device__ __forceinline__ void norm_f8(const PhxF8Rows &p) {
+    constexpr int N = Chunk<T>::N, WAVES = R / 64;
+    __shared__ double sums[WAVES];
+    const int64_t row = (int64_t)blockIdx.x * (blockDim.x / R) + threadIdx.x / R;
+    if (row >= p.M) return;  // (whole waves, and with several waves a row no workgroup)
+    const uint32_t at = threadIdx.x % R * N, K = (uint32_t)p.K;
+    Chunk<T> h[C];
+    double sum = 0;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const uint32_t k = at + c * (R * N);
+#pragma unroll
+        for (int i = 0; i < N; ++i) h[c].v[i] = 0;
+        if (k >= K) continue;
+        h[c].load((const PHX_GLOBAL T *)p.x + row * p.ldx + k);
+        if (p.r) {
+            Chunk<T> r;
+            r.load((const PHX_GLOBAL T *)p.r + row * p.ldr + k);
+            // what is stored is what the norm reads
+#pragma unroll
+            for (int i = 0; i < N; ++i) h[c].v[i] = (float)(T)(h[c].v[i] + r.v[i]);
+        }
+        if (p.h) h[c].store((PHX_GLOBAL T *)p.h + row * p.ldh + k);
+        // squares of f32 are exact in 64 bits and leave its range nowhere
+#pragma unroll
+        for (int i = 0; i < N; ++i) sum = fma((double)h[c].v[i], (double)h[c].v[i], sum);
+    }
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) sum += __shfl_xor(sum, s);
+    if (WAVES > 1) {
+        if (threadIdx.x % 64 == 0) sums[threadIdx.x / 64] = sum;
+        __syncthreads();
+        sum = sums[0];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) sum += sums[w];
+    }
+    const double factor = 1.0 / sqrt(sum / (double)p.K + (double)p.eps);
+    const float f = (float)factor;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const uint32_t k = at + c * (R * N);
+        const bool live = k < K;
+        uint32_t a = 0;
+        if (live) {
+            Chunk<T> g;
+            g.load((const PHX_GLOBAL T *)p.gain + k);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                h[c].v[i] = h[c].v[i] * g.v[i];
+                a = max(a, f8_magnitude(h[c].v[i]));
+            }
+        }
+        if (p.q) {
+            a = block_largest<Chunk<T>::LANES>(a);
+            if (live) {
+                store_codes<T>(p, row, k, h[c].v, a);
+                if (threadIdx.x % Chunk<T>::LANES == 0)
+                    ((PHX_GLOBAL float *)p.scales)[row * p.lds + k / PHX_F8_BLOCK] =
+                        a < 0x7f800000u
+                            ? (float)((double)__builtin_bit_cast(float, a) * factor / 448.0)
+                            : __builtin_nanf("");
+            }
+        }
+        if (p.y && live) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) h[c].v[i] *= f;
+            h[c].store((PHX_GLOBAL T *)p.y + row * p.ldy + k);
+        }
+    }
+}
+
+// e^x: the power of two of x log2(e), a product in two terms so that a large x
+// keeps its bits; below -100, where one plus it is one, that of -100.
+__device__ __forceinline__ float exp_of(float x) {
+    x = fmaxf(x, -100.0f);
+    const float e = 1.44269504f, rest = 1.92596303e-8f;  // log2(e) in two terms
+    const float p = x * e;
+    const float low = __builtin_fmaf(x, e, -p) + x * rest;
+    const float y = __builtin_amdgcn_exp2f(p);
+    return __builtin_isfinite(y) ? __builtin_fmaf(y * low, 0.693147181f, y) : y;
+}
+
+// A block of 128 of a row to 16 or 32 lanes; blocks of a row next to each other.
+template <typename T>
+__device__ __forceinline__ void glu_f8(const PhxF8Rows &p) {
+    constexpr int N = Chunk<T>::N, LANES = Chunk<T>::LANES;
+    const uint32_t blocks = ((uint32_t)p.K + PHX_F8_BLOCK - 1) / PHX_F8_BLOCK;
+    const int64_t unit = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+    const int64_t row = unit / blocks;
+    const uint32_t block = (uint32_t)(unit % blocks);
+    const uint32_t k = block * PHX_F8_BLOCK + threadIdx.x % LANES * N;
+    const bool live = row < p.M && k < p.K;
+    Chunk<T> u, v;
+    uint32_t a = 0;
+    if (live) {
+        const PHX_GLOBAL T *x = (const PHX_GLOBAL T *)p.x + row * p.ldx + k;
+        u.load(x);
+        v.load(x + p.K);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            u.v[i] = u.v[i] / (1.0f + exp_of(-u.v[i])) * v.v[i];
+            a = max(a, f8_magnitude(u.v[i]));
+        }
+    }
+    a = block_largest<LANES>(a);
+    if (!live) return;
+    store_codes<T>(p, row, k, u.v, a);
+    if (threadIdx.x % LANES == 0)
+        ((PHX_GLOBAL float *)p.scales)[row * p.lds + block] =
+            a < 0x7f800000u ? __builtin_bit_cast(float, a) / 448.0f : __builtin_nanf("");
+}
+
+}  // namespace
+
+#define NORM(T, suffix, R, C)                                                                   \
+    extern "C" __global__ __launch_bounds__(R < 256 ? 256 : R) void                             \
+        norm_f8_##suffix##_r##R##_c##C(PhxF8Rows p) {                                           \
+        norm_f8<T, R, C>(p);                                                                    \
+    }
+#define NORMS(R, C) NORM(_Float16, f16, R, C) NORM(float, f32, R, C)
+NORMS(64, 1)
+NORMS(64, 2)
+NORMS(64, 4)
+NORMS(256, 2)
+NORMS(256, 4)
+NORMS(1024, 1)
+NORMS(1024, 2)
+NORMS(1024, 4)
+NORM(float, f32, 1024, 8)
+extern "C" __global__ __launch_bounds__(256) void glu_f8_f16(PhxF8Rows p) { glu_f8<_Float16>(p); }
+extern "C" __global__ __launch_bounds__(256) void glu_f8_f32(PhxF8Rows p) { glu_f8<float>(p); }

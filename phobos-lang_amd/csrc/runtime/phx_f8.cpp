@@ -1,0 +1,211 @@
+// Entry points of the operators over 8-bit rows and weights: the norm, the gated
+// activation, products.  Arguments are checked here; what lies in device memory
+// (groups' starts, lists of rows) the kernels check themselves (gemm_f8.hip).
+#include <algorithm>
+#include <cmath>
+
+#include "../kernels/phx_f8.h"
+#include "phx_internal.h"
+
+using namespace phx;
+
+namespace {
+
+const char *const kRowsFile = "f8_rows.hsaco";
+const char *const kGemmFile = "gemm_f8.hsaco";
+
+// (file and entry are literals: aux_function knows them by address)
+int launch(const char *file, const char *entry, int64_t groups, uint32_t threads, hipStream_t s,
+           void *record) {
+    hipFunction_t f;
+    if (int rc = aux_function(file, entry, &f)) return rc;
+    void *args[] = {record};
+    hipError_t e = hipModuleLaunchKernel(f, (uint32_t)groups, 1, 1, threads, 1, 1, 0, s, args,
+                                         nullptr);
+    return e == hipSuccess ? PHX_OK : hip_error(e, entry);
+}
+
+bool known(phx_dtype t) { return t == PHX_F32 || t == PHX_F16; }
+int64_t size_of(phx_dtype t) { return t == PHX_F16 ? 2 : 4; }
+int64_t blocks_of(int64_t k) { return (k + PHX_F8_BLOCK - 1) / PHX_F8_BLOCK; }
+
+constexpr int64_t kMost = INT64_C(1) << 40;   // of a stride: products with 2^22 rows stay in 64 bits
+constexpr int64_t kMostRows = INT32_MAX;
+constexpr int64_t kMostThreads = UINT32_MAX;  // of a launch along one axis
+constexpr int64_t kMostK = 1 << 22;           // 256 rows of it are within 32-bit offsets
+
+// 8-bit rows, with their strides filled in.
+int check_f8(const phx_f8_rows *r, phx_f8_rows *out, const char *who) {
+    if (!r) return set_error(PHX_E_INVALID, "%s: null rows", who);
+    *out = *r;
+    if (r->rows < 0 || r->rows > kMostRows || r->k < 16 || r->k % 16 || r->k > kMostK)
+        return set_error(PHX_E_INVALID,
+                         "%s: 8-bit rows need 0 .. 2^31-1 rows of K elements, 16 <= K <= %lld with "
+                         "K%%16==0 (got %lld of %lld)",
+                         who, (long long)kMostK, (long long)r->rows, (long long)r->k);
+    const int64_t blocks = blocks_of(r->k);
+    if (!out->ld) out->ld = r->k;
+    if (!out->lds) out->lds = (blocks + 3) / 4 * 4;
+    if (out->ld < r->k || out->ld % 16 || out->ld > kMostK || out->lds < blocks || out->lds % 4 ||
+        out->lds > kMostK)
+        return set_error(PHX_E_INVALID,
+                         "%s: 8-bit rows must be at least K apart, in whole 16 bytes, and their scales "
+                         "at least ceil(K/128), in fours (got %lld, %lld)",
+                         who, (long long)r->ld, (long long)r->lds);
+    if (r->rows && (!r->codes || !r->scales || ((r->codes | r->scales) & 15)))
+        return set_error(PHX_E_INVALID, "%s: codes and scales must be 16-byte aligned", who);
+    return PHX_OK;
+}
+
+// Rows of `width` elements of type t, `ld` apart (0: dense).
+int check_rows(phx_dtype t, uint64_t ptr, int64_t width, int64_t *ld, const char *who,
+               const char *what) {
+    if (!*ld) *ld = width;
+    if (*ld < width || *ld > kMost || *ld * size_of(t) % 16)
+        return set_error(PHX_E_INVALID, "%s: rows of %s must be at least %lld elements apart, in "
+                         "whole 16-byte chunks (got %lld)", who, what, (long long)width,
+                         (long long)*ld);
+    if (!ptr || (ptr & 15))
+        return set_error(PHX_E_INVALID, "%s: %s must be 16-byte aligned", who, what);
+    return PHX_OK;
+}
+
+// ------------------------------------------------------------------ the norm
+struct NormForm {
+    int64_t threads, chunks;  // of a row, and of a thread
+    const char *entry[2];     // f16, f32
+};
+#define NORM(r, c) {r, c, {"norm_f8_f16_r" #r "_c" #c, "norm_f8_f32_r" #r "_c" #c}}
+const NormForm kNorms[] = {NORM(64, 1), NORM(64, 2), NORM(64, 4), NORM(256, 2), NORM(256, 4),
+                           NORM(1024, 1), NORM(1024, 2), NORM(1024, 4),
+                           {1024, 8, {nullptr, "norm_f8_f32_r1024_c8"}}};
+#undef NORM
+
+const NormForm *norm_form(phx_dtype t, int64_t K) {
+    const int64_t chunks = K * size_of(t) / 16;
+    for (const NormForm &f : kNorms)
+        if (chunks <= f.threads * f.chunks && f.entry[t == PHX_F16 ? 0 : 1]) return &f;
+    return nullptr;
+}
+
+// ------------------------------------------------------------------ products
+int product(phx_stream s, const phx_f8_rows *a, const phx_f8_weights *w, bool grouped,
+            uint64_t starts, uint64_t list, int64_t M, phx_dtype t, uint64_t c, float alpha,
+            float beta, int64_t ldc, const char *who) {
+    phx_f8_rows r;
+    if (!known(t)) return set_error(PHX_E_INVALID, "%s: unknown type %d", who, (int)t);
+    if (int rc = check_f8(a, &r, who)) return rc;
+    if (!w) return set_error(PHX_E_INVALID, "%s: null weights", who);
+    if (w->n < 1 || w->n > kMostRows || w->k != r.k || w->experts < 1 || w->experts > 65535)
+        return set_error(PHX_E_INVALID,
+                         "%s: weights of 1 .. 65535 experts, N > 0 and the rows' K (got %lld of %lld "
+                         "x %lld, rows of %lld)",
+                         who, (long long)w->experts, (long long)w->n, (long long)w->k,
+                         (long long)r.k);
+    if (!grouped && w->experts != 1)
+        return set_error(PHX_E_INVALID, "%s: %lld experts take a grouped product", who,
+                         (long long)w->experts);
+    if (!grouped) M = r.rows;
+    if (M < 0 || M > kMostRows)
+        return set_error(PHX_E_INVALID, "%s: %lld rows", who, (long long)M);
+    if (grouped && !list && M > r.rows)
+        return set_error(PHX_E_INVALID, "%s: %lld rows of C, %lld of A", who, (long long)M,
+                         (long long)r.rows);
+    if (!ldc) ldc = w->n;
+    if (ldc < w->n || ldc > kMost)
+        return set_error(PHX_E_INVALID, "%s: rows of C must be at least N apart (got %lld)", who,
+                         (long long)ldc);
+    if (M && (!w->codes || !w->scales || !c || (w->codes & 15) || (w->scales & 3) ||
+              (c & (size_of(t) - 1))))
+        return set_error(PHX_E_INVALID, "%s: weights' codes must be 16-byte aligned, their scales and "
+                         "C by element", who);
+    if (M && grouped && (!starts || ((starts | list) & 3)))
+        return set_error(PHX_E_INVALID, "%s: starts and list are i32 arrays", who);
+    const int64_t tiles = ((M + 15) / 16 + (grouped ? w->experts : 0)) * ((w->n + 15) / 16);
+    if (tiles > kMostThreads / 64)
+        return set_error(PHX_E_INVALID, "%s: %lld x %lld is too large", who, (long long)M,
+                         (long long)w->n);
+    if (int rc = on_device((hipStream_t)s)) return rc;
+    if (!M) return PHX_OK;
+    PhxF8Gemm p = {r.codes, r.scales, w->codes, w->scales, c, starts, list, M, w->n, r.k, r.rows,
+                   r.ld, r.lds, ldc, w->experts, alpha, beta, t == PHX_F16};
+    return launch(kGemmFile, "gemm_f8_first", tiles, 64, (hipStream_t)s, &p);
+}
+
+}  // namespace
+
+extern "C" {
+
+int phx_norm_f8(phx_stream s, phx_dtype t, uint64_t x, uint64_t r, uint64_t gain, uint64_t h,
+                uint64_t y, const phx_f8_rows *q, int64_t M, int64_t K, float eps, int64_t ldx,
+                int64_t ldr, int64_t ldh, int64_t ldy) {
+    const char *who = "norm_f8";
+    if (!known(t)) return set_error(PHX_E_INVALID, "%s: unknown type %d", who, (int)t);
+    if (M < 0 || M > kMostRows || K < 16 || K % 16 || K > PHX_F8_NORM_MOST)
+        return set_error(PHX_E_INVALID, "%s needs 0 .. 2^31-1 rows of K elements, 16 <= K <= %d with "
+                         "K%%16==0 (got %lld of %lld)",
+                         who, PHX_F8_NORM_MOST, (long long)M, (long long)K);
+    if (!(eps >= 0.0f) || std::isinf(eps))
+        return set_error(PHX_E_INVALID, "%s: eps %g", who, (double)eps);
+    phx_f8_rows o = {};
+    if (q) {
+        if (int rc = check_f8(q, &o, who)) return rc;
+        if (q->rows != M || q->k != K)
+            return set_error(PHX_E_INVALID, "%s: %lld rows of %lld, 8-bit rows %lld of %lld", who,
+                             (long long)M, (long long)K, (long long)q->rows, (long long)q->k);
+    }
+    if (M) {
+        if (int rc = check_rows(t, x, K, &ldx, who, "X")) return rc;
+        if (r)
+            if (int rc = check_rows(t, r, K, &ldr, who, "R")) return rc;
+        if (h)
+            if (int rc = check_rows(t, h, K, &ldh, who, "H")) return rc;
+        if (y)
+            if (int rc = check_rows(t, y, K, &ldy, who, "Y")) return rc;
+        if (!gain || (gain & 15))
+            return set_error(PHX_E_INVALID, "%s: the gain must be 16-byte aligned", who);
+        if (!y && !q) return set_error(PHX_E_INVALID, "%s: neither Y nor 8-bit rows", who);
+    }
+    const NormForm *f = norm_form(t, K);
+    const int64_t each = f->threads < 256 ? 256 / f->threads : 1;  // rows of a workgroup
+    const int64_t groups = (M + each - 1) / each, threads = std::max<int64_t>(f->threads, 256);
+    if (groups > kMostThreads / threads)
+        return set_error(PHX_E_INVALID, "%s: %lld rows are too many", who, (long long)M);
+    if (int rc = on_device((hipStream_t)s)) return rc;
+    if (!M) return PHX_OK;
+    PhxF8Rows p = {x, r, gain, h, y, o.codes, o.scales, M, K, ldx, ldr, ldh, ldy, o.ld, o.lds, eps};
+    return launch(kRowsFile, f->entry[t == PHX_F16 ? 0 : 1], groups, (uint32_t)threads,
+                  (hipStream_t)s, &p);
+}
+
+int phx_glu_f8(phx_stream s, phx_dtype t, uint64_t u, const phx_f8_rows *q, int64_t ldu) {
+    const char *who = "glu_f8";
+    if (!known(t)) return set_error(PHX_E_INVALID, "%s: unknown type %d", who, (int)t);
+    phx_f8_rows o;
+    if (int rc = check_f8(q, &o, who)) return rc;
+    if (o.rows)
+        if (int rc = check_rows(t, u, 2 * o.k, &ldu, who, "U")) return rc;
+    const int64_t per = 2 * size_of(t) == 4 ? 16 : 8;  // blocks of a workgroup
+    const int64_t groups = (o.rows * blocks_of(o.k) + per - 1) / per;
+    if (groups > kMostThreads / 256)
+        return set_error(PHX_E_INVALID, "%s: %lld rows of %lld are too many", who, (long long)o.rows,
+                         (long long)o.k);
+    if (int rc = on_device((hipStream_t)s)) return rc;
+    if (!o.rows) return PHX_OK;
+    PhxF8Rows p = {u, 0, 0, 0, 0, o.codes, o.scales, o.rows, o.k, ldu, 0, 0, 0, o.ld, o.lds, 0.0f};
+    return launch(kRowsFile, t == PHX_F16 ? "glu_f8_f16" : "glu_f8_f32", groups, 256, (hipStream_t)s,
+                  &p);
+}
+
+int phx_gemm_f8(phx_stream s, const phx_f8_rows *a, const phx_f8_weights *w, phx_dtype t, uint64_t c,
+                float alpha, float beta, int64_t ldc) {
+    return product(s, a, w, false, 0, 0, 0, t, c, alpha, beta, ldc, "gemm_f8");
+}
+
+int phx_gemm_f8_grouped(phx_stream s, const phx_f8_rows *a, const phx_f8_weights *w,
+                        uint64_t starts, uint64_t list, int64_t M, phx_dtype t, uint64_t c,
+                        float alpha, float beta, int64_t ldc) {
+    return product(s, a, w, true, starts, list, M, t, c, alpha, beta, ldc, "gemm_f8_grouped");
+}
+
+}  // extern "C"

@@ -48,9 +48,9 @@ KERNEL_NAMES = {
 CODE_OBJECTS = ["saxpy_fp32.hsaco", "gemm_fp32.hsaco", "gemm_fp16tc_fp32acc.hsaco",
                 "gemm_fp16.hsaco", "flash_attention_fp32.hsaco", "flash_attention_fp16.hsaco",
                 "matmul_cluster_fp32.hsaco", "gemv_w4.hsaco", "kv4.hsaco",
-                "kv4_attend.hsaco", "pages.hsaco"]
+                "kv4_attend.hsaco", "pages.hsaco", "f8_rows.hsaco", "gemm_f8.hsaco"]
 
-# phx_dtype of the decode operators
+# phx_dtype of the decode and the 8-bit operators
 F32 = 0
 F16 = 1
 
@@ -97,6 +97,20 @@ class Kv4Batch(ctypes.Structure):
                 ("lens", ctypes.c_uint64), ("q_starts", ctypes.c_uint64),
                 ("batch", ctypes.c_int64), ("max_q", ctypes.c_int64),
                 ("max_len", ctypes.c_int64), ("rows", ctypes.c_int64)]
+
+
+class F8Rows(ctypes.Structure):
+    """phx_f8_rows: rows in 8 bits, e4m3 codes and a scale for each 128 (device
+    addresses)."""
+    _fields_ = [("codes", ctypes.c_uint64), ("scales", ctypes.c_uint64), ("rows", ctypes.c_int64),
+                ("k", ctypes.c_int64), ("ld", ctypes.c_int64), ("lds", ctypes.c_int64)]
+
+
+class F8Weights(ctypes.Structure):
+    """phx_f8_weights: weights in 8 bits, e4m3 codes and a scale for each 128 x 128
+    (device addresses)."""
+    _fields_ = [("codes", ctypes.c_uint64), ("scales", ctypes.c_uint64),
+                ("experts", ctypes.c_int64), ("n", ctypes.c_int64), ("k", ctypes.c_int64)]
 
 
 _LIB = None
@@ -193,6 +207,13 @@ def lib():
     L.phx_kv4_read.argtypes = L.phx_kv4_append.argtypes
     L.phx_kv4_attention.argtypes = [_vp, _cache, _batch, ctypes.c_int, _u64, _u64, _i64,
                                     ctypes.c_float, ctypes.c_int, _i64, _i64]
+    _f8, _f8w = ctypes.POINTER(F8Rows), ctypes.POINTER(F8Weights)
+    L.phx_norm_f8.argtypes = [_vp, ctypes.c_int] + [_u64] * 5 + [_f8, _i64, _i64, ctypes.c_float] + \
+        [_i64] * 4
+    L.phx_glu_f8.argtypes = [_vp, ctypes.c_int, _u64, _f8, _i64]
+    L.phx_gemm_f8.argtypes = [_vp, _f8, _f8w, ctypes.c_int, _u64, ctypes.c_float, ctypes.c_float, _i64]
+    L.phx_gemm_f8_grouped.argtypes = [_vp, _f8, _f8w, _u64, _u64, _i64, ctypes.c_int, _u64,
+                                      ctypes.c_float, ctypes.c_float, _i64]
     L.phx_kv4_split_plan.argtypes = [_cache, _batch, _i64, ctypes.POINTER(ctypes.c_int),
                                      ctypes.POINTER(_sz)]
     _pi64, _pi32 = ctypes.POINTER(_i64), ctypes.POINTER(ctypes.c_int32)
@@ -553,6 +574,70 @@ def kv4_split_plan(cache, batch, q_heads):
     sp, ws = ctypes.c_int(), _sz()
     check(lib().phx_kv4_split_plan(cache, batch, q_heads, ctypes.byref(sp), ctypes.byref(ws)))
     return sp.value, ws.value
+
+
+def f8_quantize(w):
+    """Codes u8 [..., N, K] (e4m3) and scales f32 [..., ceil(N/128), ceil(K/128)] of
+    weights w [..., N, K], K next to each other as F8Weights has them: the largest
+    magnitude of each 128 x 128 has the code 448 or -448.  Host arrays."""
+    w = np.asarray(w, np.float64)
+    if w.ndim < 2 or not w.size:
+        raise PhxError(PHX_E_INVALID, f"f8_quantize: weights [..., N, K], got {w.shape}")
+    *lead, N, K = w.shape
+    nb, kb = -(-N // 128), -(-K // 128)
+    b = np.zeros((*lead, nb * 128, kb * 128))
+    b[..., :N, :K] = w
+    b = b.reshape(*lead, nb, 128, kb, 128)
+    a = np.abs(b).max((-3, -1))
+    with np.errstate(over="ignore"):
+        scales = (a / 448).astype(np.float32)
+    # (below 2^-126 an f32 scale keeps few bits, or none)
+    if not np.isfinite(scales).all() or (scales[a > 0] < 2.0 ** -126).any():
+        raise PhxError(PHX_E_INVALID, "f8_quantize: weights that are infinite or NaN, or that no f32 "
+                       "scale holds")
+    q = b * 448 / np.where(a > 0, a, 1)[..., :, None, :, None]
+    step = np.exp2(np.floor(np.log2(np.maximum(np.abs(q), 2.0 ** -6))) - 3)
+    q = np.rint(q / step) * step  # ties to even, as every rounding to e4m3
+    exponent = np.floor(np.log2(np.maximum(np.abs(q), 2.0 ** -6)))
+    # steps of 2^-9 from 0, of which each power of two from 2^-6 on takes eight
+    code = np.abs(q) / np.exp2(exponent - 3) + (exponent + 6) * 8
+    code = code.astype(np.uint8) | (np.signbit(q).astype(np.uint8) << 7)
+    return np.ascontiguousarray(code.reshape(*lead, nb * 128, kb * 128)[..., :N, :K]), scales
+
+
+def launch_norm_f8(stream, dtype, x, r, gain, h, y, q, M, K, eps, ldx=0, ldr=0, ldh=0, ldy=0):
+    """The root-mean-square norm of X + R (r 0: of X), which goes to H, times the
+    gain: in 8 bits to q (F8Rows or None) and as it is to Y (0: not wanted)
+    (phx_norm_f8)."""
+    e = _ESZ.get(dtype, 4)
+    check(lib().phx_norm_f8(_sh(stream), dtype, _addr(x, _span(M, ldx, K, e), "X"),
+                            _addr(r, _span(M, ldr, K, e), "R"), _addr(gain, K * e, "gain"),
+                            _addr(h, _span(M, ldh, K, e), "H"), _addr(y, _span(M, ldy, K, e), "Y"),
+                            q, M, K, eps, ldx, ldr, ldh, ldy))
+
+
+def launch_glu_f8(stream, dtype, u, q, ldu=0):
+    """silu(gate) * value of rows U [gates | values] into the 8-bit rows q
+    (phx_glu_f8)."""
+    span = _span(q.rows, ldu, 2 * q.k, _ESZ.get(dtype, 4)) if q else 0
+    check(lib().phx_glu_f8(_sh(stream), dtype, _addr(u, span, "U"), q, ldu))
+
+
+def launch_gemm_f8(stream, a, w, dtype, c, alpha=1.0, beta=0.0, ldc=0):
+    """C = alpha*A@W^T + beta*C of 8-bit rows and weights (phx_gemm_f8)."""
+    span = _span(a.rows, ldc, w.n, _ESZ.get(dtype, 4)) if a and w else 0
+    check(lib().phx_gemm_f8(_sh(stream), a, w, dtype, _addr(c, span, "C"), alpha, beta, ldc))
+
+
+def launch_gemm_f8_grouped(stream, a, w, starts, order, M, dtype, c, alpha=1.0, beta=0.0, ldc=0):
+    """The same for M rows sorted by expert: rows starts[e] up to starts[e+1] of C
+    are A's rows order[i] (order 0: A's own) times expert e's weights
+    (phx_gemm_f8_grouped)."""
+    span = _span(M, ldc, w.n, _ESZ.get(dtype, 4)) if w else 0
+    check(lib().phx_gemm_f8_grouped(_sh(stream), a, w,
+                                    _addr(starts, 4 * (w.experts + 1) if w else 0, "starts"),
+                                    _addr(order, 4 * M, "order"), M, dtype, _addr(c, span, "C"),
+                                    alpha, beta, ldc))
 
 
 def _page_list(x):
