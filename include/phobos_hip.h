@@ -504,7 +504,7 @@ typedef struct {
     uint64_t codes;  /* [rows][ld], 16-byte aligned */
     uint64_t scales; /* f32 [rows][lds], 16-byte aligned, the first ceil(k/128) of each */
     int64_t rows;
-    int64_t k;   /* at most 2^22, as ld and lds */
+    int64_t k;   /* at most 2^22, as ld; lds at most 2^20 */
     int64_t ld;  /* bytes from row to row, ld % 16 == 0 (0: k) */
     int64_t lds; /* scales from row to row, lds % 4 == 0 (0: ceil(k/512)*4) */
 } phx_f8_rows;
@@ -543,7 +543,8 @@ int phx_gemm_f8(phx_stream s, const phx_f8_rows *a, const phx_f8_weights *w, phx
  * i32 [experts+1] and list i32 [M], both in device memory.  starts ascend from 0
  * up to at most M (cut to 0 .. M; one below an earlier one counts as that one); rows of C
  * before the first and from the last on are left as they are.  A row may be
- * listed any number of times; an entry that is no row of A is a row of zeros. */
+ * listed any number of times; an entry that is no row of A is a row of zeros.  With
+ * a list A's codes and its scales are each below 2 GiB. */
 int phx_gemm_f8_grouped(phx_stream s, const phx_f8_rows *a, const phx_f8_weights *w,
                         uint64_t starts, uint64_t list, int64_t M, phx_dtype t, uint64_t c,
                         float alpha, float beta, int64_t ldc);

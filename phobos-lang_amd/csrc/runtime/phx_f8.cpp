@@ -34,6 +34,8 @@ constexpr int64_t kMostRows = INT32_MAX;
 constexpr int64_t kMostThreads = UINT32_MAX;  // of a launch along one axis
 constexpr int64_t kMostK = 1 << 22;           // 256 rows of it are within 32-bit offsets
 
+constexpr int64_t kMostScales = 1 << 20;      // and 256 rows of these
+
 // 8-bit rows, with their strides filled in.
 int check_f8(const phx_f8_rows *r, phx_f8_rows *out, const char *who) {
     if (!r) return set_error(PHX_E_INVALID, "%s: null rows", who);
@@ -47,7 +49,7 @@ int check_f8(const phx_f8_rows *r, phx_f8_rows *out, const char *who) {
     if (!out->ld) out->ld = r->k;
     if (!out->lds) out->lds = (blocks + 3) / 4 * 4;
     if (out->ld < r->k || out->ld % 16 || out->ld > kMostK || out->lds < blocks || out->lds % 4 ||
-        out->lds > kMostK)
+        out->lds > kMostScales)
         return set_error(PHX_E_INVALID,
                          "%s: 8-bit rows must be at least K apart, in whole 16 bytes, and their scales "
                          "at least ceil(K/128), in fours (got %lld, %lld)",
@@ -89,6 +91,26 @@ const NormForm *norm_form(phx_dtype t, int64_t K) {
 }
 
 // ------------------------------------------------------------------ products
+// A kernel of gemm_f8.hip: the columns and rows of a workgroup.
+struct GemmForm {
+    int64_t columns, rows;
+    uint32_t threads;
+    const char *entry;
+};
+const GemmForm kGemms[2][3] = {{{16, 16, 64, "gemm_f8_first"},
+                                {128, 128, 256, "gemm_f8_f16_2x2_4x4"},
+                                {256, 256, 512, "gemm_f8_f16_2x4_8x4"}},
+                               {{128, 128, 256, "gemm_f8_f32_2x2_4x4"},
+                                {128, 128, 256, "gemm_f8_f32_2x2_4x4"},
+                                {128, 128, 256, "gemm_f8_f32_2x2_4x4"}}};
+
+const GemmForm &gemm_form(phx_dtype t, int64_t M, int64_t N, int64_t experts) {
+    (void)N;
+    const GemmForm *f = kGemms[t == PHX_F16 ? 0 : 1];
+    if (M / experts <= 32) return f[0];
+    return f[M / experts <= 512 ? 1 : 2];
+}
+
 int product(phx_stream s, const phx_f8_rows *a, const phx_f8_weights *w, bool grouped,
             uint64_t starts, uint64_t list, int64_t M, phx_dtype t, uint64_t c, float alpha,
             float beta, int64_t ldc, const char *who) {
@@ -111,6 +133,9 @@ int product(phx_stream s, const phx_f8_rows *a, const phx_f8_weights *w, bool gr
     if (grouped && !list && M > r.rows)
         return set_error(PHX_E_INVALID, "%s: %lld rows of C, %lld of A", who, (long long)M,
                          (long long)r.rows);
+    if (list && (r.rows * r.ld > INT32_MAX || r.rows * r.lds * 4 > INT32_MAX))
+        return set_error(PHX_E_INVALID, "%s: with a list A's codes and scales are below 2 GiB (%lld rows "
+                         "%lld apart)", who, (long long)r.rows, (long long)r.ld);
     if (!ldc) ldc = w->n;
     if (ldc < w->n || ldc > kMost)
         return set_error(PHX_E_INVALID, "%s: rows of C must be at least N apart (got %lld)", who,
@@ -121,15 +146,18 @@ int product(phx_stream s, const phx_f8_rows *a, const phx_f8_weights *w, bool gr
                          "C by element", who);
     if (M && grouped && (!starts || ((starts | list) & 3)))
         return set_error(PHX_E_INVALID, "%s: starts and list are i32 arrays", who);
-    const int64_t tiles = ((M + 15) / 16 + (grouped ? w->experts : 0)) * ((w->n + 15) / 16);
-    if (tiles > kMostThreads / 64)
+    const GemmForm &f = gemm_form(t, M, w->n, w->experts);
+    const int64_t tiles = ((M + f.rows - 1) / f.rows + (grouped ? w->experts : 0)) *
+                          ((w->n + f.columns - 1) / f.columns);
+    if (tiles > kMostThreads / f.threads)
         return set_error(PHX_E_INVALID, "%s: %lld x %lld is too large", who, (long long)M,
                          (long long)w->n);
     if (int rc = on_device((hipStream_t)s)) return rc;
     if (!M) return PHX_OK;
     PhxF8Gemm p = {r.codes, r.scales, w->codes, w->scales, c, starts, list, M, w->n, r.k, r.rows,
-                   r.ld, r.lds, ldc, w->experts, alpha, beta, t == PHX_F16};
-    return launch(kGemmFile, "gemm_f8_first", tiles, 64, (hipStream_t)s, &p);
+                   r.ld, r.lds, ldc, w->experts, alpha, beta, t == PHX_F16,
+                   !(c & 15) && ldc * size_of(t) % 16 == 0};
+    return launch(kGemmFile, f.entry, tiles, f.threads, (hipStream_t)s, &p);
 }
 
 }  // namespace

@@ -39,7 +39,8 @@ def _weights(**kw):
 
 BAD_ROWS = [dict(codes=0), dict(scales=0), dict(codes=A + 8), dict(scales=A + 4), dict(rows=-1),
             dict(rows=1 << 31), dict(ld=128), dict(ld=152), dict(ld=-144), dict(ld=BIG), dict(lds=1),
-            dict(lds=3), dict(lds=6), dict(lds=-4), dict(lds=BIG)]
+            dict(lds=3), dict(lds=6), dict(lds=-4), dict(lds=BIG),
+            dict(lds=(1 << 20) + 4)]
 
 
 def _norm(rows=None, **kw):
@@ -114,7 +115,7 @@ def _grouped(rows=None, weights=None, **kw):
 
 OK = [{}, {"dtype": px.F32}, {"ldc": 7}, {"c": A + 2}, {"rows": {"k": 16}, "weights": {"k": 16}},
       {"weights": {"scales": A + 4}}, {"rows": {"ld": 160, "lds": 8}},
-      {"rows": {"rows": 200_000, "k": 16384}, "weights": {"n": 4096, "k": 16384}}]
+      {"rows": {"rows": 100_000, "k": 16384}, "weights": {"n": 4096, "k": 16384}}]
 BAD = [{"dtype": 2}, {"dtype": -1}, {"c": 0}, {"c": A + 1}, {"dtype": px.F32, "c": A + 2}, {"ldc": 4},
        {"ldc": -5}, {"ldc": BIG}, {"rows": "none"}, {"weights": "none"}, {"weights": {"n": 0}},
        {"weights": {"n": -1}}, {"weights": {"n": 1 << 31}}, {"weights": {"k": 128}},
@@ -147,6 +148,8 @@ def test_what_only_the_dense_product_refuses():
 
 
 @pytest.mark.parametrize("ok", [{"order": 0, "M": 3}, {"M": 100}, {"order": 0, "M": 0},
+                                {"rows": {"rows": (1 << 24) - 1, "k": 128}, "weights": {"k": 128}},
+                                {"rows": {"rows": 1 << 24}, "order": 0},
                                 {"weights": {"experts": 1}}, {"weights": {"experts": 65535}},
                                 {"M": 0, "starts": 0, "order": 0, "c": 0}])
 def test_grouped_takes(ok):
@@ -155,6 +158,7 @@ def test_grouped_takes(ok):
 
 @pytest.mark.parametrize("bad", [
     {"starts": 0}, {"starts": A + 2}, {"order": A + 1}, {"M": -1}, {"M": 1 << 31}, {"order": 0, "M": 4},
+    {"rows": {"rows": 1 << 24}}, {"rows": {"rows": 1 << 20, "ld": 2048}}, {"rows": {"rows": 1 << 20, "lds": 512}},
     {"weights": {"experts": 0}}, {"weights": {"experts": -3}}, {"weights": {"experts": 65536}},
     {"M": (1 << 31) - 1, "weights": {"n": (1 << 31) - 1}}])
 def test_grouped_refuses(bad):

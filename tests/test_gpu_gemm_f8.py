@@ -46,13 +46,25 @@ class Weights:
         self.values = f8.weight_values(codes, scales)
 
 
-def _whole(px, rng, M, N, K, E=1, pad=0):
-    """Whole numbers of up to 8 and scales of 1/4 .. 2: sums below 2^24 quarters."""
+def _whole(px, rng, M, N, K, E=1, pad=0, bits=32):
+    """Whole numbers of up to 8 and scales of 1/2 .. 2: sums below 2^24 quarters; for
+    f16, a few elements a row of up to 2 and scales of up to 1: below 2^11 quarters."""
     few = min(1.0, 2000 / K)
 
     def draw(*shape):
         v = rng.integers(-8, 9, shape) * (rng.random(shape) < few)
+        if bits == 16:  # |v| <= 2 in each row, 16 of them in a row of A
+            v = np.clip(v, -2, 2)
+            if len(shape) == 2:
+                keep = np.zeros(shape, bool)
+                for m in range(shape[0]):
+                    keep[m, rng.choice(K, min(K, 16), replace=False)] = True
+                v = v * keep
         return f8.codes_of(v)
+    if bits == 16:
+        kb, nb = -(-K // 128), -(-N // 128)
+        a = Rows(px, draw(M, K), 2.0 ** rng.integers(-1, 1, (M, kb)), pad)
+        return a, Weights(px, draw(E, N, K), 2.0 ** rng.integers(-1, 1, (E, nb, kb)))
     kb, nb = -(-K // 128), -(-N // 128)
     a = Rows(px, draw(M, K), 2.0 ** rng.integers(-1, 2, (M, kb)), pad)
     w = Weights(px, draw(E, N, K), 2.0 ** rng.integers(-1, 1, (E, nb, kb)))
@@ -119,12 +131,13 @@ SHAPES = [(1, 1, 16), (1, 16, 128), (2, 17, 144), (3, 5, 32), (15, 33, 112), (16
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
+@pytest.mark.parametrize("bits", [16, 32])
 @pytest.mark.parametrize("pad", [0, 1])
-def test_whole_numbers_are_exact(px_gpu, stream, M, N, K, pad):
+def test_whole_numbers_are_exact(px_gpu, stream, bits, M, N, K, pad):
     rng = np.random.default_rng(M * 7 + N * 3 + K)
-    a, w = _whole(px_gpu, rng, M, N, K, pad=pad)
+    a, w = _whole(px_gpu, rng, M, N, K, pad=pad, bits=bits)
     want = a.values @ w.values[0].T
-    got = _run(px_gpu, stream, 32, a, w, M, ldc=N + 3 * pad)
+    got = _run(px_gpu, stream, bits, a, w, M, ldc=N + 3 * pad)
     assert np.array_equal(got.astype(np.float64), want)
 
 
@@ -236,15 +249,16 @@ GROUPED = [(1, 1, 1, 16, 0), (5, 3, 17, 144, 1), (40, 7, 100, 272, 2), (16, 32, 
 
 
 @pytest.mark.parametrize("M,E,N,K,idle", GROUPED)
+@pytest.mark.parametrize("bits", [16, 32])
 @pytest.mark.parametrize("listed", [False, True])
-def test_grouped_whole_numbers_are_exact(px_gpu, stream, M, E, N, K, idle, listed):
+def test_grouped_whole_numbers_are_exact(px_gpu, stream, bits, M, E, N, K, idle, listed):
     rng = np.random.default_rng(M + E * 3 + N)
     src = max(1, M // 2) if listed else M
-    a, w = _whole(px_gpu, rng, src, N, K, E, pad=listed)
+    a, w = _whole(px_gpu, rng, src, N, K, E, pad=listed, bits=bits)
     starts = _groups(rng, E, M, idle)
     order = rng.integers(0, src, M) if listed else None
     want, _ = _want(a, w, starts, order, M)
-    got = _run(px_gpu, stream, 32, a, w, M, starts, order, ldc=N + 5)
+    got = _run(px_gpu, stream, bits, a, w, M, starts, order, ldc=N + 5)
     assert np.array_equal(got.astype(np.float64), want)
 
 
