@@ -112,74 +112,30 @@ __device__ __forceinline__ Tile tile_of(const PhxF8Gemm &p, uint32_t columns) {
     return t;
 }
 
-// The first form: a wave takes 16 columns by 16 rows, operands from memory.
-__device__ __forceinline__ void gemm_f8(const PhxF8Gemm &p) {
-    const uint32_t lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-    const uint32_t columns = (uint32_t)((p.N + 15) / 16);
-    const Tile t = tile_of<16>(p, columns);
-    if (!t.live) return;
-    const int64_t n0 = (int64_t)t.column * 16, n = n0 + r, m = t.m0 + r;
-    const uint32_t blocks = (uint32_t)((p.K + 127) / 128);
-    int64_t row = m < t.end ? p.list ? ((const PHX_GLOBAL int32_t *)p.list)[m] : m : -1;
-    if (row >= p.rows) row = -1;
-    const PHX_GLOBAL char *a = (const PHX_GLOBAL char *)p.a + row * p.lda;
-    const PHX_GLOBAL float *sa = (const PHX_GLOBAL float *)p.sa + row * p.lds;
-    const PHX_GLOBAL char *w = (const PHX_GLOBAL char *)p.w + (t.expert * p.N + n) * p.K;
-    const PHX_GLOBAL float *sw = (const PHX_GLOBAL float *)p.sw +
-                                 (t.expert * ((p.N + 127) / 128) + n0 / 128) * blocks;
-    phx_f4 acc = {0, 0, 0, 0};
-    for (uint32_t b = 0; b < blocks; ++b) {
-        phx_u4 x[2], y[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int64_t k = (int64_t)b * 128 + 64 * h + 16 * g;
-            x[h] = y[h] = (phx_u4){0, 0, 0, 0};
-            if (k < p.K && n < p.N) x[h] = *(const PHX_GLOBAL phx_u4 *)(w + k);
-            if (k < p.K && row >= 0) y[h] = *(const PHX_GLOBAL phx_u4 *)(a + k);
-        }
-        const v8i u = {(int)x[0][0], (int)x[0][1], (int)x[0][2], (int)x[0][3],
-                       (int)x[1][0], (int)x[1][1], (int)x[1][2], (int)x[1][3]};
-        const v8i v = {(int)y[0][0], (int)y[0][1], (int)y[0][2], (int)y[0][3],
-                       (int)y[1][0], (int)y[1][1], (int)y[1][2], (int)y[1][3]};
-        const phx_f4 sum = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-            u, v, (phx_f4){0, 0, 0, 0}, 0, 0, 0, 0, 0, 0);
-        const float s = row >= 0 ? sa[b] * sw[b] : 0.0f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(s, sum[i], acc[i]);
-    }
-    if (m >= t.end) return;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int64_t c = n0 + 4 * g + i;
-        if (c >= p.N) continue;
-        float o = p.alpha * acc[i];
-        const int64_t at = m * p.ldc + c;
-        if (p.half) {
-            PHX_GLOBAL _Float16 *to = (PHX_GLOBAL _Float16 *)p.c + at;
-            if (p.beta != 0.0f) o = o + p.beta * (float)*to;
-            *to = (_Float16)o;
-        } else {
-            PHX_GLOBAL float *to = (PHX_GLOBAL float *)p.c + at;
-            if (p.beta != 0.0f) o = o + p.beta * *to;
-            *to = o;
-        }
-    }
-}
-
 // ------------------------------------------------------------------ tiles
 // Where the tiles of WN x WM waves, each of NT x MT tiles of 16 columns by 16 rows,
-// lie, and what their lanes load.
+// lie, and what their lanes load. WK such sets of waves take every WK-th block of K,
+// each through its own part of LDS, and are added up at the end.
 //
-// A stage holds 128 k: a row of W or of A is 128 bytes, its 16-byte chunk c at place
+// A part holds 128 k: a row of W or of A is 128 bytes, its 16-byte chunk c at place
 // c ^ f(row), so that the 16 rows of an operand's read touch every bank once.
 // A lane's results of two neighbouring tiles of columns are eight neighbouring
 // columns: the rows of W that the tiles 2i and 2i + 1 take interleave in fours.
-template <int WN, int WM, int NT, int MT>
+template <int WN, int WM, int NT, int MT, int WK, int ST>
 struct Shape {
     static constexpr uint32_t WAVES = WN * WM, TN = 16 * WN * NT, TM = 16 * WM * MT;
-    static constexpr uint32_t STAGE = (TN + TM) * 128;
+    static constexpr uint32_t PART = (TN + TM) * 128;
+    // The rows' scales come four blocks at a time, a row's 16 bytes next to each other:
+    // with four sets or more those of a step's blocks in its stage, with fewer in
+    // places of their own, through registers.
+    static constexpr bool STAGED = WK >= 4;
+    static constexpr uint32_t SCALES = (TM < 64 ? 64 : TM) * 16, FOURS = STAGED ? WK / 4 : 1;
+    static constexpr uint32_t S_LOADS = SCALES / 1024 * FOURS;  // waves that load them
+    static constexpr uint32_t STAGE = PART * WK + (STAGED ? FOURS * SCALES : 0);
+    static constexpr uint32_t APART = STAGED ? 16 : 2 * SCALES;
     static constexpr uint32_t W_LOADS = TN / 8 / WAVES, A_LOADS = TM / 8 / WAVES;  // of 8 rows
     static_assert(TN % (8 * WAVES) == 0 && TM % (8 * WAVES) == 0, "whole loads a wave");
+    static_assert(WK == 1 || TN * TM * 4 * (WK / 2) <= PART * WK, "the sums fit where the stages were");
 
     static __device__ __forceinline__ uint32_t w_row(uint32_t tile, uint32_t r) {
         return 32 * (tile / 2) + 8 * (r / 4) + 4 * (tile % 2) + r % 4;
@@ -274,11 +230,19 @@ __device__ __forceinline__ void store8(const PhxF8Gemm &p, const float (&acc)[8]
         }
 }
 
-template <bool EXACT, int WN, int WM, int NT, int MT>
-__device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *s0, char *s1, char *sc) {
-    using S = Shape<WN, WM, NT, MT>;
+// Until at most STEPS times EACH of a wave's loads are on their way.
+template <uint32_t STEPS, uint32_t EACH>
+__device__ __forceinline__ void wait_loads() {
+    constexpr uint32_t LEFT = STEPS * EACH;
+    static_assert(LEFT < 64, "vmcnt's six bits");
+    __builtin_amdgcn_s_waitcnt(0x0f70 | (LEFT & 15) | (LEFT >> 4) << 14);
+}
+
+template <bool EXACT, int WN, int WM, int NT, int MT, int WK, int ST>
+__device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[ST], char *sc) {
+    using S = Shape<WN, WM, NT, MT, WK, ST>;
     const uint32_t lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t all = uniform(threadIdx.x >> 6), wave = all % S::WAVES, wk = all / S::WAVES;
     const uint32_t wn = wave % WN, wm = wave / WN;
     const uint32_t columns = (uint32_t)((p.N + S::TN - 1) / S::TN);
     const Tile t = tile_of<S::TM>(p, columns);
@@ -324,34 +288,36 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *s0, char *s1
         const int64_t at = source(row);
         a_off[i] = at < 0 ? kNone : (uint32_t)(at * p.lda) + a_k(i);
     }
-    {
-        const int64_t at = source(threadIdx.x % S::TM);
+    if (all < S::S_LOADS) {
+        const int64_t at = source(all % (S::SCALES / 1024) * 64 + lane);
         s_off = at < 0 ? kNone : (uint32_t)(at * p.lds * 4);
     }
-    auto load = [&](char *to, uint32_t b) {
+    // the i-th of this wave's loads of block b: 8 rows of W or of A
+    auto load = [&](char *stage, uint32_t b, uint32_t i) {
         const uint32_t k = b * 128;
-#pragma unroll
-        for (uint32_t i = 0; i < S::W_LOADS; ++i)
+        char *to = stage + wk * S::PART;
+        if (i < S::W_LOADS) {
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
                 wr, (lds_ptr)(to + (wave * S::W_LOADS + i) * 1024), 16,
                 k + w_k(i) < K ? w_off[i] : kNone, (int)k, 0, 0);
-#pragma unroll
-        for (uint32_t i = 0; i < S::A_LOADS; ++i)
+        } else {
+            const uint32_t j = i - S::W_LOADS;
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                ar, (lds_ptr)(to + S::TN * 128 + (wave * S::A_LOADS + i) * 1024), 16,
-                k + a_k(i) < K ? a_off[i] : kNone, (int)k, 0, 0);
+                ar, (lds_ptr)(to + S::TN * 128 + (wave * S::A_LOADS + j) * 1024), 16,
+                k + a_k(j) < K ? a_off[j] : kNone, (int)k, 0, 0);
+        }
     };
-    // four blocks' scales of the tile's rows at a time (waves that are more than the
-    // rows take load what others load, to the same place)
-    auto load_scales = [&](uint32_t b) {
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            sr, (lds_ptr)(sc + (b / 4 % 2) * (S::TM * 16) + wave % (S::TM / 64) * 1024), 16, s_off,
-            (int)(b * 4), 0, 0);
+    // the scales of the tile's rows of the four blocks from 4q on: this wave's share
+    auto load_scales = [&](char *to, uint32_t q) {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(sr, (lds_ptr)(to + all * 1024), 16, s_off,
+                                                 (int)((q + all / (S::SCALES / 1024)) * 16), 0, 0);
     };
-    const __attribute__((address_space(4))) float *sw =
-        (const __attribute__((address_space(4))) float *)p.sw +
-        (t.expert * ((p.N + 127) / 128) +
-         min((n0 + wn * (16 * NT)) / 128, (p.N - 1) / 128)) * blocks;
+    // the weights' scales of 64 blocks, one a lane
+    const PHX_GLOBAL float *sw = (const PHX_GLOBAL float *)p.sw +
+                                 (t.expert * ((p.N + 127) / 128) +
+                                  min((n0 + wn * (16 * NT)) / 128, (p.N - 1) / 128)) * blocks;
+    float w_scales;
+    auto load_w_scales = [&](uint32_t b) { w_scales = sw[min(b + lane, blocks - 1)]; };
 
     phx_f4 acc[NT][MT];
 #pragma unroll
@@ -372,75 +338,170 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *s0, char *s1
     }
     const uint32_t s_at = (wm * (16 * MT) + r) * 16;
 
-    auto multiply = [&](const char *from, uint32_t b, float scale) {
-        using C = Codes<EXACT>;
-        C x[MT], w;
-        float f[MT];
+    using C = Codes<EXACT>;
+    C x[MT];                 // this step's rows
+    phx_u4 w_next[2];        // the next tile of columns
+    phx_u4 x_next[MT][2];    // the next step's rows
+    float f[MT], f_next[MT], f_last[MT];
+    phx_f4 sum[MT];
+    auto read_w = [&](const char *stage, int n) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            w_next[h] = *(const phx_u4 *)(stage + wk * S::PART + w_at[n % 2][h] + n / 2 * 4096);
+    };
+    auto read_x = [&](const char *stage, int m) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            x_next[m][h] = *(const phx_u4 *)(stage + wk * S::PART + a_at[h] + m * 2048);
+    };
+    auto read_scale = [&](const char *stage, uint32_t b0, int m) {
+        const char *from = S::STAGED ? stage + WK * S::PART + wk / 4 * S::SCALES
+                                     : sc + b0 / 4 % 2 * S::SCALES;
+        return *(const float *)(from + s_at + m * 256 + (b0 + wk) % 4 * 4);
+    };
+
+    // A step: while its tiles are multiplied, the sums of the tile before are scaled, the
+    // next tile's weights read from LDS, and the blocks of ST - 1 steps ahead loaded
+    // into the stage of the step before. In its last column of tiles, where nothing
+    // of its stage is left to read, comes the one barrier: a wave's own loads of the
+    // next stage have landed before it, every wave's behind it, and behind it the
+    // next step's rows are read as this one's are used up. (Behind the last block
+    // the loads are of nothing, into what nobody reads.)
+    constexpr uint32_t AHEAD = ST - 1, EACH = S::W_LOADS + S::A_LOADS;
+    constexpr uint32_t SLOTS = (NT - 1) * MT, PER_SLOT = (EACH + SLOTS - 1) / SLOTS;
+    const bool loads_scales = all < S::S_LOADS;
+    phx_u4 scales = {0, 0, 0, 0};
+    auto pass = [&]() {
+        if (S::STAGED && loads_scales)
+            wait_loads<AHEAD - 1, EACH + 1>();
+        else
+            wait_loads<AHEAD - 1, EACH>();
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    load_w_scales(0);
+    auto step = [&](uint32_t b0, char *now, char *then, char *fill) {
+        const uint32_t b = b0 + wk;
+        const float scale =
+            __builtin_bit_cast(float, of_lane(__builtin_bit_cast(uint32_t, w_scales), b % 64));
+        if (b0 % 64 == 64 - WK) load_w_scales(b0 + WK);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-            x[m].of(*(const phx_u4 *)(from + a_at[0] + m * 2048),
-                    *(const phx_u4 *)(from + a_at[1] + m * 2048));
-            f[m] = *(const float *)(sc + (b / 4 % 2) * (S::TM * 16) + s_at + m * 256 + b % 4 * 4) * scale;
+            x[m].of(x_next[m][0], x_next[m][1]);
+            f_last[m] = f[m];
+            f[m] = f_next[m] * scale;
+            if (WK > 1) f[m] = b < blocks ? f[m] : 0.0f;
         }
-        // a tile's sum is scaled while the next tiles are multiplied
-        phx_f4 sum[MT];
-        phx_u4 next[2];
-        auto read = [&](int n) {
+        if (S::STAGED) {
+            if (loads_scales) load_scales(fill + WK * S::PART, (b0 + AHEAD * WK) / 4);
+        } else if (loads_scales) {
+            // the next four blocks' scales: loaded at the first of these four, written at
+            // the third (two steps of the four, where a step takes two)
+            if (b0 % 4 == 0)
+                scales = __builtin_bit_cast(
+                    phx_u4, __builtin_amdgcn_raw_buffer_load_b128(sr, s_off, (int)(b0 * 4 + 16), 0));
+            if (b0 % 4 == 2)
+                *(phx_u4 *)(sc + (b0 / 4 + 1) % 2 * S::SCALES + threadIdx.x * 16) = scales;
+        }
+        C w;
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-                next[h] = *(const phx_u4 *)(from + w_at[n % 2][h] + n / 2 * 4096);
-        };
-        read(0);
-#pragma unroll
-        for (int n = 0; n <= NT; ++n) {
-            if (n < NT) w.of(next[0], next[1]);
-            if (n + 1 < NT) read(n + 1);
+        for (int n = 0; n < NT; ++n) {
+            w.of(w_next[0], w_next[1]);
+            if (n + 1 < NT) read_w(now, n + 1);
+            const int done = n ? n - 1 : NT - 1;
 #pragma unroll
             for (int j = 0; j < C::STEPS; ++j)
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
-                    if (n > 0 && j == 0) {
+                    if (j == 0) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            acc[n - 1][m][i] = __builtin_fmaf(f[m], sum[m][i], acc[n - 1][m][i]);
+                            acc[done][m][i] =
+                                __builtin_fmaf(n ? f[m] : f_last[m], sum[m][i], acc[done][m][i]);
                         // (here, and not behind the branches of a later step)
-                        asm volatile("" : "+v"(acc[n - 1][m]));
+                        asm volatile("" : "+v"(acc[done][m]));
                     }
-                    if (n < NT) sum[m] = C::product(w, x[m], j, j ? sum[m] : (phx_f4){0, 0, 0, 0});
+                    sum[m] = C::product(w, x[m], j, j ? sum[m] : (phx_f4){0, 0, 0, 0});
+                    if (j == 0) {
+                        const uint32_t slot = n * MT + m;
+#pragma unroll
+                        for (uint32_t i = slot * PER_SLOT; i < (slot + 1) * PER_SLOT; ++i)
+                            if (i < EACH) load(fill, b + AHEAD * WK, i);
+                    }
                     __builtin_amdgcn_sched_barrier(0);
+                    if (n == NT - 1 && j == 0) {
+                        if (m == 0) {
+                            pass();
+                            read_w(then, 0);
+                        }
+                        read_x(then, m);
+                        f_next[m] = read_scale(then, b0 + WK, m);
+                    }
                 }
         }
     };
-    // One barrier a step: before it a wave's own loads of this step's stage have
-    // landed, and behind it every wave's have, and all reads of the other stage are
-    // done, which the next step's loads then fill.
-    load_scales(0);
-    load(s0, 0);
-    float scale = sw[0];
-    auto step = [&](uint32_t b, char *now, char *next) {
-        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
-        __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_sched_barrier(0);
-        const float f = scale;
-        // (behind the last block the loads are of nothing, into what nobody reads)
-        if ((b + 1) % 4 == 0) load_scales(b + 1);
-        load(next, b + 1);
-        scale = sw[min(b + 1, blocks - 1)];
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(now, b, f);
-    };
-    uint32_t b = 0;
-    for (; b + 2 <= blocks; b += 2) {
-        step(b, s0, s1);
-        step(b + 1, s1, s0);
+    if (!S::STAGED && loads_scales) load_scales(sc, 0);
+#pragma unroll
+    for (uint32_t u = 0; u < AHEAD; ++u) {
+        if (S::STAGED && loads_scales) load_scales(st[u] + WK * S::PART, u * WK / 4);
+#pragma unroll
+        for (uint32_t i = 0; i < EACH; ++i) load(st[u], u * WK + wk, i);
     }
-    if (b < blocks) step(b, s0, s1);
+    pass();
+    read_w(st[0], 0);
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        read_x(st[0], m);
+        f_next[m] = read_scale(st[0], 0, m);
+        f[m] = 0.0f;
+        sum[m] = (phx_f4){0, 0, 0, 0};
+    }
+    uint32_t b = 0;
+    for (; b + AHEAD * WK < blocks; b += ST * WK)
+#pragma unroll
+        for (int u = 0; u < ST; ++u)
+            step(b + u * WK, st[u], st[(u + 1) % ST], st[(u + ST - 1) % ST]);
+#pragma unroll
+    for (int u = 0; u < ST - 1; ++u)
+        if (b + u * WK < blocks) step(b + u * WK, st[u], st[(u + 1) % ST], st[(u + ST - 1) % ST]);
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            acc[NT - 1][m][i] = __builtin_fmaf(f[m], sum[m][i], acc[NT - 1][m][i]);
+    // (the loads behind the last block write zeros: before the sums, and before LDS is
+    // another workgroup's)
+    __builtin_amdgcn_s_waitcnt(0x0f70);
+    if (WK > 1) {
+        // the sets' sums to LDS; of them each wave adds up and stores its share
+        __syncthreads();
+        constexpr uint32_t SUM = S::TN * S::TM * 4;
+        auto at = [&](uint32_t set, uint32_t n, uint32_t m) {
+            char *half = set < WK / 2 ? st[0] + set * SUM : st[1] + (set - WK / 2) * SUM;
+            return (phx_f4 *)(half + ((wave * NT + n) * MT + m) * 1024 + lane * 16);
+        };
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int m = 0; m < MT; ++m) *at(wk, n, m) = acc[n][m];
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                if (((uint32_t)(n / 2 * MT + m)) % WK != wk) continue;
+                acc[n][m] = *at(0, n, m);
+#pragma unroll
+                for (int set = 1; set < WK; ++set) acc[n][m] = acc[n][m] + *at(set, n, m);
+            }
+    }
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
         const uint32_t row = wm * (16 * MT) + 16 * m + r;
         if (row >= left_m) continue;
 #pragma unroll
         for (int n = 0; n < NT; n += 2) {
+            if (WK > 1 && ((uint32_t)(n / 2 * MT + m)) % WK != wk) continue;
             const float o[8] = {acc[n][m][0], acc[n][m][1], acc[n][m][2], acc[n][m][3],
                                 acc[n + 1][m][0], acc[n + 1][m][1], acc[n + 1][m][2], acc[n + 1][m][3]};
             const int64_t c = n0 + wn * (16 * NT) + 16 * n + 8 * g;
@@ -451,15 +512,31 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *s0, char *s1
 
 }  // namespace
 
-extern "C" __global__ __launch_bounds__(64) void gemm_f8_first(PhxF8Gemm p) { gemm_f8(p); }
-
-#define TILE(EXACT, suffix, WN, WM, NT, MT)                                                     \
-    extern "C" __global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(2))) void \
-        gemm_f8_##suffix##_##WN##x##WM##_##NT##x##MT(PhxF8Gemm p) {                             \
-        using S = Shape<WN, WM, NT, MT>;                                                        \
-        __shared__ phx_u4 s0[S::STAGE / 16], s1[S::STAGE / 16], sc[2 * S::TM];                  \
-        gemm_tile<EXACT, WN, WM, NT, MT>(p, (char *)s0, (char *)s1, (char *)sc);                \
+#define STAGES_2(S) s0[S::STAGE / 16], s1[S::STAGE / 16]
+#define STAGES_3(S) STAGES_2(S), s2[S::STAGE / 16]
+#define STAGES_4(S) STAGES_3(S), s3[S::STAGE / 16]
+#define LIST_2 (char *)s0, (char *)s1
+#define LIST_3 LIST_2, (char *)s2
+#define LIST_4 LIST_3, (char *)s3
+// (each stage is an array of its own, so that the compiler sees that what is read and
+// what is being filled differ)
+#define TILE(EXACT, suffix, WN, WM, NT, MT, WK, ST)                                             \
+    extern "C" __global__ __launch_bounds__(64 * WN * WM * WK) void                             \
+        gemm_f8_##suffix##_##WN##x##WM##_##NT##x##MT##_k##WK##_s##ST(PhxF8Gemm p) {             \
+        using S = Shape<WN, WM, NT, MT, WK, ST>;                                                \
+        __shared__ phx_u4 STAGES_##ST(S), sc[S::APART / 16];                         \
+        char *const st[ST] = {LIST_##ST};                                                       \
+        gemm_tile<EXACT, WN, WM, NT, MT, WK, ST>(p, st, (char *)sc);                            \
     }
-TILE(false, f16, 2, 4, 8, 4)
-TILE(false, f16, 2, 2, 4, 4)
-TILE(true, f32, 2, 2, 4, 4)
+#define BOTH(WN, WM, NT, MT, WK, ST)                                                            \
+    TILE(false, f16, WN, WM, NT, MT, WK, ST)                                                    \
+    TILE(true, f32, WN, WM, NT, MT, WK, ST)
+BOTH(1, 1, 2, 1, 4, 4)
+BOTH(1, 1, 2, 1, 4, 2)
+BOTH(2, 1, 2, 1, 4, 3)
+BOTH(2, 2, 2, 2, 2, 4)
+BOTH(2, 2, 2, 2, 1, 4)
+BOTH(2, 2, 4, 2, 1, 3)
+TILE(true, f32, 2, 2, 4, 4, 1, 2)
+TILE(false, f16, 2, 4, 4, 2, 1, 2)
+TILE(false, f16, 2, 4, 8, 4, 1, 2)
