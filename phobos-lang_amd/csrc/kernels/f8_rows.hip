@@ -11,8 +11,8 @@ struct Chunk {  // 16 bytes of a row
     static constexpr int LANES = PHX_F8_BLOCK / N;  // of a scale's block
     float v[N];
 
-    __device__ __forceinline__ void load(const PHX_GLOBAL T *p) {
-        const phx_u4 w = *(const PHX_GLOBAL phx_u4 *)p;
+    __device__ __forceinline__ void load(const PHX_GLOBAL T *p) { of(*(const PHX_GLOBAL phx_u4 *)p); }
+    __device__ __forceinline__ void of(phx_u4 w) {
         if constexpr (sizeof(T) == 2) {
             const phx_h8 h = __builtin_bit_cast(phx_h8, w);
 #pragma unroll
@@ -54,17 +54,19 @@ __device__ __forceinline__ void store_codes(const PhxF8Rows &p, int64_t row, uin
         *(PHX_GLOBAL uint32_t *)to = out[0];
 }
 
-// R threads (waves of one workgroup) take a row, chunks of 16 bytes next to their
-// neighbours', up to C chunks a thread, which stay in registers between the sum and
-// what follows it: every byte is read once and written once.
-template <typename T, int R, int C>
+// A wave (ROWS: of four to a workgroup) or a workgroup takes a row, chunks of 16 bytes
+// next to their neighbours', up to C chunks a thread, which stay in registers
+// between the sum and what follows it: every byte is read once and written once.
+template <typename T, int C, bool ROWS>
 __device__ __forceinline__ void norm_f8(const PhxF8Rows &p) {
-    constexpr int N = Chunk<T>::N, WAVES = R / 64;
-    __shared__ double sums[WAVES];
-    const int64_t row = (int64_t)blockIdx.x * (blockDim.x / R) + threadIdx.x / R;
-    if (row >= p.M) return;  // (whole waves, and with several waves a row no workgroup)
-    const uint32_t at = threadIdx.x % R * N, K = (uint32_t)p.K;
+    constexpr int N = Chunk<T>::N;
+    __shared__ double sums[16];
+    const uint32_t R = ROWS ? 64 : blockDim.x, waves = R / 64;  // threads of a row
+    const int64_t row = ROWS ? (int64_t)blockIdx.x * 4 + threadIdx.x / 64 : (int64_t)blockIdx.x;
+    if (ROWS && row >= p.M) return;
+    const uint32_t at = (ROWS ? threadIdx.x % 64 : threadIdx.x) * N, K = (uint32_t)p.K;
     Chunk<T> h[C];
+    phx_u4 gain[C];  // (asked for with the rows: it is in use as soon as their sum is there)
     double sum = 0;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
@@ -72,6 +74,7 @@ __device__ __forceinline__ void norm_f8(const PhxF8Rows &p) {
 #pragma unroll
         for (int i = 0; i < N; ++i) h[c].v[i] = 0;
         if (k >= K) continue;
+        gain[c] = *(const PHX_GLOBAL phx_u4 *)((const PHX_GLOBAL T *)p.gain + k);
         h[c].load((const PHX_GLOBAL T *)p.x + row * p.ldx + k);
         if (p.r) {
             Chunk<T> r;
@@ -87,14 +90,13 @@ __device__ __forceinline__ void norm_f8(const PhxF8Rows &p) {
     }
 #pragma unroll
     for (int s = 1; s < 64; s <<= 1) sum += __shfl_xor(sum, s);
-    if (WAVES > 1) {
+    if (!ROWS && waves > 1) {
         if (threadIdx.x % 64 == 0) sums[threadIdx.x / 64] = sum;
         __syncthreads();
         sum = sums[0];
-#pragma unroll
-        for (int w = 1; w < WAVES; ++w) sum += sums[w];
+        for (uint32_t w = 1; w < waves; ++w) sum += sums[w];
     }
-    const double factor = 1.0 / sqrt(sum / (double)p.K + (double)p.eps);
+    const double factor = rsqrt(sum * p.inverse + (double)p.eps);
     const float f = (float)factor;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
@@ -103,7 +105,7 @@ __device__ __forceinline__ void norm_f8(const PhxF8Rows &p) {
         uint32_t a = 0;
         if (live) {
             Chunk<T> g;
-            g.load((const PHX_GLOBAL T *)p.gain + k);
+            g.of(gain[c]);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 h[c].v[i] = h[c].v[i] * g.v[i];
@@ -117,7 +119,7 @@ __device__ __forceinline__ void norm_f8(const PhxF8Rows &p) {
                 if (threadIdx.x % Chunk<T>::LANES == 0)
                     ((PHX_GLOBAL float *)p.scales)[row * p.lds + k / PHX_F8_BLOCK] =
                         a < 0x7f800000u
-                            ? (float)((double)__builtin_bit_cast(float, a) * factor / 448.0)
+                            ? (float)((double)__builtin_bit_cast(float, a) * (factor * (1 / 448.0)))
                             : __builtin_nanf("");
             }
         }
@@ -172,20 +174,18 @@ __device__ __forceinline__ void glu_f8(const PhxF8Rows &p) {
 
 }  // namespace
 
-#define NORM(T, suffix, R, C)                                                                   \
-    extern "C" __global__ __launch_bounds__(R < 256 ? 256 : R) void                             \
-        norm_f8_##suffix##_r##R##_c##C(PhxF8Rows p) {                                           \
-        norm_f8<T, R, C>(p);                                                                    \
+#define NORM(T, suffix, C)                                                                      \
+    extern "C" __global__ __launch_bounds__(1024) void norm_f8_##suffix##_c##C(PhxF8Rows p) {   \
+        norm_f8<T, C, false>(p);                                                                \
     }
-#define NORMS(R, C) NORM(_Float16, f16, R, C) NORM(float, f32, R, C)
-NORMS(64, 1)
-NORMS(64, 2)
-NORMS(64, 4)
-NORMS(256, 2)
-NORMS(256, 4)
-NORMS(1024, 1)
-NORMS(1024, 2)
-NORMS(1024, 4)
-NORM(float, f32, 1024, 8)
+#define ROWS(T, suffix, C)                                                                      \
+    extern "C" __global__ __launch_bounds__(256) void norm_f8_rows_##suffix##_c##C(PhxF8Rows p) { \
+        norm_f8<T, C, true>(p);                                                                 \
+    }
+#define NORMS(T, suffix)                                                                        \
+    ROWS(T, suffix, 1) ROWS(T, suffix, 2) NORM(T, suffix, 1) NORM(T, suffix, 2) NORM(T, suffix, 4)
+NORMS(_Float16, f16)
+NORMS(float, f32)
+NORM(float, f32, 8)
 extern "C" __global__ __launch_bounds__(256) void glu_f8_f16(PhxF8Rows p) { glu_f8<_Float16>(p); }
 extern "C" __global__ __launch_bounds__(256) void glu_f8_f32(PhxF8Rows p) { glu_f8<float>(p); }

@@ -11,6 +11,7 @@
 struct PhxF8Rows {
     uint64_t x, r, gain, h, y, q, scales;
     int64_t M, K, ldx, ldr, ldh, ldy, ldq, lds;
+    double inverse;  // 1 / K
     float eps;
 };
 

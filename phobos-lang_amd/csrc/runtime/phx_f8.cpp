@@ -74,21 +74,30 @@ int check_rows(phx_dtype t, uint64_t ptr, int64_t width, int64_t *ld, const char
 }
 
 // ------------------------------------------------------------------ the norm
+// How a norm runs: up to 128 chunks of 16 bytes a row by a wave, four rows a workgroup
+// (16384 rows of 1024, f16: 26.6 us, in workgroups of 128 threads a row 32.1); more
+// by a workgroup of as many threads as one, two, four or eight chunks each take:
+// two from 512 on (8192 rows of 8192, f16: 87 us, four 95; 4096 of 4096, f32:
+// 42.8 us, four 47.3).
 struct NormForm {
-    int64_t threads, chunks;  // of a row, and of a thread
-    const char *entry[2];     // f16, f32
+    int64_t rows;  // of a workgroup
+    uint32_t threads;
+    const char *entry;
 };
-#define NORM(r, c) {r, c, {"norm_f8_f16_r" #r "_c" #c, "norm_f8_f32_r" #r "_c" #c}}
-const NormForm kNorms[] = {NORM(64, 1), NORM(64, 2), NORM(64, 4), NORM(256, 2), NORM(256, 4),
-                           NORM(1024, 1), NORM(1024, 2), NORM(1024, 4),
-                           {1024, 8, {nullptr, "norm_f8_f32_r1024_c8"}}};
-#undef NORM
 
-const NormForm *norm_form(phx_dtype t, int64_t K) {
+NormForm norm_form(phx_dtype t, int64_t K) {
+    static const char *const names[2][6] = {
+        {"norm_f8_rows_f16_c1", "norm_f8_rows_f16_c2", "norm_f8_f16_c1", "norm_f8_f16_c2",
+         "norm_f8_f16_c4", nullptr},
+        {"norm_f8_rows_f32_c1", "norm_f8_rows_f32_c2", "norm_f8_f32_c1", "norm_f8_f32_c2",
+         "norm_f8_f32_c4", "norm_f8_f32_c8"}};
+    const char *const *name = names[t == PHX_F16 ? 0 : 1];
     const int64_t chunks = K * size_of(t) / 16;
-    for (const NormForm &f : kNorms)
-        if (chunks <= f.threads * f.chunks && f.entry[t == PHX_F16 ? 0 : 1]) return &f;
-    return nullptr;
+    if (chunks <= 128) return {4, 256, name[chunks > 64]};
+    const int64_t of_thread = chunks <= 512 ? 1 : chunks <= 2048 ? 2 : chunks <= 4096 ? 4 : 8;
+    const int64_t threads = (chunks + of_thread - 1) / of_thread;
+    return {1, (uint32_t)((threads + 63) / 64 * 64),
+            name[of_thread == 1 ? 2 : of_thread == 2 ? 3 : of_thread == 4 ? 4 : 5]};
 }
 
 // ------------------------------------------------------------------ products
@@ -231,16 +240,14 @@ int phx_norm_f8(phx_stream s, phx_dtype t, uint64_t x, uint64_t r, uint64_t gain
             return set_error(PHX_E_INVALID, "%s: the gain must be 16-byte aligned", who);
         if (!y && !q) return set_error(PHX_E_INVALID, "%s: neither Y nor 8-bit rows", who);
     }
-    const NormForm *f = norm_form(t, K);
-    const int64_t each = f->threads < 256 ? 256 / f->threads : 1;  // rows of a workgroup
-    const int64_t groups = (M + each - 1) / each, threads = std::max<int64_t>(f->threads, 256);
-    if (groups > kMostThreads / threads)
+    const NormForm f = norm_form(t, K);
+    const int64_t groups = (M + f.rows - 1) / f.rows;
+    if (groups > kMostThreads / f.threads)
         return set_error(PHX_E_INVALID, "%s: %lld rows are too many", who, (long long)M);
     if (int rc = on_device((hipStream_t)s)) return rc;
     if (!M) return PHX_OK;
-    PhxF8Rows p = {x, r, gain, h, y, o.codes, o.scales, M, K, ldx, ldr, ldh, ldy, o.ld, o.lds, eps};
-    return launch(kRowsFile, f->entry[t == PHX_F16 ? 0 : 1], groups, (uint32_t)threads,
-                  (hipStream_t)s, &p);
+    PhxF8Rows p = {x, r, gain, h, y, o.codes, o.scales, M, K, ldx, ldr, ldh, ldy, o.ld, o.lds, 1.0 / (double)K, eps};
+    return launch(kRowsFile, f.entry, groups, f.threads, (hipStream_t)s, &p);
 }
 
 int phx_glu_f8(phx_stream s, phx_dtype t, uint64_t u, const phx_f8_rows *q, int64_t ldu) {
@@ -257,7 +264,7 @@ int phx_glu_f8(phx_stream s, phx_dtype t, uint64_t u, const phx_f8_rows *q, int6
                          (long long)o.k);
     if (int rc = on_device((hipStream_t)s)) return rc;
     if (!o.rows) return PHX_OK;
-    PhxF8Rows p = {u, 0, 0, 0, 0, o.codes, o.scales, o.rows, o.k, ldu, 0, 0, 0, o.ld, o.lds, 0.0f};
+    PhxF8Rows p = {u, 0, 0, 0, 0, o.codes, o.scales, o.rows, o.k, ldu, 0, 0, 0, o.ld, o.lds, 0.0, 0.0f};
     return launch(kRowsFile, t == PHX_F16 ? "glu_f8_f16" : "glu_f8_f32", groups, 256, (hipStream_t)s,
                   &p);
 }

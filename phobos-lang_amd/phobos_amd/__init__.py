@@ -605,39 +605,45 @@ def f8_quantize(w):
     return np.ascontiguousarray(code.reshape(*lead, nb * 128, kb * 128)[..., :N, :K]), scales
 
 
+def _rows(buf, rows, ld, width, esz, what):
+    """_addr of such rows; raw addresses as they are, without working out their bytes."""
+    return buf if type(buf) is int else _addr(buf, _span(rows, ld, width, esz), what)
+
+
 def launch_norm_f8(stream, dtype, x, r, gain, h, y, q, M, K, eps, ldx=0, ldr=0, ldh=0, ldy=0):
     """The root-mean-square norm of X + R (r 0: of X), which goes to H, times the
     gain: in 8 bits to q (F8Rows or None) and as it is to Y (0: not wanted)
     (phx_norm_f8)."""
     e = _ESZ.get(dtype, 4)
-    check(lib().phx_norm_f8(_sh(stream), dtype, _addr(x, _span(M, ldx, K, e), "X"),
-                            _addr(r, _span(M, ldr, K, e), "R"), _addr(gain, K * e, "gain"),
-                            _addr(h, _span(M, ldh, K, e), "H"), _addr(y, _span(M, ldy, K, e), "Y"),
-                            q, M, K, eps, ldx, ldr, ldh, ldy))
+    check(lib().phx_norm_f8(_sh(stream), dtype, _rows(x, M, ldx, K, e, "X"), _rows(r, M, ldr, K, e, "R"),
+                            _rows(gain, 1, 0, K, e, "gain"), _rows(h, M, ldh, K, e, "H"),
+                            _rows(y, M, ldy, K, e, "Y"), q, M, K, eps, ldx, ldr, ldh, ldy))
 
 
 def launch_glu_f8(stream, dtype, u, q, ldu=0):
     """silu(gate) * value of rows U [gates | values] into the 8-bit rows q
     (phx_glu_f8)."""
-    span = _span(q.rows, ldu, 2 * q.k, _ESZ.get(dtype, 4)) if q else 0
-    check(lib().phx_glu_f8(_sh(stream), dtype, _addr(u, span, "U"), q, ldu))
+    if q:
+        u = _rows(u, q.rows, ldu, 2 * q.k, _ESZ.get(dtype, 4), "U")
+    check(lib().phx_glu_f8(_sh(stream), dtype, u, q, ldu))
 
 
 def launch_gemm_f8(stream, a, w, dtype, c, alpha=1.0, beta=0.0, ldc=0):
     """C = alpha*A@W^T + beta*C of 8-bit rows and weights (phx_gemm_f8)."""
-    span = _span(a.rows, ldc, w.n, _ESZ.get(dtype, 4)) if a and w else 0
-    check(lib().phx_gemm_f8(_sh(stream), a, w, dtype, _addr(c, span, "C"), alpha, beta, ldc))
+    if a and w:
+        c = _rows(c, a.rows, ldc, w.n, _ESZ.get(dtype, 4), "C")
+    check(lib().phx_gemm_f8(_sh(stream), a, w, dtype, c, alpha, beta, ldc))
 
 
 def launch_gemm_f8_grouped(stream, a, w, starts, order, M, dtype, c, alpha=1.0, beta=0.0, ldc=0):
     """The same for M rows sorted by expert: rows starts[e] up to starts[e+1] of C
     are A's rows order[i] (order 0: A's own) times expert e's weights
     (phx_gemm_f8_grouped)."""
-    span = _span(M, ldc, w.n, _ESZ.get(dtype, 4)) if w else 0
-    check(lib().phx_gemm_f8_grouped(_sh(stream), a, w,
-                                    _addr(starts, 4 * (w.experts + 1) if w else 0, "starts"),
-                                    _addr(order, 4 * M, "order"), M, dtype, _addr(c, span, "C"),
-                                    alpha, beta, ldc))
+    if w:
+        starts = _rows(starts, 1, 0, w.experts + 1, 4, "starts")
+        c = _rows(c, M, ldc, w.n, _ESZ.get(dtype, 4), "C")
+    check(lib().phx_gemm_f8_grouped(_sh(stream), a, w, starts, _rows(order, 1, 0, M, 4, "order"), M, dtype,
+                                    c, alpha, beta, ldc))
 
 
 def _page_list(x):
