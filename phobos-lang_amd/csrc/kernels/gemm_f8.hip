@@ -32,6 +32,23 @@ __device__ __forceinline__ uint32_t of_lane(uint32_t x, uint32_t lane) {
     return (uint32_t)__builtin_amdgcn_readlane((int)x, (int)lane);
 }
 
+// op over this lane's x and those of the lanes before it; 0 changes nothing.
+template <typename Op>
+__device__ __forceinline__ uint32_t upto(uint32_t x, Op op) {
+    // within rows of 16 lanes, then the rows' last ones to the row behind, then the
+    // lower half's last to the upper half
+#define STEP(control, rows) \
+    x = op(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, control, rows, 0xf, false))
+    STEP(0x111, 0xf);
+    STEP(0x112, 0xf);
+    STEP(0x114, 0xf);
+    STEP(0x118, 0xf);
+    STEP(0x142, 0xa);
+    STEP(0x143, 0xc);
+#undef STEP
+    return x;
+}
+
 // Tiles of the groups in their order, `columns` of them for every TM rows. The groups'
 // ranges are made to ascend, so that none overlap whatever the starts hold.
 //
@@ -59,21 +76,11 @@ __device__ __forceinline__ Tile tile_of(const PhxF8Gemm &p, uint32_t columns) {
         };
         auto range = [&](uint32_t e0, uint32_t floor, uint32_t before) {
             Range x;
-            x.begin = max(at(e0 + lane), floor);
-#pragma unroll
-            for (int s = 1; s < 64; s <<= 1) {
-                const uint32_t o = __shfl_up(x.begin, s);
-                if (lane >= s) x.begin = max(x.begin, o);
-            }
+            x.begin = upto(max(at(e0 + lane), floor),
+                           [](uint32_t a, uint32_t b) { return max(a, b); });
             x.end = e0 + lane < E ? max(x.begin, at(e0 + lane + 1)) : x.begin;
             x.tiles = (x.end - x.begin + TM - 1) / TM;
-            x.upto = x.tiles;
-#pragma unroll
-            for (int s = 1; s < 64; s <<= 1) {
-                const uint32_t o = __shfl_up(x.upto, s);
-                if (lane >= s) x.upto += o;
-            }
-            x.upto += before;
+            x.upto = before + upto(x.tiles, [](uint32_t a, uint32_t b) { return a + b; });
             return x;
         };
         Range x = range(0, 0, 0);
@@ -370,6 +377,8 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
     constexpr uint32_t AHEAD = ST - 1, EACH = S::W_LOADS + S::A_LOADS;
     constexpr uint32_t SLOTS = (NT - 1) * MT, PER_SLOT = (EACH + SLOTS - 1) / SLOTS;
     const bool loads_scales = all < S::S_LOADS;
+    // (of a last tile of rows few may be left: waves without one load and pass on)
+    const bool live = wm * (16 * MT) < left_m;
     phx_u4 scales = {0, 0, 0, 0};
     auto pass = [&]() {
         if (S::STAGED && loads_scales)
@@ -380,8 +389,31 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
         __builtin_amdgcn_sched_barrier(0);
     };
     load_w_scales(0);
+    // what a step loads besides its tiles' blocks
+    auto load_more = [&](uint32_t b0, char *fill) {
+        if (!loads_scales) return;
+        if (S::STAGED) {
+            load_scales(fill + WK * S::PART, (b0 + AHEAD * WK) / 4);
+            return;
+        }
+        // the next four blocks' scales: loaded at the first of these four, written at
+        // the third (two steps of the four, where a step takes two)
+        if (b0 % 4 == 0)
+            scales = __builtin_bit_cast(
+                phx_u4, __builtin_amdgcn_raw_buffer_load_b128(sr, s_off, (int)(b0 * 4 + 16), 0));
+        if (b0 % 4 == 2)
+            *(phx_u4 *)(sc + (b0 / 4 + 1) % 2 * S::SCALES + threadIdx.x * 16) = scales;
+    };
     auto step = [&](uint32_t b0, char *now, char *then, char *fill) {
         const uint32_t b = b0 + wk;
+        if (WM > 1 && !live) {
+            load_more(b0, fill);
+#pragma unroll
+            for (uint32_t i = 0; i < EACH; ++i) load(fill, b + AHEAD * WK, i);
+            __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the scales are written
+            pass();
+            return;
+        }
         const float scale =
             __builtin_bit_cast(float, of_lane(__builtin_bit_cast(uint32_t, w_scales), b % 64));
         if (b0 % 64 == 64 - WK) load_w_scales(b0 + WK);
@@ -392,17 +424,7 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
             f[m] = f_next[m] * scale;
             if (WK > 1) f[m] = b < blocks ? f[m] : 0.0f;
         }
-        if (S::STAGED) {
-            if (loads_scales) load_scales(fill + WK * S::PART, (b0 + AHEAD * WK) / 4);
-        } else if (loads_scales) {
-            // the next four blocks' scales: loaded at the first of these four, written at
-            // the third (two steps of the four, where a step takes two)
-            if (b0 % 4 == 0)
-                scales = __builtin_bit_cast(
-                    phx_u4, __builtin_amdgcn_raw_buffer_load_b128(sr, s_off, (int)(b0 * 4 + 16), 0));
-            if (b0 % 4 == 2)
-                *(phx_u4 *)(sc + (b0 / 4 + 1) % 2 * S::SCALES + threadIdx.x * 16) = scales;
-        }
+        load_more(b0, fill);
         C w;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -531,7 +553,7 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
 #define BOTH(WN, WM, NT, MT, WK, ST)                                                            \
     TILE(false, f16, WN, WM, NT, MT, WK, ST)                                                    \
     TILE(true, f32, WN, WM, NT, MT, WK, ST)
-BOTH(1, 1, 2, 1, 4, 4)
+TILE(false, f16, 1, 1, 2, 1, 4, 4)
 BOTH(1, 1, 2, 1, 4, 2)
 BOTH(2, 1, 2, 1, 4, 3)
 BOTH(2, 2, 2, 2, 2, 4)

@@ -115,21 +115,20 @@ struct GemmForm {
 #define FORM(t, wn, wm, nt, mt, wk, st, held, step, shared, rest)                 \
     {16 * wn * nt, 16 * wm * mt, wk, 64 * wn * wm * wk, held, step, shared, rest, \
      "gemm_f8_" #t "_" #wn "x" #wm "_" #nt "x" #mt "_k" #wk "_s" #st}
-const GemmForm kGemmF16[] = {FORM(f16, 1, 1, 2, 1, 4, 4, 1, 239, 0, 2620),
-                             FORM(f16, 1, 1, 2, 1, 4, 2, 3, 0, 293, 1650),
-                             FORM(f16, 2, 1, 2, 1, 4, 3, 1, 419, 0, 2620),
-                             FORM(f16, 2, 2, 2, 2, 2, 4, 1, 393, 0, 2810),
-                             FORM(f16, 2, 2, 2, 2, 1, 4, 2, 236, 236, 990),
-                             FORM(f16, 2, 2, 4, 2, 1, 3, 2, 377, 377, 1010),
-                             FORM(f16, 2, 4, 4, 2, 1, 2, 2, 0, 707, 0),
-                             FORM(f16, 2, 4, 8, 4, 1, 2, 1, 1308, 0, 3550)};
-const GemmForm kGemmF32[] = {FORM(f32, 1, 1, 2, 1, 4, 4, 1, 374, 0, 2630),
-                             FORM(f32, 1, 1, 2, 1, 4, 2, 3, 0, 304, 1820),
-                             FORM(f32, 2, 1, 2, 1, 4, 3, 1, 548, 0, 2770),
-                             FORM(f32, 2, 2, 2, 2, 2, 4, 1, 659, 0, 3130),
-                             FORM(f32, 2, 2, 2, 2, 1, 4, 2, 438, 386, 1000),
-                             FORM(f32, 2, 2, 4, 2, 1, 3, 2, 696, 612, 1760),
-                             FORM(f32, 2, 2, 4, 4, 1, 2, 2, 593, 1054, 2240)};
+const GemmForm kGemmF16[] = {FORM(f16, 1, 1, 2, 1, 4, 4, 1, 193, 38, 2189),
+                             FORM(f16, 1, 1, 2, 1, 4, 2, 3, 64, 292, 1887),
+                             FORM(f16, 2, 1, 2, 1, 4, 3, 1, 174, 418, 2406),
+                             FORM(f16, 2, 2, 2, 2, 2, 4, 1, 175, 131, 5104),
+                             FORM(f16, 2, 2, 2, 2, 1, 4, 2, 277, 156, 1363),
+                             FORM(f16, 2, 2, 4, 2, 1, 3, 2, 562, 13, 1998),
+                             FORM(f16, 2, 4, 4, 2, 1, 2, 2, 940, 227, 52),
+                             FORM(f16, 2, 4, 8, 4, 1, 2, 1, 1392, 0, 1029)};
+const GemmForm kGemmF32[] = {FORM(f32, 1, 1, 2, 1, 4, 2, 3, 121, 294, 2199),
+                             FORM(f32, 2, 1, 2, 1, 4, 3, 1, 457, 32, 3189),
+                             FORM(f32, 2, 2, 2, 2, 2, 4, 1, 681, 14, 2192),
+                             FORM(f32, 2, 2, 2, 2, 1, 4, 2, 409, 350, 1686),
+                             FORM(f32, 2, 2, 4, 2, 1, 3, 2, 809, 592, 962),
+                             FORM(f32, 2, 2, 4, 4, 1, 2, 2, 1189, 1050, 971)};
 #undef FORM
 
 int64_t estimate(const GemmForm &f, int64_t M, int64_t N, int64_t K, int64_t experts) {

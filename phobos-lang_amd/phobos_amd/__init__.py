@@ -605,33 +605,31 @@ def f8_quantize(w):
     return np.ascontiguousarray(code.reshape(*lead, nb * 128, kb * 128)[..., :N, :K]), scales
 
 
-def _rows(buf, rows, ld, width, esz, what):
-    """_addr of such rows; raw addresses as they are, without working out their bytes."""
-    return buf if type(buf) is int else _addr(buf, _span(rows, ld, width, esz), what)
-
-
 def launch_norm_f8(stream, dtype, x, r, gain, h, y, q, M, K, eps, ldx=0, ldr=0, ldh=0, ldy=0):
     """The root-mean-square norm of X + R (r 0: of X), which goes to H, times the
     gain: in 8 bits to q (F8Rows or None) and as it is to Y (0: not wanted)
     (phx_norm_f8)."""
-    e = _ESZ.get(dtype, 4)
-    check(lib().phx_norm_f8(_sh(stream), dtype, _rows(x, M, ldx, K, e, "X"), _rows(r, M, ldr, K, e, "R"),
-                            _rows(gain, 1, 0, K, e, "gain"), _rows(h, M, ldh, K, e, "H"),
-                            _rows(y, M, ldy, K, e, "Y"), q, M, K, eps, ldx, ldr, ldh, ldy))
+    # (raw addresses are nothing to be looked at, and that takes 1 us of 5)
+    if not (type(x) is type(r) is type(gain) is type(h) is type(y) is int):
+        e = _ESZ.get(dtype, 4)
+        x, r = _addr(x, _span(M, ldx, K, e), "X"), _addr(r, _span(M, ldr, K, e), "R")
+        gain = _addr(gain, K * e, "gain")
+        h, y = _addr(h, _span(M, ldh, K, e), "H"), _addr(y, _span(M, ldy, K, e), "Y")
+    check(lib().phx_norm_f8(_sh(stream), dtype, x, r, gain, h, y, q, M, K, eps, ldx, ldr, ldh, ldy))
 
 
 def launch_glu_f8(stream, dtype, u, q, ldu=0):
     """silu(gate) * value of rows U [gates | values] into the 8-bit rows q
     (phx_glu_f8)."""
-    if q:
-        u = _rows(u, q.rows, ldu, 2 * q.k, _ESZ.get(dtype, 4), "U")
+    if type(u) is not int and q:
+        u = _addr(u, _span(q.rows, ldu, 2 * q.k, _ESZ.get(dtype, 4)), "U")
     check(lib().phx_glu_f8(_sh(stream), dtype, u, q, ldu))
 
 
 def launch_gemm_f8(stream, a, w, dtype, c, alpha=1.0, beta=0.0, ldc=0):
     """C = alpha*A@W^T + beta*C of 8-bit rows and weights (phx_gemm_f8)."""
-    if a and w:
-        c = _rows(c, a.rows, ldc, w.n, _ESZ.get(dtype, 4), "C")
+    if type(c) is not int and a and w:
+        c = _addr(c, _span(a.rows, ldc, w.n, _ESZ.get(dtype, 4)), "C")
     check(lib().phx_gemm_f8(_sh(stream), a, w, dtype, c, alpha, beta, ldc))
 
 
@@ -639,11 +637,10 @@ def launch_gemm_f8_grouped(stream, a, w, starts, order, M, dtype, c, alpha=1.0, 
     """The same for M rows sorted by expert: rows starts[e] up to starts[e+1] of C
     are A's rows order[i] (order 0: A's own) times expert e's weights
     (phx_gemm_f8_grouped)."""
-    if w:
-        starts = _rows(starts, 1, 0, w.experts + 1, 4, "starts")
-        c = _rows(c, M, ldc, w.n, _ESZ.get(dtype, 4), "C")
-    check(lib().phx_gemm_f8_grouped(_sh(stream), a, w, starts, _rows(order, 1, 0, M, 4, "order"), M, dtype,
-                                    c, alpha, beta, ldc))
+    if not (type(starts) is type(order) is type(c) is int) and w:
+        starts, order = _addr(starts, 4 * (w.experts + 1), "starts"), _addr(order, 4 * M, "order")
+        c = _addr(c, _span(M, ldc, w.n, _ESZ.get(dtype, 4)), "C")
+    check(lib().phx_gemm_f8_grouped(_sh(stream), a, w, starts, order, M, dtype, c, alpha, beta, ldc))
 
 
 def _page_list(x):
