@@ -6,6 +6,8 @@
 // The inner sum is one v_mfma_f32_16x16x128 of the codes, scaled in f32. The
 // weights are its A operand, so that a lane holds four neighbouring columns of
 // one row of C, and one row's scale.
+#include <type_traits>
+
 #include "f8.h"
 
 namespace {
@@ -189,52 +191,34 @@ struct Codes<true> {
     }
 };
 
-// Stores a lane's eight columns of a row of C.
+// Stores a lane's eight columns of a row of C, which may start at any element: memory
+// takes 16 bytes there too.
+template <typename T>
 __device__ __forceinline__ void store8(const PhxF8Gemm &p, const float (&acc)[8], int64_t m, int64_t n) {
-    const int64_t at = m * p.ldc + n;
-    float o[8];
+    typedef T v8 __attribute__((ext_vector_type(8)));
+    typedef v8 loose __attribute__((aligned(sizeof(T))));
+    PHX_GLOBAL T *to = (PHX_GLOBAL T *)p.c + m * p.ldc + n;
+    const bool whole = n + 8 <= p.N;
+    v8 o;
+    if (p.beta != 0.0f) {
+        v8 old;
+        if (whole)
+            old = *(const PHX_GLOBAL loose *)to;
+        else
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = p.alpha * acc[i];
-    if (p.half) {
-        PHX_GLOBAL _Float16 *to = (PHX_GLOBAL _Float16 *)p.c + at;
-        if (p.wide && n + 8 <= p.N) {
-            phx_h8 h;
-            if (p.beta != 0.0f) {
-                h = *(PHX_GLOBAL phx_h8 *)to;
+            for (int i = 0; i < 8; ++i) old[i] = n + i < p.N ? to[i] : (T)0;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) o[i] = o[i] + p.beta * (float)h[i];
-            }
+        for (int i = 0; i < 8; ++i) o[i] = (T)(p.alpha * acc[i] + p.beta * (float)old[i]);
+    } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) h[i] = (_Float16)o[i];
-            *(PHX_GLOBAL phx_h8 *)to = h;
-            return;
-        }
+        for (int i = 0; i < 8; ++i) o[i] = (T)(p.alpha * acc[i]);
+    }
+    if (whole)
+        *(PHX_GLOBAL loose *)to = o;
+    else
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (n + i < p.N) {
-                if (p.beta != 0.0f) o[i] = o[i] + p.beta * (float)to[i];
-                to[i] = (_Float16)o[i];
-            }
-        return;
-    }
-    PHX_GLOBAL float *to = (PHX_GLOBAL float *)p.c + at;
-    if (p.wide && n + 8 <= p.N) {
-        phx_f4 v[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            v[h] = (phx_f4){o[4 * h], o[4 * h + 1], o[4 * h + 2], o[4 * h + 3]};
-            if (p.beta != 0.0f) v[h] = v[h] + p.beta * ((PHX_GLOBAL phx_f4 *)to)[h];
-        }
-        ((PHX_GLOBAL phx_f4 *)to)[0] = v[0];
-        ((PHX_GLOBAL phx_f4 *)to)[1] = v[1];
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (n + i < p.N) {
-            if (p.beta != 0.0f) o[i] = o[i] + p.beta * to[i];
-            to[i] = o[i];
-        }
+            if (n + i < p.N) to[i] = o[i];
 }
 
 // Until at most STEPS times EACH of a wave's loads are on their way.
@@ -377,8 +361,6 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
     constexpr uint32_t AHEAD = ST - 1, EACH = S::W_LOADS + S::A_LOADS;
     constexpr uint32_t SLOTS = (NT - 1) * MT, PER_SLOT = (EACH + SLOTS - 1) / SLOTS;
     const bool loads_scales = all < S::S_LOADS;
-    // (of a last tile of rows few may be left: waves without one load and pass on)
-    const bool live = wm * (16 * MT) < left_m;
     phx_u4 scales = {0, 0, 0, 0};
     auto pass = [&]() {
         if (S::STAGED && loads_scales)
@@ -406,14 +388,6 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
     };
     auto step = [&](uint32_t b0, char *now, char *then, char *fill) {
         const uint32_t b = b0 + wk;
-        if (WM > 1 && !live) {
-            load_more(b0, fill);
-#pragma unroll
-            for (uint32_t i = 0; i < EACH; ++i) load(fill, b + AHEAD * WK, i);
-            __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the scales are written
-            pass();
-            return;
-        }
         const float scale =
             __builtin_bit_cast(float, of_lane(__builtin_bit_cast(uint32_t, w_scales), b % 64));
         if (b0 % 64 == 64 - WK) load_w_scales(b0 + WK);
@@ -478,14 +452,27 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
         f[m] = 0.0f;
         sum[m] = (phx_f4){0, 0, 0, 0};
     }
-    uint32_t b = 0;
-    for (; b + AHEAD * WK < blocks; b += ST * WK)
+    auto steps = [&](auto one) {
+        uint32_t b = 0;
+        for (; b + AHEAD * WK < blocks; b += ST * WK)
 #pragma unroll
-        for (int u = 0; u < ST; ++u)
-            step(b + u * WK, st[u], st[(u + 1) % ST], st[(u + ST - 1) % ST]);
+            for (int u = 0; u < ST; ++u)
+                one(b + u * WK, st[u], st[(u + 1) % ST], st[(u + ST - 1) % ST]);
 #pragma unroll
-    for (int u = 0; u < ST - 1; ++u)
-        if (b + u * WK < blocks) step(b + u * WK, st[u], st[(u + 1) % ST], st[(u + ST - 1) % ST]);
+        for (int u = 0; u < ST - 1; ++u)
+            if (b + u * WK < blocks) one(b + u * WK, st[u], st[(u + 1) % ST], st[(u + ST - 1) % ST]);
+    };
+    // (of a last tile of rows few may be left: waves without one load and pass on)
+    if (WM == 1 || wm * (16 * MT) < left_m)
+        steps(step);
+    else
+        steps([&](uint32_t b0, char *, char *, char *fill) {
+            load_more(b0, fill);
+#pragma unroll
+            for (uint32_t i = 0; i < EACH; ++i) load(fill, b0 + wk + AHEAD * WK, i);
+            __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the scales are written
+            pass();
+        });
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -527,7 +514,7 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
             const float o[8] = {acc[n][m][0], acc[n][m][1], acc[n][m][2], acc[n][m][3],
                                 acc[n + 1][m][0], acc[n + 1][m][1], acc[n + 1][m][2], acc[n + 1][m][3]};
             const int64_t c = n0 + wn * (16 * NT) + 16 * n + 8 * g;
-            if (c < p.N) store8(p, o, t.m0 + row, c);
+            if (c < p.N) store8<std::conditional_t<EXACT, float, _Float16>>(p, o, t.m0 + row, c);
         }
     }
 }

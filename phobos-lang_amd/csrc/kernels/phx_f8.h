@@ -20,5 +20,4 @@ struct PhxF8Gemm {
     uint64_t a, sa, w, sw, c, starts, list;
     int64_t M, N, K, rows, lda, lds, ldc, experts;
     float alpha, beta;
-    int32_t half, wide;  // C is f16; its rows start 16-byte aligned
 };

@@ -103,9 +103,10 @@ NormForm norm_form(phx_dtype t, int64_t K) {
 // ------------------------------------------------------------------ products
 // A kernel of gemm_f8.hip: the columns and rows of a workgroup, how many blocks of K
 // it takes in a step, and how many workgroups a CU holds.  Of its time, fitted to
-// 225 shapes a type (1 to 4096 rows, K 512 to 8192; grouped: 1 to 512 rows each of
-// 5 to 61 experts): a step takes `step` ns, or `shared` for every workgroup of the
-// CU where that is more, and what is before and behind the steps `rest`.
+// the choices among the kernels over 225 shapes a type (1 to 4096 rows, K 512 to
+// 8192; grouped: 1 to 512 rows each of 5 to 61 experts): a step takes `step` ns, or
+// `shared` for every workgroup of the CU where that is more, and what is before
+// and behind the steps `rest`.
 struct GemmForm {
     int64_t columns, rows, blocks;
     uint32_t threads;
@@ -115,20 +116,20 @@ struct GemmForm {
 #define FORM(t, wn, wm, nt, mt, wk, st, held, step, shared, rest)                 \
     {16 * wn * nt, 16 * wm * mt, wk, 64 * wn * wm * wk, held, step, shared, rest, \
      "gemm_f8_" #t "_" #wn "x" #wm "_" #nt "x" #mt "_k" #wk "_s" #st}
-const GemmForm kGemmF16[] = {FORM(f16, 1, 1, 2, 1, 4, 4, 1, 193, 38, 2189),
-                             FORM(f16, 1, 1, 2, 1, 4, 2, 3, 64, 292, 1887),
-                             FORM(f16, 2, 1, 2, 1, 4, 3, 1, 174, 418, 2406),
-                             FORM(f16, 2, 2, 2, 2, 2, 4, 1, 175, 131, 5104),
-                             FORM(f16, 2, 2, 2, 2, 1, 4, 2, 277, 156, 1363),
-                             FORM(f16, 2, 2, 4, 2, 1, 3, 2, 562, 13, 1998),
-                             FORM(f16, 2, 4, 4, 2, 1, 2, 2, 940, 227, 52),
-                             FORM(f16, 2, 4, 8, 4, 1, 2, 1, 1392, 0, 1029)};
-const GemmForm kGemmF32[] = {FORM(f32, 1, 1, 2, 1, 4, 2, 3, 121, 294, 2199),
-                             FORM(f32, 2, 1, 2, 1, 4, 3, 1, 457, 32, 3189),
-                             FORM(f32, 2, 2, 2, 2, 2, 4, 1, 681, 14, 2192),
-                             FORM(f32, 2, 2, 2, 2, 1, 4, 2, 409, 350, 1686),
-                             FORM(f32, 2, 2, 4, 2, 1, 3, 2, 809, 592, 962),
-                             FORM(f32, 2, 2, 4, 4, 1, 2, 2, 1189, 1050, 971)};
+const GemmForm kGemmF16[] = {FORM(f16, 1, 1, 2, 1, 4, 4, 1, 198, 68, 2300),
+                             FORM(f16, 1, 1, 2, 1, 4, 2, 3, 61, 307, 1945),
+                             FORM(f16, 2, 1, 2, 1, 4, 3, 1, 208, 506, 2407),
+                             FORM(f16, 2, 2, 2, 2, 2, 4, 1, 199, 120, 4375),
+                             FORM(f16, 2, 2, 2, 2, 1, 4, 2, 288, 60, 1978),
+                             FORM(f16, 2, 2, 4, 2, 1, 3, 2, 544, 0, 1662),
+                             FORM(f16, 2, 4, 4, 2, 1, 2, 2, 944, 225, 0),
+                             FORM(f16, 2, 4, 8, 4, 1, 2, 1, 1408, 0, 393)};
+const GemmForm kGemmF32[] = {FORM(f32, 1, 1, 2, 1, 4, 2, 3, 24, 276, 2268),
+                             FORM(f32, 2, 1, 2, 1, 4, 3, 1, 297, 68, 4202),
+                             FORM(f32, 2, 2, 2, 2, 2, 4, 1, 682, 23, 1967),
+                             FORM(f32, 2, 2, 2, 2, 1, 4, 2, 391, 351, 1648),
+                             FORM(f32, 2, 2, 4, 2, 1, 3, 2, 806, 591, 958),
+                             FORM(f32, 2, 2, 4, 4, 1, 2, 2, 1187, 1050, 961)};
 #undef FORM
 
 int64_t estimate(const GemmForm &f, int64_t M, int64_t N, int64_t K, int64_t experts) {
@@ -143,11 +144,12 @@ int64_t estimate(const GemmForm &f, int64_t M, int64_t N, int64_t K, int64_t exp
     return groups / round * ns(f.held) + (left ? ns((left + 255) / 256) : 0);
 }
 
-// The kernel that is estimated fastest. Over those shapes the choice takes 5.6 % (f16)
-// and 3.8 % (f32) longer than the fastest of them; one kernel alone 26 % (64 x 64) and
-// more. 8192 x 16384 x 8192 f16: 256 x 256 935 us; 1 x 4096 x 4096: 32 x 16 6 us, 64
-// x 64 10 us, 256 x 256 42 us; 1 x 16384 x 8192: 32 x 16 with two stages, of which a
-// CU holds three, 27 us, with four stages 36 us.
+// The kernel that is estimated fastest. Over those shapes its time is 1.013 (f16) and
+// 1.014 (f32) times that of the fastest one, at most 1.24 and 1.35 times; any one
+// kernel for all is 1.26 times and more. 8192 x 16384 x 8192 f16: 256 x 256 930 us;
+// 1 x 4096 x 4096: 32 x 16 with four stages 5.9 us, 64 x 64 10 us, 256 x 256 42 us;
+// 1 x 16384 x 8192: 32 x 16 with two stages, of which a CU holds three, 27.6 us,
+// with four stages 36 us.
 const GemmForm &gemm_form(phx_dtype t, int64_t M, int64_t N, int64_t K, int64_t experts) {
     const GemmForm *first = t == PHX_F16 ? std::begin(kGemmF16) : std::begin(kGemmF32);
     const GemmForm *last = t == PHX_F16 ? std::end(kGemmF16) : std::end(kGemmF32);
@@ -200,8 +202,7 @@ int product(phx_stream s, const phx_f8_rows *a, const phx_f8_weights *w, bool gr
     if (int rc = on_device((hipStream_t)s)) return rc;
     if (!M) return PHX_OK;
     PhxF8Gemm p = {r.codes, r.scales, w->codes, w->scales, c, starts, list, M, w->n, r.k, r.rows,
-                   r.ld, r.lds, ldc, w->experts, alpha, beta, t == PHX_F16,
-                   !(c & 15) && ldc * size_of(t) % 16 == 0};
+                   r.ld, r.lds, ldc, w->experts, alpha, beta};
     return launch(kGemmFile, f.entry, tiles, f.threads, (hipStream_t)s, &p);
 }
 
