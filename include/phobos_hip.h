@@ -517,12 +517,13 @@ typedef struct {
 } phx_f8_weights;
 
 /* The root-mean-square norm of M rows of K (at most 32768) elements of type t:
- * H = round(X + R), or X where r is 0, stored where h is not 0 (it may be x or r);
+ * H = round(X + R), or X where r is 0, stored where h is not 0;
  * f = 1/sqrt(mean(H^2) + eps); of t = H * gain (f32 products) the codes go to q,
  * with the scales a * f / 448 (nullable), and round(f * t) to Y (0: not wanted).
  * The squares are summed in 64 bits.  gain is [K] of type t.  Rows are ldx, ldr,
  * ldh and ldy elements apart (0: K), start 16-byte aligned and in whole 16-byte
- * chunks.  q has M rows of K.  Outputs overlap nothing else. */
+ * chunks.  q has M rows of K.  One of H and Y may be X, one R (with their
+ * strides); apart from that outputs overlap nothing. */
 int phx_norm_f8(phx_stream s, phx_dtype t, uint64_t x, uint64_t r, uint64_t gain, uint64_t h,
                 uint64_t y, const phx_f8_rows *q, int64_t M, int64_t K, float eps, int64_t ldx,
                 int64_t ldr, int64_t ldh, int64_t ldy);
@@ -535,7 +536,10 @@ int phx_glu_f8(phx_stream s, phx_dtype t, uint64_t u, const phx_f8_rows *q, int6
  * (0: n): the products of a row's and a weight's codes in a block of 128 of K are
  * summed, then scaled by both scales and added in f32; C is rounded once from
  * fl(fl(alpha*acc) + fl(beta*c)), not read when beta == 0.  C overlaps no other
- * operand. */
+ * operand.  With t f32 every product enters whole.  With t f16 of the products of
+ * eight neighbouring codes what is below 2^-13 of their largest is cut off, all
+ * that the e4m3 matrix instruction keeps: 1.4e-5 of an ordinary result's norm,
+ * where the rounding to f16 is 2.1e-4. */
 int phx_gemm_f8(phx_stream s, const phx_f8_rows *a, const phx_f8_weights *w, phx_dtype t, uint64_t c,
                 float alpha, float beta, int64_t ldc);
 /* The same for M rows of C sorted by expert: row i, starts[e] <= i < starts[e+1],

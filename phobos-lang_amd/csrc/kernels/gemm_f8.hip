@@ -248,7 +248,7 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
         (void *)(p.w + (t.expert * p.N + n0) * p.K), 0, (int)(left_n * p.K), 0x00020000);
     // A: the tile's rows, or with a list all of them
     const int64_t base = p.list ? 0 : t.m0, left_m = min(t.end - t.m0, (int64_t)S::TM);
-    const int64_t rows = p.list ? p.rows : left_m;
+    const int64_t rows = p.list ? max(p.rows, (int64_t)1) : left_m;  // (none: nothing is read)
     const __amdgpu_buffer_rsrc_t ar = __builtin_amdgcn_make_buffer_rsrc(
         (void *)(p.a + base * p.lda), 0, (int)((rows - 1) * p.lda + p.K), 0x00020000);
     const __amdgpu_buffer_rsrc_t sr = __builtin_amdgcn_make_buffer_rsrc(

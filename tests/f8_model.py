@@ -32,7 +32,7 @@ def blocks_of(t):
     M, K = t.shape
     kb = -(-K // 128)
     b = np.zeros((M, kb, 128), t.dtype)
-    b.reshape(M, -1)[:, :K] = t
+    b.reshape(M, kb * 128)[:, :K] = t
     return b
 
 
@@ -46,7 +46,7 @@ def quotients(t):
     with np.errstate(invalid="ignore"):
         q = np.where(a[..., None] == 0, b, 448 * b / np.where(a == 0, 1, a)[..., None])
     q = np.where(bad[..., None], np.nan, q)
-    return q.reshape(t.shape[0], -1)[:, :K], a
+    return q.reshape(t.shape[0], b.shape[1] * 128)[:, :K], a
 
 
 def norm(x, r, gain, eps):

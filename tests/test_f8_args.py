@@ -194,3 +194,32 @@ def test_f8_quantize_of_zeros_and_what_it_refuses():
         assert _rc(lambda: px.f8_quantize(w)) == px.PHX_E_INVALID
     for bad in (np.zeros(16), np.zeros((0, 16)), 3.0):
         assert _rc(lambda: px.f8_quantize(bad)) == px.PHX_E_INVALID
+
+
+# ---------------------------------------------------------------- buffers that are too small
+def _buffer(nbytes):
+    b = px.DeviceBuffer.__new__(px.DeviceBuffer)
+    b.nbytes, b.ptr = nbytes, A
+    return b
+
+
+@pytest.mark.parametrize("which,bytes_", [("x", 2 * (2 * 152 + 144)), ("r", 2 * 3 * 144), ("gain", 288),
+                                          ("h", 2 * 3 * 144), ("y", 2 * 3 * 144)])
+def test_norm_looks_at_its_buffers(which, bytes_):
+    assert _norm(**{which: _buffer(bytes_), "ldx": 152}) == px.PHX_E_NOT_INIT
+    with pytest.raises(px.PhxError, match="buffer holds"):
+        px.launch_norm_f8(None, px.F16, *(_buffer(bytes_ - 1) if n == which else A
+                                          for n in ("x", "r", "gain", "h", "y")), _rows(), 3, 144, 1e-5, 152)
+
+
+def test_the_others_look_at_theirs():
+    r, w = _rows(), _weights(experts=4)
+    one = _weights()
+    for good, call in [(2 * 3 * 288, lambda b: px.launch_glu_f8(None, px.F16, b, r)),
+                       (4 * (2 * 9 + 5), lambda b: px.launch_gemm_f8(None, r, one, px.F32, b, ldc=9)),
+                       (2 * 7 * 5, lambda b: px.launch_gemm_f8_grouped(None, r, w, A, A, 7, px.F16, b)),
+                       (20, lambda b: px.launch_gemm_f8_grouped(None, r, w, b, A, 7, px.F16, A)),
+                       (28, lambda b: px.launch_gemm_f8_grouped(None, r, w, A, b, 7, px.F16, A))]:
+        assert _rc(lambda: call(_buffer(good))) == px.PHX_E_NOT_INIT
+        with pytest.raises(px.PhxError, match="buffer holds"):
+            call(_buffer(good - 1))

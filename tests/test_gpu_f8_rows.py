@@ -142,6 +142,23 @@ def test_norm_strides_and_outputs(px_gpu, stream, bits):
 
 
 @pytest.mark.parametrize("bits", [16, 32])
+@pytest.mark.parametrize("K", [528, 2064, 20000])
+def test_norm_with_y_in_place(px_gpu, stream, bits, K):
+    # Y over X, and H over R
+    px = px_gpu
+    dt, t = _t(px, bits)
+    rng = np.random.default_rng(K)
+    x, r = (rng.standard_normal((5, K)).astype(t) for _ in range(2))
+    gain = rng.standard_normal(K).astype(t)
+    dx, dr, dg = (px.DeviceBuffer.from_array(v) for v in (x, r, gain))
+    codes, scales, rows = _f8_out(px, 5, K)
+    px.launch_norm_f8(stream, dt, dx, dr, dg, dr, dx, rows, 5, K, 1e-5)
+    stream.synchronize()
+    got = [dr.download(t, (5, K)), dx.download(t, (5, K)), codes.get(), scales.get()]
+    _check_norm(got, x, r, gain, 1e-5)
+
+
+@pytest.mark.parametrize("bits", [16, 32])
 def test_norm_codes_at_ties(px_gpu, stream, bits):
     # 448 in every block, so that a value is its own quotient: all codes' values,
     # the middles between them, and what is next to those
