@@ -542,10 +542,10 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
     TILE(true, f32, WN, WM, NT, MT, WK, ST)
 TILE(false, f16, 1, 1, 2, 1, 4, 4)
 BOTH(1, 1, 2, 1, 4, 2)
-BOTH(2, 1, 2, 1, 4, 3)
+TILE(false, f16, 2, 1, 2, 1, 4, 3)
 BOTH(2, 2, 2, 2, 2, 4)
 BOTH(2, 2, 2, 2, 1, 4)
 BOTH(2, 2, 4, 2, 1, 3)
 TILE(true, f32, 2, 2, 4, 4, 1, 2)
-TILE(false, f16, 2, 4, 4, 2, 1, 2)
+TILE(false, f16, 2, 4, 8, 2, 1, 3)
 TILE(false, f16, 2, 4, 8, 4, 1, 2)

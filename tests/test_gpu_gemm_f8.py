@@ -144,8 +144,8 @@ SHAPES = [(1, 1, 16), (1, 16, 128), (2, 17, 144), (3, 5, 32), (15, 33, 112), (16
 
 # more tiles of every kind than the GPU runs at a time, last ones short
 LARGE = [(2049, 4111, 272), (4100, 4090, 144), (1, 16500, 528), (40, 16390, 272), (700, 9000, 144),
-         (8200, 300, 400), (1, 12000, 4144), (33, 3000, 4144), (33, 8000, 2064), (100, 4000, 2064),
-         (17, 16000, 2064)]
+         (8200, 300, 400), (1, 12000, 4144), (33, 3000, 4144), (33, 6000, 4144), (100, 4000, 2064),
+         (17, 16000, 2064), (300, 16000, 528)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES + LARGE)
