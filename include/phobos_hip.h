@@ -534,9 +534,9 @@ int phx_norm_f8(phx_stream s, phx_dtype t, uint64_t x, uint64_t r, uint64_t gain
 int phx_glu_f8(phx_stream s, phx_dtype t, uint64_t u, const phx_f8_rows *q, int64_t ldu);
 /* C = alpha * A @ W^T + beta * C of type t, [A's rows, n], rows ldc elements apart
  * (0: n): the products of a row's and a weight's codes in a block of 128 of K are
- * summed, then scaled by both scales and added in f32; C is rounded once from
- * fl(fl(alpha*acc) + fl(beta*c)), not read when beta == 0.  C overlaps no other
- * operand.  With t f32 every product enters whole.  With t f16 of the products of
+ * summed, then scaled by the f32 product of both scales and added in f32; C is
+ * rounded once from fl(fl(alpha*acc) + fl(beta*c)), not read when beta == 0.  C
+ * overlaps no other operand.  With t f32 every product enters whole.  With t f16 of the products of
  * eight neighbouring codes what is below 2^-13 of their largest is cut off, all
  * that the e4m3 matrix instruction keeps: 1.4e-5 of an ordinary result's norm,
  * where the rounding to f16 is 2.1e-4. */

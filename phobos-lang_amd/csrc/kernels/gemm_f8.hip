@@ -3,9 +3,28 @@
 //
 //   acc[m,n] = sum over blocks b of sa[m,b] sw[n/128,b] * sum over k in b of a[m,k] w[n,k]
 //
-// The inner sum is one v_mfma_f32_16x16x128 of the codes, scaled in f32. The
-// weights are its A operand, so that a lane holds four neighbouring columns of
-// one row of C, and one row's scale.
+// f16 outputs: the inner sum is one v_mfma_f32_16x16x128 of the codes. Of eight
+// neighbouring products it keeps what is above 2^-13 of the largest (measured with
+// one large and one small product; the sums of eight are added in f32): 1.4e-5 of an
+// ordinary result's norm, where the rounding to f16 is 2.1e-4.
+// f32 outputs, which that would show in, take the codes as f16, exactly, and four
+// v_mfma_f32_16x16x32: 1.1e-7, at half the rate.
+// The inner sum is scaled and added in f32 by vector instructions, four for each
+// 16 x 16, which run while the matrix cores work on the next one. The weights are the
+// A operand, so that a lane holds neighbouring columns of one row of C, whose
+// scales' product is one number.
+//
+// Large products are bound by the power that the card may take, and by LDS: a 256 x 256
+// tile's step of 128 k reads 192 KiB of operands from LDS and writes 64 KiB into it, at
+// 128 and about 64 bytes a cycle 2560 cycles, in which the matrix cores have 2048 to do.
+// 8192 x 16384 x 8192, f16: 930 us (2360 TFLOP/s; a large 8-bit product of a library,
+// with one scale for all, 3330) at 1.8 GHz, the matrix cores busy 63 % of the cycles.
+// Few rows are bound by the weights' bytes: 1 x 16384 x 8192 27.6 us (4.9 TB/s), 64 rows
+// 33.9 us (4.0 TB/s). Between them, tiles that fill the GPU but once, it is the
+// latency of a step: 1000 x 1000 x 4144, f32, 17.4 us in 17 steps of 256 k.
+// (Also measured, at the same speed or slower: rows staged through registers instead of
+// loaded into LDS directly; waves of 64 x 64 that read less LDS but are half as many;
+// loads spread over the whole step; a raised wave priority; 2 or 8 rows of tiles deep.)
 #include <type_traits>
 
 #include "f8.h"
@@ -64,15 +83,15 @@ __device__ __forceinline__ Tile tile_of(const PhxF8Gemm &p, uint32_t columns) {
     t.live = false;
     t.expert = 0;
     t.end = p.M;
-    uint32_t tiles = (uint32_t)((p.M + TM - 1) / TM), first = 0, id;
-    int64_t begin = 0;
+    uint32_t begin = 0, tiles = (uint32_t)((p.M + TM - 1) / TM), in;  // of the group; in it
     if (!p.starts) {
-        id = phx_xcd_swizzle_any(blockIdx.x, gridDim.x);
+        in = uniform(phx_xcd_swizzle_any(blockIdx.x, gridDim.x));
     } else {
-        const uint32_t lane = threadIdx.x & 63, E = (uint32_t)p.experts, M = (uint32_t)p.M;
+        const uint32_t lane = threadIdx.x & 63, E = (uint32_t)p.experts;
         const PHX_GLOBAL int32_t *starts = (const PHX_GLOBAL int32_t *)p.starts;
-        auto at = [&](uint32_t e) { return (uint32_t)min(max(starts[min(e, E)], 0), (int32_t)M); };
-        // 64 experts' first and last row, and how many tiles there are up to each
+        auto at = [&](uint32_t e) { return (uint32_t)min(max(starts[min(e, E)], 0), (int32_t)p.M); };
+        // 64 experts' first row and the one past the last, their tiles, and how many there
+        // are up to each
         struct Range {
             uint32_t begin, end, tiles, upto;
         };
@@ -86,37 +105,30 @@ __device__ __forceinline__ Tile tile_of(const PhxF8Gemm &p, uint32_t columns) {
             return x;
         };
         Range x = range(0, 0, 0);
-        uint32_t total = of_lane(x.upto, 63);
-        if (E > 64) {
-            uint32_t floor = of_lane(x.end, 63);
-            for (uint32_t e0 = 64; e0 < E; e0 += 64) {
-                const Range y = range(e0, floor, total);
-                floor = of_lane(y.end, 63);
-                total = of_lane(y.upto, 63);
-            }
+        uint32_t total = of_lane(x.upto, 63), floor = of_lane(x.end, 63);
+        for (uint32_t e0 = 64; e0 < E; e0 += 64) {
+            const Range y = range(e0, floor, total);
+            floor = of_lane(y.end, 63);
+            total = of_lane(y.upto, 63);
         }
         if (blockIdx.x >= total * columns) return t;
-        id = phx_xcd_swizzle_any(blockIdx.x, total * columns);
-        const uint32_t wanted = id / columns;
+        const uint32_t id = uniform(phx_xcd_swizzle_any(blockIdx.x, total * columns));
         uint32_t e0 = 0;
-        while (of_lane(x.upto, 63) <= wanted) {
+        while (of_lane(x.upto, 63) <= id / columns) {
             e0 += 64;
             x = range(e0, of_lane(x.end, 63), of_lane(x.upto, 63));
         }
-        const uint32_t l = uniform(__builtin_ctzll(__ballot(x.upto > wanted)));
-        t.expert = e0 + l;
-        t.expert = uniform((uint32_t)t.expert);
+        const uint32_t l = uniform(__builtin_ctzll(__ballot(x.upto > id / columns)));
+        t.expert = uniform(e0 + l);
         begin = of_lane(x.begin, l);
         t.end = of_lane(x.end, l);
         tiles = of_lane(x.tiles, l);
-        first = of_lane(x.upto, l) - tiles;
+        in = uniform(id - (of_lane(x.upto, l) - tiles) * columns);
     }
-    id = uniform(id);
-    const uint32_t in = id - first * columns;
     const uint32_t top = in / (kDeep * columns) * kDeep, rest = in % (kDeep * columns);
     const uint32_t deep = min(tiles - top, kDeep);
     t.column = uniform(rest / deep);
-    t.m0 = uniform((uint32_t)begin + (top + rest % deep) * TM);
+    t.m0 = uniform(begin + (top + rest % deep) * TM);
     t.live = true;
     return t;
 }
@@ -135,12 +147,14 @@ struct Shape {
     static constexpr uint32_t WAVES = WN * WM, TN = 16 * WN * NT, TM = 16 * WM * MT;
     static constexpr uint32_t PART = (TN + TM) * 128;
     // The rows' scales come four blocks at a time, a row's 16 bytes next to each other:
-    // with four sets or more those of a step's blocks in its stage, with fewer in
-    // places of their own, through registers.
-    static constexpr bool STAGED = WK >= 4;
-    static constexpr uint32_t SCALES = (TM < 64 ? 64 : TM) * 16, FOURS = STAGED ? WK / 4 : 1;
-    static constexpr uint32_t S_LOADS = SCALES / 1024 * FOURS;  // waves that load them
-    static constexpr uint32_t STAGE = PART * WK + (STAGED ? FOURS * SCALES : 0);
+    // with four sets, which take four blocks a step, in its stage; with fewer in places
+    // of their own, through registers (loaded into LDS directly, each read of them
+    // would wait for the latest such load).
+    static_assert(WK == 1 || WK == 2 || WK == 4, "a step within four blocks");
+    static constexpr bool STAGED = WK == 4;
+    static constexpr uint32_t SCALES = (TM < 64 ? 64 : TM) * 16;
+    static constexpr uint32_t S_LOADS = SCALES / 1024;  // waves that load them
+    static constexpr uint32_t STAGE = PART * WK + (STAGED ? SCALES : 0);
     static constexpr uint32_t APART = STAGED ? 16 : 2 * SCALES;
     static constexpr uint32_t W_LOADS = TN / 8 / WAVES, A_LOADS = TM / 8 / WAVES;  // of 8 rows
     static_assert(TN % (8 * WAVES) == 0 && TM % (8 * WAVES) == 0, "whole loads a wave");
@@ -221,12 +235,11 @@ __device__ __forceinline__ void store8(const PhxF8Gemm &p, const float (&acc)[8]
             if (n + i < p.N) to[i] = o[i];
 }
 
-// Until at most STEPS times EACH of a wave's loads are on their way.
-template <uint32_t STEPS, uint32_t EACH>
-__device__ __forceinline__ void wait_loads() {
-    constexpr uint32_t LEFT = STEPS * EACH;
+// Until at most LEFT of a wave's loads are on their way, and nothing to or from LDS.
+template <uint32_t LEFT>
+__device__ __forceinline__ void wait_for() {
     static_assert(LEFT < 64, "vmcnt's six bits");
-    __builtin_amdgcn_s_waitcnt(0x0f70 | (LEFT & 15) | (LEFT >> 4) << 14);
+    __builtin_amdgcn_s_waitcnt(0x0070 | (LEFT & 15) | (LEFT >> 4) << 14);
 }
 
 template <bool EXACT, int WN, int WM, int NT, int MT, int WK, int ST>
@@ -280,7 +293,7 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
         a_off[i] = at < 0 ? kNone : (uint32_t)(at * p.lda) + a_k(i);
     }
     if (all < S::S_LOADS) {
-        const int64_t at = source(all % (S::SCALES / 1024) * 64 + lane);
+        const int64_t at = source(all * 64 + lane);
         s_off = at < 0 ? kNone : (uint32_t)(at * p.lds * 4);
     }
     // the i-th of this wave's loads of block b: 8 rows of W or of A
@@ -298,10 +311,12 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
                 k + a_k(j) < K ? a_off[j] : kNone, (int)k, 0, 0);
         }
     };
-    // the scales of the tile's rows of the four blocks from 4q on: this wave's share
+    // the scales of the tile's rows of the four blocks from 4q on: where this wave's
+    // share is (behind the rows' end nowhere), and into LDS
+    auto scales_at = [&](uint32_t q) { return 4 * q < (uint32_t)p.lds ? s_off : kNone; };
     auto load_scales = [&](char *to, uint32_t q) {
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(sr, (lds_ptr)(to + all * 1024), 16, s_off,
-                                                 (int)((q + all / (S::SCALES / 1024)) * 16), 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(sr, (lds_ptr)(to + all * 1024), 16, scales_at(q),
+                                                 (int)(q * 16), 0, 0);
     };
     // the weights' scales of 64 blocks, one a lane
     const PHX_GLOBAL float *sw = (const PHX_GLOBAL float *)p.sw +
@@ -346,7 +361,7 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
             x_next[m][h] = *(const phx_u4 *)(stage + wk * S::PART + a_at[h] + m * 2048);
     };
     auto read_scale = [&](const char *stage, uint32_t b0, int m) {
-        const char *from = S::STAGED ? stage + WK * S::PART + wk / 4 * S::SCALES
+        const char *from = S::STAGED ? stage + WK * S::PART
                                      : sc + b0 / 4 % 2 * S::SCALES;
         return *(const float *)(from + s_at + m * 256 + (b0 + wk) % 4 * 4);
     };
@@ -364,10 +379,12 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
     phx_u4 scales = {0, 0, 0, 0};
     auto pass = [&]() {
         if (S::STAGED && loads_scales)
-            wait_loads<AHEAD - 1, EACH + 1>();
+            wait_for<(AHEAD - 1) * (EACH + 1)>();
         else
-            wait_loads<AHEAD - 1, EACH>();
+            wait_for<(AHEAD - 1) * EACH>();
+        asm volatile("" ::: "memory");  // no access moves across
         __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
     };
     load_w_scales(0);
@@ -378,11 +395,13 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
             load_scales(fill + WK * S::PART, (b0 + AHEAD * WK) / 4);
             return;
         }
-        // the next four blocks' scales: loaded at the first of these four, written at
-        // the third (two steps of the four, where a step takes two)
+        // the next four blocks' scales: loaded at the first of these four, written at the
+        // third (at the two steps of the four, where a step takes two), behind two
+        // barriers or more since what was there was read
         if (b0 % 4 == 0)
             scales = __builtin_bit_cast(
-                phx_u4, __builtin_amdgcn_raw_buffer_load_b128(sr, s_off, (int)(b0 * 4 + 16), 0));
+                phx_u4, __builtin_amdgcn_raw_buffer_load_b128(sr, scales_at(b0 / 4 + 1),
+                                                              (int)(b0 * 4 + 16), 0));
         if (b0 % 4 == 2)
             *(phx_u4 *)(sc + (b0 / 4 + 1) % 2 * S::SCALES + threadIdx.x * 16) = scales;
     };
@@ -470,7 +489,6 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
             load_more(b0, fill);
 #pragma unroll
             for (uint32_t i = 0; i < EACH; ++i) load(fill, b0 + wk + AHEAD * WK, i);
-            __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the scales are written
             pass();
         });
 #pragma unroll
@@ -480,7 +498,7 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
             acc[NT - 1][m][i] = __builtin_fmaf(f[m], sum[m][i], acc[NT - 1][m][i]);
     // (the loads behind the last block write zeros: before the sums, and before LDS is
     // another workgroup's)
-    __builtin_amdgcn_s_waitcnt(0x0f70);
+    wait_for<0>();
     if (WK > 1) {
         // the sets' sums to LDS; of them each wave adds up and stores its share
         __syncthreads();
@@ -533,7 +551,7 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
     extern "C" __global__ __launch_bounds__(64 * WN * WM * WK) void                             \
         gemm_f8_##suffix##_##WN##x##WM##_##NT##x##MT##_k##WK##_s##ST(PhxF8Gemm p) {             \
         using S = Shape<WN, WM, NT, MT, WK, ST>;                                                \
-        __shared__ phx_u4 STAGES_##ST(S), sc[S::APART / 16];                         \
+        __shared__ phx_u4 STAGES_##ST(S), sc[S::APART / 16];                                    \
         char *const st[ST] = {LIST_##ST};                                                       \
         gemm_tile<EXACT, WN, WM, NT, MT, WK, ST>(p, st, (char *)sc);                            \
     }
