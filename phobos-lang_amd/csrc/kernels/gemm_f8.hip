@@ -40,7 +40,7 @@ constexpr uint32_t kNone = 0x80000000u;  // an offset past every resource's end:
 // Where a tile of TM rows lies: its expert, and C's rows from m0 up to end.
 struct Tile {
     int64_t m0, end, expert;
-    uint32_t column;  // in tiles
+    uint32_t column, rows;  // in tiles: its column, and the group's rows
     bool live;
 };
 
@@ -129,6 +129,7 @@ __device__ __forceinline__ Tile tile_of(const PhxF8Gemm &p, uint32_t columns) {
     const uint32_t deep = min(tiles - top, kDeep);
     t.column = uniform(rest / deep);
     t.m0 = uniform(begin + (top + rest % deep) * TM);
+    t.rows = tiles;
     t.live = true;
     return t;
 }
@@ -254,6 +255,16 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
     const int64_t n0 = (int64_t)t.column * S::TN;
     const uint32_t blocks = (uint32_t)((p.K + 127) / 128);
     const uint32_t K = (uint32_t)p.K;
+    // Of few rows every workgroup reads weights of its own, all at the same k at the same
+    // time, rows of W apart, which memory is slower with than it need be: they start
+    // at different blocks instead and go round (in fours, as the scales come). 64 x 16384
+    // x 8192: 29.6 us, all from the first on 34; 32 experts with 62 rows each of 4096
+    // x 4096: 128 and 151. (With more rows neighbours share what they read: 256 x 256
+    // tiles would take 1 to 4 % longer so.)
+    const uint32_t turn = S::TM > 64 || t.rows > kDeep || blocks % 4 ? 0 : t.column * 12 % blocks;
+    auto turned = [&](uint32_t b) {
+        return b >= blocks ? b : b + turn >= blocks ? b + turn - blocks : b + turn;
+    };
 
     // W: rows of this tile up to N's end
     const int64_t left_n = min(p.N - n0, (int64_t)S::TN);
@@ -298,7 +309,7 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
     }
     // the i-th of this wave's loads of block b: 8 rows of W or of A
     auto load = [&](char *stage, uint32_t b, uint32_t i) {
-        const uint32_t k = b * 128;
+        const uint32_t k = turned(b) * 128;
         char *to = stage + wk * S::PART;
         if (i < S::W_LOADS) {
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
@@ -311,19 +322,20 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
                 k + a_k(j) < K ? a_off[j] : kNone, (int)k, 0, 0);
         }
     };
-    // the scales of the tile's rows of the four blocks from 4q on: where this wave's
-    // share is (behind the rows' end nowhere), and into LDS
-    auto scales_at = [&](uint32_t q) { return 4 * q < (uint32_t)p.lds ? s_off : kNone; };
-    auto load_scales = [&](char *to, uint32_t q) {
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(sr, (lds_ptr)(to + all * 1024), 16, scales_at(q),
-                                                 (int)(q * 16), 0, 0);
+    // the scales of the tile's rows of the four blocks from b on: where this wave's share
+    // is (behind the rows' end nowhere), and into LDS
+    auto scales_at = [&](uint32_t b) { return b < (uint32_t)p.lds ? s_off : kNone; };
+    auto load_scales = [&](char *to, uint32_t b) {
+        b = turned(b);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(sr, (lds_ptr)(to + all * 1024), 16, scales_at(b),
+                                                 (int)(b * 4), 0, 0);
     };
     // the weights' scales of 64 blocks, one a lane
     const PHX_GLOBAL float *sw = (const PHX_GLOBAL float *)p.sw +
                                  (t.expert * ((p.N + 127) / 128) +
                                   min((n0 + wn * (16 * NT)) / 128, (p.N - 1) / 128)) * blocks;
     float w_scales;
-    auto load_w_scales = [&](uint32_t b) { w_scales = sw[min(b + lane, blocks - 1)]; };
+    auto load_w_scales = [&](uint32_t b) { w_scales = sw[min(turned(b + lane), blocks - 1)]; };
 
     phx_f4 acc[NT][MT];
 #pragma unroll
@@ -392,16 +404,17 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
     auto load_more = [&](uint32_t b0, char *fill) {
         if (!loads_scales) return;
         if (S::STAGED) {
-            load_scales(fill + WK * S::PART, (b0 + AHEAD * WK) / 4);
+            load_scales(fill + WK * S::PART, b0 + AHEAD * WK);
             return;
         }
         // the next four blocks' scales: loaded at the first of these four, written at the
         // third (at the two steps of the four, where a step takes two), behind two
         // barriers or more since what was there was read
-        if (b0 % 4 == 0)
+        if (b0 % 4 == 0) {
+            const uint32_t b = turned(b0 + 4);
             scales = __builtin_bit_cast(
-                phx_u4, __builtin_amdgcn_raw_buffer_load_b128(sr, scales_at(b0 / 4 + 1),
-                                                              (int)(b0 * 4 + 16), 0));
+                phx_u4, __builtin_amdgcn_raw_buffer_load_b128(sr, scales_at(b), (int)(b * 4), 0));
+        }
         if (b0 % 4 == 2)
             *(phx_u4 *)(sc + (b0 / 4 + 1) % 2 * S::SCALES + threadIdx.x * 16) = scales;
     };
@@ -458,7 +471,7 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
     if (!S::STAGED && loads_scales) load_scales(sc, 0);
 #pragma unroll
     for (uint32_t u = 0; u < AHEAD; ++u) {
-        if (S::STAGED && loads_scales) load_scales(st[u] + WK * S::PART, u * WK / 4);
+        if (S::STAGED && loads_scales) load_scales(st[u] + WK * S::PART, u * WK);
 #pragma unroll
         for (uint32_t i = 0; i < EACH; ++i) load(st[u], u * WK + wk, i);
     }

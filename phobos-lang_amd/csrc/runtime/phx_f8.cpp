@@ -103,7 +103,7 @@ NormForm norm_form(phx_dtype t, int64_t K) {
 // ------------------------------------------------------------------ products
 // A kernel of gemm_f8.hip: the columns and rows of a workgroup, how many blocks of K
 // it takes in a step, and how many workgroups a CU holds.  Of its time, fitted to
-// the choices among the kernels over 268 shapes a type (1 to 4096 rows, K 512 to
+// the choices among the kernels over 286 shapes a type (1 to 4096 rows, K 512 to
 // 8192; grouped: 1 to 512 rows each of 5 to 61 experts): a step takes `step` ns, or
 // `shared` for every workgroup of the CU where that is more, and what is before
 // and behind the steps `rest`.
@@ -116,19 +116,19 @@ struct GemmForm {
 #define FORM(t, wn, wm, nt, mt, wk, st, held, step, shared, rest)                 \
     {16 * wn * nt, 16 * wm * mt, wk, 64 * wn * wm * wk, held, step, shared, rest, \
      "gemm_f8_" #t "_" #wn "x" #wm "_" #nt "x" #mt "_k" #wk "_s" #st}
-const GemmForm kGemmF16[] = {FORM(f16, 1, 1, 2, 1, 4, 4, 1, 157, 0, 2352),
-                             FORM(f16, 1, 1, 2, 1, 4, 2, 3, 9, 288, 1904),
-                             FORM(f16, 2, 1, 2, 1, 4, 3, 1, 422, 0, 2434),
-                             FORM(f16, 2, 2, 2, 2, 2, 4, 1, 173, 0, 4838),
-                             FORM(f16, 2, 2, 2, 2, 1, 4, 2, 226, 136, 1635),
-                             FORM(f16, 2, 2, 4, 2, 1, 3, 2, 557, 19, 1069),
-                             FORM(f16, 2, 4, 8, 2, 1, 3, 1, 762, 0, 746),
-                             FORM(f16, 2, 4, 8, 4, 1, 2, 1, 1318, 0, 109)};
-const GemmForm kGemmF32[] = {FORM(f32, 1, 1, 2, 1, 4, 2, 3, 327, 290, 2235),
-                             FORM(f32, 2, 2, 2, 2, 2, 4, 1, 659, 0, 2420),
-                             FORM(f32, 2, 2, 2, 2, 1, 4, 2, 420, 350, 1760),
-                             FORM(f32, 2, 2, 4, 2, 1, 3, 2, 806, 591, 965),
-                             FORM(f32, 2, 2, 4, 4, 1, 2, 2, 1190, 1052, 937)};
+const GemmForm kGemmF16[] = {FORM(f16, 1, 1, 2, 1, 4, 4, 1, 148, 0, 2549),
+                             FORM(f16, 1, 1, 2, 1, 4, 2, 3, 9, 289, 1970),
+                             FORM(f16, 2, 1, 2, 1, 4, 3, 1, 413, 0, 2048),
+                             FORM(f16, 2, 2, 2, 2, 2, 4, 1, 340, 0, 2477),
+                             FORM(f16, 2, 2, 2, 2, 1, 4, 2, 212, 127, 2107),
+                             FORM(f16, 2, 2, 4, 2, 1, 3, 2, 559, 28, 974),
+                             FORM(f16, 2, 4, 8, 2, 1, 3, 1, 766, 0, 504),
+                             FORM(f16, 2, 4, 8, 4, 1, 2, 1, 1314, 0, 58)};
+const GemmForm kGemmF32[] = {FORM(f32, 1, 1, 2, 1, 4, 2, 3, 77, 313, 2117),
+                             FORM(f32, 2, 2, 2, 2, 2, 4, 1, 687, 0, 1760),
+                             FORM(f32, 2, 2, 2, 2, 1, 4, 2, 370, 357, 1616),
+                             FORM(f32, 2, 2, 4, 2, 1, 3, 2, 807, 589, 988),
+                             FORM(f32, 2, 2, 4, 4, 1, 2, 2, 1191, 1050, 957)};
 #undef FORM
 
 int64_t estimate(const GemmForm &f, int64_t M, int64_t N, int64_t K, int64_t experts) {
@@ -144,7 +144,7 @@ int64_t estimate(const GemmForm &f, int64_t M, int64_t N, int64_t K, int64_t exp
 }
 
 // The kernel that is estimated fastest. Over those shapes its time is 1.012 (f16) and
-// 1.011 (f32) times that of the fastest one, at most 1.21 and 1.29 times; any one
+// 1.008 (f32) times that of the fastest one, at most 1.28 and 1.35 times; any one
 // kernel for all is 1.26 times and more. 8192 x 16384 x 8192 f16: 256 x 256 930 us,
 // 256 x 128 1079; 384 x 16384 x 8192: 256 x 128 68 us, 256 x 256 102; 1 x 4096 x
 // 4096: 32 x 16 with four stages 5.9 us, 64 x 64 10, 256 x 256 42; 1 x 16384 x

@@ -139,12 +139,13 @@ SHAPES = [(1, 1, 16), (1, 16, 128), (2, 17, 144), (3, 5, 32), (15, 33, 112), (16
           (17, 40, 400), (33, 100, 80), (64, 15, 528), (48, 257, 1040), (1, 1000, 4144), (4, 64, 8192),
           (65, 130, 2064), (5, 4099, 64), (1, 31, 16384), (127, 129, 272), (128, 128, 1024),
           (129, 300, 640), (200, 1030, 384), (256, 256, 512), (300, 520, 1040), (257, 255, 2048),
-          (513, 700, 128), (1000, 1000, 16), (1030, 2050, 656)]
+          (513, 700, 128), (1000, 1000, 16), (1030, 2050, 656), (5, 700, 2048), (64, 300, 1024), (100, 500, 512),
+          (33, 9000, 3584), (256, 260, 1536)]
 
 
 # more tiles of every kind than the GPU runs at a time, last ones short
 LARGE = [(2049, 4111, 272), (4100, 4090, 144), (1, 16500, 528), (40, 16390, 272), (700, 9000, 144),
-         (8200, 300, 400), (1, 12000, 4144), (33, 3000, 4144), (33, 6000, 4144), (100, 4000, 2064),
+         (8200, 300, 400), (1, 12000, 4144), (33, 3000, 4144), (33, 6000, 4144), (100, 4000, 4144),
          (17, 16000, 2064), (300, 16000, 528)]
 
 
@@ -271,7 +272,8 @@ def _want(a, w, starts, order, M):
 
 GROUPED = [(1, 1, 1, 16, 0), (5, 3, 17, 144, 1), (40, 7, 100, 272, 2), (16, 32, 260, 1040, 18),
            (300, 4, 130, 400, 0), (1000, 6, 257, 256, 1), (700, 64, 140, 128, 30), (3, 200, 33, 64, 190),
-           (129, 130, 16, 528, 3), (2000, 3, 300, 272, 1), (60, 2, 2050, 400, 0)]
+           (129, 130, 16, 528, 3), (2000, 3, 300, 272, 1), (60, 2, 2050, 400, 0), (50, 9, 300, 1024, 3), (200, 3, 500, 512, 0),
+           (9, 4, 5000, 2048, 1)]
 
 
 @pytest.mark.parametrize("M,E,N,K,idle", GROUPED)
