@@ -102,10 +102,10 @@ NormForm norm_form(phx_dtype t, int64_t K) {
 
 // ------------------------------------------------------------------ products
 // A kernel of gemm_f8.hip: the columns and rows of a workgroup, how many blocks of K
-// it takes in a step, and how many workgroups a CU holds.  Of its time, fitted to
-// the choices among the kernels over 286 shapes a type (1 to 4096 rows, K 512 to
-// 8192; grouped: 1 to 512 rows each of 5 to 61 experts): a step takes `step` ns, or
-// `shared` for every workgroup of the CU where that is more, and what is before
+// it takes in a step, and how many workgroups a CU holds.  What its time is made of,
+// fitted to the choices among the kernels over 502 shapes a type (1 to 4096 rows, K
+// 64 to 8192; grouped: 1 to 512 rows each of 5 to 61 experts): a step takes `step`
+// ns, or `shared` for every workgroup of the CU where that is more, and what is before
 // and behind the steps `rest`.
 struct GemmForm {
     int64_t columns, rows, blocks;
@@ -116,19 +116,19 @@ struct GemmForm {
 #define FORM(t, wn, wm, nt, mt, wk, st, held, step, shared, rest)                 \
     {16 * wn * nt, 16 * wm * mt, wk, 64 * wn * wm * wk, held, step, shared, rest, \
      "gemm_f8_" #t "_" #wn "x" #wm "_" #nt "x" #mt "_k" #wk "_s" #st}
-const GemmForm kGemmF16[] = {FORM(f16, 1, 1, 2, 1, 4, 4, 1, 148, 0, 2549),
-                             FORM(f16, 1, 1, 2, 1, 4, 2, 3, 9, 289, 1970),
-                             FORM(f16, 2, 1, 2, 1, 4, 3, 1, 413, 0, 2048),
-                             FORM(f16, 2, 2, 2, 2, 2, 4, 1, 340, 0, 2477),
-                             FORM(f16, 2, 2, 2, 2, 1, 4, 2, 212, 127, 2107),
-                             FORM(f16, 2, 2, 4, 2, 1, 3, 2, 559, 28, 974),
-                             FORM(f16, 2, 4, 8, 2, 1, 3, 1, 766, 0, 504),
-                             FORM(f16, 2, 4, 8, 4, 1, 2, 1, 1314, 0, 58)};
-const GemmForm kGemmF32[] = {FORM(f32, 1, 1, 2, 1, 4, 2, 3, 77, 313, 2117),
-                             FORM(f32, 2, 2, 2, 2, 2, 4, 1, 687, 0, 1760),
-                             FORM(f32, 2, 2, 2, 2, 1, 4, 2, 370, 357, 1616),
-                             FORM(f32, 2, 2, 4, 2, 1, 3, 2, 807, 589, 988),
-                             FORM(f32, 2, 2, 4, 4, 1, 2, 2, 1191, 1050, 957)};
+const GemmForm kGemmF16[] = {FORM(f16, 1, 1, 2, 1, 4, 4, 1, 189, 0, 2313),
+                             FORM(f16, 1, 1, 2, 1, 4, 2, 3, 1, 288, 1528),
+                             FORM(f16, 2, 1, 2, 1, 4, 3, 1, 486, 0, 1600),
+                             FORM(f16, 2, 2, 2, 2, 2, 4, 1, 371, 0, 1911),
+                             FORM(f16, 2, 2, 2, 2, 1, 4, 2, 220, 188, 1546),
+                             FORM(f16, 2, 2, 4, 2, 1, 3, 2, 415, 14, 1413),
+                             FORM(f16, 2, 4, 8, 2, 1, 3, 1, 527, 0, 1406),
+                             FORM(f16, 2, 4, 8, 4, 1, 2, 1, 910, 0, 2038)};
+const GemmForm kGemmF32[] = {FORM(f32, 1, 1, 2, 1, 4, 2, 3, 689, 459, 1322),
+                             FORM(f32, 2, 2, 2, 2, 2, 4, 1, 759, 0, 1343),
+                             FORM(f32, 2, 2, 2, 2, 1, 4, 2, 411, 356, 1109),
+                             FORM(f32, 2, 2, 4, 2, 1, 3, 2, 814, 585, 976),
+                             FORM(f32, 2, 2, 4, 4, 1, 2, 2, 1173, 1045, 1020)};
 #undef FORM
 
 int64_t estimate(const GemmForm &f, int64_t M, int64_t N, int64_t K, int64_t experts) {
@@ -143,8 +143,8 @@ int64_t estimate(const GemmForm &f, int64_t M, int64_t N, int64_t K, int64_t exp
     return groups / round * ns(f.held) + (left ? ns((left + 255) / 256) : 0);
 }
 
-// The kernel that is estimated fastest. Over those shapes its time is 1.012 (f16) and
-// 1.008 (f32) times that of the fastest one, at most 1.28 and 1.35 times; any one
+// The kernel that is estimated fastest. Over those shapes its time is 1.014 (f16) and
+// 1.010 (f32) times that of the fastest one, at most 1.33 and 1.28 times; any one
 // kernel for all is 1.26 times and more. 8192 x 16384 x 8192 f16: 256 x 256 930 us,
 // 256 x 128 1079; 384 x 16384 x 8192: 256 x 128 68 us, 256 x 256 102; 1 x 4096 x
 // 4096: 32 x 16 with four stages 5.9 us, 64 x 64 10, 256 x 256 42; 1 x 16384 x
