@@ -57,6 +57,13 @@ __device__ __forceinline__ void store_codes(const PhxF8Rows &p, int64_t row, uin
 // A wave (ROWS: of four to a workgroup) or a workgroup takes a row, chunks of 16 bytes
 // next to their neighbours', up to C chunks a thread, which stay in registers
 // between the sum and what follows it: every byte is read once and written once.
+// Long runs are bound by memory: 16384 rows of 8192, f16, with the sum, 162-166 us
+// (5.8 TB/s; a copy, which writes as much as it reads, 5.1), the vector instructions
+// busy two thirds of it (the squares in 64 bits, the codes' exact quotients). Fewer
+// rows than the GPU holds at once are one chain of load, sum, divide and store: 1000
+// of 4144, f32, 9.1 us, one of 4096, f16, 3.1. A row per workgroup rather than several
+// turns of a wave: a second reading would come from memory. (Two chunks a thread, not
+// four or one, where there are many rows: the figures are with the rule that chooses.)
 template <typename T, int C, bool ROWS>
 __device__ __forceinline__ void norm_f8(const PhxF8Rows &p) {
     constexpr int N = Chunk<T>::N;
@@ -142,7 +149,10 @@ __device__ __forceinline__ float exp_of(float x) {
     return __builtin_isfinite(y) ? __builtin_fmaf(y * low, 0.693147181f, y) : y;
 }
 
-// A block of 128 of a row to 16 or 32 lanes; blocks of a row next to each other.
+// A block of 128 of a row to 16 or 32 lanes; blocks of a row next to each other. No
+// lane needs more than its own block's, so a launch is as wide as its data. Bound by
+// memory: 4133 rows of 5520, f32, 43 us (4.8 TB/s); 32 of 4096, f16, 3.4 us, one
+// chain of load and store.
 template <typename T>
 __device__ __forceinline__ void glu_f8(const PhxF8Rows &p) {
     constexpr int N = Chunk<T>::N, LANES = Chunk<T>::LANES;

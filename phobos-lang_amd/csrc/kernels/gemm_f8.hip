@@ -14,17 +14,18 @@
 // A operand, so that a lane holds neighbouring columns of one row of C, whose
 // scales' product is one number.
 //
-// Large products are bound by the power that the card may take, and by LDS: a 256 x 256
-// tile's step of 128 k reads 192 KiB of operands from LDS and writes 64 KiB into it, at
-// 128 and about 64 bytes a cycle 2560 cycles, in which the matrix cores have 2048 to do.
-// 8192 x 16384 x 8192, f16: 930 us (2360 TFLOP/s; a large 8-bit product of a library,
-// with one scale for all, 3330) at 1.8 GHz, the matrix cores busy 63 % of the cycles.
-// Few rows are bound by the weights' bytes: 1 x 16384 x 8192 27.6 us (4.9 TB/s), 64 rows
-// 33.9 us (4.0 TB/s). Between them, tiles that fill the GPU but once, it is the
+// Large products: 8192 x 16384 x 8192, f16, 920-935 us (2370 TFLOP/s; a library's 8-bit
+// product, with one scale for all, 3330). The card is at its power limit, 1.8 GHz; of
+// the cycles the matrix cores are busy 63 %, the vector instructions 51 %, LDS 28 %. A
+// 256 x 256 tile alone on the chip, at 2.4 GHz, takes 1.18 us for 128 k and 0.76 without
+// the 64 KiB that it loads into LDS for them; in the full chip 1.8 us.
+// Few rows are bound by the weights' bytes: 64 x 16384 x 8192 29.2 us (4.7 TB/s), 1 row
+// 28.3 us (4.8 TB/s). Between them, where the tiles fill the GPU but once, it is the
 // latency of a step: 1000 x 1000 x 4144, f32, 17.4 us in 17 steps of 256 k.
 // (Also measured, at the same speed or slower: rows staged through registers instead of
 // loaded into LDS directly; waves of 64 x 64 that read less LDS but are half as many;
-// loads spread over the whole step; a raised wave priority; 2 or 8 rows of tiles deep.)
+// loads spread over the whole step; a raised wave priority; 2 or 8 rows of tiles deep;
+// the codes' conversions to f16 spread over the products of the tile before.)
 #include <type_traits>
 
 #include "f8.h"
