@@ -158,6 +158,9 @@ struct Shape {
     static constexpr uint32_t S_LOADS = SCALES / 1024;  // waves that load them
     static constexpr uint32_t STAGE = PART * WK + (STAGED ? SCALES : 0);
     static constexpr uint32_t APART = STAGED ? 16 : 2 * SCALES;
+    // How many tiles of columns before it is used W is read from LDS: four where there are
+    // registers left for them (2048 x 4096 x 4096 36.6 us, one 37.4).
+    static constexpr int D = NT == 8 && MT == 2 ? 4 : 1;
     static constexpr uint32_t W_LOADS = TN / 8 / WAVES, A_LOADS = TM / 8 / WAVES;  // of 8 rows
     static_assert(TN % (8 * WAVES) == 0 && TM % (8 * WAVES) == 0, "whole loads a wave");
     static_assert(WK == 1 || TN * TM * 4 * (WK / 2) <= PART * WK, "the sums fit where the stages were");
@@ -274,7 +277,8 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
     // x 8192: 29.6 us, all from the first on 34; 32 experts with 62 rows each of 4096
     // x 4096: 128 and 151. (With more rows neighbours share what they read: 256 x 256
     // tiles would take 1 to 4 % longer so.)
-    const uint32_t turn = S::TM > 64 || t.rows > kDeep || blocks % 4 ? 0 : t.column * 12 % blocks;
+    constexpr bool TURNS = S::TM <= 64;
+    const uint32_t turn = !TURNS || t.rows > kDeep || blocks % 4 ? 0 : t.column * 12 % blocks;
     auto turned = [&](uint32_t b) {
         return b >= blocks ? b : b + turn >= blocks ? b + turn - blocks : b + turn;
     };
@@ -320,6 +324,18 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
         const int64_t at = source(all * 64 + lane);
         s_off = at < 0 ? kNone : (uint32_t)(at * p.lds * 4);
     }
+    // Of block b the chunks behind K's end are nowhere: they stay so, as nothing but what
+    // lies behind it is loaded after the last block. (Where W's blocks go round each load
+    // looks by itself: 2 to 3 % of a step's time.)
+    auto cut = [&](uint32_t b) {
+        if (TURNS || b * 128 + 128 <= K) return;
+#pragma unroll
+        for (uint32_t i = 0; i < S::W_LOADS; ++i)
+            if (b * 128 + w_k(i) >= K) w_off[i] = kNone;
+#pragma unroll
+        for (uint32_t i = 0; i < S::A_LOADS; ++i)
+            if (b * 128 + a_k(i) >= K) a_off[i] = kNone;
+    };
     // the i-th of this wave's loads of block b: 8 rows of W or of A
     auto load = [&](char *stage, uint32_t b, uint32_t i) {
         const uint32_t k = turned(b) * 128;
@@ -327,12 +343,12 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
         if (i < S::W_LOADS) {
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
                 wr, (lds_ptr)(to + (wave * S::W_LOADS + i) * 1024), 16,
-                k + w_k(i) < K ? w_off[i] : kNone, (int)k, 0, 0);
+                TURNS && k + w_k(i) >= K ? kNone : w_off[i], (int)k, 0, 0);
         } else {
             const uint32_t j = i - S::W_LOADS;
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
                 ar, (lds_ptr)(to + S::TN * 128 + (wave * S::A_LOADS + j) * 1024), 16,
-                k + a_k(j) < K ? a_off[j] : kNone, (int)k, 0, 0);
+                TURNS && k + a_k(j) >= K ? kNone : a_off[j], (int)k, 0, 0);
         }
     };
     // the scales of the tile's rows of the four blocks from b on: where this wave's share
@@ -369,16 +385,17 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
     }
     const uint32_t s_at = (wm * (16 * MT) + r) * 16;
 
+    constexpr int D = S::D;
     using C = Codes<EXACT>;
     C x[MT];                 // this step's rows
-    phx_u4 w_next[2];        // the next tile of columns
+    phx_u4 w_next[D][2];     // the next tiles of columns
     phx_u4 x_next[MT][2];    // the next step's rows
     float f[MT], f_next[MT], f_last[MT];
     phx_f4 sum[MT];
     auto read_w = [&](const char *stage, int n) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-            w_next[h] = *(const phx_u4 *)(stage + wk * S::PART + w_at[n % 2][h] + n / 2 * 4096);
+            w_next[n % D][h] = *(const phx_u4 *)(stage + wk * S::PART + w_at[n % 2][h] + n / 2 * 4096);
     };
     auto read_x = [&](const char *stage, int m) {
 #pragma unroll
@@ -393,13 +410,13 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
 
     // A step: while its tiles are multiplied, the sums of the tile before are scaled, the
     // next tile's weights read from LDS, and the blocks of ST - 1 steps ahead loaded
-    // into the stage of the step before. In its last column of tiles, where nothing
+    // into the stage of the step before. In its last D columns of tiles, where nothing
     // of its stage is left to read, comes the one barrier: a wave's own loads of the
     // next stage have landed before it, every wave's behind it, and behind it the
     // next step's rows are read as this one's are used up. (Behind the last block
     // the loads are of nothing, into what nobody reads.)
     constexpr uint32_t AHEAD = ST - 1, EACH = S::W_LOADS + S::A_LOADS;
-    constexpr uint32_t SLOTS = (NT - 1) * MT, PER_SLOT = (EACH + SLOTS - 1) / SLOTS;
+    constexpr uint32_t SLOTS = (NT - D) * MT, PER_SLOT = (EACH + SLOTS - 1) / SLOTS;
     const bool loads_scales = all < S::S_LOADS;
     phx_u4 scales = {0, 0, 0, 0};
     auto pass = [&]() {
@@ -444,11 +461,12 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
             if (WK > 1) f[m] = b < blocks ? f[m] : 0.0f;
         }
         load_more(b0, fill);
+        cut(b + AHEAD * WK);
         C w;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            w.of(w_next[0], w_next[1]);
-            if (n + 1 < NT) read_w(now, n + 1);
+            w.of(w_next[n % D][0], w_next[n % D][1]);
+            if (n + D < NT) read_w(now, n + D);
             const int done = n ? n - 1 : NT - 1;
 #pragma unroll
             for (int j = 0; j < C::STEPS; ++j)
@@ -470,13 +488,13 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
                             if (i < EACH) load(fill, b + AHEAD * WK, i);
                     }
                     __builtin_amdgcn_sched_barrier(0);
-                    if (n == NT - 1 && j == 0) {
-                        if (m == 0) {
-                            pass();
-                            read_w(then, 0);
+                    if (n >= NT - D && j == 0) {
+                        if (n == NT - D && m == 0) pass();
+                        if (m == 0) read_w(then, n - (NT - D));
+                        if (n == NT - D) {
+                            read_x(then, m);
+                            f_next[m] = read_scale(then, b0 + WK, m);
                         }
-                        read_x(then, m);
-                        f_next[m] = read_scale(then, b0 + WK, m);
                     }
                 }
         }
@@ -484,12 +502,14 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
     if (!S::STAGED && loads_scales) load_scales(sc, 0);
 #pragma unroll
     for (uint32_t u = 0; u < AHEAD; ++u) {
+        cut(u * WK + wk);
         if (S::STAGED && loads_scales) load_scales(st[u] + WK * S::PART, u * WK);
 #pragma unroll
         for (uint32_t i = 0; i < EACH; ++i) load(st[u], u * WK + wk, i);
     }
     pass();
-    read_w(st[0], 0);
+#pragma unroll
+    for (int n = 0; n < D; ++n) read_w(st[0], n);
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
         read_x(st[0], m);
@@ -513,6 +533,7 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
     else
         steps([&](uint32_t b0, char *, char *, char *fill) {
             load_more(b0, fill);
+            cut(b0 + wk + AHEAD * WK);
 #pragma unroll
             for (uint32_t i = 0; i < EACH; ++i) load(fill, b0 + wk + AHEAD * WK, i);
             pass();
@@ -587,7 +608,9 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
 TILE(false, f16, 1, 1, 2, 1, 4, 4)
 BOTH(1, 1, 2, 1, 4, 2)
 TILE(false, f16, 2, 1, 2, 1, 4, 3)
-BOTH(2, 2, 2, 2, 2, 4)
+BOTH(2, 1, 2, 2, 2, 3)
+TILE(false, f16, 2, 2, 2, 2, 2, 4)
+TILE(true, f32, 1, 2, 4, 2, 4, 2)
 BOTH(2, 2, 2, 2, 1, 4)
 BOTH(2, 2, 4, 2, 1, 3)
 TILE(true, f32, 2, 2, 4, 4, 1, 2)

@@ -116,19 +116,21 @@ struct GemmForm {
 #define FORM(t, wn, wm, nt, mt, wk, st, held, step, shared, rest)                 \
     {16 * wn * nt, 16 * wm * mt, wk, 64 * wn * wm * wk, held, step, shared, rest, \
      "gemm_f8_" #t "_" #wn "x" #wm "_" #nt "x" #mt "_k" #wk "_s" #st}
-const GemmForm kGemmF16[] = {FORM(f16, 1, 1, 2, 1, 4, 4, 1, 189, 0, 2313),
-                             FORM(f16, 1, 1, 2, 1, 4, 2, 3, 1, 288, 1528),
-                             FORM(f16, 2, 1, 2, 1, 4, 3, 1, 486, 0, 1600),
-                             FORM(f16, 2, 2, 2, 2, 2, 4, 1, 371, 0, 1911),
-                             FORM(f16, 2, 2, 2, 2, 1, 4, 2, 220, 188, 1546),
-                             FORM(f16, 2, 2, 4, 2, 1, 3, 2, 415, 14, 1413),
-                             FORM(f16, 2, 4, 8, 2, 1, 3, 1, 527, 0, 1406),
-                             FORM(f16, 2, 4, 8, 4, 1, 2, 1, 910, 0, 2038)};
-const GemmForm kGemmF32[] = {FORM(f32, 1, 1, 2, 1, 4, 2, 3, 689, 459, 1322),
-                             FORM(f32, 2, 2, 2, 2, 2, 4, 1, 759, 0, 1343),
-                             FORM(f32, 2, 2, 2, 2, 1, 4, 2, 411, 356, 1109),
-                             FORM(f32, 2, 2, 4, 2, 1, 3, 2, 814, 585, 976),
-                             FORM(f32, 2, 2, 4, 4, 1, 2, 2, 1173, 1045, 1020)};
+const GemmForm kGemmF16[] = {FORM(f16, 1, 1, 2, 1, 4, 4, 1, 191, 4, 2331),
+                             FORM(f16, 1, 1, 2, 1, 4, 2, 3, 0, 298, 1650),
+                             FORM(f16, 2, 1, 2, 1, 4, 3, 1, 498, 0, 1519),
+                             FORM(f16, 2, 1, 2, 2, 2, 3, 2, 0, 277, 1629),
+                             FORM(f16, 2, 2, 2, 2, 2, 4, 1, 372, 73, 1515),
+                             FORM(f16, 2, 2, 2, 2, 1, 4, 2, 190, 146, 1495),
+                             FORM(f16, 2, 2, 4, 2, 1, 3, 2, 380, 255, 1306),
+                             FORM(f16, 2, 4, 8, 2, 1, 3, 1, 552, 3, 1567),
+                             FORM(f16, 2, 4, 8, 4, 1, 2, 1, 939, 2, 2173)};
+const GemmForm kGemmF32[] = {FORM(f32, 1, 1, 2, 1, 4, 2, 3, 930, 402, 1227),
+                             FORM(f32, 2, 1, 2, 2, 2, 3, 2, 649, 441, 1079),
+                             FORM(f32, 1, 2, 4, 2, 4, 2, 1, 1358, 0, 1512),
+                             FORM(f32, 2, 2, 2, 2, 1, 4, 2, 455, 332, 1018),
+                             FORM(f32, 2, 2, 4, 2, 1, 3, 2, 780, 478, 889),
+                             FORM(f32, 2, 2, 4, 4, 1, 2, 2, 1209, 774, 751)};
 #undef FORM
 
 int64_t estimate(const GemmForm &f, int64_t M, int64_t N, int64_t K, int64_t experts) {
@@ -144,8 +146,8 @@ int64_t estimate(const GemmForm &f, int64_t M, int64_t N, int64_t K, int64_t exp
 }
 
 // The kernel that is estimated fastest. Over those shapes its time is 1.014 (f16) and
-// 1.010 (f32) times that of the fastest one, at most 1.33 and 1.28 times; any one
-// kernel for all is 1.26 times and more. 8192 x 16384 x 8192 f16: 256 x 256 930 us,
+// 1.007 (f32) times that of the fastest one, at most 1.34 and 1.27 times; any one
+// kernel for all is 1.24 times and more. 8192 x 16384 x 8192 f16: 256 x 256 930 us,
 // 256 x 128 1079; 384 x 16384 x 8192: 256 x 128 68 us, 256 x 256 102; 1 x 4096 x
 // 4096: 32 x 16 with four stages 5.9 us, 64 x 64 10, 256 x 256 42; 1 x 16384 x
 // 8192: 32 x 16 with two stages, of which a CU holds three, 27.6 us, with four 36.
