@@ -73,7 +73,13 @@ __device__ __forceinline__ void norm_f8(const PhxF8Rows &p) {
     if (ROWS && row >= p.M) return;
     const uint32_t at = (ROWS ? threadIdx.x % 64 : threadIdx.x) * N, K = (uint32_t)p.K;
     Chunk<T> h[C];
-    phx_u4 gain[C];  // (asked for with the rows: it is in use as soon as their sum is there)
+    // (asked for with the rows: it is in use as soon as their sum is there; of eight chunks a
+    // thread, for all of which there are no registers, one ahead)
+    constexpr int EARLY = C == 8 ? 1 : C;
+    phx_u4 gain[C];
+    auto load_gain = [&](int c, uint32_t k) {
+        gain[c] = *(const PHX_GLOBAL phx_u4 *)((const PHX_GLOBAL T *)p.gain + k);
+    };
     double sum = 0;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
@@ -81,7 +87,7 @@ __device__ __forceinline__ void norm_f8(const PhxF8Rows &p) {
 #pragma unroll
         for (int i = 0; i < N; ++i) h[c].v[i] = 0;
         if (k >= K) continue;
-        gain[c] = *(const PHX_GLOBAL phx_u4 *)((const PHX_GLOBAL T *)p.gain + k);
+        if (c < EARLY) load_gain(c, k);
         h[c].load((const PHX_GLOBAL T *)p.x + row * p.ldx + k);
         if (p.r) {
             Chunk<T> r;
@@ -105,11 +111,18 @@ __device__ __forceinline__ void norm_f8(const PhxF8Rows &p) {
     }
     const double factor = rsqrt(sum * p.inverse + (double)p.eps);
     const float f = (float)factor;
+    // (rows of the smallest or largest f32, where f has few bits or none)
+    const bool plain = __builtin_amdgcn_readfirstlane(f >= 0x1p-126f && f <= 0x1.fp127f);
 #pragma unroll
     for (int c = 0; c < C; ++c) {
         const uint32_t k = at + c * (R * N);
         const bool live = k < K;
         uint32_t a = 0;
+        if (EARLY < C) {
+            if (c + 1 < C && k + R * N < K) load_gain(c + 1, k + R * N);
+            // (else the chunks are worked on together, in more registers than there are)
+            __builtin_amdgcn_sched_barrier(0);
+        }
         if (live) {
             Chunk<T> g;
             g.of(gain[c]);
@@ -131,8 +144,13 @@ __device__ __forceinline__ void norm_f8(const PhxF8Rows &p) {
             }
         }
         if (p.y && live) {
+            if (plain) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) h[c].v[i] *= f;
+                for (int i = 0; i < N; ++i) h[c].v[i] *= f;
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; ++i) h[c].v[i] = (float)((double)h[c].v[i] * factor);
+            }
             h[c].store((PHX_GLOBAL T *)p.y + row * p.ldy + k);
         }
     }

@@ -190,6 +190,14 @@ def test_norm_tiny_and_large_f32(px_gpu, stream, exponent):
     _check_norm(got, x, None, gain, 0.0, want_y=abs(exponent) < 105)
 
 
+@pytest.mark.parametrize("exponent", [-146, -135, -128, -126, 110, 124])
+def test_norm_y_where_no_f32_holds_the_factor(px_gpu, stream, exponent):
+    rng = np.random.default_rng(300 + exponent)
+    x = np.ldexp(rng.standard_normal((3, 640)), exponent).astype(np.float32)
+    gain = np.ones(640, np.float32)
+    _check_norm(_norm(px_gpu, stream, 32, x, None, gain, 0.0), x, None, gain, 0.0)
+
+
 @pytest.mark.parametrize("bits", [16, 32])
 def test_norm_zeros_infinities_and_nan(px_gpu, stream, bits):
     px = px_gpu
