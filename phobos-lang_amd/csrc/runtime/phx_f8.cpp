@@ -195,8 +195,10 @@ int product(phx_stream s, const phx_f8_rows *a, const phx_f8_weights *w, bool gr
     if (M && grouped && (!starts || ((starts | list) & 3)))
         return set_error(PHX_E_INVALID, "%s: starts and list are i32 arrays", who);
     const GemmForm &f = gemm_form(t, M, w->n, r.k, w->experts);
-    const int64_t tiles = ((M + f.rows - 1) / f.rows + (grouped ? w->experts : 0)) *
-                          ((w->n + f.columns - 1) / f.columns);
+    // (groups of rows: each that has any has a first tile, and only whole tiles behind it add
+    // one; workgroups behind what there is read the starts and end)
+    const int64_t live = std::min(grouped ? w->experts : 1, M);
+    const int64_t tiles = (live + (M - live) / f.rows) * ((w->n + f.columns - 1) / f.columns);
     if (tiles > kMostThreads / f.threads)
         return set_error(PHX_E_INVALID, "%s: %lld x %lld is too large", who, (long long)M,
                          (long long)w->n);

@@ -290,6 +290,18 @@ def test_grouped_whole_numbers_are_exact(px_gpu, stream, bits, M, E, N, K, idle,
     assert np.array_equal(got.astype(np.float64), want)
 
 
+@pytest.mark.parametrize("each,E", [(1, 9), (17, 9), (33, 5), (65, 40), (129, 5), (257, 5), (257, 30)])
+@pytest.mark.parametrize("bits", [16, 32])
+def test_groups_of_one_row_more_than_whole_tiles(px_gpu, stream, bits, each, E):
+    # as many tiles as M rows of E groups can have
+    rng = np.random.default_rng(each)
+    M = each * E
+    a, w = _whole(px_gpu, rng, M, 270, 144, E, bits=bits)
+    starts = np.arange(E + 1) * each
+    got = _run(px_gpu, stream, bits, a, w, M, starts)
+    assert np.array_equal(got.astype(np.float64), _want(a, w, starts, None, M))
+
+
 @pytest.mark.parametrize("M,E,N,K,idle", [(50, 9, 300, 1040, 3), (1500, 8, 520, 400, 1)])
 @pytest.mark.parametrize("bits", [16, 32])
 def test_grouped_normal_inputs_onto_c(px_gpu, stream, bits, M, E, N, K, idle):
