@@ -34,11 +34,12 @@ struct Chunk {  // 16 bytes of a row
     }
 };
 
-// The largest magnitude of a block, in all its lanes.
+// The largest magnitude of a block, in all its lanes (of a row's `lanes`, if they are fewer).
 template <int LANES>
-__device__ __forceinline__ uint32_t block_largest(uint32_t a) {
+__device__ __forceinline__ uint32_t block_largest(uint32_t a, uint32_t lanes = LANES) {
 #pragma unroll
-    for (int s = 1; s < LANES; s <<= 1) a = max(a, (uint32_t)__shfl_xor((int)a, s));
+    for (uint32_t s = 1; s < LANES; s <<= 1)
+        if (s < lanes) a = max(a, (uint32_t)__shfl_xor((int)a, (int)s));
     return a;
 }
 
@@ -54,8 +55,16 @@ __device__ __forceinline__ void store_codes(const PhxF8Rows &p, int64_t row, uin
         *(PHX_GLOBAL uint32_t *)to = out[0];
 }
 
-// A wave (ROWS: of four to a workgroup) or a workgroup takes a row, chunks of 16 bytes
-// next to their neighbours', up to C chunks a thread, which stay in registers
+// The threads that a row is given: a workgroup, or (ROWS) a wave or the 2, 4 .. 32 lanes that
+// its chunks take.
+template <typename T, int C, bool ROWS>
+__device__ __forceinline__ uint32_t threads_of_row(uint32_t K) {
+    if (!ROWS) return blockDim.x;
+    const uint32_t chunks = K / Chunk<T>::N;
+    return C > 1 || chunks > 32 ? 64 : 1u << (32 - __builtin_clz(chunks - 1));
+}
+
+// Threads next to each other take a row, chunks of 16 bytes next to their neighbours', up to C chunks a thread, which stay in registers
 // between the sum and what follows it: every byte is read once and written once.
 // Long runs are bound by memory: 16384 rows of 8192, f16, with the sum, 162-166 us
 // (5.8 TB/s; a copy, which writes as much as it reads, 5.1), the vector instructions
@@ -68,10 +77,10 @@ template <typename T, int C, bool ROWS>
 __device__ __forceinline__ void norm_f8(const PhxF8Rows &p) {
     constexpr int N = Chunk<T>::N;
     __shared__ double sums[16];
-    const uint32_t R = ROWS ? 64 : blockDim.x, waves = R / 64;  // threads of a row
-    const int64_t row = ROWS ? (int64_t)blockIdx.x * 4 + threadIdx.x / 64 : (int64_t)blockIdx.x;
-    if (ROWS && row >= p.M) return;
-    const uint32_t at = (ROWS ? threadIdx.x % 64 : threadIdx.x) * N, K = (uint32_t)p.K;
+    const uint32_t K = (uint32_t)p.K, R = threads_of_row<T, C, ROWS>(K), waves = R / 64;
+    const int64_t row = ROWS ? (int64_t)blockIdx.x * (256 / R) + threadIdx.x / R : (int64_t)blockIdx.x;
+    const uint32_t at = (ROWS ? threadIdx.x % R : threadIdx.x) * N;
+    if (ROWS && row >= p.M) return;  // (lanes of another row need none of it)
     Chunk<T> h[C];
     // (asked for with the rows: it is in use as soon as their sum is there; of eight chunks a
     // thread, for all of which there are no registers, one ahead)
@@ -102,7 +111,8 @@ __device__ __forceinline__ void norm_f8(const PhxF8Rows &p) {
         for (int i = 0; i < N; ++i) sum = fma((double)h[c].v[i], (double)h[c].v[i], sum);
     }
 #pragma unroll
-    for (int s = 1; s < 64; s <<= 1) sum += __shfl_xor(sum, s);
+    for (uint32_t s = 1; s < 64; s <<= 1)
+        if (!ROWS || s < R) sum += __shfl_xor(sum, (int)s);
     if (!ROWS && waves > 1) {
         if (threadIdx.x % 64 == 0) sums[threadIdx.x / 64] = sum;
         __syncthreads();
@@ -112,7 +122,8 @@ __device__ __forceinline__ void norm_f8(const PhxF8Rows &p) {
     const double factor = rsqrt(sum * p.inverse + (double)p.eps);
     const float f = (float)factor;
     // (rows of the smallest or largest f32, where f has few bits or none)
-    const bool plain = __builtin_amdgcn_readfirstlane(f >= 0x1p-126f && f <= 0x1.fp127f);
+    const bool plain = f >= 0x1p-126f && f <= 0x1.fp127f;
+    const bool all_plain = ROWS ? __all(plain) : __builtin_amdgcn_readfirstlane(plain);
 #pragma unroll
     for (int c = 0; c < C; ++c) {
         const uint32_t k = at + c * (R * N);
@@ -133,10 +144,10 @@ __device__ __forceinline__ void norm_f8(const PhxF8Rows &p) {
             }
         }
         if (p.q) {
-            a = block_largest<Chunk<T>::LANES>(a);
+            a = block_largest<Chunk<T>::LANES>(a, ROWS ? R : 64);
             if (live) {
                 store_codes<T>(p, row, k, h[c].v, a);
-                if (threadIdx.x % Chunk<T>::LANES == 0)
+                if (at % PHX_F8_BLOCK == 0)
                     ((PHX_GLOBAL float *)p.scales)[row * p.lds + k / PHX_F8_BLOCK] =
                         a < 0x7f800000u
                             ? (float)((double)__builtin_bit_cast(float, a) * (factor * (1 / 448.0)))
@@ -144,12 +155,13 @@ __device__ __forceinline__ void norm_f8(const PhxF8Rows &p) {
             }
         }
         if (p.y && live) {
-            if (plain) {
+            if (all_plain) {
 #pragma unroll
                 for (int i = 0; i < N; ++i) h[c].v[i] *= f;
             } else {
 #pragma unroll
-                for (int i = 0; i < N; ++i) h[c].v[i] = (float)((double)h[c].v[i] * factor);
+                for (int i = 0; i < N; ++i)
+                    h[c].v[i] = plain ? h[c].v[i] * f : (float)((double)h[c].v[i] * factor);
             }
             h[c].store((PHX_GLOBAL T *)p.y + row * p.ldy + k);
         }

@@ -74,10 +74,11 @@ int check_rows(phx_dtype t, uint64_t ptr, int64_t width, int64_t *ld, const char
 }
 
 // ------------------------------------------------------------------ the norm
-// How a norm runs: up to 128 chunks of 16 bytes a row by a wave, four rows a workgroup
-// (16384 rows of 1024, f16: 26.6 us, in workgroups of 128 threads a row 32.1); more
-// by a workgroup of as many threads as one, two, four or eight chunks each take:
-// two from 512 on (8192 rows of 8192, f16: 87 us, four 95; 4096 of 4096, f32:
+// How a norm runs: up to 64 chunks of 16 bytes a row by as many lanes, a power of two
+// (781250 rows of 128, f16, with the sum: 124 us, by a wave each 335); up to 128 by a
+// wave (16384 rows of 1024, f16: 26.6 us, by 128 threads of a workgroup of their own
+// 32.1); more by a workgroup of as many threads as one, two, four or eight chunks each
+// take: two from 512 on (8192 rows of 8192, f16: 87 us, four 95; 4096 of 4096, f32:
 // 42.8 us, four 47.3).
 struct NormForm {
     int64_t rows;  // of a workgroup
@@ -93,7 +94,9 @@ NormForm norm_form(phx_dtype t, int64_t K) {
          "norm_f8_f32_c4", "norm_f8_f32_c8"}};
     const char *const *name = names[t == PHX_F16 ? 0 : 1];
     const int64_t chunks = K * size_of(t) / 16;
-    if (chunks <= 128) return {4, 256, name[chunks > 64]};
+    int64_t lanes = 2;
+    while (lanes < chunks && lanes < 64) lanes *= 2;
+    if (chunks <= 128) return {256 / lanes, 256, name[chunks > 64]};
     const int64_t of_thread = chunks <= 512 ? 1 : chunks <= 2048 ? 2 : chunks <= 4096 ? 4 : 8;
     const int64_t threads = (chunks + of_thread - 1) / of_thread;
     return {1, (uint32_t)((threads + 63) / 64 * 64),

@@ -125,6 +125,33 @@ def test_norm(px_gpu, stream, bits, K, M):
         _check_norm(got, x, res, gain, 1e-5)
 
 
+@pytest.mark.parametrize("K", [16, 32, 48, 64, 80, 112, 128, 144, 256, 272])
+@pytest.mark.parametrize("bits", [16, 32])
+@pytest.mark.parametrize("M", [3, 127, 300])
+def test_norm_short_rows(px_gpu, stream, bits, K, M):
+    # several rows a wave, the last ones' lanes idle
+    rng = np.random.default_rng(K * M + bits)
+    _, t = _t(px_gpu, bits)
+    x = (rng.standard_normal((M, K)) * 10.0 ** rng.uniform(-2, 2, (M, 1))).astype(t)
+    r = rng.standard_normal((M, K)).astype(t)
+    gain = (1 + 0.2 * rng.standard_normal(K)).astype(t)
+    _check_norm(_norm(px_gpu, stream, bits, x, r, gain, 1e-5, pad=1), x, r, gain, 1e-5)
+
+
+def test_norm_short_rows_of_every_size(px_gpu, stream):
+    # neighbours in a wave, of which some have a factor that no f32 holds
+    rng = np.random.default_rng(31)
+    exponents = np.array([0, -146, 3, 124, -130, 0, 20])[np.arange(60) % 7]
+    x = np.ldexp(rng.standard_normal((60, 64)), exponents[:, None]).astype(np.float32)
+    gain = np.ones(64, np.float32)
+    got = _norm(px_gpu, stream, 32, x, None, gain, 0.0)
+    _check_norm(got, x, None, gain, 0.0)
+    for m in (0, 5, 6):  # a row's bits are its own
+        alone = _norm(px_gpu, stream, 32, x[m:m + 1], None, gain, 0.0)
+        for a, b in zip(alone, got):
+            assert np.array_equal(a[0], b[m])
+
+
 @pytest.mark.parametrize("bits", [16, 32])
 def test_norm_strides_and_outputs(px_gpu, stream, bits):
     rng = np.random.default_rng(2)
