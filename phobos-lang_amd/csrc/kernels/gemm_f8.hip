@@ -98,9 +98,9 @@ __device__ __forceinline__ Tile tile_of(const PhxF8Gemm &p, uint32_t columns) {
         };
         auto range = [&](uint32_t e0, uint32_t floor, uint32_t before) {
             Range x;
-            x.begin = upto(max(at(e0 + lane), floor),
-                           [](uint32_t a, uint32_t b) { return max(a, b); });
-            x.end = e0 + lane < E ? max(x.begin, at(e0 + lane + 1)) : x.begin;
+            const uint32_t first = at(e0 + lane), last = at(e0 + lane + 1);
+            x.begin = upto(max(first, floor), [](uint32_t a, uint32_t b) { return max(a, b); });
+            x.end = e0 + lane < E ? max(x.begin, last) : x.begin;
             x.tiles = (x.end - x.begin + TM - 1) / TM;
             x.upto = before + upto(x.tiles, [](uint32_t a, uint32_t b) { return a + b; });
             return x;
@@ -294,12 +294,21 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
         (void *)(p.a + base * p.lda), 0, (int)((rows - 1) * p.lda + p.K), 0x00020000);
     const __amdgpu_buffer_rsrc_t sr = __builtin_amdgcn_make_buffer_rsrc(
         (void *)(p.sa + base * p.lds * 4), 0, (int)(rows * p.lds * 4), 0x00020000);
-    // a row of the tile in A, or none
-    auto source = [&](uint32_t row) -> int64_t {
-        if (row >= left_m) return -1;
-        if (!p.list) return row;
-        const int64_t i = ((const PHX_GLOBAL int32_t *)p.list)[t.m0 + row];
-        return i >= 0 && i < p.rows ? i : -1;
+    // the rows of this wave's loads, and the entries of the list that say where they are
+    auto a_row = [&](uint32_t i) {
+        return i < S::A_LOADS ? (wave * S::A_LOADS + i) * 8 + lane / 8 : all * 64 + lane;
+    };
+    int32_t entry[S::A_LOADS + 1];
+    if (p.list) {
+#pragma unroll
+        for (uint32_t i = 0; i <= S::A_LOADS; ++i)
+            entry[i] = ((const PHX_GLOBAL int32_t *)p.list)[t.m0 + min((int64_t)a_row(i), left_m - 1)];
+    }
+    // the i-th's row in A, or none
+    auto source = [&](uint32_t i) -> int64_t {
+        if (a_row(i) >= left_m) return -1;
+        if (!p.list) return a_row(i);
+        return entry[i] >= 0 && entry[i] < p.rows ? entry[i] : -1;
     };
     // the k of a lane's chunk in a load's row
     auto w_k = [&](uint32_t i) {
@@ -314,16 +323,17 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
         const uint32_t row = (wave * S::W_LOADS + i) * 8 + lane / 8;
         w_off[i] = row * K + w_k(i);  // (rows past N's end lie past the resource's)
     }
+    auto find_rows = [&]() {
 #pragma unroll
-    for (uint32_t i = 0; i < S::A_LOADS; ++i) {
-        const uint32_t row = (wave * S::A_LOADS + i) * 8 + lane / 8;
-        const int64_t at = source(row);
-        a_off[i] = at < 0 ? kNone : (uint32_t)(at * p.lda) + a_k(i);
-    }
-    if (all < S::S_LOADS) {
-        const int64_t at = source(all * 64 + lane);
-        s_off = at < 0 ? kNone : (uint32_t)(at * p.lds * 4);
-    }
+        for (uint32_t i = 0; i < S::A_LOADS; ++i) {
+            const int64_t at = source(i);
+            a_off[i] = at < 0 ? kNone : (uint32_t)(at * p.lda) + a_k(i);
+        }
+        if (all < S::S_LOADS) {
+            const int64_t at = source(S::A_LOADS);
+            s_off = at < 0 ? kNone : (uint32_t)(at * p.lds * 4);
+        }
+    };
     // Of block b the chunks behind K's end are nowhere: they stay so, as nothing but what
     // lies behind it is loaded after the last block. (Where W's blocks go round each load
     // looks by itself: 2 to 3 % of a step's time.)
@@ -499,13 +509,18 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
                 }
         }
     };
+    // (the first weights before A's rows are looked up in the list)
+    cut(wk);
+#pragma unroll
+    for (uint32_t i = 0; i < S::W_LOADS; ++i) load(st[0], wk, i);
+    find_rows();
     if (!S::STAGED && loads_scales) load_scales(sc, 0);
 #pragma unroll
     for (uint32_t u = 0; u < AHEAD; ++u) {
         cut(u * WK + wk);
         if (S::STAGED && loads_scales) load_scales(st[u] + WK * S::PART, u * WK);
 #pragma unroll
-        for (uint32_t i = 0; i < EACH; ++i) load(st[u], u * WK + wk, i);
+        for (uint32_t i = u ? 0 : S::W_LOADS; i < EACH; ++i) load(st[u], u * WK + wk, i);
     }
     pass();
 #pragma unroll
