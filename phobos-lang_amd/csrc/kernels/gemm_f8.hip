@@ -14,18 +14,23 @@
 // A operand, so that a lane holds neighbouring columns of one row of C, whose
 // scales' product is one number.
 //
-// Large products: 8192 x 16384 x 8192, f16, 920-935 us (2370 TFLOP/s; a library's 8-bit
-// product, with one scale for all, 3330). The card is at its power limit, 1.8 GHz; of
-// the cycles the matrix cores are busy 63 %, the vector instructions 51 %, LDS 28 %. A
-// 256 x 256 tile alone on the chip, at 2.4 GHz, takes 1.18 us for 128 k and 0.76 without
-// the 64 KiB that it loads into LDS for them; in the full chip 1.8 us.
-// Few rows are bound by the weights' bytes: 64 x 16384 x 8192 29.2 us (4.7 TB/s), 1 row
-// 28.3 us (4.8 TB/s). Between them, where the tiles fill the GPU but once, it is the
-// latency of a step: 1000 x 1000 x 4144, f32, 17.4 us in 17 steps of 256 k.
+// Large products: 8192 x 16384 x 8192, f16, 902-912 us (2430 TFLOP/s; a library's 8-bit
+// product, with one scale for all, 660 to 800 with its inputs). The card is at its power
+// limit, 1.8 GHz; of the cycles the matrix cores are busy 65 %, the vector instructions
+// 48 %, LDS 29 %. A 256 x 256 tile alone on the chip, at 2.4 GHz, takes 1.18 us for 128 k
+// and 0.76 without the 64 KiB that it loads into LDS for them; in the full chip 1.75 us.
+// What is before and behind a tile's steps, 3 to 5 us, nothing hides where a CU holds one
+// workgroup: it is a fifth of 16384 rows over 61 experts of 4096 x 2048, 210 us.
+// Few rows are bound by the weights' bytes: 64 x 16384 x 8192 29.1 us (4.8 TB/s), 1 row
+// 25.5 us (5.3 TB/s). Between them, where the tiles fill the GPU but once, it is the
+// length of a step: 1000 x 1000 x 4144, f32, 16.9 us in 9 steps of 512 k.
 // (Also measured, at the same speed or slower: rows staged through registers instead of
-// loaded into LDS directly; waves of 64 x 64 that read less LDS but are half as many;
-// loads spread over the whole step; a raised wave priority; 2 or 8 rows of tiles deep;
-// the codes' conversions to f16 spread over the products of the tile before.)
+// loaded into LDS directly; waves of 64 x 64 that read less LDS, as many or half as many,
+// and one wave a SIMD of 128 x 64; loads spread over the whole step; a raised wave
+// priority; 2 or 8 rows of tiles deep; the codes' conversions to f16 spread over the
+// products of the tile before; W read ahead into L2 by a wave of its own; 256 columns of
+// 16 for one row; results that change lanes, so that stores take whole rows: 2 % more for
+// whole 16 bytes.)
 #include <type_traits>
 
 #include "f8.h"

@@ -150,7 +150,7 @@ int64_t estimate(const GemmForm &f, int64_t M, int64_t N, int64_t K, int64_t exp
 
 // The kernel that is estimated fastest. Over those shapes its time is 1.014 (f16) and
 // 1.007 (f32) times that of the fastest one, at most 1.34 and 1.27 times; any one
-// kernel for all is 1.24 times and more. 8192 x 16384 x 8192 f16: 256 x 256 930 us,
+// kernel for all is 1.24 times and more. 8192 x 16384 x 8192 f16: 256 x 256 905 us,
 // 256 x 128 1079; 384 x 16384 x 8192: 256 x 128 68 us, 256 x 256 102; 1 x 4096 x
 // 4096: 32 x 16 with four stages 5.9 us, 64 x 64 10, 256 x 256 42; 1 x 16384 x
 // 8192: 32 x 16 with two stages, of which a CU holds three, 27.6 us, with four 36.
