@@ -64,13 +64,14 @@ __device__ __forceinline__ uint32_t threads_of_row(uint32_t K) {
     return C > 1 || chunks > 32 ? 64 : 1u << (32 - __builtin_clz(chunks - 1));
 }
 
-// Threads next to each other take a row, chunks of 16 bytes next to their neighbours', up to C chunks a thread, which stay in registers
-// between the sum and what follows it: every byte is read once and written once.
+// Threads next to each other take a row, chunks of 16 bytes next to their neighbours', up
+// to C chunks a thread, which stay in registers between the sum and what follows it: every
+// byte is read once and written once.
 // Long runs are bound by memory: 16384 rows of 8192, f16, with the sum, 162-166 us
 // (5.8 TB/s; a copy, which writes as much as it reads, 5.1), the vector instructions
 // busy two thirds of it (the squares in 64 bits, the codes' exact quotients). Fewer
 // rows than the GPU holds at once are one chain of load, sum, divide and store: 1000
-// of 4144, f32, 9.1 us, one of 4096, f16, 3.1. A row per workgroup rather than several
+// of 4144, f32, 9.3 us, one of 4096, f16, 3.0. A row per workgroup rather than several
 // turns of a wave: a second reading would come from memory. (Two chunks a thread, not
 // four or one, where there are many rows: the figures are with the rule that chooses.)
 template <typename T, int C, bool ROWS>

@@ -136,7 +136,8 @@ const GemmForm kGemmF32[] = {FORM(f32, 1, 1, 2, 1, 4, 2, 3, 930, 402, 1227),
                              FORM(f32, 2, 2, 4, 4, 1, 2, 2, 1209, 774, 751)};
 #undef FORM
 
-int64_t estimate(const GemmForm &f, int64_t M, int64_t N, int64_t K, int64_t experts) {
+// (in 64-bit floating point: sizes that are refused later would overflow)
+double estimate(const GemmForm &f, int64_t M, int64_t N, int64_t K, int64_t experts) {
     // (which experts have how many rows is not known here: all have some)
     const int64_t live = std::min(experts, M);
     const int64_t tiles = experts == 1 ? (M + f.rows - 1) / f.rows
@@ -145,7 +146,7 @@ int64_t estimate(const GemmForm &f, int64_t M, int64_t N, int64_t K, int64_t exp
     const int64_t steps = (blocks_of(K) + f.blocks - 1) / f.blocks, round = 256 * f.held;
     auto ns = [&](int64_t each) { return steps * std::max(f.step, each * f.shared) + f.rest; };
     const int64_t left = groups % round;
-    return groups / round * ns(f.held) + (left ? ns((left + 255) / 256) : 0);
+    return (double)(groups / round) * ns(f.held) + (left ? ns((left + 255) / 256) : 0);
 }
 
 // The kernel that is estimated fastest. Over those shapes its time is 1.014 (f16) and
@@ -157,9 +158,13 @@ int64_t estimate(const GemmForm &f, int64_t M, int64_t N, int64_t K, int64_t exp
 const GemmForm &gemm_form(phx_dtype t, int64_t M, int64_t N, int64_t K, int64_t experts) {
     const GemmForm *first = t == PHX_F16 ? std::begin(kGemmF16) : std::begin(kGemmF32);
     const GemmForm *last = t == PHX_F16 ? std::end(kGemmF16) : std::end(kGemmF32);
-    return *std::min_element(first, last, [&](const GemmForm &a, const GemmForm &b) {
-        return estimate(a, M, N, K, experts) < estimate(b, M, N, K, experts);
-    });
+    const GemmForm *best = first;
+    double least = INFINITY;
+    for (; first != last; ++first) {
+        const double ns = estimate(*first, M, N, K, experts);
+        if (ns < least) best = first, least = ns;
+    }
+    return *best;
 }
 
 int product(phx_stream s, const phx_f8_rows *a, const phx_f8_weights *w, bool grouped,
