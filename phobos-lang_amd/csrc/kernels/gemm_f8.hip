@@ -154,12 +154,13 @@ struct Shape {
     static constexpr uint32_t WAVES = WN * WM, TN = 16 * WN * NT, TM = 16 * WM * MT;
     static constexpr uint32_t PART = (TN + TM) * 128;
     // The rows' scales come four blocks at a time, a row's 16 bytes next to each other:
-    // with four sets, which take four blocks a step, in its stage; with fewer in places
-    // of their own, through registers (loaded into LDS directly, each read of them
-    // would wait for the latest such load).
-    static_assert(WK == 1 || WK == 2 || WK == 4, "a step within four blocks");
-    static constexpr bool STAGED = WK == 4;
-    static constexpr uint32_t SCALES = (TM < 64 ? 64 : TM) * 16;
+    // with four or eight sets, which take four or eight blocks a step, in its stage; with
+    // fewer in places of their own, through registers (loaded into LDS directly, each read
+    // of them would wait for the latest such load).
+    static_assert(WK == 1 || WK == 2 || WK == 4 || WK == 8, "steps and fours of blocks");
+    static constexpr bool STAGED = WK >= 4;
+    static constexpr uint32_t ROWS = TM < 64 ? 64 : TM;       // that have a place
+    static constexpr uint32_t SCALES = ROWS * (WK == 8 ? 32 : 16);
     static constexpr uint32_t S_LOADS = SCALES / 1024;  // waves that load them
     static constexpr uint32_t STAGE = PART * WK + (STAGED ? SCALES : 0);
     static constexpr uint32_t APART = STAGED ? 16 : 2 * SCALES;
@@ -301,7 +302,7 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
         (void *)(p.sa + base * p.lds * 4), 0, (int)(rows * p.lds * 4), 0x00020000);
     // the rows of this wave's loads, and the entries of the list that say where they are
     auto a_row = [&](uint32_t i) {
-        return i < S::A_LOADS ? (wave * S::A_LOADS + i) * 8 + lane / 8 : all * 64 + lane;
+        return i < S::A_LOADS ? (wave * S::A_LOADS + i) * 8 + lane / 8 : all * 64 % S::ROWS + lane;
     };
     int32_t entry[S::A_LOADS + 1];
     if (p.list) {
@@ -370,7 +371,7 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
     // is (behind the rows' end nowhere), and into LDS
     auto scales_at = [&](uint32_t b) { return b < (uint32_t)p.lds ? s_off : kNone; };
     auto load_scales = [&](char *to, uint32_t b) {
-        b = turned(b);
+        b = turned(b + all * 64 / S::ROWS * 4);
         __builtin_amdgcn_raw_ptr_buffer_load_lds(sr, (lds_ptr)(to + all * 1024), 16, scales_at(b),
                                                  (int)(b * 4), 0, 0);
     };
@@ -418,7 +419,7 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
             x_next[m][h] = *(const phx_u4 *)(stage + wk * S::PART + a_at[h] + m * 2048);
     };
     auto read_scale = [&](const char *stage, uint32_t b0, int m) {
-        const char *from = S::STAGED ? stage + WK * S::PART
+        const char *from = S::STAGED ? stage + WK * S::PART + wk / 4 * (S::ROWS * 16)
                                      : sc + b0 / 4 % 2 * S::SCALES;
         return *(const float *)(from + s_at + m * 256 + (b0 + wk) % 4 * 4);
     };
@@ -627,6 +628,7 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
     TILE(true, f32, WN, WM, NT, MT, WK, ST)
 TILE(false, f16, 1, 1, 2, 1, 4, 4)
 BOTH(1, 1, 2, 1, 4, 2)
+TILE(true, f32, 1, 1, 2, 1, 8, 3)
 TILE(false, f16, 2, 1, 2, 1, 4, 3)
 BOTH(2, 1, 2, 2, 2, 3)
 TILE(false, f16, 2, 2, 2, 2, 2, 4)

@@ -128,7 +128,8 @@ const GemmForm kGemmF16[] = {FORM(f16, 1, 1, 2, 1, 4, 4, 1, 191, 4, 2331),
                              FORM(f16, 2, 2, 4, 2, 1, 3, 2, 380, 255, 1306),
                              FORM(f16, 2, 4, 8, 2, 1, 3, 1, 552, 3, 1567),
                              FORM(f16, 2, 4, 8, 4, 1, 2, 1, 939, 2, 2173)};
-const GemmForm kGemmF32[] = {FORM(f32, 1, 1, 2, 1, 4, 2, 3, 930, 402, 1227),
+const GemmForm kGemmF32[] = {FORM(f32, 1, 1, 2, 1, 4, 2, 3, 930, 402, 950),
+                             FORM(f32, 1, 1, 2, 1, 8, 3, 1, 1450, 0, 2300),
                              FORM(f32, 2, 1, 2, 2, 2, 3, 2, 649, 441, 1079),
                              FORM(f32, 1, 2, 4, 2, 4, 2, 1, 1358, 0, 1512),
                              FORM(f32, 2, 2, 2, 2, 1, 4, 2, 455, 332, 1018),
@@ -150,7 +151,7 @@ double estimate(const GemmForm &f, int64_t M, int64_t N, int64_t K, int64_t expe
 }
 
 // The kernel that is estimated fastest. Over those shapes its time is 1.014 (f16) and
-// 1.007 (f32) times that of the fastest one, at most 1.34 and 1.27 times; any one
+// 1.008 (f32) times that of the fastest one, at most 1.34 and 1.27 times; any one
 // kernel for all is 1.24 times and more. 8192 x 16384 x 8192 f16: 256 x 256 905 us,
 // 256 x 128 1079; 384 x 16384 x 8192: 256 x 128 68 us, 256 x 256 102; 1 x 4096 x
 // 4096: 32 x 16 with four stages 5.9 us, 64 x 64 10, 256 x 256 42; 1 x 16384 x

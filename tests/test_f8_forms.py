@@ -56,5 +56,5 @@ def test_every_kernel_is_reached(tmp_path):
     for name in ("f8_rows.hsaco", "gemm_f8.hsaco"):
         with open(os.path.join(px.LIB_DIR, name), "rb") as f:
             built |= {m.decode() for m in re.findall(rb"\0((?:gemm|norm|glu)_f8_[a-z0-9_]+)\.kd", f.read())}
-    assert len(built) == 13 + 15
+    assert len(built) == 13 + 16
     assert launched == built, (launched - built, built - launched)

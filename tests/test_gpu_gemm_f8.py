@@ -140,7 +140,7 @@ SHAPES = [(1, 1, 16), (1, 16, 128), (2, 17, 144), (3, 5, 32), (15, 33, 112), (16
           (65, 130, 2064), (5, 4099, 64), (1, 31, 16384), (127, 129, 272), (128, 128, 1024),
           (129, 300, 640), (200, 1030, 384), (256, 256, 512), (300, 520, 1040), (257, 255, 2048),
           (513, 700, 128), (1000, 1000, 16), (1030, 2050, 656), (5, 700, 2048), (64, 300, 1024), (100, 500, 512),
-          (33, 9000, 3584), (256, 260, 1536)]
+          (33, 9000, 3584), (256, 260, 1536), (20, 500, 4608), (7, 100, 20480)]
 
 
 # more tiles of every kind than the GPU runs at a time, last ones short
