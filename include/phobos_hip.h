@@ -528,8 +528,8 @@ int phx_norm_f8(phx_stream s, phx_dtype t, uint64_t x, uint64_t r, uint64_t gain
                 uint64_t y, const phx_f8_rows *q, int64_t M, int64_t K, float eps, int64_t ldx,
                 int64_t ldr, int64_t ldh, int64_t ldy);
 /* The gated activation: of each row of U, the gates [0, K) and the values
- * [K, 2K) next to them, gate / (1 + exp(-gate)) * value in f32 (within 2^-20)
- * into the rows q, with the scales a / 448.  Rows of U (type t) are ldu elements
+ * [K, 2K) next to them, gate / (1 + exp(-gate)) * value in f32 (within 2^-20 for
+ * every gate; a subnormal one within 2^-149) into the rows q, with the scales a / 448.  Rows of U (type t) are ldu elements
  * apart (0: 2K), start 16-byte aligned and in whole 16-byte chunks. */
 int phx_glu_f8(phx_stream s, phx_dtype t, uint64_t u, const phx_f8_rows *q, int64_t ldu);
 /* C = alpha * A @ W^T + beta * C of type t, [A's rows, n], rows ldc elements apart

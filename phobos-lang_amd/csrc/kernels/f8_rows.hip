@@ -169,17 +169,35 @@ __device__ __forceinline__ void norm_f8(const PhxF8Rows &p) {
     }
 }
 
-// e^x: the power of two of x log2(e), a product in two terms so that a large x
-// keeps its bits; below -100, where one plus it is one, that of -100. FAR: also where it
-// is infinite.
-template <bool FAR>
+// x log2(e) in two terms, so that a large x keeps its bits.
+struct Power {
+    float high, low;
+    __device__ __forceinline__ explicit Power(float x) {
+        const float e = 1.44269504f, rest = 1.92596303e-8f;  // log2(e) in two terms
+        high = x * e;
+        low = __builtin_fmaf(x, rest, __builtin_fmaf(x, e, -high));
+    }
+};
+
+// e^x for x up to 80; below -100, where one plus it is one, that of -100.
 __device__ __forceinline__ float exp_of(float x) {
-    x = fmaxf(x, -100.0f);
-    const float e = 1.44269504f, rest = 1.92596303e-8f;  // log2(e) in two terms
-    const float p = x * e;
-    const float low = __builtin_fmaf(x, rest, __builtin_fmaf(x, e, -p));
-    const float y = __builtin_amdgcn_exp2f(p);
-    return !FAR || __builtin_isfinite(y) ? __builtin_fmaf(y * low, 0.693147181f, y) : y;
+    const Power p(fmaxf(x, -100.0f));
+    const float y = __builtin_amdgcn_exp2f(p.high);
+    return __builtin_fmaf(y * p.low, 0.693147181f, y);
+}
+
+// gate * e^gate * value: the activation of gates below -80, where 1 + e^gate is 1. From
+// -88.7 on e^-gate is no f32 any more, and e^gate not one of all its bits, but their product
+// with a large value is: the power of two is taken in halves, before and behind the product.
+// (Where the first half leaves bits or all of the value below 2^-126, the result is 0.)
+__device__ __forceinline__ float far_value(float gate, float value) {
+    const float x = fmaxf(gate, -400.0f);  // (e^-400 times any two values is 0)
+    const Power p(x);
+    const float whole = rintf(p.high);
+    const float e = __builtin_amdgcn_exp2f((p.high - whole) + p.low);
+    const int n = (int)whole, half = n / 2;
+    const float t = ldexpf(x * e * ldexpf(value, half), n - half);
+    return gate == -INFINITY ? __builtin_nanf("") : t;
 }
 
 // A block of 128 of a row to 16 or 32 lanes; blocks of a row next to each other. No
@@ -203,16 +221,22 @@ __device__ __forceinline__ void glu_f8(const PhxF8Rows &p) {
         u.load(x);
         v.load(x + p.K);
         float t[N];
-        bool far = false;
+        uint32_t far = 0, least = ~0u;  // of the gates' bits, their magnitudes
 #pragma unroll
         for (int i = 0; i < N; ++i) {
+            far = max(far, __builtin_bit_cast(uint32_t, u.v[i]));
+            if (sizeof(T) == 4) least = min(least, f8_magnitude(u.v[i]));
             // (the reciprocal within 2^-23 of itself, as long as it is no denormal)
-            far |= u.v[i] < -80.0f;
-            t[i] = u.v[i] * __builtin_amdgcn_rcpf(1.0f + exp_of<false>(-u.v[i])) * v.v[i];
+            t[i] = u.v[i] * __builtin_amdgcn_rcpf(1.0f + exp_of(-u.v[i])) * v.v[i];
         }
-        if (far) {
+        // Gates below -80; f32 ones below 2^-124, of which half may not have its bits.
+        if (far > __builtin_bit_cast(uint32_t, -80.0f) || least < 3u << 23) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) t[i] = u.v[i] / (1.0f + exp_of<true>(-u.v[i])) * v.v[i];
+            for (int i = 0; i < N; ++i) {
+                if (u.v[i] < -80.0f) t[i] = far_value(u.v[i], v.v[i]);
+                if (sizeof(T) == 4 && fabsf(u.v[i]) < 0x1p-124f)
+                    t[i] = (u.v[i] * 0x1p24f) * (v.v[i] * 0x1p-25f);
+            }
         }
 #pragma unroll
         for (int i = 0; i < N; ++i) {
