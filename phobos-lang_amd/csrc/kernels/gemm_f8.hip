@@ -119,9 +119,12 @@ __device__ __forceinline__ Tile tile_of(const PhxF8Gemm &p, uint32_t columns) {
         }
         if (blockIdx.x >= total * columns) return t;
         const uint32_t id = uniform(phx_xcd_swizzle_any(blockIdx.x, total * columns));
+        // (starts that are written while they are read, against what is asked for, may end
+        // before this tile now: it is left out)
         uint32_t e0 = 0;
         while (of_lane(x.upto, 63) <= id / columns) {
             e0 += 64;
+            if (e0 >= E) return t;
             x = range(e0, of_lane(x.end, 63), of_lane(x.upto, 63));
         }
         const uint32_t l = uniform(__builtin_ctzll(__ballot(x.upto > id / columns)));
