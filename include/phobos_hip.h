@@ -520,7 +520,8 @@ typedef struct {
  * H = round(X + R), or X where r is 0, stored where h is not 0;
  * f = 1/sqrt(mean(H^2) + eps); of t = H * gain (f32 products) the codes go to q,
  * with the scales a * f / 448 (nullable), and round(f * t) to Y (0: not wanted).
- * The squares are summed in 64 bits.  gain is [K] of type t.  Rows are ldx, ldr,
+ * The squares are summed in 64 bits.  (A row of zeros with an eps of 0 has codes of 0
+ * and, f being infinite, scales and a Y of NaN.)  gain is [K] of type t.  Rows are ldx, ldr,
  * ldh and ldy elements apart (0: K), start 16-byte aligned and in whole 16-byte
  * chunks.  q has M rows of K.  One of H and Y may be X, one R (with their
  * strides); apart from that outputs overlap nothing. */
@@ -528,9 +529,10 @@ int phx_norm_f8(phx_stream s, phx_dtype t, uint64_t x, uint64_t r, uint64_t gain
                 uint64_t y, const phx_f8_rows *q, int64_t M, int64_t K, float eps, int64_t ldx,
                 int64_t ldr, int64_t ldh, int64_t ldy);
 /* The gated activation: of each row of U, the gates [0, K) and the values
- * [K, 2K) next to them, gate / (1 + exp(-gate)) * value in f32 (within 2^-20 for
- * every gate; a subnormal one within 2^-149) into the rows q, with the scales a / 448.  Rows of U (type t) are ldu elements
- * apart (0: 2K), start 16-byte aligned and in whole 16-byte chunks. */
+ * [K, 2K) next to them, gate / (1 + exp(-gate)) * value in f32 (within 2^-20
+ * for every gate; a subnormal one within 2^-149), into the rows q, with the scales
+ * a / 448.  Rows of U (type t) are ldu elements apart (0: 2K), start 16-byte aligned
+ * and in whole 16-byte chunks. */
 int phx_glu_f8(phx_stream s, phx_dtype t, uint64_t u, const phx_f8_rows *q, int64_t ldu);
 /* C = alpha * A @ W^T + beta * C of type t, [A's rows, n], rows ldc elements apart
  * (0: n): the products of a row's and a weight's codes in a block of 128 of K are
@@ -539,7 +541,9 @@ int phx_glu_f8(phx_stream s, phx_dtype t, uint64_t u, const phx_f8_rows *q, int6
  * overlaps no other operand.  With t f32 every product enters whole.  With t f16,
  * of the products of eight neighbouring codes, what is below 2^-13 of their
  * largest is cut off, all that the e4m3 matrix instruction keeps: 1.4e-5 of an
- * ordinary result's norm, where the rounding to f16 is 2.1e-4. */
+ * ordinary result's norm, where the rounding to f16 is 2.1e-4.  Where large products
+ * cancel, what they leave may be off by many of its own steps; t f32, at up to twice
+ * the time, is the way to results without that. */
 int phx_gemm_f8(phx_stream s, const phx_f8_rows *a, const phx_f8_weights *w, phx_dtype t, uint64_t c,
                 float alpha, float beta, int64_t ldc);
 /* The same for M rows of C sorted by expert: row i, starts[e] <= i < starts[e+1],

@@ -202,9 +202,10 @@ __device__ __forceinline__ float far_value(float gate, float value) {
 
 // A block of 128 of a row to 16 or 32 lanes; blocks of a row next to each other. No
 // lane needs more than its own block's, so a launch is as wide as its data. Bound by
-// memory: 4133 rows of 5520, f32, 38.6 us (5.3 TB/s; with a division of f32 for every
-// value 43); 16384 of 8192, f16, 141 us (4.8 TB/s; 174); 32 of 4096, f16, 3.4 us, one
-// chain of load and store.
+// memory: 4133 rows of 5520, f32, 38.9 us (5.3 TB/s; with a division of f32 for every
+// value 43); 16384 of 8192, f16, 143 us (4.7 TB/s; 174), f32 204 (5.9 TB/s); 32 of 4096,
+// f16, 3.7 us, one chain of load and store. Blocks of fewer than 128 leave lanes idle:
+// 1562500 rows of 64, f16, 186 us (2.7 TB/s).
 template <typename T>
 __device__ __forceinline__ void glu_f8(const PhxF8Rows &p) {
     constexpr int N = Chunk<T>::N, LANES = Chunk<T>::LANES;

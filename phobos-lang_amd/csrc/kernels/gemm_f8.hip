@@ -7,23 +7,27 @@
 // neighbouring products it keeps what is above 2^-13 of the largest (measured with
 // one large and one small product; the sums of eight are added in f32): 1.4e-5 of an
 // ordinary result's norm, where the rounding to f16 is 2.1e-4.
-// f32 outputs, which that would show in, take the codes as f16, exactly, and four
-// v_mfma_f32_16x16x32: 1.1e-7, at half the rate.
+// Where large products cancel it shows. That is the price of twice the rate: f32
+// outputs, which it would show in everywhere, take the codes as f16, exactly, and four
+// v_mfma_f32_16x16x32: 1.1e-7, 8192 x 16384 x 8192 1860 us instead of 920.
 // The inner sum is scaled and added in f32 by vector instructions, four for each
 // 16 x 16, which run while the matrix cores work on the next one. The weights are the
 // A operand, so that a lane holds neighbouring columns of one row of C, whose
 // scales' product is one number.
 //
-// Large products: 8192 x 16384 x 8192, f16, 902-912 us (2430 TFLOP/s; a library's 8-bit
+// Large products: 8192 x 16384 x 8192, f16, 902-932 us (2360-2440 TFLOP/s; a library 8-bit
 // product, with one scale for all, 660 to 800 with its inputs). The card is at its power
 // limit, 1.8 GHz; of the cycles the matrix cores are busy 65 %, the vector instructions
 // 48 %, LDS 29 %. A 256 x 256 tile alone on the chip, at 2.4 GHz, takes 1.18 us for 128 k
 // and 0.76 without the 64 KiB that it loads into LDS for them; in the full chip 1.75 us.
 // What is before and behind a tile's steps, 3 to 5 us, nothing hides where a CU holds one
-// workgroup: it is a fifth of 16384 rows over 61 experts of 4096 x 2048, 210 us.
-// Few rows are bound by the weights' bytes: 64 x 16384 x 8192 29.1 us (4.8 TB/s), 1 row
-// 25.5 us (5.3 TB/s). Between them, where the tiles fill the GPU but once, it is the
-// length of a step: 1000 x 1000 x 4144, f32, 16.9 us in 9 steps of 512 k.
+// workgroup: it is a fifth of 16384 rows over 61 experts of 4096 x 2048, 208-214 us. There
+// the groups' last tiles cost more still: of the 91 to 94 tiles of 256 rows 60 are not full
+// and 22 to 30 hold 128 rows or fewer, so that 30 % of the rows worked on are none.
+// Few rows are bound by the weights' bytes: 64 x 16384 x 8192 29.3 us (4.8 TB/s), 1 row
+// 25.3 us (5.3 TB/s). Between them, where the tiles fill the GPU but once, it is the
+// length of a step: 1000 x 1000 x 4144, f32, 17 us in 9 steps of 512 k; 384 x 16384 x 8192,
+// f16, 70 us in 64 steps of 1.06 us on 192 CUs.
 // (Also measured, at the same speed or slower: rows staged through registers instead of
 // loaded into LDS directly; waves of 64 x 64 that read less LDS, as many or half as many,
 // and one wave a SIMD of 128 x 64; loads spread over the whole step; a raised wave
@@ -168,7 +172,7 @@ struct Shape {
     static constexpr uint32_t STAGE = PART * WK + (STAGED ? SCALES : 0);
     static constexpr uint32_t APART = STAGED ? 16 : 2 * SCALES;
     // How many tiles of columns before it is used W is read from LDS: four where there are
-    // registers left for them (2048 x 4096 x 4096 36.6 us, one 37.4).
+    // registers left for them (2048 x 4096 x 4096: 2 % on one box, none on another).
     static constexpr int D = NT == 8 && MT == 2 ? 4 : 1;
     static constexpr uint32_t W_LOADS = TN / 8 / WAVES, A_LOADS = TM / 8 / WAVES;  // of 8 rows
     static_assert(TN % (8 * WAVES) == 0 && TM % (8 * WAVES) == 0, "whole loads a wave");
@@ -242,7 +246,7 @@ __device__ __forceinline__ void store8(const PhxF8Gemm &p, const float (&acc)[8]
         for (int i = 0; i < 8; ++i) o[i] = (T)(p.alpha * acc[i]);
     }
     // (between two dwords the 16 bytes take longer than a half, three dwords and a half:
-    // 1475 x 13175 x 96 27.6 us, so 21.8, 13174 columns 18.7)
+    // 1475 x 13175 x 96 27.6 us, so 22.4, 13174 columns 18.8)
     if constexpr (sizeof(T) == 2) if (whole && ((uint64_t)to & 2)) {
         typedef T v6 __attribute__((ext_vector_type(6)));
         typedef uint32_t u3 __attribute__((ext_vector_type(3)));
@@ -283,8 +287,8 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
     // Of few rows every workgroup reads weights of its own, all at the same k at the same
     // time, rows of W apart, which memory is slower with than it need be: they start
     // at different blocks instead and go round (in fours, as the scales come). 64 x 16384
-    // x 8192: 29.6 us, all from the first on 34; 32 experts with 62 rows each of 4096
-    // x 4096: 128 and 151. (With more rows neighbours share what they read: 256 x 256
+    // x 8192: 31 us, all from the first on 35; 1 x 16384 x 8192: 29.8 and 32.4; f32, 40 rows
+    // over 14 experts of 2048 x 4096: 30.4 and 32.5. (With more rows neighbours share what they read: 256 x 256
     // tiles would take 1 to 4 % longer so.)
     constexpr bool TURNS = S::TM <= 64;
     const uint32_t turn = !TURNS || t.rows > kDeep || blocks % 4 ? 0 : t.column * 12 % blocks;

@@ -76,7 +76,7 @@ int check_rows(phx_dtype t, uint64_t ptr, int64_t width, int64_t *ld, const char
 // ------------------------------------------------------------------ the norm
 // How a norm runs: up to 64 chunks of 16 bytes a row by as many lanes, a power of two
 // (781250 rows of 128, f16, with the sum: 124 us, by a wave each 335); up to 128 by a
-// wave (16384 rows of 1024, f16: 26.6 us, by 128 threads of a workgroup of their own
+// wave (16384 rows of 1024, f16: 26.9 us, by 128 threads of a workgroup of their own
 // 32.1); more by a workgroup of as many threads as one, two, four or eight chunks each
 // take: two from 512 on (8192 rows of 8192, f16: 87 us, four 95; 4096 of 4096, f32:
 // 42.8 us, four 47.3).
@@ -105,11 +105,12 @@ NormForm norm_form(phx_dtype t, int64_t K) {
 
 // ------------------------------------------------------------------ products
 // A kernel of gemm_f8.hip: the columns and rows of a workgroup, how many blocks of K
-// it takes in a step, and how many workgroups a CU holds.  What its time is made of,
-// fitted to the choices among the kernels over 502 shapes a type (1 to 4096 rows, K
-// 64 to 8192; grouped: 1 to 512 rows each of 5 to 61 experts): a step takes `step`
-// ns, or `shared` for every workgroup of the CU where that is more, and what is before
-// and behind the steps `rest`.
+// it takes in a step, and how many workgroups a CU holds.  What it is weighed by: `step`
+// for each step, or `shared` for every workgroup of the CU where that is more, and `rest`
+// for what is before and behind the steps.  The constants are fitted to which kernel is
+// the fastest over 502 shapes a type (1 to 4096 rows, K 64 to 8192; grouped: 1 to 512 rows
+// each of 5 to 61 experts), not to its time: that is 1.1 to 4.1 times the sum in ns for
+// f16, half of the shapes above 2.1, and 0.65 to 5.3 times, above 1.6, for f32.
 struct GemmForm {
     int64_t columns, rows, blocks;
     uint32_t threads;
@@ -137,7 +138,7 @@ const GemmForm kGemmF32[] = {FORM(f32, 1, 1, 2, 1, 4, 2, 3, 930, 402, 950),
                              FORM(f32, 2, 2, 4, 4, 1, 2, 2, 1209, 774, 751)};
 #undef FORM
 
-// (in 64-bit floating point: sizes that are refused later would overflow)
+// (in 64-bit floating point: sizes that are refused later would overflow; a weight, no time)
 double estimate(const GemmForm &f, int64_t M, int64_t N, int64_t K, int64_t experts) {
     // (which experts have how many rows is not known here: all have some)
     const int64_t live = std::min(experts, M);
@@ -145,25 +146,27 @@ double estimate(const GemmForm &f, int64_t M, int64_t N, int64_t K, int64_t expe
                                        : std::max(live, M / f.rows + live / 2);
     const int64_t groups = tiles * ((N + f.columns - 1) / f.columns);
     const int64_t steps = (blocks_of(K) + f.blocks - 1) / f.blocks, round = 256 * f.held;
-    auto ns = [&](int64_t each) { return steps * std::max(f.step, each * f.shared) + f.rest; };
+    auto of = [&](int64_t each) { return steps * std::max(f.step, each * f.shared) + f.rest; };
     const int64_t left = groups % round;
-    return (double)(groups / round) * ns(f.held) + (left ? ns((left + 255) / 256) : 0);
+    return (double)(groups / round) * of(f.held) + (left ? of((left + 255) / 256) : 0);
 }
 
-// The kernel that is estimated fastest. Over those shapes its time is 1.014 (f16) and
-// 1.008 (f32) times that of the fastest one, at most 1.34 and 1.27 times; any one
-// kernel for all is 1.24 times and more. 8192 x 16384 x 8192 f16: 256 x 256 905 us,
-// 256 x 128 1079; 384 x 16384 x 8192: 256 x 128 68 us, 256 x 256 102; 1 x 4096 x
-// 4096: 32 x 16 with four stages 5.9 us, 64 x 64 10, 256 x 256 42; 1 x 16384 x
-// 8192: 32 x 16 with two stages, of which a CU holds three, 27.6 us, with four 36.
+// The kernel that weighs least. Over those shapes its time is 1.013 (f16) and 1.007
+// (f32) times that of the fastest one, at most 1.32 and 1.27 times; any one kernel for
+// all is 1.24 times and more. (Columns x rows; f16.) 8192 x 16384 x 8192: 256 x 256
+// 922 us, 256 x 128 1058; 384 x 16384 x 8192: 256 x 128 70 us, 256 x 256 100; 1 x 4096
+// x 4096: 32 x 16 with four stages 6.4 us, with two 8.2, 64 x 64 9.5, 256 x 256 30; 64 x
+// 16384 x 8192: 64 x 64 over two blocks 29.4 us, over one 30.5, 64 x 32 36.7. Not the
+// fastest: 257 x 8192 x 8192, 64 x 64 43.8 us, 128 x 64 38.3; 1 x 16384 x 8192, 64 x 16
+// 25.5 us, 32 x 16 with two stages 24.8.
 const GemmForm &gemm_form(phx_dtype t, int64_t M, int64_t N, int64_t K, int64_t experts) {
     const GemmForm *first = t == PHX_F16 ? std::begin(kGemmF16) : std::begin(kGemmF32);
     const GemmForm *last = t == PHX_F16 ? std::end(kGemmF16) : std::end(kGemmF32);
     const GemmForm *best = first;
     double least = INFINITY;
     for (; first != last; ++first) {
-        const double ns = estimate(*first, M, N, K, experts);
-        if (ns < least) best = first, least = ns;
+        const double w = estimate(*first, M, N, K, experts);
+        if (w < least) best = first, least = w;
     }
     return *best;
 }
