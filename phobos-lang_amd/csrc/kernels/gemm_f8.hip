@@ -172,7 +172,7 @@ struct Shape {
     static constexpr uint32_t STAGE = PART * WK + (STAGED ? SCALES : 0);
     static constexpr uint32_t APART = STAGED ? 16 : 2 * SCALES;
     // How many tiles of columns before it is used W is read from LDS: four where there are
-    // registers left for them (2048 x 4096 x 4096: 2 % on one box, none on another).
+    // registers left for them (2048 x 4096 x 4096: up to 2 %).
     static constexpr int D = NT == 8 && MT == 2 ? 4 : 1;
     static constexpr uint32_t W_LOADS = TN / 8 / WAVES, A_LOADS = TM / 8 / WAVES;  // of 8 rows
     static_assert(TN % (8 * WAVES) == 0 && TM % (8 * WAVES) == 0, "whole loads a wave");
@@ -288,8 +288,8 @@ __device__ __forceinline__ void gemm_tile(const PhxF8Gemm &p, char *const (&st)[
     // time, rows of W apart, which memory is slower with than it need be: they start
     // at different blocks instead and go round (in fours, as the scales come). 64 x 16384
     // x 8192: 31 us, all from the first on 35; 1 x 16384 x 8192: 29.8 and 32.4; f32, 40 rows
-    // over 14 experts of 2048 x 4096: 30.4 and 32.5. (With more rows neighbours share what they read: 256 x 256
-    // tiles would take 1 to 4 % longer so.)
+    // over 14 experts of 2048 x 4096: 30.4 and 32.5. (With more rows neighbours share what
+    // they read: 256 x 256 tiles would take 1 to 4 % longer so.)
     constexpr bool TURNS = S::TM <= 64;
     const uint32_t turn = !TURNS || t.rows > kDeep || blocks % 4 ? 0 : t.column * 12 % blocks;
     auto turned = [&](uint32_t b) {
